@@ -414,6 +414,64 @@ int nf4_qkv_rope_bwd(const void *dq, const void *dk, const void *dv, const float
                      const float *sin_t, void *dqkv, int64_t ld_dqkv, int64_t tokens, int n_heads,
                      int n_kv, int head_dim, int dtype, void *stream);
 
+/* ------------------------------------------ serving: a paged cache and attention over it */
+
+/* A paged key/value cache and one step's sequences.  Position j of sequence b lies in page
+ * table[b * ld_table + j / page_size], slot j % page_size; key/value head h of it starts
+ * page * page_stride + slot * slot_stride + h * head_stride 16-bit elements after k (and v), its
+ * head_dim values consecutive.  A table entry outside [0, pages) names no page: appends to it
+ * are dropped and its keys are not seen.  lens[b] is the sequence's length with the call's own
+ * tokens.  page_size is a power of two, head_dim 64 or 128, the strides multiples of 8 and k, v
+ * 16-byte aligned; width * page_size at most 2^30. */
+typedef struct nf4_paged_kv {
+    void *k;
+    void *v;
+    int64_t page_stride;
+    int64_t slot_stride;
+    int64_t head_stride;
+    const int32_t *table; /* device, [batch, ld_table] */
+    int64_t ld_table;
+    const int32_t *lens;  /* device, [batch] */
+    int32_t pages;
+    int32_t page_size;
+    int32_t width;        /* table entries of a sequence */
+    int32_t batch;
+    int32_t n_kv;
+    int32_t head_dim;
+} nf4_paged_kv;
+
+/* One step's q|k|v projection (qkv [tokens, ld_qkv], columns as in nf4_qkv_rope) into q
+ * [tokens, n_heads, head_dim] and the cache.  Sequence b brings the tokens cu_q[b] ..
+ * cu_q[b + 1] - 1 (device, [batch + 1], from 0 on, not decreasing), or tokens / batch each when
+ * cu_q is NULL; the i-th of its n is at position p = lens[b] - n + i.  Per pair i < head_dim / 2:
+ * lo' = lo cos[p][i] - hi sin[p][i], hi' = hi cos[p][i] + lo sin[p][i] on q and k in fp32 (cos,
+ * sin fp32 [rope_rows, head_dim / 2]), rounded once.  A token whose position is not in
+ * [0, rope_rows), or that is past the last offset, gets a q of zeros and no place in the cache;
+ * one past the table keeps its q only. */
+int nf4_paged_append(const nf4_paged_kv *kv, const void *qkv, int64_t ld_qkv, const float *cos_t,
+                     const float *sin_t, int64_t rope_rows, const int32_t *cu_q, void *q,
+                     int64_t tokens, int n_heads, int dtype, void *stream);
+
+/* Attention of a step's queries (q: token ld_tok, head ld_head elements apart, multiples of 8)
+ * over the cache, positions as in nf4_paged_append.  The query at p sees key j <= p where
+ * window == 0, j > p - window or j < sinks; with s = scale * q.k over them, out
+ * [tokens, n_heads, head_dim] = sum softmax(s) v and lse [tokens, n_heads] (fp32, may be NULL)
+ * = log sum exp(s).  A query that sees no key gets zeros and -inf.  Query head h reads
+ * key/value head h / (n_heads / n_kv).
+ * shared > 0: positions below it are read through sequence 0's table row for every sequence,
+ * once for the whole batch (a prefix that all of them start with).
+ * max_q and max_len are the longest run of new tokens and the longest length as the host knows
+ * them (0: unknown).  They choose the launch shape only: longer sequences are still right.
+ * Workspace: nf4_paged_attn_workspace bytes, 16-byte aligned. */
+size_t nf4_paged_attn_workspace(const nf4_paged_kv *kv, const int32_t *cu_q, int64_t tokens,
+                                int n_heads, int64_t window, int64_t sinks, int64_t shared,
+                                int64_t max_q, int64_t max_len);
+int nf4_paged_attn(const nf4_paged_kv *kv, const void *q, int64_t ld_tok, int64_t ld_head,
+                   const int32_t *cu_q, void *out, float *lse, int64_t tokens, int n_heads,
+                   float scale, int64_t window, int64_t sinks, int64_t shared, int64_t max_q,
+                   int64_t max_len, int dtype, void *workspace, size_t workspace_bytes,
+                   void *stream);
+
 /* -------------------------------------------------------------------------- small helpers */
 
 /* out[rows, cols] = silu(gate) * up, and its gradient (the SwiGLU step between the gate/up and

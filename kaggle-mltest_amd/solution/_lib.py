@@ -54,6 +54,16 @@ class NF4LoraJob(ctypes.Structure):
     ]
 
 
+class NF4PagedKV(ctypes.Structure):
+    """struct nf4_paged_kv (include/nf4_mi355x.h), 88 bytes."""
+    _fields_ = [
+        ("k", c_void_p), ("v", c_void_p), ("page_stride", c_int64), ("slot_stride", c_int64),
+        ("head_stride", c_int64), ("table", c_void_p), ("ld_table", c_int64), ("lens", c_void_p),
+        ("pages", c_int32), ("page_size", c_int32), ("width", c_int32), ("batch", c_int32),
+        ("n_kv", c_int32), ("head_dim", c_int32),
+    ]
+
+
 _SIGNATURES = {
     "nf4_abi_version": (c_int, []),
     "nf4_status_string": (ctypes.c_char_p, [c_int]),
@@ -140,6 +150,14 @@ _SIGNATURES = {
                              c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "nf4_qkv_rope_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                  c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "nf4_paged_append": (c_int, [ctypes.POINTER(NF4PagedKV), c_void_p, c_int64, c_void_p,
+                                 c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int,
+                                 c_void_p]),
+    "nf4_paged_attn_workspace": (c_size_t, [ctypes.POINTER(NF4PagedKV), c_void_p, c_int64, c_int,
+                                            c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "nf4_paged_attn": (c_int, [ctypes.POINTER(NF4PagedKV), c_void_p, c_int64, c_int64, c_void_p,
+                               c_void_p, c_void_p, c_int64, c_int, c_float, c_int64, c_int64,
+                               c_int64, c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
 }
 
 EXPORTS = tuple(_SIGNATURES)

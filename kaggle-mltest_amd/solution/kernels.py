@@ -9,7 +9,7 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import DTYPE_CODE, NF4Lora, NF4LoraJob, check, load, stream_of
+from ._lib import DTYPE_CODE, NF4Lora, NF4LoraJob, NF4PagedKV, check, load, stream_of
 from .quant_state import weight_array, weight_desc
 
 GEMM_DTYPES = (torch.float16, torch.bfloat16)
@@ -653,3 +653,150 @@ def int8_swiglu_bwd(acc: torch.Tensor, sd: torch.Tensor, cs: torch.Tensor,
                                      2 * inter, sq.data_ptr(), _code(gu.dtype), stream_of(acc)),
           "nf4_int8_swiglu_bwd")
     return q, sq
+
+
+# ------------------------------------------------- serving: a paged cache, attention over it
+
+class PagedKV:
+    """One layer's paged key/value cache and the step's sequences, as the paged calls take them.
+
+    `k_pages`, `v_pages`: [pages, page_size, n_kv, head_dim] float16 or bfloat16 views of one
+    layout (any order of the first three dimensions in memory: head-major pages come as
+    `pages.transpose(1, 2)`); `table`: int32 [batch, width], the page of every page_size
+    positions of a sequence (an entry outside the cache, -1 say, names no page: appends there are
+    dropped, its keys are not seen); `lens`: int32 [batch], each sequence's length with the
+    step's own tokens.  The layout is checked and packed once; the tensors' contents are read on
+    the device by every call, so a program updates `table` and `lens` in place between steps (a
+    captured graph then replays with the new lengths).  Layers of a model share `table` and
+    `lens`."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, table: torch.Tensor,
+                 lens: torch.Tensor):
+        _check_device(k_pages, v_pages, table, lens)
+        if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
+            raise ValueError("k_pages and v_pages are [pages, page_size, n_kv, head_dim] of one dtype")
+        if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+            raise ValueError("k_pages and v_pages share their strides, head_dim contiguous")
+        if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
+            raise ValueError("table is an int32 [batch, width] tensor with contiguous rows")
+        if lens.dtype != torch.int32 or tuple(lens.shape) != (table.shape[0],) \
+                or not lens.is_contiguous():
+            raise ValueError("lens is a contiguous int32 [batch] tensor")
+        if len({t.device for t in (k_pages, v_pages, table, lens)}) != 1:
+            raise ValueError("the cache, its table and lens are on one device")
+        self.k_pages, self.v_pages, self.table, self.lens = k_pages, v_pages, table, lens
+        self.dtype, self.code = k_pages.dtype, _code(k_pages.dtype)
+        self.batch, self.width = (int(d) for d in table.shape)
+        pages, self.page_size, self.n_kv, self.head_dim = (int(d) for d in k_pages.shape)
+        ld_table = max(int(table.stride(0)), self.width)  # one row's stride says nothing
+        self.desc = NF4PagedKV(
+            k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1),
+            k_pages.stride(2), table.data_ptr(), ld_table, lens.data_ptr(), pages,
+            self.page_size, self.width, self.batch, self.n_kv, self.head_dim)
+        self.ref = ctypes.byref(self.desc)
+
+
+def _check_cu(cu_q, cache: PagedKV):
+    if cu_q is None:
+        return None
+    if not cu_q.is_cuda or cu_q.dtype != torch.int32 or tuple(cu_q.shape) != (cache.batch + 1,) \
+            or not cu_q.is_contiguous():
+        raise ValueError("cu_q is a contiguous int32 [batch + 1] device tensor")
+    return cu_q.data_ptr()
+
+
+def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache: PagedKV,
+                 cu_q: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotated q [tokens, n_heads, head_dim] of a step's q|k|v projection (`qkv`
+    [tokens, (n_heads + 2 n_kv) head_dim], rows any multiple of 8 apart); its rotated k and its v
+    go to the cache, the i-th of a sequence's n tokens to position lens - n + i.  `cos`, `sin`:
+    fp32 [positions, head_dim / 2] (rope_table); `cu_q`: int32 offsets of the sequences' tokens,
+    None when each brings tokens / batch."""
+    dim, kv = cache.head_dim, cache.n_kv
+    if qkv.dim() != 2 or qkv.dtype != cache.dtype or qkv.stride(1) != 1 or qkv.shape[1] % dim:
+        raise ValueError("qkv is a row-contiguous [tokens, (n_heads + 2 n_kv) head_dim] tensor of "
+                         "the cache's dtype")
+    _check_device(qkv, cos, sin)
+    tokens, heads = qkv.shape[0], qkv.shape[1] // dim - 2 * kv
+    if heads < 1 or heads % kv:
+        raise ValueError("n_heads is a multiple of the cache's n_kv")
+    for t in (cos, sin):
+        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] * 2 != dim \
+                or t.shape != cos.shape or not t.is_contiguous():
+            raise ValueError("cos and sin are contiguous fp32 [positions, head_dim / 2] tables")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=qkv.dtype, device=qkv.device)
+    else:
+        _check_out(out, (tokens, heads, dim), qkv)
+    ld = qkv.stride(0) if tokens > 1 else qkv.shape[1]
+    st = load().nf4_paged_append(cache.ref, qkv.data_ptr(), ld, cos.data_ptr(), sin.data_ptr(),
+                                 cos.shape[0], _check_cu(cu_q, cache), out.data_ptr(), tokens,
+                                 heads, cache.code, stream_of(qkv))
+    if st:
+        check(st, "nf4_paged_append")
+    return out
+
+
+def _check_out(out, shape, like):
+    if tuple(out.shape) != shape or out.dtype != like.dtype or out.device != like.device \
+            or not out.is_contiguous():
+        raise ValueError(f"out is a contiguous {list(shape)} tensor of the input's dtype")
+
+
+def _attention(q, cache, shared, cu_q, scale, window, sinks, max_q, max_len, out, lse):
+    if q.dim() != 3 or q.dtype != cache.dtype or q.shape[2] != cache.head_dim or q.stride(2) != 1:
+        raise ValueError("q is [tokens, n_heads, head_dim] of the cache's dtype, head_dim contiguous")
+    _check_device(q)
+    tokens, heads, dim = q.shape
+    if heads < 1 or heads % cache.n_kv:
+        raise ValueError("n_heads is a multiple of the cache's n_kv")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    else:
+        _check_out(out, (tokens, heads, dim), q)
+    stats = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if lse else None
+    lib = load()
+    cu = _check_cu(cu_q, cache)
+    window, sinks, max_q, max_len = window or 0, sinks or 0, max_q or 0, max_len or 0
+    nbytes = lib.nf4_paged_attn_workspace(cache.ref, cu, tokens, heads, window, sinks, shared,
+                                          max_q, max_len)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
+    st = lib.nf4_paged_attn(cache.ref, q.data_ptr(), q.stride(0), q.stride(1), cu, out.data_ptr(),
+                            _p(stats), tokens, heads, dim ** -0.5 if scale is None else scale,
+                            window, sinks, shared, max_q, max_len, cache.code, _p(ws), nbytes,
+                            stream_of(q))
+    if st:
+        check(st, "nf4_paged_attn")
+    return (out, stats) if lse else out
+
+
+def paged_attention(q: torch.Tensor, cache: PagedKV, cu_q: torch.Tensor | None = None,
+                    scale: float | None = None, window: int = 0, sinks: int = 0, max_q: int = 0,
+                    max_len: int = 0, out: torch.Tensor | None = None, lse: bool = False):
+    """Causal attention of a step's queries over the cache: out [tokens, n_heads, head_dim] (and
+    with `lse` the fp32 log-sum-exp [tokens, n_heads]).  The i-th of a sequence's n tokens is at
+    position p = lens - n + i and sees key j <= p where window == 0, j > p - window or j < sinks;
+    a query that sees nothing gives zeros and -inf.  `scale`: head_dim ** -0.5 by default.
+    `max_q`, `max_len`: the longest run of new tokens and the longest length, as far as the host
+    knows them; they only choose the launch shape (unknown: from the tensors' shapes), and a
+    sequence beyond them is still right."""
+    return _attention(q, cache, 0, cu_q, scale, window, sinks, max_q, max_len, out, lse)
+
+
+def shared_prefix_attention(q: torch.Tensor, cache: PagedKV, shared: int,
+                            cu_q: torch.Tensor | None = None, scale: float | None = None,
+                            window: int = 0, sinks: int = 0, max_q: int = 0, max_len: int = 0,
+                            out: torch.Tensor | None = None, lse: bool = False):
+    """paged_attention for a batch whose sequences start with the same `shared` positions: their
+    keys are read once for all sequences, through the first row of the cache's table (which must
+    name their pages); every other position is the sequence's own, as in paged_attention."""
+    return _attention(q, cache, int(shared), cu_q, scale, window, sinks, max_q, max_len, out, lse)
+
+
+def rope_table(positions: int, head_dim: int, base: float, device):
+    """(cos, sin) fp32 [positions, head_dim / 2] of paged_append: angles
+    position * base ** (-2 i / head_dim), formed in 64 bits, so that far positions are as exact
+    as near ones."""
+    inv = base ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
+    ang = torch.arange(positions, dtype=torch.float64)[:, None] * inv
+    return ang.cos().float().to(device), ang.sin().float().to(device)
