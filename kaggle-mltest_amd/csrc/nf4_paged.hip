@@ -47,6 +47,16 @@ __device__ __forceinline__ Seq seq_at(const Cache &c, int b) {
     return s;
 }
 
+// The same for a b that is the wave's, in scalar registers (loop bounds and branches then are
+// scalar ones).
+__device__ __forceinline__ Seq seq_uniform(const Cache &c, int b) {
+    Seq s = seq_at(c, b);
+    s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
+    s.n = __builtin_amdgcn_readfirstlane(s.n);
+    s.p0 = __builtin_amdgcn_readfirstlane(s.p0);
+    return s;
+}
+
 // The sequence of token t: with offsets, how many sequences end at or before it (64 at a time).
 __device__ __forceinline__ int seq_of_token(const Cache &c, int t) {
     if (!c.cu) return t / c.uniform;
@@ -152,34 +162,55 @@ __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
 // the lane, and the scores leave the first product in the register layout that the second one
 // takes as its operand.
 //
-// Parts.  A launch covers the positions [shared, end) of each sequence through its own table
-// row, or (prefix) [0, shared) through row 0 for the rows of the whole batch.  The tiles that
-// some row of a workgroup sees (sink tiles, then window tiles) are cut into `splits` pieces; with
-// one piece in all the workgroup writes the output, else (maximum, sum, unscaled output) in fp32
-// for paged_attn_join_kernel.
+// Parts.  A sequence's positions [shared, end) are read through its own table row, [0, shared)
+// through row 0 for the rows of the whole batch.  Both are cut into pieces where there are too
+// few rows to fill the card; what a piece leaves is (maximum, sum, unscaled output) in fp32 for
+// paged_attn_join_kernel, and the output itself where the piece is all there is of a row.
 
 struct Query {
     const uint16_t *q;
     int64_t ld_tok, ld_head;
     uint16_t *out;
     float *lse;
-    float *part_o;   // [tokens * n_heads][pieces][D]
-    float2 *part_ml; // [tokens * n_heads][pieces]
-    int pieces;      // of all the parts
+    float *part_o;    // tiled parts: [tokens * n_heads][dense][D]
+    float2 *part_ml;  // [tokens * n_heads][dense]
+    int dense;        // pieces of the tiled parts; 0: their rows are written to `out`
     int n_heads, group, window, sinks, shared;
-    float scale;     // of the scores in units of log 2, positive
-    uint32_t flip;   // sign bits of a query pair, where the scale is negative
+    float scale;      // of the scores in units of log 2, positive
+    uint32_t flip;    // sign bits of a query pair, where the scale is negative
 };
 
-struct Part {
+struct Part {       // a tiled part
     int prefix;     // 1: positions below `shared`, the whole batch's rows
     int splits;     // pieces of this part
     int first;      // index of its first piece
     int min_tiles;  // tiles of a piece, at least
-    int blocks;     // row blocks (tiled kernel)
+    int blocks;     // row blocks
+    int groups;     // workgroups
+};
+
+struct Few {         // the parts of few rows
+    float *part_o;   // [slots * n_kv][rows of an item][D]
+    float2 *part_ml; // [slots * n_kv][rows of an item]
+    int groups;      // workgroups a key/value head
+    int min_units;   // work of one, at least
+    int whole;       // 1: an item each
+    int items;       // at most
+    int seqs, prefix; // entries: sequences, and 1 for the prefix if it has few rows
+    int direct;      // 1: an item in one piece is written to `out`
 };
 
 constexpr int kNowhere = -(1 << 30);  // the position of a row that is not there
+
+// The 16 slots from position k (a multiple of 16) on, in page e of the keys or values of a head
+// (`base`, 16-bit elements), as a buffer resource: an entry that names no page, or pos past the
+// end, is an empty one, from which every load gives zeros.
+__device__ __forceinline__ rsrc_t slots16(const Cache &c, const uint16_t *base, int e, int k, int row_bytes) {
+    const int64_t at = e * c.page_stride + (k & ((1 << c.page_shift) - 1)) * c.slot_stride;
+    const bool there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
+    return make_rsrc(reinterpret_cast<const char *>(base) + uniform64(there ? at * 2 : 0),
+                     there ? c.slot_stride * 30 + row_bytes : 0);
+}
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
@@ -215,10 +246,10 @@ struct Range {
     int sink0, sinks_n, win0, n;  // tiles
     int i0, i1;                   // of this piece
 
-    __device__ __forceinline__ void set(const Cache &c, const Query &a, const Part &part, int piece) {
+    __device__ __forceinline__ void set(const Cache &c, const Query &a, int prefix) {
         const int end = pmax + 1 < c.cap ? pmax + 1 : c.cap;
-        lo = part.prefix ? 0 : a.shared;
-        hi = part.prefix && a.shared < end ? a.shared : end;
+        lo = prefix ? 0 : a.shared;
+        hi = prefix && a.shared < end ? a.shared : end;
         int first = lo;
         if (a.window && pmin >= a.window && pmin - a.window + 1 > lo) first = pmin - a.window + 1;
         const int se = a.window ? (a.sinks < hi ? a.sinks : hi) : lo;
@@ -231,8 +262,12 @@ struct Range {
             sinks_n = (s1 < win0 ? s1 : win0) - sink0;
             n = sinks_n + (w1 > win0 ? w1 - win0 : 0);
         }
-        int per = (n + part.splits - 1) / part.splits;
-        per = per > part.min_tiles ? per : part.min_tiles;
+        i0 = 0;
+        i1 = n;
+    }
+    __device__ __forceinline__ void cut(int splits, int min_tiles, int piece) {
+        int per = (n + splits - 1) / splits;
+        per = per > min_tiles ? per : min_tiles;
         i0 = piece * per < n ? piece * per : n;
         i1 = i0 + per < n ? i0 + per : n;
     }
@@ -294,39 +329,191 @@ __device__ __forceinline__ u32x4_t load_q(const Query &a, int tok, int head, int
 
 // ------------------------------------------------------------- few rows (decoding)
 //
-// At most 16 RB rows (more are taken in turns): the bytes of the cache are all that counts, and
-// no key is used often enough for LDS to pay.  Each of a workgroup's 4 waves takes every fourth
-// 32-key slab on its own, straight from memory into MFMA operands: a lane loads 16 bytes of a key
-// (rows of K are A-operand rows as they lie) and 16 bytes (8 channels) of 8 of its V rows, and
-// turns the 8x8 block of V into operands by byte permutes, which is free beside the memory
-// (channel e of each lane's 8 forms one product, so the order of channels is a permuted one).
-// The next slab's keys are loaded as soon as the scores are formed and its values as soon as they
-// are used, so that a wave always has loads in flight; the 4 waves' results meet in LDS.
+// Work.  An item is at most 16 RB rows of a sequence (more are further items) and all that they
+// see; it costs a unit to begin and one for every step, a slab of 32 keys for each of the
+// workgroup's W waves.  Lengths are known on the device only, so every workgroup adds up all
+// sequences' units (64 at a time, a lane each) and takes an equal share of the total, which ends
+// and begins inside items: all workgroups are resident and finish together, however uneven the
+// lengths (a fixed number of pieces per sequence instead: 64 sequences of 40 to 16000 keys
+// 399 us).  A piece's slot is its workgroup's number plus its item's: two pieces of one
+// workgroup, or two workgroups in one item, never have the same.
 
-template <int DT, int D, int RB, bool SMALL>
-__global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void paged_attn_few_kernel(const Cache c, const Query a,
-                                                             const Part part) {
+template <int D>
+constexpr int few_lds(int waves, int rb) { return waves * 16 * rb * ((D + 4) * 4 + 8); }
+
+struct Units {
+    int64_t total, base, up;   // units: of all entries; before this chunk; to this lane's end
+    int ibase, iup;            // items, alike
+    int b0, steps, blocks;     // first entry of the chunk; this lane's entry
+    int pmin, pmax;            // positions of the whole batch (if a prefix is an entry)
+};
+
+// `div` of an equal cut: the first unit of workgroup g of n
+__device__ __forceinline__ int64_t first_unit(int64_t total, int g, int n) {
+    const uint64_t x = static_cast<uint64_t>(g) * static_cast<uint64_t>(total);
+    if (x >> 32) return static_cast<int64_t>(x / static_cast<uint32_t>(n));
+    return static_cast<uint32_t>(x) / static_cast<uint32_t>(n);
+}
+
+// the workgroup whose share holds unit u: the largest g with g total < (u + 1) n
+__device__ __forceinline__ int group_of(int64_t total, int64_t u, int n) {
+    const uint64_t x = static_cast<uint64_t>(u + 1) * static_cast<uint32_t>(n) - 1;
+    if ((x | static_cast<uint64_t>(total)) >> 32) return static_cast<int>(x / static_cast<uint64_t>(total));
+    return static_cast<uint32_t>(x) / static_cast<uint32_t>(total);
+}
+
+__device__ __forceinline__ int groups_used(const Few &f, int64_t total) {
+    const int64_t n = total / f.min_units;
+    return n < 1 ? 1 : n < f.groups ? static_cast<int>(n) : f.groups;
+}
+
+template <int W, int RB>
+__device__ __forceinline__ void load_units(Units &u, const Cache &c, const Query &a, const Few &f,
+                                           int b0) {
+    const int l = threadIdx.x & 63, e = b0 + l;
+    u.b0 = b0;
+    u.steps = u.blocks = 0;
+    if (e < f.seqs + f.prefix) {
+        Range<5> rg;
+        int rows = c.tokens * a.group;
+        rg.pmin = u.pmin;
+        rg.pmax = u.pmax;
+        if (e < f.seqs) {
+            const Seq s = seq_at(c, e);
+            rows = s.n * a.group;
+            rg.pmin = s.p0;
+            rg.pmax = s.p0 + s.n - 1;
+        }
+        rg.set(c, a, e == f.seqs);
+        u.blocks = (rows + 16 * RB - 1) / (16 * RB);
+        u.steps = (rg.n + W - 1) / W;
+    }
+    u.up = static_cast<int64_t>(u.blocks) * (f.whole ? 1 : u.steps + 1);
+    u.iup = u.blocks;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t x = __shfl_up(u.up, o);
+        const int y = __shfl_up(u.iup, o);
+        if (l >= o) {
+            u.up += x;
+            u.iup += y;
+        }
+    }
+}
+
+__device__ __forceinline__ int64_t last_lane(int64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), 63);
+    const int hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), 63);
+    return (static_cast<int64_t>(hi) << 32) | lo;
+}
+
+__device__ __forceinline__ int64_t lane_of(int64_t v, int l) {
+    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(v), l);
+    const int hi = __builtin_amdgcn_readlane(static_cast<int>(v >> 32), l);
+    return (static_cast<int64_t>(hi) << 32) | lo;
+}
+
+// The total, and the chunk of the first 64 entries.
+template <int W, int RB>
+__device__ __forceinline__ void all_units(Units &u, const Cache &c, const Query &a, const Few &f) {
+    u.pmin = 0x7fffffff;
+    u.pmax = kNowhere;
+    if (f.prefix) {
+        for (int b0 = 0; b0 < f.seqs; b0 += 64) {
+            const int e = b0 + (threadIdx.x & 63);
+            if (e >= f.seqs) continue;
+            const Seq s = seq_at(c, e);
+            if (s.n == 0) continue;
+            u.pmin = s.p0 < u.pmin ? s.p0 : u.pmin;
+            u.pmax = s.p0 + s.n - 1 > u.pmax ? s.p0 + s.n - 1 : u.pmax;
+        }
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int x = __shfl_xor(u.pmin, o), z = __shfl_xor(u.pmax, o);
+            u.pmin = x < u.pmin ? x : u.pmin;
+            u.pmax = z > u.pmax ? z : u.pmax;
+        }
+        u.pmin = __builtin_amdgcn_readfirstlane(u.pmin);
+        u.pmax = __builtin_amdgcn_readfirstlane(u.pmax);
+    }
+    u.total = u.base = 0;
+    u.ibase = 0;
+    const int n = f.seqs + f.prefix;
+    for (int b0 = 0; b0 < n; b0 += 64) {
+        load_units<W, RB>(u, c, a, f, b0);
+        u.total += last_lane(u.up);
+    }
+    if (n > 64) load_units<W, RB>(u, c, a, f, 0);
+}
+
+template <int W, int RB>
+__device__ __forceinline__ void next_units(Units &u, const Cache &c, const Query &a, const Few &f) {
+    u.base += last_lane(u.up);
+    u.ibase += __builtin_amdgcn_readlane(u.iup, 63);
+    load_units<W, RB>(u, c, a, f, u.b0 + 64);
+}
+
+// The bytes of the cache are all that counts, and no key is used often enough for LDS to pay.
+// Each wave takes every W-th 32-key slab on its own, straight from memory into MFMA operands: a
+// lane loads 16 bytes of a key (rows of K are A-operand rows as they lie) and 16 bytes (8
+// channels) of 8 of its V rows, and turns the 8x8 block of V into operands by byte permutes,
+// which is free beside the memory (channel e of each lane's 8 forms one product, so the order of
+// channels is a permuted one).  The next slab's keys are loaded as soon as the scores are formed
+// and its values as soon as they are used, so that a wave always has loads in flight; the waves'
+// results meet in LDS.
+
+template <int DT, int D, int RB, bool SMALL, int W>
+__device__ __forceinline__ void few_body(const Cache &c, const Query &a, const Few &f, int block,
+                                         uint8_t *lds) {
     constexpr int KC = D / 32, VE = D / 16, LD = D + 4;  // K chunks, V values a lane, LDS row
-    __shared__ float s_o[4][16 * RB][LD];
-    __shared__ float s_ml[4][16 * RB][2];
+    float *s_o = reinterpret_cast<float *>(lds);                           // [W][16 RB][LD]
+    float2 *s_ml = reinterpret_cast<float2 *>(s_o + W * 16 * RB * LD);     // [W][16 RB]
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     const int g = l >> 4, n = l & 15;
-    const int kvh = blockIdx.x % c.n_kv, y = blockIdx.x / c.n_kv;
-    const int piece = y % part.splits, item = y / part.splits;
-    const int b = part.prefix ? 0 : item;
-    Seq s = {0, c.tokens, 0};
-    if (!part.prefix) s = seq_at(c, b);
-    const int rows = s.n * a.group;
-    const int32_t *tab = c.table + b * c.ld_table;
-    const char *kb = reinterpret_cast<const char *>(c.k + kvh * c.head_stride);
-    const char *vb = reinterpret_cast<const char *>(c.v + kvh * c.head_stride);
-    const uint32_t stride2 = static_cast<uint32_t>(c.slot_stride) * 2;
+    const int kvh = block % c.n_kv, group = block / c.n_kv;
+    const uint16_t *kb = c.k + kvh * c.head_stride, *vb = c.v + kvh * c.head_stride;
+    const int stride2 = static_cast<int>(c.slot_stride) * 2;
     const int page_mask = (1 << c.page_shift) - 1;
 
-    for (int r0 = part.prefix ? item * 16 * RB : 0; r0 < rows; r0 += 16 * RB) {
+    Units u;
+    all_units<W, RB>(u, c, a, f);
+    const int used = f.whole ? 0 : groups_used(f, u.total);
+    if (f.whole ? group >= u.total : group >= used) return;
+    const int64_t u1 = f.whole ? group + 1 : first_unit(u.total, group + 1, used);
+    int64_t at = f.whole ? group : first_unit(u.total, group, used);
+    while (at < u1) {
+        // the item that unit `at` falls into
+        uint64_t past = __ballot(u.base + u.up > at);
+        while (!past) {
+            if (u.b0 + 64 >= f.seqs + f.prefix) return;  // lengths that changed under the kernel
+            next_units<W, RB>(u, c, a, f);
+            past = __ballot(u.base + u.up > at);
+        }
+        const int lane = __builtin_ctzll(past);
+        const int b = u.b0 + lane, steps = __builtin_amdgcn_readlane(u.steps, lane);
+        const int blocks = __builtin_amdgcn_readlane(u.blocks, lane);
+        const int per = f.whole ? 1 : steps + 1;
+        int64_t start = u.base + lane_of(u.up, lane) - static_cast<int64_t>(blocks) * per;
+        const int blk = blocks == 1 ? 0 : static_cast<int>((at - start) / per);
+        start += static_cast<int64_t>(blk) * per;
+        const int item = u.ibase + __builtin_amdgcn_readlane(u.iup, lane) - blocks + blk;
+        const int64_t next = start + per < u1 ? start + per : u1;
+        int st0 = static_cast<int>(at - start) - 1, st1 = static_cast<int>(next - start) - 1;
+        st0 = st0 < 0 ? 0 : st0;
+        if (f.whole) st1 = steps;
+        at = next;
+        if (item >= f.items) return;             // offsets that decrease
+        if (st1 <= st0 && steps) continue;       // no more than its beginning
+        const bool single = st0 == 0 && st1 == steps;
+
+        const bool prefix = b == f.seqs;
+        Seq s = {0, c.tokens, 0};
+        if (!prefix) s = seq_uniform(c, b);
+        const int rows = s.n * a.group, r0 = blk * 16 * RB;
+        const int32_t *tab = c.table + (prefix ? 0 : b) * c.ld_table;
         // this lane's rows and their positions
         u32x4_t q[RB][KC];
-        int pos[RB], pmin = 0x7fffffff, pmax = kNowhere;
+        int pos[RB];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             const int r = r0 + rb * 16 + n;
@@ -335,23 +522,17 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void paged_attn_few_kernel(co
             for (int k = 0; k < KC; ++k) q[rb][k] = (u32x4_t){0, 0, 0, 0};
             if (r < rows) {
                 const int tok = s.q0 + r / a.group, head = kvh * a.group + r % a.group;
-                pos[rb] = part.prefix ? position_of(c, tok) : s.p0 + r / a.group;
-                pmin = pos[rb] < pmin ? pos[rb] : pmin;
-                pmax = pos[rb] > pmax ? pos[rb] : pmax;
+                pos[rb] = prefix ? position_of(c, tok) : s.p0 + r / a.group;
 #pragma unroll
                 for (int k = 0; k < KC; ++k) q[rb][k] = load_q(a, tok, head, k * 32 + g * 8);
             }
         }
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-            const int x = __shfl_xor(pmin, o), z = __shfl_xor(pmax, o);
-            pmin = x < pmin ? x : pmin;
-            pmax = z > pmax ? z : pmax;
-        }
-        Range<5> rg;
-        rg.pmin = __builtin_amdgcn_readfirstlane(pmin);
-        rg.pmax = __builtin_amdgcn_readfirstlane(pmax);
-        rg.set(c, a, part, piece);
+        Range<5> rg;  // of all the entry's rows, as its steps were counted
+        rg.pmin = prefix ? u.pmin : s.p0;
+        rg.pmax = prefix ? u.pmax : s.p0 + s.n - 1;
+        rg.set(c, a, prefix);
+        rg.i0 = st0 * W;
+        rg.i1 = st1 * W < rg.n ? st1 * W : rg.n;
 
         float m[RB], sum[RB];
         float4_t acc[RB][VE];
@@ -364,8 +545,9 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void paged_attn_few_kernel(co
         }
 
         // page entries of the slab at key k: of its two 16-key halves, or (pages under 16) of
-        // key k + l % 32
-        auto entry = [&](int k, int half) {
+        // key k + l % 32; none past the item's end
+        auto entry = [&](int i, int k, int half) {
+            if (i >= rg.i1) return -1;
             if constexpr (SMALL) {
                 const int j = k + (l & 31);
                 return j < c.cap ? tab[j >> c.page_shift] : -1;
@@ -374,56 +556,61 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void paged_attn_few_kernel(co
             }
         };
         auto good = [&](int e) { return static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages); };
-        // key i (0 .. 31) of the slab, in bytes of k or v: where there is no page, page 0's
-        auto slot = [&](int e0, int e1, int k, int i) -> int64_t {
-            int e;
-            if constexpr (SMALL) e = __shfl(e0, i);
-            else e = i < 16 ? e0 : e1;
-            e = good(e) ? e : 0;
-            return (e * c.page_stride + ((k + i) & page_mask) * c.slot_stride) * 2;
-        };
         u32x4_t kr[2][KC];
         u32x4_t vr[8];
-        // a half slab's page and first slot are the wave's (a scalar base), the rest the lane's
+        // Every load is issued, whether its page is there or not: the waits then are exact.
         auto load_k = [&](int e0, int e1, int k) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const char *p = SMALL ? kb + slot(e0, e1, k, h * 16 + n) : kb + slot(e0, e1, k, h * 16);
-                const uint32_t o = SMALL ? g * 16 : n * stride2 + g * 16;
+                if constexpr (SMALL) {
+                    const int e = __shfl(e0, h * 16 + n);
+                    const uint16_t *p = kb + (good(e) ? e * c.page_stride + ((k + h * 16 + n) & page_mask) * c.slot_stride : 0);
 #pragma unroll
-                for (int x = 0; x < KC; ++x)
-                    kr[h][x] = *reinterpret_cast<const u32x4_t *>(p + (o + x * 64));
+                    for (int x = 0; x < KC; ++x) {
+                        kr[h][x] = (u32x4_t){0, 0, 0, 0};
+                        if (good(e)) kr[h][x] = *reinterpret_cast<const u32x4_t *>(p + g * 8 + x * 32);
+                    }
+                } else {
+                    const rsrc_t r = slots16(c, kb, h ? e1 : e0, k + h * 16, D * 2);
+#pragma unroll
+                    for (int x = 0; x < KC; ++x) kr[h][x] = bload16(r, n * stride2 + g * 16 + x * 64);
+                }
             }
         };
         auto load_v = [&](int e0, int e1, int k) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int h = j >> 2, i = g * 4 + (j & 3);
-                const char *p = SMALL ? vb + slot(e0, e1, k, h * 16 + i) : vb + slot(e0, e1, k, h * 16);
-                const uint32_t o = SMALL ? n * VE * 2 : i * stride2 + n * VE * 2;
-                if constexpr (D == 128) {
-                    vr[j] = *reinterpret_cast<const u32x4_t *>(p + o);
-                } else {
-                    const u32x2_t t = *reinterpret_cast<const u32x2_t *>(p + o);
-                    vr[j] = (u32x4_t){t.x, t.y, 0, 0};
+            for (int h = 0; h < 2; ++h) {
+                rsrc_t r;
+                if constexpr (!SMALL) r = slots16(c, vb, h ? e1 : e0, k + h * 16, D * 2);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if constexpr (SMALL) {
+                        const int i = h * 16 + g * 4 + j, e = __shfl(e0, i);
+                        vr[h * 4 + j] = (u32x4_t){0, 0, 0, 0};
+                        if (good(e)) {
+                            const u32x2_t *p = reinterpret_cast<const u32x2_t *>(
+                                vb + e * c.page_stride + ((k + i) & page_mask) * c.slot_stride + n * VE);
+                            const u32x2_t lo = p[0], hi = p[D == 128 ? 1 : 0];
+                            vr[h * 4 + j] = (u32x4_t){lo.x, lo.y, hi.x, hi.y};
+                        }
+                    } else if constexpr (D == 128) {
+                        vr[h * 4 + j] = bload16(r, (g * 4 + j) * stride2 + n * 16);
+                    } else {
+                        const u32x2_t t = __builtin_bit_cast(
+                            u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, (g * 4 + j) * stride2 + n * 8, 0, 0));
+                        vr[h * 4 + j] = (u32x4_t){t.x, t.y, 0, 0};
+                    }
                 }
             }
         };
 
-        int i = rg.i0 + w, k = rg.key0(i), e0 = -1, e1 = -1, f0 = -1, f1 = -1;
-        if (i < rg.i1) {
-            e0 = entry(k, 0);
-            e1 = entry(k, 1);
-            load_k(e0, e1, k);
-            load_v(e0, e1, k);
-        }
-        int k2 = rg.key0(i + 4);
-        if (i + 4 < rg.i1) {
-            f0 = entry(k2, 0);
-            f1 = entry(k2, 1);
-        }
+        bool odd_seen = false;
+        int i = rg.i0 + w, k = rg.key0(i), k2 = rg.key0(i + W);
+        int e0 = entry(i, k, 0), e1 = entry(i, k, 1);
+        int f0 = entry(i + W, k2, 0), f1 = entry(i + W, k2, 1);
+        load_k(e0, e1, k);
+        load_v(e0, e1, k);
         while (i < rg.i1) {
-            const bool more = i + 4 < rg.i1;
             float4_t st[RB][2];
 #pragma unroll
             for (int rb = 0; rb < RB; ++rb)
@@ -436,7 +623,7 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void paged_attn_few_kernel(co
             uint32_t ok;  // keys whose page is there
             if constexpr (SMALL) ok = static_cast<uint32_t>(__ballot(good(e0)));
             else ok = (good(e0) ? 0xffffu : 0u) | (good(e1) ? 0xffff0000u : 0u);
-            if (more) load_k(f0, f1, k2);
+            load_k(f0, f1, k2);
             const bool full = rg.full(a, k) && ok == 0xffffffffu;
             bool odd = false;  // an infinity or NaN among values that not every row sees
             if (!full) {
@@ -480,31 +667,9 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void paged_attn_few_kernel(co
                                    pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
             }
             if (__any(odd)) {
-                // 0 times such a value is no 0: they are added to the rows that see them (a
-                // probability above 0 leaves an infinity or NaN what it is) and leave the products
-#pragma unroll 1
-                for (int key = 0; key < 32; ++key) {
-                    if (!((ok >> key) & 1) || !rg.any(a, k + key)) continue;
-                    const char *p = vb + (tab[(k + key) >> c.page_shift] * c.page_stride +
-                                          ((k + key) & page_mask) * c.slot_stride) * 2;
-                    bool see[RB];
-#pragma unroll
-                    for (int rb = 0; rb < RB; ++rb) see[rb] = rg.sees(a, pos[rb], k + key);
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) {
-                        const u32x2_t *vp = reinterpret_cast<const u32x2_t *>(p + (g * 4 + x) * VE * 2);
-#pragma unroll
-                        for (int e = 0; e < VE; e += 4) {
-                            const u32x2_t t = vp[e / 4];
-#pragma unroll
-                            for (int z = 0; z < 4; ++z) {
-                                const float o = odd_part<DT>(z & 1 ? t[z >> 1] >> 16 : t[z >> 1]);
-#pragma unroll
-                                for (int rb = 0; rb < RB; ++rb) acc[rb][e + z][x] += see[rb] ? o : 0.f;
-                            }
-                        }
-                    }
-                }
+                // 0 times such a value is no 0: zeros take their place, below they are added to
+                // the rows that see them
+                odd_seen = true;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
@@ -519,72 +684,95 @@ __global__ __launch_bounds__(256, RB == 1 ? 3 : 2) void paged_attn_few_kernel(co
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) acc[rb][e] = mfma16<DT>(f, pf[rb], acc[rb][e]);
             }
-            if (more) {
-                load_v(f0, f1, k2);
-                e0 = f0;
-                e1 = f1;
-                const int k3 = rg.key0(i + 8);
-                if (i + 8 < rg.i1) {
-                    f0 = entry(k3, 0);
-                    f1 = entry(k3, 1);
-                }
-                k = k2;
-                k2 = k3;
-            }
-            i += 4;
+            load_v(f0, f1, k2);
+            e0 = f0;
+            e1 = f1;
+            k = k2;
+            k2 = rg.key0(i + 2 * W);
+            f0 = entry(i + 2 * W, k2, 0);
+            f1 = entry(i + 2 * W, k2, 1);
+            i += W;
         }
 
-        // the 4 waves' parts: each scaled to the common maximum, summed over LDS in wave order
+        if (odd_seen) {
+            // infinities and NaN among values that not every row sees: a probability above 0
+            // leaves them what they are
+#pragma unroll 1
+            for (i = rg.i0 + w; i < rg.i1; i += W) {
+                k = rg.key0(i);
+#pragma unroll 1
+                for (int key = k; key < k + 32; ++key) {
+                    if (!rg.any(a, key)) continue;
+                    const int e = sload(tab + (key >> c.page_shift));
+                    if (!good(e) || rg.full(a, k)) continue;
+                    const uint16_t *p = vb + e * c.page_stride + (key & page_mask) * c.slot_stride;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+#pragma unroll
+                        for (int z = 0; z < VE; ++z) {
+                            const float o = odd_part<DT>(p[(g * 4 + x) * VE + z]);
+#pragma unroll
+                            for (int rb = 0; rb < RB; ++rb)
+                                acc[rb][z][x] += rg.sees(a, pos[rb], key) ? o : 0.f;
+                        }
+                }
+            }
+        }
+
+        // the waves' parts: each scaled to the common maximum, summed over LDS in wave order
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             sum[rb] += __shfl_xor(sum[rb], 16);
             sum[rb] += __shfl_xor(sum[rb], 32);
-            if (g == 0) {
-                s_ml[w][rb * 16 + n][0] = m[rb];
-                s_ml[w][rb * 16 + n][1] = sum[rb];
+            const int row = w * 16 * RB + rb * 16 + n;
+            if (g == 0) s_ml[row] = make_float2(m[rb], sum[rb]);
+            if (r0 + rb * 16 + n < rows) {
+#pragma unroll
+                for (int x = 0; x < 4; ++x)
+#pragma unroll
+                    for (int e = 0; e < VE; e += 4)
+                        *reinterpret_cast<float4_t *>(s_o + row * LD + (g * 4 + x) * VE + e) =
+                            (float4_t){acc[rb][e][x], acc[rb][e + 1][x], acc[rb][e + 2][x],
+                                       acc[rb][e + 3][x]};
             }
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-#pragma unroll
-                for (int e = 0; e < VE; e += 4)
-                    *reinterpret_cast<float4_t *>(&s_o[w][rb * 16 + n][(g * 4 + x) * VE + e]) =
-                        (float4_t){acc[rb][e][x], acc[rb][e + 1][x], acc[rb][e + 2][x], acc[rb][e + 3][x]};
         }
         __syncthreads();
-        for (int u = threadIdx.x; u < 16 * RB * (D / 8); u += 256) {
-            const int r = u / (D / 8), d = (u % (D / 8)) * 8;
+        for (int v = threadIdx.x; v < 16 * RB * (D / 4); v += W * 64) {
+            const int r = v / (D / 4), d = (v % (D / 4)) * 4;
             if (r0 + r >= rows) continue;
-            float mm = -INFINITY, ll = 0.f, o[8] = {};
+            float mm = -INFINITY, ll = 0.f;
+            float4_t o = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int x = 0; x < 4; ++x) mm = fmaxf(mm, s_ml[x][r][0]);
+            for (int x = 0; x < W; ++x) mm = fmaxf(mm, s_ml[x * 16 * RB + r].x);
 #pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const float mw = s_ml[x][r][0], f = mw == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mw - mm);
-                ll += s_ml[x][r][1] * f;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] += s_o[x][r][d + e] * f;
+            for (int x = 0; x < W; ++x) {
+                const float2 ml = s_ml[x * 16 * RB + r];
+                const float fx = ml.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml.x - mm);
+                ll += ml.y * fx;
+                o += *reinterpret_cast<const float4_t *>(s_o + (x * 16 * RB + r) * LD + d) * fx;
             }
-            const int64_t row = static_cast<int64_t>(s.q0 + (r0 + r) / a.group) * a.n_heads +
-                                kvh * a.group + (r0 + r) % a.group;
-            if (a.pieces == 1) {
+            if (single && f.direct) {
+                const int64_t row = static_cast<int64_t>(s.q0 + (r0 + r) / a.group) * a.n_heads +
+                                    kvh * a.group + (r0 + r) % a.group;
                 const float inv = ll == 0.f ? 0.f : 1.f / ll;
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] *= inv;
-                *reinterpret_cast<u32x4_t *>(a.out + row * D + d) = pack8<DT>(o);
+                *reinterpret_cast<u32x2_t *>(a.out + row * D + d) =
+                    (u32x2_t){pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
                 if (a.lse && d == 0) a.lse[row] = ll == 0.f ? -INFINITY : mm * kLn2 + logf(ll);
             } else {
-                const int64_t at = row * a.pieces + part.first + piece;
-                if (mm != -INFINITY) {
-                    float4_t *po = reinterpret_cast<float4_t *>(a.part_o + at * D + d);
-                    po[0] = (float4_t){o[0], o[1], o[2], o[3]};
-                    po[1] = (float4_t){o[4], o[5], o[6], o[7]};
-                }
-                if (d == 0) a.part_ml[at] = make_float2(mm, ll);
+                const int64_t slot = (static_cast<int64_t>(group + item) * c.n_kv + kvh) * 16 * RB + r;
+                if (mm != -INFINITY) *reinterpret_cast<float4_t *>(f.part_o + slot * D + d) = o;
+                if (d == 0) f.part_ml[slot] = make_float2(mm, ll);
             }
         }
-        if (part.prefix) return;  // the other rows are other workgroups'
         __syncthreads();
     }
+}
+
+template <int DT, int D, int RB, bool SMALL, int W>
+__global__ __launch_bounds__(64 * W, W == 4 && RB == 1 ? 3 : 2) void paged_attn_few_kernel(
+    const Cache c, const Query a, const Few f) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds<D>(W, RB)];
+    few_body<DT, D, RB, SMALL, W>(c, a, f, blockIdx.x, lds);
 }
 
 // ------------------------------------------------------------------ many rows (prompts)
@@ -606,18 +794,22 @@ __device__ __forceinline__ u32x2_t tr_read(const uint8_t *s, int off) {
 
 constexpr int kRows = 128;
 
+template <int D>
+constexpr int kTileLds = 4 * 64 * D * 2 + 64;  // two stages of K and V, and a few words
+
 template <int DT, int D, bool SMALL>
-__global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, const Query a,
-                                                                 const Part part) {
+__device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const Part &part, int block,
+                                          uint8_t *lds) {
     constexpr int CH = D / 8, KS = D / 16, DT32 = D / 32;  // 16-byte chunks of a row, k steps, d tiles
     constexpr int RPP = 256 / CH, PASS = 64 / RPP;         // rows a pass of the workgroup loads
-    __shared__ __attribute__((aligned(16))) uint8_t s_k[2][64 * D * 2];
-    __shared__ __attribute__((aligned(16))) uint8_t s_v[2][64 * D * 2];
-    __shared__ int s_odd[2];  // the stage's tile, where its values hold an infinity or NaN
-    __shared__ int s_p[8];
+    constexpr int STAGE = 64 * D * 2;
+    uint8_t *s_k = lds, *s_v = lds + 2 * STAGE;                // [2][STAGE]
+    int *s_odd = reinterpret_cast<int *>(lds + 4 * STAGE);  // [2]: the stage's tile, where its
+                                                            // values hold an infinity or NaN
+    int *s_p = s_odd + 4;                                   // [8]
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
     const int g = l >> 5, n = l & 31;
-    const int kvh = blockIdx.x % c.n_kv, y = blockIdx.x / c.n_kv;
+    const int kvh = block % c.n_kv, y = block / c.n_kv;
     const int piece = y % part.splits;
     int blk = y / part.splits, b = 0;
     Seq s = {0, c.tokens, 0};
@@ -644,8 +836,10 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
             }
             blk -= __builtin_amdgcn_readlane(upto, 63);
         }
-        s = seq_at(c, b);
+        s = seq_uniform(c, b);
     }
+    const uint16_t *kb = c.k + kvh * c.head_stride, *vb = c.v + kvh * c.head_stride;
+    const int stride2 = static_cast<int>(c.slot_stride) * 2;
     const int r0 = blk * kRows, rows = s.n * a.group;
     const int32_t *tab = c.table + b * c.ld_table;
     const int page_mask = (1 << c.page_shift) - 1;
@@ -687,21 +881,22 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
         rg.pmin = s.p0 + r0 / a.group;
         rg.pmax = s.p0 + (last - 1) / a.group;
     }
-    rg.set(c, a, part, piece);
+    rg.set(c, a, part.prefix);
+    rg.cut(part.splits, part.min_tiles, piece);
 
     float m = -INFINITY, sum = 0.f;
+    bool odd_seen = false;
     float16_t acc[DT32];
 #pragma unroll
     for (int x = 0; x < DT32; ++x) acc[x] = (float16_t){};
 
-    // ---- staging: thread's row of a pass and its chunk
+    // ---- staging: a thread's row of a pass and its 16 bytes of it in LDS, and the chunk of the
+    // row that belongs there
     const int srow = tid / CH, sch = tid % CH;
-    auto k_at = [&](int row, int ch) {  // byte of a K chunk in its stage
-        return row * D * 2 + ((ch ^ (D == 128 ? (row & 15) : ((row >> 1) & 7))) << 4);
-    };
-    auto v_at = [&](int row, int ch) {
-        return row * D * 2 + ((ch ^ (D == 128 ? (row & 3) << 2 : ((row >> 1) & 1) << 2)) << 4);
-    };
+    const int kch = sch ^ (D == 128 ? srow & 15 : (srow >> 1) & 7);
+    const int vch0 = sch ^ (D == 128 ? (srow & 3) << 2 : ((srow >> 1) & 1) << 2);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+                              (__attribute__((address_space(3))) uint8_t *)lds)) + w * 1024;
     auto good = [&](int e) { return static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages); };
     // page entries of the tile at key k: of its 16-key quarters, or (pages under 16) key k + l's
     struct Entries { int e[4]; };
@@ -726,46 +921,48 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
             return v;
         }
     };
-    u32x4_t kst[PASS], vst[PASS];
-    auto load = [&](const Entries &t, int k) {
+    const int ko = (srow & 15) * stride2 + kch * 16, vo = (srow & 15) * stride2 + vch0 * 16;
+    // tile k into stage st: by DMA, a pass of a wave within one of the tile's 16-key quarters
+    auto send = [&](int st, const Entries &t, int k) {
 #pragma unroll
         for (int x = 0; x < PASS; ++x) {
-            const int row = x * RPP + srow;
-            int e;
-            if constexpr (SMALL) e = __shfl(t.e[0], row);
-            else if constexpr (D == 128) e = t.e[x];
-            else e = w < 2 ? t.e[2 * x] : t.e[2 * x + 1];
-            e = good(e) ? e : 0;
-            const int64_t at = e * c.page_stride + kvh * c.head_stride +
-                               ((k + row) & page_mask) * c.slot_stride + sch * 8;
-            kst[x] = *reinterpret_cast<const u32x4_t *>(c.k + at);
-            vst[x] = *reinterpret_cast<const u32x4_t *>(c.v + at);
+            if constexpr (SMALL) {
+                const int row = x * RPP + srow, e = __shfl(t.e[0], row);
+                const int64_t at = e * c.page_stride + ((k + row) & page_mask) * c.slot_stride;
+                u32x4_t kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
+                if (good(e)) {
+                    kx = *reinterpret_cast<const u32x4_t *>(kb + at + kch * 8);
+                    vx = *reinterpret_cast<const u32x4_t *>(vb + at + vch0 * 8);
+                }
+                *reinterpret_cast<u32x4_t *>(s_k + st * STAGE + row * D * 2 + sch * 16) = kx;
+                *reinterpret_cast<u32x4_t *>(s_v + st * STAGE + row * D * 2 + sch * 16) = vx;
+            } else {
+                const int e = D == 128 ? t.e[x] : w < 2 ? t.e[(2 * x) & 3] : t.e[(2 * x + 1) & 3];
+                const int k16 = k + (x * RPP + (D == 128 ? 0 : (w >> 1) * 16));
+                const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + st * STAGE + x * 4096);
+                lds_dma16(at, ko, slots16(c, kb, e, k16, D * 2), 0);
+                lds_dma16(at + 2 * STAGE, vo, slots16(c, vb, e, k16, D * 2), 0);
+            }
         }
     };
-    auto store = [&](int st, int i, int k, uint64_t ok) {
-        if (!rg.full(a, k) || ~ok) {
-            bool odd = false;
-#pragma unroll
-            for (int x = 0; x < PASS; ++x) {
-                const int row = x * RPP + srow;
-                if (!((ok >> row) & 1) || !rg.any(a, k + row)) vst[x] = (u32x4_t){0, 0, 0, 0};
-#pragma unroll
-                for (int z = 0; z < 4; ++z) odd |= not_finite<DT>(vst[x][z]);
-            }
-            if (odd) {
-#pragma unroll
-                for (int x = 0; x < PASS; ++x)
-#pragma unroll
-                    for (int z = 0; z < 4; ++z) vst[x][z] = finite_or_zero<DT>(vst[x][z]);
-                s_odd[st] = i;
-            }
-        }
+    // what this wave loaded of a tile that not every row sees whole: the values of keys that no
+    // row sees become zeros; infinities and NaN too (0 times one is no 0), and s_odd says so
+    auto clean = [&](int st, int i, int k, uint64_t ok) {
+        bool odd = false;
 #pragma unroll
         for (int x = 0; x < PASS; ++x) {
             const int row = x * RPP + srow;
-            *reinterpret_cast<u32x4_t *>(s_k[st] + k_at(row, sch)) = kst[x];
-            *reinterpret_cast<u32x4_t *>(s_v[st] + v_at(row, sch)) = vst[x];
+            u32x4_t *p = reinterpret_cast<u32x4_t *>(s_v + st * STAGE + row * D * 2 + sch * 16);
+            u32x4_t v = *p;
+            if (!((ok >> row) & 1) || !rg.any(a, k + row)) v = (u32x4_t){0, 0, 0, 0};
+#pragma unroll
+            for (int z = 0; z < 4; ++z) {
+                odd |= not_finite<DT>(v[z]);
+                v[z] = finite_or_zero<DT>(v[z]);
+            }
+            *p = v;
         }
+        if (odd) s_odd[st] = i;
     };
 
     // ---- operand addresses of this lane
@@ -776,40 +973,55 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
     const int vx = D == 128 ? (vkey & 3) << 2 : ((vkey >> 1) & 1) << 2;
 
     Entries cur{}, nxt{};
-    int k = 0, k2 = 0;
-    uint64_t ok = 0;
+    int k = rg.key0(rg.i0), k2 = rg.key0(rg.i0 + 1);
     if (tid < 2) s_odd[tid] = -1;
     __syncthreads();
     if (rg.i0 < rg.i1) {
-        k = rg.key0(rg.i0);
         cur = entries(k);
-        load(cur, k);
-        ok = there(cur);
-        store(0, rg.i0, k, ok);
-        k2 = rg.key0(rg.i0 + 1);
+        send(0, cur, k);
         if (rg.i0 + 1 < rg.i1) nxt = entries(k2);
     }
-    __syncthreads();
     for (int i = rg.i0; i < rg.i1; ++i) {
         const int st = (i - rg.i0) & 1;
-        const bool more = i + 1 < rg.i1;
-        if (more) load(nxt, k2);
+        const uint64_t ok = there(cur);
+        const bool full = rg.full(a, k) && !~ok;
+        if constexpr (!SMALL) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if (!full) clean(st, i, k, ok);
+        __syncthreads();  // every wave's part of tile i is there, and tile i - 1 is read
+        // scores, 32 keys each
+        u32x4_t kf[2][KS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < KS; ++x)
+                kf[h][x] = *reinterpret_cast<const u32x4_t *>(
+                    s_k + st * STAGE + h * 32 * D * 2 + krow + (((2 * x + g) ^ kx) << 4));
+        if (i + 1 < rg.i1) send(st ^ 1, nxt, k2);
         Entries nxt2{};
         const int k3 = rg.key0(i + 2);
         if (i + 2 < rg.i1) nxt2 = entries(k3);
-        // scores, 32 keys each
+        __builtin_amdgcn_sched_barrier(0);
         float16_t sc[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             sc[h] = (float16_t){};
 #pragma unroll
-            for (int x = 0; x < KS; ++x) {
-                const u32x4_t f = *reinterpret_cast<const u32x4_t *>(
-                    s_k[st] + h * 32 * D * 2 + krow + (((2 * x + g) ^ kx) << 4));
-                sc[h] = mfma32<DT>(f, q[x], sc[h]);
-            }
+            for (int x = 0; x < KS; ++x) sc[h] = mfma32<DT>(kf[h][x], q[x], sc[h]);
         }
-        const bool full = rg.full(a, k) && !~ok;
+        // V^T operands: keys of step x, channels of tile d; the first half's latency passes
+        // during the softmax
+        u32x4_t vf[2][DT32];
+        auto read_v = [&](int x, u32x4_t (&f)[DT32]) {
+#pragma unroll
+            for (int d = 0; d < DT32; ++d) {
+                const int at = st * STAGE + vbase + (((d * 4 + vch) ^ vx) << 4) + x * 16 * D * 2;
+                const u32x2_t lo = tr_read(s_v, at), hi = tr_read(s_v, at + 8 * D * 2);
+                f[d] = (u32x4_t){lo.x, lo.y, hi.x, hi.y};
+            }
+        };
+        read_v(0, vf[0]);
+        read_v(1, vf[1]);
+        __builtin_amdgcn_sched_barrier(0);
         if (!full) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -823,7 +1035,9 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
 #pragma unroll
         for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
         top = fmaxf(top, __shfl_xor(top, 32)) * a.scale;
-        if (__any(top > m)) {
+        // m is a maximum of earlier tiles: probabilities up to 2^8 are let be (their sums are in
+        // fp32, their rounding is relative), so that few tiles rescale
+        if (__any(top > m + 8.f)) {
             const float mn = fmaxf(m, top), alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
             sum *= alpha;
 #pragma unroll
@@ -843,49 +1057,45 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
             pf[x] = (u32x4_t){pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]),
                               pack2<DT>(p[6], p[7])};
         }
-        if (s_odd[st] == i) {
-            // as in the few-rows kernel: the stage holds zeros in their place
+        odd_seen |= s_odd[st] == i;
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+#pragma unroll
+            for (int d = 0; d < DT32; ++d) acc[d] = mfma32<DT>(vf[x & 1][d], pf[x], acc[d]);
+            if (x < 2) read_v(x + 2, vf[x & 1]);
+        }
+        cur = nxt;
+        nxt = nxt2;
+        k = k2;
+        k2 = k3;
+    }
+
+    if (odd_seen) {
+        // as in the few-rows kernel: the stages held zeros in their place
 #pragma unroll 1
-            for (int key = 0; key < 64; ++key) {
-                if (!((ok >> key) & 1) || !rg.any(a, k + key)) continue;
-                const uint16_t *p = c.v + tab[(k + key) >> c.page_shift] * c.page_stride +
-                                    kvh * c.head_stride + ((k + key) & page_mask) * c.slot_stride;
-                const bool see = rg.sees(a, pos, k + key);
+        for (int i = rg.i0; i < rg.i1; ++i) {
+            k = rg.key0(i);
+            if (rg.full(a, k)) continue;
+#pragma unroll 1
+            for (int key = k; key < k + 64; ++key) {
+                if (!rg.any(a, key)) continue;
+                const int e = tab[key >> c.page_shift];
+                if (!good(e) || !rg.sees(a, pos, key)) continue;
+                const uint16_t *p =
+                    vb + e * c.page_stride + (key & page_mask) * c.slot_stride;
 #pragma unroll
                 for (int x = 0; x < DT32; ++x)
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        const u32x2_t t = *reinterpret_cast<const u32x2_t *>(p + x * 32 + e * 2 + g * 4);
-#pragma unroll
-                        for (int z = 0; z < 4; ++z) {
-                            const float o = odd_part<DT>(z & 1 ? t[z >> 1] >> 16 : t[z >> 1]);
-                            acc[x][e + z] += see ? o : 0.f;
-                        }
-                    }
+                    for (int z = 0; z < 16; ++z)
+                        acc[x][z] += odd_part<DT>(p[x * 32 + (z >> 2) * 8 + g * 4 + (z & 3)]);
             }
         }
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-#pragma unroll
-            for (int d = 0; d < DT32; ++d) {  // V^T operand: keys of step x, channels of tile d
-                const int at = vbase + (((d * 4 + vch) ^ vx) << 4) + x * 16 * D * 2;
-                const u32x2_t lo = tr_read(s_v[st], at), hi = tr_read(s_v[st], at + 8 * D * 2);
-                acc[d] = mfma32<DT>((u32x4_t){lo.x, lo.y, hi.x, hi.y}, pf[x], acc[d]);
-            }
-        if (more) {
-            ok = there(nxt);
-            store(st ^ 1, i + 1, k2, ok);
-        }
-        k = k2;
-        k2 = k3;
-        nxt = nxt2;
-        __syncthreads();
     }
 
     sum += __shfl_xor(sum, 32);
     if (!live) return;
     const int64_t row = static_cast<int64_t>(tok) * a.n_heads + head;
-    if (a.pieces == 1) {
+    if (a.dense == 0) {
         const float inv = sum == 0.f ? 0.f : 1.f / sum;
         uint16_t *o = a.out + row * D + g * 4;
 #pragma unroll
@@ -897,7 +1107,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
                               pack2<DT>(acc[x][e + 2] * inv, acc[x][e + 3] * inv)};
         if (a.lse && g == 0) a.lse[row] = sum == 0.f ? -INFINITY : m * kLn2 + logf(sum);
     } else {
-        const int64_t at = row * a.pieces + part.first + piece;
+        const int64_t at = row * a.dense + part.first + piece;
         if (m != -INFINITY) {
             float *o = a.part_o + at * D + g * 4;
 #pragma unroll
@@ -911,24 +1121,122 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
     }
 }
 
+template <int DT, int D, bool SMALL>
+__global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, const Query a,
+                                                                 const Part own, const Part pre) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kTileLds<D>];
+    const int block = blockIdx.x;
+    if (block < pre.groups) tile_body<DT, D, SMALL>(c, a, pre, block, lds);
+    else tile_body<DT, D, SMALL>(c, a, own, block - pre.groups, lds);
+}
+
+// A prefix of many rows and few rows of each sequence in one launch, their workgroups in turn:
+// the first are bound by arithmetic, the second by memory.
+template <int DT, int D, int RB, bool SMALL>
+__global__ __launch_bounds__(256, 2) void paged_attn_both_kernel(const Cache c, const Query a,
+                                                                 const Few f, const Part pre) {
+    constexpr int LDS = kTileLds<D> > few_lds<D>(4, RB) ? kTileLds<D> : few_lds<D>(4, RB);
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+    const int nf = f.groups * c.n_kv, both = 2 * (nf < pre.groups ? nf : pre.groups);
+    const int i = blockIdx.x;
+    if (i < both ? (i & 1) == 0 : pre.groups > nf)
+        tile_body<DT, D, SMALL>(c, a, pre, i < both ? i >> 1 : i - nf, lds);
+    else
+        few_body<DT, D, RB, SMALL, 4>(c, a, f, i < both ? i >> 1 : i - pre.groups, lds);
+}
+
 // One workgroup per output row: O = sum_i 2^(m_i - m) O_i / sum_i 2^(m_i - m) l_i over its
-// pieces, in order; a piece that saw nothing has m_i = -inf and no O_i.
-template <int DT, int D>
-__global__ __launch_bounds__(D) void paged_attn_join_kernel(const Query a) {
+// pieces; a piece that saw nothing has m_i = -inf and no O_i.  A thread takes 4 channels of every
+// kJoinThreads / (D / 4)-th piece, the threads of a channel meet in LDS in order: few rows of many
+// pieces (one long sequence) are bound by the latency of their loads, which one thread a channel
+// took one piece at a time (342 pieces of 28 rows: 120 us).
+constexpr int kJoinThreads = 256;
+
+template <int DT, int D, int RB>
+__global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Cache c, const Query a,
+                                                                       const Few f) {
+    constexpr int COLS = D / 4, LANES = kJoinThreads / COLS, R = 16 * RB;
+    __shared__ float4_t s_o[LANES][COLS];
+    __shared__ float s_m[LANES], s_l[LANES];
     const int64_t row = blockIdx.x;
-    const float2 *ml = a.part_ml + row * a.pieces;
-    const float *o = a.part_o + row * a.pieces * D + threadIdx.x;
-    float m = -INFINITY;
-    for (int i = 0; i < a.pieces; ++i) m = fmaxf(m, ml[i].x);
-    float l = 0.f, v = 0.f;
-    for (int i = 0; i < a.pieces; ++i) {
-        if (ml[i].x == -INFINITY) continue;
-        const float f = __builtin_amdgcn_exp2f(ml[i].x - m);
-        l += ml[i].y * f;
-        v += o[static_cast<int64_t>(i) * D] * f;
+    const int col = threadIdx.x % COLS, lane = threadIdx.x / COLS;
+    int n[2] = {0, 0};        // pieces of few rows: of the sequence's item and of the prefix's
+    int64_t slot[2] = {0, 0}; // row of the first
+    if (f.groups) {
+        const int tok = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
+        const int kvh = head / a.group, b = seq_of_token(c, tok);
+        const int q0 = b < f.seqs ? seq_at(c, b).q0 : 0;
+        Units u;
+        all_units<4, RB>(u, c, a, f);
+        const int used = groups_used(f, u.total);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const int e = x ? f.seqs : b, r = (x ? tok : tok - q0) * a.group + head % a.group;
+            if ((x ? !f.prefix : b >= f.seqs) || r < 0) continue;
+            while (e >= u.b0 + 64) next_units<4, RB>(u, c, a, f);
+            if (e < u.b0) continue;
+            const int at = e - u.b0, blocks = __builtin_amdgcn_readlane(u.blocks, at);
+            const int steps = __builtin_amdgcn_readlane(u.steps, at), blk = r / R;
+            const int item = u.ibase + __builtin_amdgcn_readlane(u.iup, at) - blocks + blk;
+            if (blk >= blocks || item >= f.items) continue;
+            const int64_t start = u.base + lane_of(u.up, at) - static_cast<int64_t>(blocks - blk) * (steps + 1);
+            const int first = group_of(u.total, steps ? start + 1 : start, used);
+            n[x] = group_of(u.total, start + steps, used) - first + 1;
+            slot[x] = (static_cast<int64_t>(first + item) * c.n_kv + kvh) * R + r % R;
+        }
+        if (f.direct && n[0] == 1) return;  // written
     }
-    a.out[row * D + threadIdx.x] = round16<DT>(l == 0.f ? 0.f : v / l);
-    if (a.lse && threadIdx.x == 0) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+    const int few = n[0] + n[1], all = few + a.dense;
+    float m = -INFINITY, l = 0.f;
+    float4_t v = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = lane; i0 < all; i0 += 4 * LANES) {
+        float2 t[4];
+        float4_t o[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int i = i0 + x * LANES;
+            t[x] = make_float2(-INFINITY, 0.f);
+            o[x] = (float4_t){0.f, 0.f, 0.f, 0.f};
+            if (i < all) {
+                const int64_t at = i < n[0] ? slot[0] + static_cast<int64_t>(i) * c.n_kv * R
+                                   : i < few ? slot[1] + static_cast<int64_t>(i - n[0]) * c.n_kv * R
+                                             : row * a.dense + i - few;
+                t[x] = (i < few ? f.part_ml : a.part_ml)[at];
+                o[x] = reinterpret_cast<const float4_t *>((i < few ? f.part_o : a.part_o) + at * D)[col];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if (t[x].x == -INFINITY) continue;
+            const float mn = fmaxf(m, t[x].x);
+            const float fo = __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(t[x].x - mn);
+            l = l * fo + t[x].y * fn;
+            v = v * fo + o[x] * fn;
+            m = mn;
+        }
+    }
+    s_o[lane][col] = v;
+    if (col == 0) {
+        s_m[lane] = m;
+        s_l[lane] = l;
+    }
+    __syncthreads();
+    if (lane) return;
+#pragma unroll
+    for (int i = 0; i < LANES; ++i) m = fmaxf(m, s_m[i]);
+    l = 0.f;
+    v = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < LANES; ++i) {
+        if (s_m[i] == -INFINITY) continue;
+        const float fi = __builtin_amdgcn_exp2f(s_m[i] - m);
+        l += s_l[i] * fi;
+        v += s_o[i][col] * fi;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    reinterpret_cast<u32x2_t *>(a.out + row * D)[col] =
+        (u32x2_t){pack2<DT>(v[0] * inv, v[1] * inv), pack2<DT>(v[2] * inv, v[3] * inv)};
+    if (a.lse && col == 0) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // --------------------------------------------------------------------------------- host
@@ -940,8 +1248,8 @@ int fill_cache(Cache &c, const nf4_paged_kv *kv, const int32_t *cu_q, int64_t to
         tokens < 0 || n_heads < 1 || n_heads % kv->n_kv || kv->ld_table < kv->width)
         return NF4_ERR_ARG;
     // a position and a token times its heads stay 32-bit
-    if (static_cast<int64_t>(kv->width) * kv->page_size > (1 << 30) || tokens > (1 << 26) ||
-        n_heads > 1024 || kv->batch > (1 << 20))
+    if (static_cast<int64_t>(kv->width) * kv->page_size > (1 << 30) || n_heads > 1024 ||
+        tokens > (1 << 23) || tokens * n_heads > (1 << 30) || kv->batch > (1 << 20))
         return NF4_ERR_UNSUPPORTED;
     if (!cu_q && (kv->batch ? tokens % kv->batch : tokens)) return NF4_ERR_ARG;
     if (kv->head_dim != 64 && kv->head_dim != 128) return NF4_ERR_UNSUPPORTED;
@@ -978,99 +1286,118 @@ int cut(int64_t v) { return static_cast<int>(v < (1 << 30) ? v : 1 << 30); }
 
 int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
 
-// How a part runs: the kernel (rb row blocks of 16 in the few-rows kernel, 0 the tiled one), its
-// items (sequences, or row blocks) and its pieces.
-struct PartPlan {
-    Part part;
-    int rb, items;
-};
-
 struct Plan {
-    PartPlan own, pre;
-    int pieces;
+    Few few;          // groups 0: none
+    Part own, pre;    // groups 0: none
+    int rb, waves;    // of the few-rows kernel
+    int64_t dense, slots;
     size_t bytes;
 };
 
-// `rows` rows at most of each of `items` sequences (prefix: items 1, the batch's rows) over
-// `keys` keys at most.  Few rows go to the kernel without LDS staging; the tiles are cut until
-// the launch has kFewGroups (kTileGroups) workgroups, or pieces of one slab a wave (4 tiles).
-constexpr int kFewRows = 32, kFewGroups = 2048, kTileGroups = 512;
+// Sequences whose rows are few go to the kernel without LDS staging.  Its launch fills the card
+// once (kFewSlots workgroups); where no sequence is longer than kWholeKeys and all of them fit
+// the card, a workgroup of 8 waves takes a whole sequence, and there is nothing to join.  Tiled
+// parts are cut until the launch has kTileSlots workgroups.
+constexpr int kFewRows = 32, kFewSlots = 768, kTileSlots = 512, kWholeKeys = 1024;
 
-PartPlan plan_part(bool prefix, int64_t rows, int64_t blocks, int items, int n_kv, int64_t keys) {
-    PartPlan p{};
-    const bool few = rows <= kFewRows;
-    p.rb = !few ? 0 : rows <= 16 ? 1 : 2;
-    p.items = few ? (prefix ? 1 : items) : static_cast<int>(blocks);
-    const int tiles = ceil_div(keys, few ? 32 : 64) + 1;
-    const int64_t groups = static_cast<int64_t>(p.items) * n_kv;
-    int64_t splits = (few ? kFewGroups : kTileGroups) / (groups ? groups : 1);
-    splits = splits < 1 ? 1 : splits > ceil_div(tiles, 4) ? ceil_div(tiles, 4) : splits;
-    const int per = ceil_div(ceil_div(tiles, splits), 4) * 4;
-    p.part = Part{prefix ? 1 : 0, ceil_div(tiles, per), 0, per, static_cast<int>(blocks)};
+Part tile_part(bool prefix, int64_t blocks, int n_kv, int64_t keys, int slots) {
+    Part p{};
+    const int tiles = ceil_div(keys, 64) + 1;
+    const int64_t groups = blocks * n_kv;
+    int64_t splits = slots / (groups ? groups : 1);
+    splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
+    p.prefix = prefix ? 1 : 0;
+    p.min_tiles = ceil_div(tiles, splits);
+    p.splits = ceil_div(tiles, p.min_tiles);
+    p.blocks = static_cast<int>(blocks);
+    p.groups = cut(groups * p.splits);
     return p;
 }
 
 Plan make_plan(const Cache &c, int n_heads, int window, int sinks, int shared, int64_t max_q,
                int64_t max_len, int head_dim) {
-    const int64_t group = n_heads / c.n_kv;
+    const int64_t group = n_heads / c.n_kv, all_rows = c.tokens * group;
     int64_t longest = c.cu ? (max_q && max_q < c.tokens ? max_q : c.tokens) : c.uniform;
     const int64_t len = max_len && max_len < c.cap ? max_len : c.cap;
     int64_t span = len > shared ? len - shared : 0;
     if (window && span > static_cast<int64_t>(window) + longest + sinks) span = window + longest + sinks;
+    const int64_t pre_keys = len < shared ? len : shared;
     const int seqs = c.batch + (c.cu ? 1 : 0);  // with offsets: and the tokens past the last
-    const int64_t blocks = c.cu ? c.tokens * group / kRows + seqs
-                                : static_cast<int64_t>(c.batch) * ceil_div(longest * group, kRows);
+    const bool few_own = longest * group <= kFewRows, few_pre = shared && all_rows <= kFewRows;
     Plan p{};
-    p.own = plan_part(false, longest * group, blocks, seqs, c.n_kv, span);
-    p.pieces = p.own.part.splits;
-    if (shared) {
-        const int64_t rows = c.tokens * group;
-        p.pre = plan_part(true, rows, ceil_div(rows, kRows), 1, c.n_kv, len < shared ? len : shared);
-        p.own.part.first = p.pre.part.splits;
-        p.pieces += p.pre.part.splits;
+    if (few_own) {
+        Few &f = p.few;
+        p.rb = (few_pre ? all_rows : longest * group) <= 16 ? 1 : 2;
+        f.seqs = seqs;
+        f.prefix = few_pre ? 1 : 0;
+        f.direct = shared ? 0 : 1;
+        f.items = static_cast<int>(all_rows / (16 * p.rb)) + seqs +
+                  (few_pre ? ceil_div(all_rows, 16 * p.rb) : 0);
+        f.whole = !shared && p.rb == 1 && span <= kWholeKeys &&
+                  static_cast<int64_t>(f.items) * c.n_kv <= 2 * 256;
+        p.waves = f.whole ? 8 : 4;
+        f.min_units = 2;
+        int64_t units = f.items * (span / (32 * p.waves) + 2) + pre_keys / 128 + 2;
+        int64_t groups = ceil_div(shared && !few_pre ? kTileSlots / 2 : kFewSlots, c.n_kv);
+        groups = groups < units / f.min_units ? groups : units / f.min_units;
+        f.groups = f.whole ? f.items : static_cast<int>(groups < 1 ? 1 : groups);
+        if (!f.whole) p.slots = f.groups + f.items;
+    } else {
+        const int64_t blocks = c.cu ? all_rows / kRows + seqs
+                                    : static_cast<int64_t>(c.batch) * ceil_div(longest * group, kRows);
+        p.own = tile_part(false, blocks, c.n_kv, span, kTileSlots);
     }
-    if (p.pieces > 1)
-        p.bytes = static_cast<size_t>(c.tokens) * n_heads * p.pieces * (4 * head_dim + 8);
+    if (shared && !few_pre)
+        p.pre = tile_part(true, ceil_div(all_rows, kRows), c.n_kv, pre_keys,
+                          few_own ? kTileSlots / 2 : kTileSlots);
+    p.own.first = p.pre.groups ? p.pre.splits : 0;
+    p.dense = p.own.first + (p.own.groups ? p.own.splits : 0);
+    if (!shared && p.dense == 1) p.dense = 0;
+    p.bytes = (p.dense * c.tokens * n_heads + p.slots * c.n_kv * 16 * p.rb) * (4 * head_dim + 8);
     return p;
 }
 
-template <int DT, int D>
-int launch_part(const Cache &c, const Query &a, const PartPlan &p, hipStream_t s) {
-    const int64_t groups = static_cast<int64_t>(p.items) * p.part.splits * c.n_kv;
+template <int DT, int D, bool SMALL>
+int launch(const Cache &c, const Query &a, const Plan &p, hipStream_t s) {
+    const int64_t nf = static_cast<int64_t>(p.few.groups) * c.n_kv;
+    const int64_t groups = nf + p.pre.groups + p.own.groups;
     if (groups == 0) return NF4_OK;
-    if (groups > 0x7fffffff) return NF4_ERR_UNSUPPORTED;
+    if (groups > (1 << 23)) return NF4_ERR_UNSUPPORTED;
     const dim3 grid(static_cast<unsigned>(groups));
-    const bool small = c.page_shift < 4;
-#define NF4_FEW(RB, SMALL)                                                                          \
-    hipLaunchKernelGGL((paged_attn_few_kernel<DT, D, RB, SMALL>), grid, dim3(256), 0, s, c, a, p.part)
-#define NF4_TILE(SMALL)                                                                             \
-    hipLaunchKernelGGL((paged_attn_tile_kernel<DT, D, SMALL>), grid, dim3(256), 0, s, c, a, p.part)
-    if (p.rb == 0) {
-        if (small) NF4_TILE(true);
-        else NF4_TILE(false);
-    } else if (p.rb == 1) {
-        if (small) NF4_FEW(1, true);
-        else NF4_FEW(1, false);
-    } else {
-        if (small) NF4_FEW(2, true);
-        else NF4_FEW(2, false);
-    }
+#define NF4_FEW(RB, W)                                                                              \
+    hipLaunchKernelGGL((paged_attn_few_kernel<DT, D, RB, SMALL, W>), grid, dim3(64 * W), 0, s, c, a, \
+                       p.few)
+#define NF4_BOTH(RB)                                                                                \
+    hipLaunchKernelGGL((paged_attn_both_kernel<DT, D, RB, SMALL>), grid, dim3(256), 0, s, c, a,      \
+                       p.few, p.pre)
+    if (nf == 0)
+        hipLaunchKernelGGL((paged_attn_tile_kernel<DT, D, SMALL>), grid, dim3(256), 0, s, c, a, p.own,
+                           p.pre);
+    else if (p.pre.groups)
+        if (p.rb == 1) NF4_BOTH(1);
+        else NF4_BOTH(2);
+    else if (p.few.whole) NF4_FEW(1, 8);
+    else if (p.rb == 1) NF4_FEW(1, 4);
+    else NF4_FEW(2, 4);
 #undef NF4_FEW
-#undef NF4_TILE
+#undef NF4_BOTH
+    const int st = status_of(hipGetLastError());
+    if (st != NF4_OK || p.bytes == 0) return st;
+    const dim3 rows(static_cast<unsigned>(c.tokens * a.n_heads));
+#define NF4_JOIN(RB)                                                                                \
+    hipLaunchKernelGGL((paged_attn_join_kernel<DT, D, RB>), rows, dim3(kJoinThreads), 0, s, c, a, p.few)
+    if (p.rb == 2) NF4_JOIN(2);
+    else NF4_JOIN(1);
+#undef NF4_JOIN
     return status_of(hipGetLastError());
 }
 
-template <int DT, int D>
-int launch(const Cache &c, const Query &a, const Plan &p, hipStream_t s) {
-    if (a.shared) {
-        const int st = launch_part<DT, D>(c, a, p.pre, s);
-        if (st != NF4_OK) return st;
-    }
-    const int st = launch_part<DT, D>(c, a, p.own, s);
-    if (st != NF4_OK || p.pieces == 1) return st;
-    hipLaunchKernelGGL((paged_attn_join_kernel<DT, D>), dim3(static_cast<unsigned>(c.tokens * a.n_heads)),
-                       dim3(D), 0, s, a);
-    return status_of(hipGetLastError());
+template <int DT>
+int launch_of(const Cache &c, const Query &a, const Plan &p, int head_dim, hipStream_t s) {
+    const bool small = c.page_shift < 4;
+    if (head_dim == 128)
+        return small ? launch<DT, 128, true>(c, a, p, s) : launch<DT, 128, false>(c, a, p, s);
+    return small ? launch<DT, 64, true>(c, a, p, s) : launch<DT, 64, false>(c, a, p, s);
 }
 
 }  // namespace
@@ -1141,17 +1468,18 @@ extern "C" int nf4_paged_attn(const nf4_paged_kv *kv, const void *q, int64_t ld_
     a.shared = cut(shared);
     a.flip = scale < 0.f ? 0x80008000u : 0u;
     a.scale = fmaxf(fabsf(scale) * kLog2e, 1e-30f);  // not 0: a hidden score is -inf
-    const Plan p = make_plan(c, n_heads, a.window, a.sinks, a.shared, max_q, max_len, kv->head_dim);
-    a.pieces = p.pieces;
+    Plan p = make_plan(c, n_heads, a.window, a.sinks, a.shared, max_q, max_len, kv->head_dim);
+    a.dense = p.dense;
     if (p.bytes) {
         if (!workspace || workspace_bytes < p.bytes) return NF4_ERR_WORKSPACE;
         if (!aligned(workspace, 16)) return NF4_ERR_UNSUPPORTED;
+        const int64_t rows = p.dense * tokens * n_heads, few = p.slots * c.n_kv * 16 * p.rb;
         a.part_o = static_cast<float *>(workspace);
-        a.part_ml = reinterpret_cast<float2 *>(a.part_o + tokens * n_heads * p.pieces * kv->head_dim);
+        p.few.part_o = a.part_o + rows * kv->head_dim;
+        a.part_ml = reinterpret_cast<float2 *>(p.few.part_o + few * kv->head_dim);
+        p.few.part_ml = a.part_ml + rows;
     }
     auto s = static_cast<hipStream_t>(stream);
-    const bool wide = kv->head_dim == 128;
-    if (dtype == NF4_BF16)
-        return wide ? launch<NF4_BF16, 128>(c, a, p, s) : launch<NF4_BF16, 64>(c, a, p, s);
-    return wide ? launch<NF4_F16, 128>(c, a, p, s) : launch<NF4_F16, 64>(c, a, p, s);
+    return dtype == NF4_BF16 ? launch_of<NF4_BF16>(c, a, p, kv->head_dim, s)
+                             : launch_of<NF4_F16>(c, a, p, kv->head_dim, s);
 }
