@@ -202,14 +202,55 @@ struct Few {         // the parts of few rows
 
 constexpr int kNowhere = -(1 << 30);  // the position of a row that is not there
 
-// The 16 slots from position k (a multiple of 16) on, in page e of the keys or values of a head
-// (`base`, 16-bit elements), as a buffer resource: an entry that names no page, or pos past the
-// end, is an empty one, from which every load gives zeros.
-__device__ __forceinline__ rsrc_t slots16(const Cache &c, const uint16_t *base, int e, int k, int row_bytes) {
-    const int64_t at = e * c.page_stride + (k & ((1 << c.page_shift) - 1)) * c.slot_stride;
-    const bool there = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages);
-    return make_rsrc(reinterpret_cast<const char *>(base) + uniform64(there ? at * 2 : 0),
-                     there ? c.slot_stride * 30 + row_bytes : 0);
+// A window of 64 pages of a sequence, a lane each, and the next 64 entries on their way: a page's
+// offset is then a lane read away, where a scalar load of each entry would be waited for together
+// with the LDS reads.
+struct Pages {
+    int64_t off;   // lane l: byte offset of page first + l, or -1 where the entry names no page
+    int next;      // entry first + 64 + l
+    int first;
+
+    __device__ __forceinline__ int entry(const Cache &c, const int32_t *tab, int i) const {
+        return i < (c.cap >> c.page_shift) ? tab[i] : -1;
+    }
+    __device__ __forceinline__ void set(const Cache &c, int e) {
+        off = static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages) ? e * c.page_stride * 2 : -1;
+    }
+    __device__ __forceinline__ void begin() { first = -(1 << 30); }
+    // the window that holds `page` (the wave's); windows begin where they are first asked for
+    __device__ __forceinline__ void hold(const Cache &c, const int32_t *tab, int page) {
+        if (page >= first && page < first + 64) return;
+        const int l = threadIdx.x & 63;
+        if (page >= first + 64 && page < first + 128) {
+            first += 64;
+            set(c, next);
+        } else {
+            first = page;
+            set(c, entry(c, tab, first + l));
+        }
+        next = entry(c, tab, first + 64 + l);
+    }
+    // a page of the window, in keys or values of a head (`base`), as a buffer resource: one that
+    // is not there, or not wanted, is an empty one, from which every load gives zeros
+    __device__ __forceinline__ rsrc_t rsrc(const Cache &c, const uint16_t *base, bool want, int page,
+                                           int row_bytes, bool &there) const {
+        const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(off), page - first);
+        const int hi = __builtin_amdgcn_readlane(static_cast<int>(off >> 32), page - first);
+        there = want && hi >= 0;
+        const char *p = reinterpret_cast<const char *>(base) +
+                        (there ? static_cast<int64_t>(static_cast<uint64_t>(hi) << 32 | lo) : 0);
+        const int bytes = ((1 << c.page_shift) - 1) * static_cast<int>(c.slot_stride) * 2 + row_bytes;
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(p), static_cast<short>(0),
+                                                 there ? bytes : 0, 0x00020000);
+    }
+    // byte of position k's slot in its page
+    __device__ __forceinline__ static int slot(const Cache &c, int k) {
+        return (k & ((1 << c.page_shift) - 1)) * static_cast<int>(c.slot_stride) * 2;
+    }
+};
+
+__device__ __forceinline__ u32x4_t bload16s(rsrc_t r, int off, int soff) {
+    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 0));
 }
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -544,60 +585,73 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
             for (int e = 0; e < VE; ++e) acc[rb][e] = (float4_t){0.f, 0.f, 0.f, 0.f};
         }
 
-        // page entries of the slab at key k: of its two 16-key halves, or (pages under 16) of
-        // key k + l % 32; none past the item's end
-        auto entry = [&](int i, int k, int half) {
-            if (i >= rg.i1) return -1;
-            if constexpr (SMALL) {
-                const int j = k + (l & 31);
-                return j < c.cap ? tab[j >> c.page_shift] : -1;
-            } else {
-                return k + half * 16 < c.cap ? sload(tab + ((k + half * 16) >> c.page_shift)) : -1;
-            }
+        // pages under 16 slots (SMALL): the entry of key k + l % 32; none past the item's end
+        auto entry = [&](int i, int k) {
+            const int j = k + (l & 31);
+            return i < rg.i1 && j < c.cap ? tab[j >> c.page_shift] : -1;
         };
         auto good = [&](int e) { return static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages); };
         u32x4_t kr[2][KC];
         u32x4_t vr[8];
+        Pages pg;
+        pg.begin();
         // Every load is issued, whether its page is there or not: the waits then are exact.
-        auto load_k = [&](int e0, int e1, int k) {
+        // Returns the slab's keys whose page is there.
+        auto load_k = [&](int i, int k, int e) -> uint32_t {
+            uint32_t ok = 0;
+            if constexpr (SMALL) {
+                ok = static_cast<uint32_t>(__ballot(good(e)));
+            } else if (i < rg.i1) {
+                pg.hold(c, tab, k >> c.page_shift);
+            }
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 if constexpr (SMALL) {
-                    const int e = __shfl(e0, h * 16 + n);
-                    const uint16_t *p = kb + (good(e) ? e * c.page_stride + ((k + h * 16 + n) & page_mask) * c.slot_stride : 0);
+                    const int eh = __shfl(e, h * 16 + n);
+                    const uint16_t *p = kb + (good(eh) ? eh * c.page_stride + ((k + h * 16 + n) & page_mask) * c.slot_stride : 0);
 #pragma unroll
                     for (int x = 0; x < KC; ++x) {
                         kr[h][x] = (u32x4_t){0, 0, 0, 0};
-                        if (good(e)) kr[h][x] = *reinterpret_cast<const u32x4_t *>(p + g * 8 + x * 32);
+                        if (good(eh)) kr[h][x] = *reinterpret_cast<const u32x4_t *>(p + g * 8 + x * 32);
                     }
                 } else {
-                    const rsrc_t r = slots16(c, kb, h ? e1 : e0, k + h * 16, D * 2);
+                    const int kh = k + h * 16;
+                    bool there;
+                    const rsrc_t r = pg.rsrc(c, kb, i < rg.i1, kh >> c.page_shift, D * 2, there);
+                    ok |= there ? 0xffffu << (16 * h) : 0;
+                    const int so = Pages::slot(c, kh);
 #pragma unroll
-                    for (int x = 0; x < KC; ++x) kr[h][x] = bload16(r, n * stride2 + g * 16 + x * 64);
+                    for (int x = 0; x < KC; ++x) kr[h][x] = bload16s(r, n * stride2 + g * 16 + x * 64, so);
                 }
             }
+            return ok;
         };
-        auto load_v = [&](int e0, int e1, int k) {
+        auto load_v = [&](int i, int k, int e) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 rsrc_t r;
-                if constexpr (!SMALL) r = slots16(c, vb, h ? e1 : e0, k + h * 16, D * 2);
+                int so = 0;
+                if constexpr (!SMALL) {
+                    bool there;
+                    r = pg.rsrc(c, vb, i < rg.i1, (k + h * 16) >> c.page_shift, D * 2, there);
+                    so = Pages::slot(c, k + h * 16);
+                }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     if constexpr (SMALL) {
-                        const int i = h * 16 + g * 4 + j, e = __shfl(e0, i);
+                        const int i = h * 16 + g * 4 + j, eh = __shfl(e, i);
                         vr[h * 4 + j] = (u32x4_t){0, 0, 0, 0};
-                        if (good(e)) {
+                        if (good(eh)) {
                             const u32x2_t *p = reinterpret_cast<const u32x2_t *>(
-                                vb + e * c.page_stride + ((k + i) & page_mask) * c.slot_stride + n * VE);
+                                vb + eh * c.page_stride + ((k + i) & page_mask) * c.slot_stride + n * VE);
                             const u32x2_t lo = p[0], hi = p[D == 128 ? 1 : 0];
                             vr[h * 4 + j] = (u32x4_t){lo.x, lo.y, hi.x, hi.y};
                         }
                     } else if constexpr (D == 128) {
-                        vr[h * 4 + j] = bload16(r, (g * 4 + j) * stride2 + n * 16);
+                        vr[h * 4 + j] = bload16s(r, (g * 4 + j) * stride2 + n * 16, so);
                     } else {
                         const u32x2_t t = __builtin_bit_cast(
-                            u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, (g * 4 + j) * stride2 + n * 8, 0, 0));
+                            u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, (g * 4 + j) * stride2 + n * 8, so, 0));
                         vr[h * 4 + j] = (u32x4_t){t.x, t.y, 0, 0};
                     }
                 }
@@ -605,11 +659,16 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
         };
 
         bool odd_seen = false;
-        int i = rg.i0 + w, k = rg.key0(i), k2 = rg.key0(i + W);
-        int e0 = entry(i, k, 0), e1 = entry(i, k, 1);
-        int f0 = entry(i + W, k2, 0), f1 = entry(i + W, k2, 1);
-        load_k(e0, e1, k);
-        load_v(e0, e1, k);
+        int i = rg.i0 + w, k = rg.key0(i), k2 = rg.key0(i + W), e0 = -1, e1 = -1;
+        uint32_t ok = 0;  // keys whose page is there
+        if (i < rg.i1) {
+            if constexpr (SMALL) {
+                e0 = entry(i, k);
+                e1 = entry(i + W, k2);
+            }
+            ok = load_k(i, k, e0);
+            load_v(i, k, e0);
+        }
         while (i < rg.i1) {
             float4_t st[RB][2];
 #pragma unroll
@@ -620,10 +679,7 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
 #pragma unroll
                     for (int x = 0; x < KC; ++x) st[rb][h] = mfma16<DT>(kr[h][x], q[rb][x], st[rb][h]);
                 }
-            uint32_t ok;  // keys whose page is there
-            if constexpr (SMALL) ok = static_cast<uint32_t>(__ballot(good(e0)));
-            else ok = (good(e0) ? 0xffffu : 0u) | (good(e1) ? 0xffff0000u : 0u);
-            load_k(f0, f1, k2);
+            const uint32_t ok2 = load_k(i + W, k2, e1);
             const bool full = rg.full(a, k) && ok == 0xffffffffu;
             bool odd = false;  // an infinity or NaN among values that not every row sees
             if (!full) {
@@ -684,14 +740,15 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
 #pragma unroll
                 for (int rb = 0; rb < RB; ++rb) acc[rb][e] = mfma16<DT>(f, pf[rb], acc[rb][e]);
             }
-            load_v(f0, f1, k2);
-            e0 = f0;
-            e1 = f1;
-            k = k2;
-            k2 = rg.key0(i + 2 * W);
-            f0 = entry(i + 2 * W, k2, 0);
-            f1 = entry(i + 2 * W, k2, 1);
+            load_v(i + W, k2, e1);
+            ok = ok2;
             i += W;
+            k = k2;
+            k2 = rg.key0(i + W);
+            if constexpr (SMALL) {
+                e0 = e1;
+                e1 = entry(i + W, k2);
+            }
         }
 
         if (odd_seen) {
@@ -787,9 +844,13 @@ __global__ __launch_bounds__(64 * W, W == 4 && RB == 1 ? 3 : 2) void paged_attn_
 typedef short v4i16_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16_t lds_v4i16_t;
 
-__device__ __forceinline__ u32x2_t tr_read(const uint8_t *s, int off) {
+// by LDS address
+__device__ __forceinline__ u32x2_t tr_read(uint32_t at) {
     return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        (lds_v4i16_t *)((__attribute__((address_space(3))) uint8_t *)s + off)));
+        reinterpret_cast<lds_v4i16_t *>(static_cast<uintptr_t>(at))));
+}
+__device__ __forceinline__ u32x4_t lds16(uint32_t at) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t *>(static_cast<uintptr_t>(at));
 }
 
 constexpr int kRows = 128;
@@ -898,36 +959,19 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
                               (__attribute__((address_space(3))) uint8_t *)lds)) + w * 1024;
     auto good = [&](int e) { return static_cast<uint32_t>(e) < static_cast<uint32_t>(c.pages); };
-    // page entries of the tile at key k: of its 16-key quarters, or (pages under 16) key k + l's
-    struct Entries { int e[4]; };
-    auto entries = [&](int k) {
-        Entries t;
-        if constexpr (SMALL) {
-            t.e[0] = k + l < c.cap ? tab[(k + l) >> c.page_shift] : -1;
-        } else {
-#pragma unroll
-            for (int x = 0; x < 4; ++x)
-                t.e[x] = k + 16 * x < c.cap ? sload(tab + ((k + 16 * x) >> c.page_shift)) : -1;
-        }
-        return t;
-    };
-    auto there = [&](const Entries &t) -> uint64_t {  // keys whose page is there
-        if constexpr (SMALL) {
-            return __ballot(good(t.e[0]));
-        } else {
-            uint64_t v = 0;
-#pragma unroll
-            for (int x = 0; x < 4; ++x) v |= good(t.e[x]) ? 0xffffull << (16 * x) : 0;
-            return v;
-        }
-    };
+    Pages pg;
+    pg.begin();
     const int ko = (srow & 15) * stride2 + kch * 16, vo = (srow & 15) * stride2 + vch0 * 16;
-    // tile k into stage st: by DMA, a pass of a wave within one of the tile's 16-key quarters
-    auto send = [&](int st, const Entries &t, int k) {
+    // tile k into stage st, and which of its keys' pages are there: by DMA, a pass of a wave
+    // within one of the tile's 16-key quarters
+    auto send = [&](int st, int k) -> uint64_t {
+        uint64_t ok = 0;
+        if constexpr (SMALL) {
+            const int mine = k + l < c.cap ? tab[(k + l) >> c.page_shift] : -1;
+            ok = __ballot(good(mine));
 #pragma unroll
-        for (int x = 0; x < PASS; ++x) {
-            if constexpr (SMALL) {
-                const int row = x * RPP + srow, e = __shfl(t.e[0], row);
+            for (int x = 0; x < PASS; ++x) {
+                const int row = x * RPP + srow, e = __shfl(mine, row);
                 const int64_t at = e * c.page_stride + ((k + row) & page_mask) * c.slot_stride;
                 u32x4_t kx = {0, 0, 0, 0}, vx = {0, 0, 0, 0};
                 if (good(e)) {
@@ -936,14 +980,23 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
                 }
                 *reinterpret_cast<u32x4_t *>(s_k + st * STAGE + row * D * 2 + sch * 16) = kx;
                 *reinterpret_cast<u32x4_t *>(s_v + st * STAGE + row * D * 2 + sch * 16) = vx;
-            } else {
-                const int e = D == 128 ? t.e[x] : w < 2 ? t.e[(2 * x) & 3] : t.e[(2 * x + 1) & 3];
-                const int k16 = k + (x * RPP + (D == 128 ? 0 : (w >> 1) * 16));
-                const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + st * STAGE + x * 4096);
-                lds_dma16(at, ko, slots16(c, kb, e, k16, D * 2), 0);
-                lds_dma16(at + 2 * STAGE, vo, slots16(c, vb, e, k16, D * 2), 0);
+            }
+        } else {
+            pg.hold(c, tab, k >> c.page_shift);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                bool there;
+                const int k16 = k + x * 16, page = k16 >> c.page_shift;
+                const rsrc_t rk = pg.rsrc(c, kb, true, page, D * 2, there), rv = pg.rsrc(c, vb, true, page, D * 2, there);
+                ok |= there ? 0xffffull << (16 * x) : 0;
+                if (D == 64 && (x & 1) != w >> 1) continue;
+                const int so = Pages::slot(c, k16);
+                const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + st * STAGE + (D == 128 ? x : x >> 1) * 4096);
+                lds_dma16(at, ko, rk, so);
+                lds_dma16(at + 2 * STAGE, vo, rv, so);
             }
         }
+        return ok;
     };
     // what this wave loaded of a tile that not every row sees whole: the values of keys that no
     // row sees become zeros; infinities and NaN too (0 times one is no 0), and s_odd says so
@@ -966,40 +1019,35 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
     };
 
     // ---- operand addresses of this lane
-    const int krow = n * D * 2, kx = D == 128 ? (n & 15) : ((n >> 1) & 7);
+    // (chunk numbers change by exclusive or: so do the addresses, whose low bits they are)
+    const uint32_t lds_k = lds0 - w * 1024;
+    const uint32_t kbase = lds_k + n * D * 2 + ((g ^ (D == 128 ? (n & 15) : ((n >> 1) & 7))) << 4);
     const int vkey = g * 4 + ((l & 15) >> 2);  // key (of 16) and chunk that it points at
     const int vch = ((l >> 4) & 1) * 2 + ((l & 3) >> 1);
-    const int vbase = vkey * D * 2 + (l & 1) * 8;
-    const int vx = D == 128 ? (vkey & 3) << 2 : ((vkey >> 1) & 1) << 2;
+    const uint32_t vbase = lds_k + 2 * STAGE + vkey * D * 2 + (l & 1) * 8 +
+                           ((vch ^ (D == 128 ? (vkey & 3) << 2 : ((vkey >> 1) & 1) << 2)) << 4);
 
-    Entries cur{}, nxt{};
-    int k = rg.key0(rg.i0), k2 = rg.key0(rg.i0 + 1);
+    int k = rg.key0(rg.i0);
+    uint64_t ok = 0;
     if (tid < 2) s_odd[tid] = -1;
     __syncthreads();
-    if (rg.i0 < rg.i1) {
-        cur = entries(k);
-        send(0, cur, k);
-        if (rg.i0 + 1 < rg.i1) nxt = entries(k2);
-    }
+    if (rg.i0 < rg.i1) ok = send(0, k);
     for (int i = rg.i0; i < rg.i1; ++i) {
         const int st = (i - rg.i0) & 1;
-        const uint64_t ok = there(cur);
         const bool full = rg.full(a, k) && !~ok;
         if constexpr (!SMALL) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         if (!full) clean(st, i, k, ok);
         __syncthreads();  // every wave's part of tile i is there, and tile i - 1 is read
         // scores, 32 keys each
         u32x4_t kf[2][KS];
+        const uint32_t ka = kbase + st * STAGE, va = vbase + st * STAGE;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int x = 0; x < KS; ++x)
-                kf[h][x] = *reinterpret_cast<const u32x4_t *>(
-                    s_k + st * STAGE + h * 32 * D * 2 + krow + (((2 * x + g) ^ kx) << 4));
-        if (i + 1 < rg.i1) send(st ^ 1, nxt, k2);
-        Entries nxt2{};
-        const int k3 = rg.key0(i + 2);
-        if (i + 2 < rg.i1) nxt2 = entries(k3);
+            for (int x = 0; x < KS; ++x) kf[h][x] = lds16((ka ^ (x << 5)) + h * 64 * D);
+        const int k2 = rg.key0(i + 1);
+        uint64_t ok2 = 0;
+        if (i + 1 < rg.i1) ok2 = send(st ^ 1, k2);
         __builtin_amdgcn_sched_barrier(0);
         float16_t sc[2];
 #pragma unroll
@@ -1014,8 +1062,8 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         auto read_v = [&](int x, u32x4_t (&f)[DT32]) {
 #pragma unroll
             for (int d = 0; d < DT32; ++d) {
-                const int at = st * STAGE + vbase + (((d * 4 + vch) ^ vx) << 4) + x * 16 * D * 2;
-                const u32x2_t lo = tr_read(s_v, at), hi = tr_read(s_v, at + 8 * D * 2);
+                const uint32_t at = (va ^ (d << 6)) + x * 32 * D;
+                const u32x2_t lo = tr_read(at), hi = tr_read(at + 16 * D);
                 f[d] = (u32x4_t){lo.x, lo.y, hi.x, hi.y};
             }
         };
@@ -1064,10 +1112,8 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
             for (int d = 0; d < DT32; ++d) acc[d] = mfma32<DT>(vf[x & 1][d], pf[x], acc[d]);
             if (x < 2) read_v(x + 2, vf[x & 1]);
         }
-        cur = nxt;
-        nxt = nxt2;
         k = k2;
-        k2 = k3;
+        ok = ok2;
     }
 
     if (odd_seen) {
@@ -1394,7 +1440,8 @@ int launch(const Cache &c, const Query &a, const Plan &p, hipStream_t s) {
 
 template <int DT>
 int launch_of(const Cache &c, const Query &a, const Plan &p, int head_dim, hipStream_t s) {
-    const bool small = c.page_shift < 4;
+    // per-lane page addresses: for pages under 16 slots, and for pages that span 2^31 bytes
+    const bool small = c.page_shift < 4 || c.slot_stride * 2 << c.page_shift >= 0x7fffffff;
     if (head_dim == 128)
         return small ? launch<DT, 128, true>(c, a, p, s) : launch<DT, 128, false>(c, a, p, s);
     return small ? launch<DT, 64, true>(c, a, p, s) : launch<DT, 64, false>(c, a, p, s);
