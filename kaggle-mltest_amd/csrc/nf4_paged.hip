@@ -192,6 +192,8 @@ struct Part {       // a tiled part
 struct Few {         // the parts of few rows
     float *part_o;   // [slots * n_kv][rows of an item][D]
     float2 *part_ml; // [slots * n_kv][rows of an item]
+    int2 *where;     // [1 + prefix][tokens * group]: (first slot, pieces * 64 + row in the item)
+    int slots;       // all of them
     int groups;      // workgroups a key/value head
     int min_units;   // work of one, at least
     int whole;       // 1: an item each
@@ -249,8 +251,14 @@ struct Pages {
     }
 };
 
+// Loads of the few-rows kernel, not temporal (aux bit 1): a step reads its cache once, and lines
+// that evict others on their way cost 2-4 % (131071 keys 60.6 -> 59.1 us, 64 sequences
+// 212.7 -> 206.4 us).
 __device__ __forceinline__ u32x4_t bload16s(rsrc_t r, int off, int soff) {
-    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 0));
+    return __builtin_bit_cast(u32x4_t, __builtin_amdgcn_raw_buffer_load_b128(r, off, soff, 2));
+}
+__device__ __forceinline__ u32x2_t bload8s(rsrc_t r, int off, int soff) {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 2));
 }
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
@@ -517,35 +525,52 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
     const int page_mask = (1 << c.page_shift) - 1;
 
     Units u;
-    all_units<W, RB>(u, c, a, f);
-    const int used = f.whole ? 0 : groups_used(f, u.total);
-    if (f.whole ? group >= u.total : group >= used) return;
-    const int64_t u1 = f.whole ? group + 1 : first_unit(u.total, group + 1, used);
-    int64_t at = f.whole ? group : first_unit(u.total, group, used);
+    int used = 0;
+    int64_t at = group, u1 = group + 1;
+    const bool plain = W == 8 && !c.cu;  // whole sequences of at most 16 rows: item b is sequence b
+    if (plain) {
+        if (group >= f.seqs) return;
+    } else {
+        all_units<W, RB>(u, c, a, f);
+        used = f.whole ? 0 : groups_used(f, u.total);
+        if (f.whole ? group >= u.total : group >= used) return;
+        if (!f.whole) {
+            u1 = first_unit(u.total, group + 1, used);
+            at = first_unit(u.total, group, used);
+        }
+    }
     while (at < u1) {
         // the item that unit `at` falls into
-        uint64_t past = __ballot(u.base + u.up > at);
-        while (!past) {
-            if (u.b0 + 64 >= f.seqs + f.prefix) return;  // lengths that changed under the kernel
-            next_units<W, RB>(u, c, a, f);
-            past = __ballot(u.base + u.up > at);
+        int b = group, item = group, blk = 0, st0 = 0, st1 = 0, steps = 0, pieces = 1;
+        bool single = true;
+        if (!plain) {
+            uint64_t past = __ballot(u.base + u.up > at);
+            while (!past) {
+                if (u.b0 + 64 >= f.seqs + f.prefix) return;  // lengths that changed under the kernel
+                next_units<W, RB>(u, c, a, f);
+                past = __ballot(u.base + u.up > at);
+            }
+            const int lane = __builtin_ctzll(past);
+            b = u.b0 + lane;
+            steps = __builtin_amdgcn_readlane(u.steps, lane);
+            const int blocks = __builtin_amdgcn_readlane(u.blocks, lane);
+            const int per = f.whole ? 1 : steps + 1;
+            int64_t start = u.base + lane_of(u.up, lane) - static_cast<int64_t>(blocks) * per;
+            blk = blocks == 1 ? 0 : static_cast<int>((at - start) / per);
+            start += static_cast<int64_t>(blk) * per;
+            item = u.ibase + __builtin_amdgcn_readlane(u.iup, lane) - blocks + blk;
+            const int64_t next = start + per < u1 ? start + per : u1;
+            st0 = static_cast<int>(at - start) - 1;
+            st1 = f.whole ? steps : static_cast<int>(next - start) - 1;
+            st0 = st0 < 0 ? 0 : st0;
+            at = next;
+            if (item >= f.items) return;        // offsets that decrease
+            if (st1 <= st0 && steps) continue;  // no more than its beginning
+            single = st0 == 0 && st1 == steps;
+            if (!single && st0 == 0) pieces = group_of(u.total, start + steps, used) - group + 1;
+        } else {
+            at = u1;
         }
-        const int lane = __builtin_ctzll(past);
-        const int b = u.b0 + lane, steps = __builtin_amdgcn_readlane(u.steps, lane);
-        const int blocks = __builtin_amdgcn_readlane(u.blocks, lane);
-        const int per = f.whole ? 1 : steps + 1;
-        int64_t start = u.base + lane_of(u.up, lane) - static_cast<int64_t>(blocks) * per;
-        const int blk = blocks == 1 ? 0 : static_cast<int>((at - start) / per);
-        start += static_cast<int64_t>(blk) * per;
-        const int item = u.ibase + __builtin_amdgcn_readlane(u.iup, lane) - blocks + blk;
-        const int64_t next = start + per < u1 ? start + per : u1;
-        int st0 = static_cast<int>(at - start) - 1, st1 = static_cast<int>(next - start) - 1;
-        st0 = st0 < 0 ? 0 : st0;
-        if (f.whole) st1 = steps;
-        at = next;
-        if (item >= f.items) return;             // offsets that decrease
-        if (st1 <= st0 && steps) continue;       // no more than its beginning
-        const bool single = st0 == 0 && st1 == steps;
 
         const bool prefix = b == f.seqs;
         Seq s = {0, c.tokens, 0};
@@ -572,8 +597,10 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
         rg.pmin = prefix ? u.pmin : s.p0;
         rg.pmax = prefix ? u.pmax : s.p0 + s.n - 1;
         rg.set(c, a, prefix);
-        rg.i0 = st0 * W;
-        rg.i1 = st1 * W < rg.n ? st1 * W : rg.n;
+        if (!plain) {
+            rg.i0 = st0 * W;
+            rg.i1 = st1 * W < rg.n ? st1 * W : rg.n;
+        }
 
         float m[RB], sum[RB];
         float4_t acc[RB][VE];
@@ -650,8 +677,7 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
                     } else if constexpr (D == 128) {
                         vr[h * 4 + j] = bload16s(r, (g * 4 + j) * stride2 + n * 16, so);
                     } else {
-                        const u32x2_t t = __builtin_bit_cast(
-                            u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, (g * 4 + j) * stride2 + n * 8, so, 0));
+                        const u32x2_t t = bload8s(r, (g * 4 + j) * stride2 + n * 8, so);
                         vr[h * 4 + j] = (u32x4_t){t.x, t.y, 0, 0};
                     }
                 }
@@ -821,12 +847,18 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
                 if (d == 0) f.part_ml[slot] = make_float2(mm, ll);
             }
         }
+        if (W != 8 && kvh == 0 && st0 == 0) {  // the item's first piece says where its rows are
+            const int r = threadIdx.x;
+            if (r < 16 * RB && r0 + r < rows)
+                f.where[(prefix ? c.tokens * a.group : 0) + s.q0 * a.group + r0 + r] =
+                    make_int2(group + item, pieces * 64 + r);
+        }
         __syncthreads();
     }
 }
 
 template <int DT, int D, int RB, bool SMALL, int W>
-__global__ __launch_bounds__(64 * W, W == 4 && RB == 1 ? 3 : 2) void paged_attn_few_kernel(
+__global__ __launch_bounds__(64 * W, 2) void paged_attn_few_kernel(
     const Cache c, const Query a, const Few f) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds<D>(W, RB)];
     few_body<DT, D, RB, SMALL, W>(c, a, f, blockIdx.x, lds);
@@ -983,6 +1015,19 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
             }
         } else {
             pg.hold(c, tab, k >> c.page_shift);
+            if (c.page_shift >= 6) {  // the tile is in one page
+                bool there;
+                const int page = k >> c.page_shift, so = Pages::slot(c, k);
+                const rsrc_t rk = pg.rsrc(c, kb, true, page, D * 2, there), rv = pg.rsrc(c, vb, true, page, D * 2, there);
+                const uint32_t at = __builtin_amdgcn_readfirstlane(lds0 + st * STAGE);
+                const int so1 = so + (D == 64 ? (w >> 1) * 16 : 0) * stride2;
+#pragma unroll
+                for (int x = 0; x < PASS; ++x) {
+                    lds_dma16(at + x * 4096, ko, rk, so1 + x * RPP * stride2);
+                    lds_dma16(at + 2 * STAGE + x * 4096, vo, rv, so1 + x * RPP * stride2);
+                }
+                return there ? ~0ull : 0;
+            }
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
                 bool there;
@@ -1210,25 +1255,16 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Cac
     int64_t slot[2] = {0, 0}; // row of the first
     if (f.groups) {
         const int tok = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
-        const int kvh = head / a.group, b = seq_of_token(c, tok);
-        const int q0 = b < f.seqs ? seq_at(c, b).q0 : 0;
-        Units u;
-        all_units<4, RB>(u, c, a, f);
-        const int used = groups_used(f, u.total);
+        const int kvh = head / a.group;
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-            const int e = x ? f.seqs : b, r = (x ? tok : tok - q0) * a.group + head % a.group;
-            if ((x ? !f.prefix : b >= f.seqs) || r < 0) continue;
-            while (e >= u.b0 + 64) next_units<4, RB>(u, c, a, f);
-            if (e < u.b0) continue;
-            const int at = e - u.b0, blocks = __builtin_amdgcn_readlane(u.blocks, at);
-            const int steps = __builtin_amdgcn_readlane(u.steps, at), blk = r / R;
-            const int item = u.ibase + __builtin_amdgcn_readlane(u.iup, at) - blocks + blk;
-            if (blk >= blocks || item >= f.items) continue;
-            const int64_t start = u.base + lane_of(u.up, at) - static_cast<int64_t>(blocks - blk) * (steps + 1);
-            const int first = group_of(u.total, steps ? start + 1 : start, used);
-            n[x] = group_of(u.total, start + steps, used) - first + 1;
-            slot[x] = (static_cast<int64_t>(first + item) * c.n_kv + kvh) * R + r % R;
+            if (x && !f.prefix) continue;
+            const int2 w = f.where[(x ? c.tokens * a.group : 0) + tok * a.group + head % a.group];
+            const int p = w.y >> 6, r = w.y & 63;
+            // (offsets that decrease leave tokens that no item has: nothing past the slots is read)
+            if (w.x < 0 || p < 1 || r >= R || w.x >= f.slots || p > f.slots - w.x) continue;
+            n[x] = p;
+            slot[x] = (static_cast<int64_t>(w.x) * c.n_kv + kvh) * R + r;
         }
         if (f.direct && n[0] == 1) return;  // written
     }
@@ -1336,15 +1372,17 @@ struct Plan {
     Few few;          // groups 0: none
     Part own, pre;    // groups 0: none
     int rb, waves;    // of the few-rows kernel
-    int64_t dense, slots;
+    int64_t dense, slots, where;
     size_t bytes;
 };
 
-// Sequences whose rows are few go to the kernel without LDS staging.  Its launch fills the card
-// once (kFewSlots workgroups); where no sequence is longer than kWholeKeys and all of them fit
+// Sequences whose rows are few go to the kernel without LDS staging.  Its launch is a workgroup
+// on every CU (kFewSlots): 64 KB in flight on each are enough for the memory's rate, and more
+// workgroups mean shorter shares and more pieces (131071 keys, 64 ragged sequences: 512
+// workgroups 63.5 and 215 us, 256 60.6 and 212.7).  Where no sequence is longer than kWholeKeys and all of them fit
 // the card, a workgroup of 8 waves takes a whole sequence, and there is nothing to join.  Tiled
 // parts are cut until the launch has kTileSlots workgroups.
-constexpr int kFewRows = 32, kFewSlots = 768, kTileSlots = 512, kWholeKeys = 1024;
+constexpr int kFewRows = 32, kFewSlots = 256, kTileSlots = 512, kWholeKeys = 1024;
 
 Part tile_part(bool prefix, int64_t blocks, int n_kv, int64_t keys, int slots) {
     Part p{};
@@ -1384,10 +1422,13 @@ Plan make_plan(const Cache &c, int n_heads, int window, int sinks, int shared, i
         p.waves = f.whole ? 8 : 4;
         f.min_units = 2;
         int64_t units = f.items * (span / (32 * p.waves) + 2) + pre_keys / 128 + 2;
-        int64_t groups = ceil_div(shared && !few_pre ? kTileSlots / 2 : kFewSlots, c.n_kv);
+        int64_t groups = ceil_div(kFewSlots, c.n_kv);
         groups = groups < units / f.min_units ? groups : units / f.min_units;
-        f.groups = f.whole ? f.items : static_cast<int>(groups < 1 ? 1 : groups);
-        if (!f.whole) p.slots = f.groups + f.items;
+        f.groups = f.whole ? (c.cu ? f.items : seqs) : static_cast<int>(groups < 1 ? 1 : groups);
+        if (!f.whole) {
+            p.slots = f.slots = f.groups + f.items;
+            p.where = all_rows * (1 + f.prefix);
+        }
     } else {
         const int64_t blocks = c.cu ? all_rows / kRows + seqs
                                     : static_cast<int64_t>(c.batch) * ceil_div(longest * group, kRows);
@@ -1399,7 +1440,8 @@ Plan make_plan(const Cache &c, int n_heads, int window, int sinks, int shared, i
     p.own.first = p.pre.groups ? p.pre.splits : 0;
     p.dense = p.own.first + (p.own.groups ? p.own.splits : 0);
     if (!shared && p.dense == 1) p.dense = 0;
-    p.bytes = (p.dense * c.tokens * n_heads + p.slots * c.n_kv * 16 * p.rb) * (4 * head_dim + 8);
+    p.bytes = (p.dense * c.tokens * n_heads + p.slots * c.n_kv * 16 * p.rb) * (4 * head_dim + 8) +
+              p.where * 8;
     return p;
 }
 
@@ -1525,6 +1567,7 @@ extern "C" int nf4_paged_attn(const nf4_paged_kv *kv, const void *q, int64_t ld_
         p.few.part_o = a.part_o + rows * kv->head_dim;
         a.part_ml = reinterpret_cast<float2 *>(p.few.part_o + few * kv->head_dim);
         p.few.part_ml = a.part_ml + rows;
+        p.few.where = reinterpret_cast<int2 *>(p.few.part_ml + few);
     }
     auto s = static_cast<hipStream_t>(stream);
     return dtype == NF4_BF16 ? launch_of<NF4_BF16>(c, a, p, kv->head_dim, s)

@@ -713,25 +713,28 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache:
     fp32 [positions, head_dim / 2] (rope_table); `cu_q`: int32 offsets of the sequences' tokens,
     None when each brings tokens / batch."""
     dim, kv = cache.head_dim, cache.n_kv
-    if qkv.dim() != 2 or qkv.dtype != cache.dtype or qkv.stride(1) != 1 or qkv.shape[1] % dim:
+    if qkv.dim() != 2 or qkv.dtype != cache.dtype or qkv.stride(1) != 1:
         raise ValueError("qkv is a row-contiguous [tokens, (n_heads + 2 n_kv) head_dim] tensor of "
                          "the cache's dtype")
-    _check_device(qkv, cos, sin)
-    tokens, heads = qkv.shape[0], qkv.shape[1] // dim - 2 * kv
-    if heads < 1 or heads % kv:
-        raise ValueError("n_heads is a multiple of the cache's n_kv")
-    for t in (cos, sin):
-        if t.dtype != torch.float32 or t.dim() != 2 or t.shape[1] * 2 != dim \
-                or t.shape != cos.shape or not t.is_contiguous():
-            raise ValueError("cos and sin are contiguous fp32 [positions, head_dim / 2] tables")
+    if not (qkv.is_cuda and cos.is_cuda and sin.is_cuda):
+        _check_device(qkv, cos, sin)
+    tokens, cols = qkv.shape
+    heads = cols // dim - 2 * kv
+    if heads < 1 or heads % kv or cols % dim:
+        raise ValueError("qkv has (n_heads + 2 n_kv) head_dim columns, n_heads a multiple of the "
+                         "cache's n_kv")
+    rope = cos.shape
+    if len(rope) != 2 or rope[1] * 2 != dim or rope != sin.shape or cos.dtype != torch.float32 \
+            or sin.dtype != torch.float32 or not (cos.is_contiguous() and sin.is_contiguous()):
+        raise ValueError("cos and sin are contiguous fp32 [positions, head_dim / 2] tables")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=qkv.dtype, device=qkv.device)
+        out = qkv.new_empty((tokens, heads, dim))
     else:
         _check_out(out, (tokens, heads, dim), qkv)
-    ld = qkv.stride(0) if tokens > 1 else qkv.shape[1]
-    st = load().nf4_paged_append(cache.ref, qkv.data_ptr(), ld, cos.data_ptr(), sin.data_ptr(),
-                                 cos.shape[0], _check_cu(cu_q, cache), out.data_ptr(), tokens,
-                                 heads, cache.code, stream_of(qkv))
+    st = load().nf4_paged_append(cache.ref, qkv.data_ptr(), qkv.stride(0) if tokens > 1 else cols,
+                                 cos.data_ptr(), sin.data_ptr(), rope[0],
+                                 None if cu_q is None else _check_cu(cu_q, cache), out.data_ptr(),
+                                 tokens, heads, cache.code, stream_of(qkv))
     if st:
         check(st, "nf4_paged_append")
     return out
@@ -746,17 +749,18 @@ def _check_out(out, shape, like):
 def _attention(q, cache, shared, cu_q, scale, window, sinks, max_q, max_len, out, lse):
     if q.dim() != 3 or q.dtype != cache.dtype or q.shape[2] != cache.head_dim or q.stride(2) != 1:
         raise ValueError("q is [tokens, n_heads, head_dim] of the cache's dtype, head_dim contiguous")
-    _check_device(q)
+    if not q.is_cuda:
+        _check_device(q)
     tokens, heads, dim = q.shape
     if heads < 1 or heads % cache.n_kv:
         raise ValueError("n_heads is a multiple of the cache's n_kv")
     if out is None:
-        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+        out = q.new_empty((tokens, heads, dim))
     else:
         _check_out(out, (tokens, heads, dim), q)
     stats = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if lse else None
     lib = load()
-    cu = _check_cu(cu_q, cache)
+    cu = None if cu_q is None else _check_cu(cu_q, cache)
     window, sinks, max_q, max_len = window or 0, sinks or 0, max_q or 0, max_len or 0
     nbytes = lib.nf4_paged_attn_workspace(cache.ref, cu, tokens, heads, window, sinks, shared,
                                           max_q, max_len)
