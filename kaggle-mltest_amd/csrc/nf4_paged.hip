@@ -876,6 +876,13 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_few_kernel(
 typedef short v4i16_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16_t lds_v4i16_t;
 
+// the value of lane l ^ 32
+__device__ __forceinline__ float other_half(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
 // by LDS address
 __device__ __forceinline__ u32x2_t tr_read(uint32_t at) {
     return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -1094,6 +1101,9 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         uint64_t ok2 = 0;
         if (i + 1 < rg.i1) ok2 = send(st ^ 1, k2);
         __builtin_amdgcn_sched_barrier(0);
+        // a wave at its products goes before one at its softmax (512 -> 494 us for the 8192-token
+        // prompt: the other has its instructions under them)
+        __builtin_amdgcn_s_setprio(1);
         float16_t sc[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -1112,6 +1122,7 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
                 f[d] = (u32x4_t){lo.x, lo.y, hi.x, hi.y};
             }
         };
+        __builtin_amdgcn_s_setprio(0);
         read_v(0, vf[0]);
         read_v(1, vf[1]);
         __builtin_amdgcn_sched_barrier(0);
@@ -1127,7 +1138,7 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         float top = sc[0][0];
 #pragma unroll
         for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
-        top = fmaxf(top, __shfl_xor(top, 32)) * a.scale;
+        top = fmaxf(top, other_half(top)) * a.scale;
         // m is a maximum of earlier tiles: probabilities up to 2^8 are let be (their sums are in
         // fp32, their rounding is relative), so that few tiles rescale
         if (__any(top > m + 8.f)) {
@@ -1151,12 +1162,14 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
                               pack2<DT>(p[6], p[7])};
         }
         odd_seen |= s_odd[st] == i;
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
 #pragma unroll
             for (int d = 0; d < DT32; ++d) acc[d] = mfma32<DT>(vf[x & 1][d], pf[x], acc[d]);
             if (x < 2) read_v(x + 2, vf[x & 1]);
         }
+        __builtin_amdgcn_s_setprio(0);
         k = k2;
         ok = ok2;
     }
@@ -1183,7 +1196,7 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         }
     }
 
-    sum += __shfl_xor(sum, 32);
+    sum += other_half(sum);
     if (!live) return;
     const int64_t row = static_cast<int64_t>(tok) * a.n_heads + head;
     if (a.dense == 0) {
