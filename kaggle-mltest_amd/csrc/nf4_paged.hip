@@ -807,6 +807,7 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
         for (int rb = 0; rb < RB; ++rb) {
             sum[rb] += __shfl_xor(sum[rb], 16);
             sum[rb] += __shfl_xor(sum[rb], 32);
+            if (m[rb] == -INFINITY && sum[rb] != sum[rb]) m[rb] = 0.f;  // NaN scores only: not nothing
             const int row = w * 16 * RB + rb * 16 + n;
             if (g == 0) s_ml[row] = make_float2(m[rb], sum[rb]);
             if (r0 + rb * 16 + n < rows) {
@@ -1197,6 +1198,7 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
     }
 
     sum += other_half(sum);
+    if (m == -INFINITY && sum != sum) m = 0.f;  // NaN scores only: not nothing
     if (!live) return;
     const int64_t row = static_cast<int64_t>(tok) * a.n_heads + head;
     if (a.dense == 0) {
@@ -1258,80 +1260,83 @@ constexpr int kJoinThreads = 256;
 
 template <int DT, int D, int RB>
 __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Cache c, const Query a,
-                                                                       const Few f) {
+                                                                       const Few f, int64_t rows) {
     constexpr int COLS = D / 4, LANES = kJoinThreads / COLS, R = 16 * RB;
     __shared__ float4_t s_o[LANES][COLS];
     __shared__ float s_m[LANES], s_l[LANES];
-    const int64_t row = blockIdx.x;
     const int col = threadIdx.x % COLS, lane = threadIdx.x / COLS;
-    int n[2] = {0, 0};        // pieces of few rows: of the sequence's item and of the prefix's
-    int64_t slot[2] = {0, 0}; // row of the first
-    if (f.groups) {
-        const int tok = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
-        const int kvh = head / a.group;
+    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
+        int n[2] = {0, 0};        // pieces of few rows: of the sequence's item and of the prefix's
+        int64_t slot[2] = {0, 0}; // row of the first
+        if (f.groups) {
+            const int tok = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
+            const int kvh = head / a.group;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            if (x && !f.prefix) continue;
-            const int2 w = f.where[(x ? c.tokens * a.group : 0) + tok * a.group + head % a.group];
-            const int p = w.y >> 6, r = w.y & 63;
-            // (offsets that decrease leave tokens that no item has: nothing past the slots is read)
-            if (w.x < 0 || p < 1 || r >= R || w.x >= f.slots || p > f.slots - w.x) continue;
-            n[x] = p;
-            slot[x] = (static_cast<int64_t>(w.x) * c.n_kv + kvh) * R + r;
+            for (int x = 0; x < 2; ++x) {
+                if (x && !f.prefix) continue;
+                const int2 w = f.where[(x ? c.tokens * a.group : 0) + tok * a.group + head % a.group];
+                const int p = w.y >> 6, r = w.y & 63;
+                // (offsets that decrease leave tokens that no item has: nothing past the slots is read)
+                if (w.x < 0 || p < 1 || r >= R || w.x >= f.slots || p > f.slots - w.x) continue;
+                n[x] = p;
+                slot[x] = (static_cast<int64_t>(w.x) * c.n_kv + kvh) * R + r;
+            }
+            if (f.direct && n[0] == 1) continue;  // written
         }
-        if (f.direct && n[0] == 1) return;  // written
-    }
-    const int few = n[0] + n[1], all = few + a.dense;
-    float m = -INFINITY, l = 0.f;
-    float4_t v = {0.f, 0.f, 0.f, 0.f};
-    for (int i0 = lane; i0 < all; i0 += 4 * LANES) {
-        float2 t[4];
-        float4_t o[4];
+        const int few = n[0] + n[1], all = few + a.dense;
+        float m = -INFINITY, l = 0.f;
+        float4_t v = {0.f, 0.f, 0.f, 0.f};
+        for (int i0 = lane; i0 < all; i0 += 4 * LANES) {
+            float2 t[4];
+            float4_t o[4];
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const int i = i0 + x * LANES;
-            t[x] = make_float2(-INFINITY, 0.f);
-            o[x] = (float4_t){0.f, 0.f, 0.f, 0.f};
-            if (i < all) {
-                const int64_t at = i < n[0] ? slot[0] + static_cast<int64_t>(i) * c.n_kv * R
-                                   : i < few ? slot[1] + static_cast<int64_t>(i - n[0]) * c.n_kv * R
-                                             : row * a.dense + i - few;
-                t[x] = (i < few ? f.part_ml : a.part_ml)[at];
-                o[x] = reinterpret_cast<const float4_t *>((i < few ? f.part_o : a.part_o) + at * D)[col];
+            for (int x = 0; x < 4; ++x) {
+                const int i = i0 + x * LANES;
+                t[x] = make_float2(-INFINITY, 0.f);
+                o[x] = (float4_t){0.f, 0.f, 0.f, 0.f};
+                if (i < all) {
+                    const int64_t at = i < n[0] ? slot[0] + static_cast<int64_t>(i) * c.n_kv * R
+                                       : i < few ? slot[1] + static_cast<int64_t>(i - n[0]) * c.n_kv * R
+                                                 : row * a.dense + i - few;
+                    t[x] = (i < few ? f.part_ml : a.part_ml)[at];
+                    o[x] = reinterpret_cast<const float4_t *>((i < few ? f.part_o : a.part_o) + at * D)[col];
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                if (t[x].x == -INFINITY) continue;
+                const float mn = fmaxf(m, t[x].x);
+                const float fo = __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(t[x].x - mn);
+                l = l * fo + t[x].y * fn;
+                v = v * fo + o[x] * fn;
+                m = mn;
             }
         }
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            if (t[x].x == -INFINITY) continue;
-            const float mn = fmaxf(m, t[x].x);
-            const float fo = __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(t[x].x - mn);
-            l = l * fo + t[x].y * fn;
-            v = v * fo + o[x] * fn;
-            m = mn;
+        s_o[lane][col] = v;
+        if (col == 0) {
+            s_m[lane] = m;
+            s_l[lane] = l;
         }
-    }
-    s_o[lane][col] = v;
-    if (col == 0) {
-        s_m[lane] = m;
-        s_l[lane] = l;
-    }
-    __syncthreads();
-    if (lane) return;
+        __syncthreads();
+        if (lane == 0) {
 #pragma unroll
-    for (int i = 0; i < LANES; ++i) m = fmaxf(m, s_m[i]);
-    l = 0.f;
-    v = (float4_t){0.f, 0.f, 0.f, 0.f};
+            for (int i = 0; i < LANES; ++i) m = fmaxf(m, s_m[i]);
+            l = 0.f;
+            v = (float4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < LANES; ++i) {
-        if (s_m[i] == -INFINITY) continue;
-        const float fi = __builtin_amdgcn_exp2f(s_m[i] - m);
-        l += s_l[i] * fi;
-        v += s_o[i][col] * fi;
+            for (int i = 0; i < LANES; ++i) {
+                if (s_m[i] == -INFINITY) continue;
+                const float fi = __builtin_amdgcn_exp2f(s_m[i] - m);
+                l += s_l[i] * fi;
+                v += s_o[i][col] * fi;
+            }
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            reinterpret_cast<u32x2_t *>(a.out + row * D)[col] =
+                (u32x2_t){pack2<DT>(v[0] * inv, v[1] * inv), pack2<DT>(v[2] * inv, v[3] * inv)};
+            if (a.lse && col == 0) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
+        }
+        __syncthreads();
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    reinterpret_cast<u32x2_t *>(a.out + row * D)[col] =
-        (u32x2_t){pack2<DT>(v[0] * inv, v[1] * inv), pack2<DT>(v[2] * inv, v[3] * inv)};
-    if (a.lse && col == 0) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // --------------------------------------------------------------------------------- host
@@ -1484,9 +1489,11 @@ int launch(const Cache &c, const Query &a, const Plan &p, hipStream_t s) {
 #undef NF4_BOTH
     const int st = status_of(hipGetLastError());
     if (st != NF4_OK || p.bytes == 0) return st;
-    const dim3 rows(static_cast<unsigned>(c.tokens * a.n_heads));
+    const int64_t rows = static_cast<int64_t>(c.tokens) * a.n_heads;
+    const dim3 joins(static_cast<unsigned>(rows < (1 << 20) ? rows : 1 << 20));
 #define NF4_JOIN(RB)                                                                                \
-    hipLaunchKernelGGL((paged_attn_join_kernel<DT, D, RB>), rows, dim3(kJoinThreads), 0, s, c, a, p.few)
+    hipLaunchKernelGGL((paged_attn_join_kernel<DT, D, RB>), joins, dim3(kJoinThreads), 0, s, c, a,   \
+                       p.few, rows)
     if (p.rb == 2) NF4_JOIN(2);
     else NF4_JOIN(1);
 #undef NF4_JOIN

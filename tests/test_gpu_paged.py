@@ -309,3 +309,92 @@ def test_other_stream_and_repeat(cuda):
         again = kernels.paged_attention(q, cache)
     stream.synchronize()
     assert torch.equal(first, again)
+
+
+# ---- many sequences, long tables, layouts that need 64-bit addresses
+
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("shared", [0, 40])
+def test_many_ragged_sequences(cuda, ragged, shared):
+    """More than two chunks of 64 sequences, of 0 to 1300 positions, cut into equal shares."""
+    from solution import kernels
+
+    banner("many sequences", ragged, shared)
+    g = torch.Generator().manual_seed(20)
+    lens = [shared + int(n) for n in torch.randint(0, 40, (131,), generator=g)]
+    lens[5], lens[70], lens[130], lens[64] = shared + 1300, shared + 700, shared + 333, shared
+    new = [1] * 131
+    if ragged:
+        for b in (0, 63, 64, 100):
+            new[b] = b % 3  # some bring nothing, one two tokens
+    s = ref.Setup(cuda, BF16, 4, 2, 64, 16, lens, new, seed=21, shared=shared)
+    kw = dict(max_q=max(new), max_len=max(lens)) if ragged else {}
+    _check(_run(kernels, s, cuda, shared=shared, cu_q=s.cu_d() if ragged else None, **kw),
+           ref.attention(s, shared=shared), BF16)
+
+
+@pytest.mark.parametrize("new,page", [(1, 16), (40, 16), (40, 8), (3, 32)])
+def test_table_of_many_pages(cuda, new, page):
+    """Lengths of several windows of 64 table entries, some entries missing, with and without a
+    window of keys that starts far behind the sinks."""
+    from solution import kernels
+
+    banner("many pages", new, page)
+    s = ref.Setup(cuda, F16, 2, 1, 64, page, [4100], [new], seed=22)
+    s.table[0, 70], s.table[0, 100:103] = -1, 1 << 22
+    for window, sinks in ((0, 0), (1500, 5)):
+        _check(_run(kernels, s, cuda, window, sinks, cu_q=s.cu_d(), max_q=new, max_len=4100),
+               ref.attention(s, window, sinks), F16)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_slots_far_apart(cuda, new):
+    """Slot-major caches: a page's slots lie further apart than 32-bit byte offsets reach."""
+    from solution import kernels
+
+    banner("slots far apart", new)
+    pages, page, kv, dim = 72000, 64, 4, 64
+    k = torch.empty((page, pages, kv, dim), dtype=F16, device=cuda).transpose(0, 1)
+    v = torch.empty((page, pages, kv, dim), dtype=F16, device=cuda).transpose(0, 1)
+    s = ref.Setup(cuda, F16, 8, kv, dim, page, [300, 90], [new, new], seed=23)
+    far = s.table.clone()
+    far[far >= 0] += pages - s.k.shape[0]
+    k[-s.k.shape[0]:], v[-s.k.shape[0]:] = s.k, s.v
+    cache = kernels.PagedKV(k, v, far.to(cuda), torch.tensor(s.lens, dtype=torch.int32, device=cuda))
+    _check(kernels.paged_attention(s.q.to(cuda), cache, lse=True), ref.attention(s), F16)
+
+
+def test_values_not_finite_that_some_rows_see(cuda):
+    """An infinity or NaN among the values reaches the rows that see its key, in that channel, and
+    no other row; few rows and many."""
+    from solution import kernels
+
+    for new in (3, 40):
+        banner("values not finite", new)
+        s = ref.Setup(cuda, F16, 4, 2, 64, 16, [100], [new], seed=24)
+        want = ref.attention(s)
+        j = 100 - new // 2 - 1  # a position in the middle of the new tokens
+        s.v[int(s.table[0, j // 16]), j % 16, 1, 7] = math.inf
+        o, l = _run(kernels, s, cuda)
+        p = torch.arange(100 - new, 100)
+        hit = torch.zeros(o.shape, dtype=torch.bool)
+        hit[p >= j, 2:, 7] = True
+        assert (o.cpu()[hit] == math.inf).all()
+        o = torch.where(hit.to(cuda), torch.zeros_like(o), o)
+        want[0][hit] = 0
+        _check((o, l), want, F16)
+
+
+def test_queries_that_are_nan(cuda):
+    """A query of NaN gives NaN (not the zeros of a query that sees nothing), pieces or not."""
+    from solution import kernels
+
+    for lens, new, shared in (([90], 1, 0), ([3000, 40], 1, 0), ([300], 40, 0), ([200, 190], 1, 150)):
+        banner("NaN queries", lens, new, shared)
+        s = ref.Setup(cuda, BF16, 4, 2, 64, 16, lens, [new] * len(lens), seed=25, shared=shared)
+        want = ref.attention(s, shared=shared)
+        s.q[-1, 1] = math.nan
+        o, l = _run(kernels, s, cuda, shared=shared)
+        assert o[-1, 1].isnan().all() and l[-1, 1].isnan()
+        o[-1, 1], l[-1, 1] = want[0][-1, 1].to(o), want[1][-1, 1].to(l)
+        _check((o, l), want, BF16)

@@ -106,3 +106,24 @@ def test_rope_table_far_positions():
     ang = 131072 * 1e6 ** (-torch.arange(32, dtype=torch.float64) / 32)
     assert (cos[-1].double() - ang.cos()).abs().max() < 1e-7
     assert (sin[-1].double() - ang.sin()).abs().max() < 1e-7
+
+
+def test_rows_past_32_bits_are_refused(lib):
+    """Tokens times heads stay under 2^30: what counts rows is 32 bits wide."""
+    kv = _kv(n_kv=1, batch=1)
+    assert _attn(lib, kv, tokens=1 << 21, heads=1024, ld=1 << 16, cu=1 << 12) == UNSUPPORTED
+    assert _attn(lib, kv, tokens=(1 << 23) + 1, heads=1, cu=1 << 12) == UNSUPPORTED
+
+
+@pytest.mark.parametrize("batch,width,max_len", [(1, 64, 500), (1, 1 << 16, 0), (64, 1000, 16000)])
+def test_workspace_is_bounded(lib, batch, width, max_len):
+    """Decoding: no workspace where a workgroup takes each sequence whole; else pieces of at most
+    one workgroup per CU and one per sequence, whatever the lengths."""
+    kv = _kv(batch=batch, width=width, ld_table=width)
+    n = lib.nf4_paged_attn_workspace(ctypes.byref(kv), None, batch, 4, 0, 0, 0, 1, max_len)
+    if max_len == 500:
+        assert n == 0
+    else:
+        # (workgroups of a key/value head + sequences) x 2 heads x 16 rows of 64 + 2 floats, and
+        # a pair for each of the rows
+        assert 0 < n <= (128 + 2 * batch) * 2 * 16 * (64 * 4 + 8) + batch * 2 * 8
