@@ -286,6 +286,11 @@ __device__ __forceinline__ int position_of(const Cache &c, int t) {
     return s.p0 + t - s.q0;
 }
 
+// The lowest n bits.
+__device__ __forceinline__ uint64_t below(int n) {
+    return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+
 // What a workgroup's rows (positions pmin .. pmax) see of a part: keys of [lo, hi) that are at
 // most at the row's position, and past its window's start or below `sinks`; tiles of 2^SH keys,
 // first those of the sinks, then those of the windows.
@@ -333,6 +338,18 @@ struct Range {
     __device__ __forceinline__ bool any(const Query &a, int j) const {
         return j >= lo && j < hi && (!a.window || pmin - a.window < j || j < a.sinks);
     }
+    // the keys of the tile at k that some row sees, and that the row at position p sees, as bits
+    // (a few instructions for a tile, where the tests below are a dozen for each key)
+    __device__ __forceinline__ uint64_t any_bits(const Query &a, int k) const {
+        uint64_t m = below(hi - k) & ~below(lo - k);
+        if (a.window) m &= ~below(pmin - k - a.window + 1) | below(a.sinks - k);
+        return m;
+    }
+    __device__ __forceinline__ uint64_t seen_bits(const Query &a, int p, int k) const {
+        uint64_t m = below((hi < p + 1 ? hi : p + 1) - k) & ~below(lo - k);
+        if (a.window) m &= ~below(p - k - a.window + 1) | below(a.sinks - k);
+        return m;
+    }
     // the row at position p sees key j
     __device__ __forceinline__ bool sees(const Query &a, int p, int j) const {
         return j >= lo && j < hi && j <= p && (!a.window || p - a.window < j || j < a.sinks);
@@ -344,6 +361,14 @@ template <int DT>
 __device__ __forceinline__ bool not_finite(uint32_t w) {
     constexpr uint32_t e = DT == NF4_BF16 ? 0x7f80u : 0x7c00u;
     return (w & e) == e || ((w >> 16) & e) == e;
+}
+
+// 0 where all 8 values of a chunk are finite, else NaN; added to `c`.
+template <int DT>
+__device__ __forceinline__ float odd_sum(const u32x4_t &r, float c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = dot2<DT>(r[i], 0, c);
+    return c;
 }
 
 template <int DT>
@@ -709,16 +734,20 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
             const bool full = rg.full(a, k) && ok == 0xffffffffu;
             bool odd = false;  // an infinity or NaN among values that not every row sees
             if (!full) {
+                const uint32_t any = static_cast<uint32_t>(rg.any_bits(a, k)) & ok;
+                float zero = 0.f;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const int key = (j >> 2) * 16 + g * 4 + (j & 3);
-                    if (!((ok >> key) & 1) || !rg.any(a, k + key)) vr[j] = (u32x4_t){0, 0, 0, 0};
+                    if (!(((any >> (g * 4)) >> ((j >> 2) * 16 + (j & 3))) & 1)) vr[j] = (u32x4_t){0, 0, 0, 0};
+                    zero = odd_sum<DT>(vr[j], zero);
+                }
+                odd = rg.pmin != rg.pmax && zero != 0.f;  // (rows of one token see the same keys)
 #pragma unroll
-                    for (int x = 0; x < VE / 2; ++x) odd |= not_finite<DT>(vr[j][x]);
+                for (int rb = 0; rb < RB; ++rb) {
+                    const uint32_t see = (static_cast<uint32_t>(rg.seen_bits(a, pos[rb], k)) & ok) >> (g * 4);
 #pragma unroll
-                    for (int rb = 0; rb < RB; ++rb)
-                        if (!((ok >> key) & 1) || !rg.sees(a, pos[rb], k + key))
-                            st[rb][j >> 2][j & 3] = -INFINITY;
+                    for (int j = 0; j < 8; ++j)
+                        if (!((see >> ((j >> 2) * 16 + (j & 3))) & 1)) st[rb][j >> 2][j & 3] = -INFINITY;
                 }
             }
             u32x4_t pf[RB];
@@ -1054,21 +1083,26 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
     // what this wave loaded of a tile that not every row sees whole: the values of keys that no
     // row sees become zeros; infinities and NaN too (0 times one is no 0), and s_odd says so
     auto clean = [&](int st, int i, int k, uint64_t ok) {
-        bool odd = false;
+        const uint64_t any = rg.any_bits(a, k) & ok;
+        u32x4_t v[PASS];
+        float zero = 0.f;
 #pragma unroll
         for (int x = 0; x < PASS; ++x) {
             const int row = x * RPP + srow;
             u32x4_t *p = reinterpret_cast<u32x4_t *>(s_v + st * STAGE + row * D * 2 + sch * 16);
-            u32x4_t v = *p;
-            if (!((ok >> row) & 1) || !rg.any(a, k + row)) v = (u32x4_t){0, 0, 0, 0};
-#pragma unroll
-            for (int z = 0; z < 4; ++z) {
-                odd |= not_finite<DT>(v[z]);
-                v[z] = finite_or_zero<DT>(v[z]);
-            }
-            *p = v;
+            v[x] = *p;
+            if (!((any >> row) & 1)) *p = v[x] = (u32x4_t){0, 0, 0, 0};
+            zero = odd_sum<DT>(v[x], zero);
         }
-        if (odd) s_odd[st] = i;
+        if (zero != 0.f) {
+#pragma unroll
+            for (int x = 0; x < PASS; ++x) {
+#pragma unroll
+                for (int z = 0; z < 4; ++z) v[x][z] = finite_or_zero<DT>(v[x][z]);
+                *reinterpret_cast<u32x4_t *>(s_v + st * STAGE + (x * RPP + srow) * D * 2 + sch * 16) = v[x];
+            }
+            s_odd[st] = i;
+        }
     };
 
     // ---- operand addresses of this lane
@@ -1128,13 +1162,14 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         read_v(1, vf[1]);
         __builtin_amdgcn_sched_barrier(0);
         if (!full) {
+            const uint64_t see = (rg.seen_bits(a, pos, k) & ok) >> (g * 4);
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
+            for (int h = 0; h < 2; ++h) {
+                const uint32_t half = static_cast<uint32_t>(see >> (h * 32));
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int key = h * 32 + (e >> 2) * 8 + g * 4 + (e & 3);
-                    if (!((ok >> key) & 1) || !rg.sees(a, pos, k + key)) sc[h][e] = -INFINITY;
-                }
+                for (int e = 0; e < 16; ++e)
+                    if (!((half >> ((e >> 2) * 8 + (e & 3))) & 1)) sc[h][e] = -INFINITY;
+            }
         }
         float top = sc[0][0];
 #pragma unroll
