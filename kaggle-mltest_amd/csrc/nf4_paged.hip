@@ -108,7 +108,8 @@ constexpr int kAppendThreads = 256;
 
 // One workgroup per token.  A thread takes 8 rotary pairs of a head (16 bytes of its low half
 // and 16 of its high half): lo' = lo cos - hi sin, hi' = hi cos + lo sin in fp32, each rounded
-// once; v heads are copied the same way.
+// once; v heads are copied the same way.  Bound by memory: 8081 tokens of 28 + 4 + 4 heads, 153 MB,
+// in 28.2 us (5.4 TB/s); a step of one token is its launch, 2.5 us.
 template <int DT>
 __global__ __launch_bounds__(kAppendThreads) void paged_append_kernel(
     const Cache c, const uint16_t *qkv, int64_t ld, const float *cs, const float *sn, int rope_rows,
@@ -536,6 +537,13 @@ __device__ __forceinline__ void next_units(Units &u, const Cache &c, const Query
 // and its values as soon as they are used, so that a wave always has loads in flight; the waves'
 // results meet in LDS.
 
+//
+// Bound by memory.  bf16, 4 heads of 128: 64 ragged sequences, 1.14 GB, in 199 us (5.7 TB/s, what
+// a plain read of this card reaches); 131071 keys of one, 268 MB, in 51.5 us (5.2 TB/s) and 5 us
+// for the join.  Up to kWholeKeys keys of a sequence it is latency: length, page entries, keys,
+// the sums over LDS, 9.4 us.  (SMALL: an address a lane, for pages under 16 slots and pages whose
+// slots span 2^31 bytes.)
+
 template <int DT, int D, int RB, bool SMALL, int W>
 __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const Few &f, int block,
                                          uint8_t *lds) {
@@ -896,12 +904,18 @@ __global__ __launch_bounds__(64 * W, 2) void paged_attn_few_kernel(
 
 // ------------------------------------------------------------------ many rows (prompts)
 //
-// 128 rows a workgroup, 32 a wave on v_mfma_f32_32x32x16, over 64-key tiles: K and V tiles go
-// through LDS, loaded into registers while the tile before is used (two LDS stages, one barrier
-// a tile).  16-byte chunk ch of K's row r lies at chunk ch ^ (r & 15) (128 channels; 64: ch ^
-// (r / 2 & 7)): the 16 lanes that LDS serves at a time then read 16 rows from 16 different bank
-// groups.  V is read transposed (ds_read_b64_tr_b16: 4 keys of a channel a lane) from rows whose
-// 64-byte blocks are exchanged by the key's low bits, 4 keys x 64 bytes on all banks.
+// 128 rows a workgroup, 32 a wave on v_mfma_f32_32x32x16, over 64-key tiles: K and V tiles go to
+// LDS by DMA while the tile before is used (two stages, one barrier a tile; two workgroups a CU).
+// 16-byte chunk ch of K's row r lies at chunk ch ^ (r & 15) (128 channels; 64: ch ^ (r / 2 & 7)):
+// the 16 lanes that LDS serves at a time then read 16 rows from 16 different bank groups.  V is
+// read transposed (ds_read_b64_tr_b16: 4 keys of a channel a lane) from rows whose 64-byte blocks
+// are exchanged by the key's low bits, 4 keys x 64 bytes on all banks.  No bank conflicts counted.
+//
+// 8192 new tokens, 28 heads of 128 over 4, bf16: 495-505 us, 950-970 TFLOP/s, where a library's
+// 8192^3 product reaches 1140.  The matrix pipe is in use 46 % of the cycles, and the clock falls
+// to 1.95 GHz under the load: the power cap bounds it.  Measured against it: the next tile's
+// scores formed beside this one's exponentials within a wave (fewer cycles, a lower clock: 495 us,
+// and 5-15 % slower with few tiles), the same with 256 rows a workgroup (510 us).
 
 typedef short v4i16_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16_t lds_v4i16_t;
@@ -1175,8 +1189,10 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
 #pragma unroll
         for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
         top = fmaxf(top, other_half(top)) * a.scale;
-        // m is a maximum of earlier tiles: probabilities up to 2^8 are let be (their sums are in
-        // fp32, their rounding is relative), so that few tiles rescale
+        // m is a maximum of earlier tiles: probabilities up to 2^8 are let be, so that few tiles
+        // rescale (a new maximum at every tile: 3-5 % slower).  Their sums are in fp32 and their
+        // rounding to 16 bits is relative; the largest one's, which is 1 with an exact maximum,
+        // then counts too: 2.2e-3 instead of 1.9e-3 of an output in bf16, whose own is 1.6e-3
         if (__any(top > m + 8.f)) {
             const float mn = fmaxf(m, top), alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
             sum *= alpha;
@@ -1271,8 +1287,11 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
     else tile_body<DT, D, SMALL>(c, a, own, block - pre.groups, lds);
 }
 
-// A prefix of many rows and few rows of each sequence in one launch, their workgroups in turn:
-// the first are bound by arithmetic, the second by memory.
+// A prefix of many rows and few rows of each sequence in one launch, their workgroups in turn, one
+// of each on a CU: the first are bound by arithmetic and latency, the second by memory.  128
+// sequences behind 16384 positions 78 us, the prefix alone as long; two launches 100 us and more
+// (of 8 sequences 26 us instead of 14), more and shorter pieces of the prefix 99 us: they wait for
+// the other part's workgroups.
 template <int DT, int D, int RB, bool SMALL>
 __global__ __launch_bounds__(256, 2) void paged_attn_both_kernel(const Cache c, const Query a,
                                                                  const Few f, const Part pre) {
@@ -1291,7 +1310,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_both_kernel(const Cache c, 
 // kJoinThreads / (D / 4)-th piece, the threads of a channel meet in LDS in order: few rows of many
 // pieces (one long sequence) are bound by the latency of their loads, which one thread a channel
 // took one piece at a time (342 pieces of 28 rows: 120 us).
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinShift = 20;  // rows of a grid's first dimension: 2^20
 
 template <int DT, int D, int RB>
 __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Cache c, const Query a,
@@ -1300,78 +1319,76 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Cac
     __shared__ float4_t s_o[LANES][COLS];
     __shared__ float s_m[LANES], s_l[LANES];
     const int col = threadIdx.x % COLS, lane = threadIdx.x / COLS;
-    for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
-        int n[2] = {0, 0};        // pieces of few rows: of the sequence's item and of the prefix's
-        int64_t slot[2] = {0, 0}; // row of the first
-        if (f.groups) {
-            const int tok = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
-            const int kvh = head / a.group;
+    const int64_t row = blockIdx.x + (static_cast<int64_t>(blockIdx.y) << kJoinShift);
+    if (row >= rows) return;
+    int n[2] = {0, 0};        // pieces of few rows: of the sequence's item and of the prefix's
+    int64_t slot[2] = {0, 0}; // row of the first
+    if (f.groups) {
+        const int tok = static_cast<int>(row / a.n_heads), head = static_cast<int>(row % a.n_heads);
+        const int kvh = head / a.group;
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                if (x && !f.prefix) continue;
-                const int2 w = f.where[(x ? c.tokens * a.group : 0) + tok * a.group + head % a.group];
-                const int p = w.y >> 6, r = w.y & 63;
-                // (offsets that decrease leave tokens that no item has: nothing past the slots is read)
-                if (w.x < 0 || p < 1 || r >= R || w.x >= f.slots || p > f.slots - w.x) continue;
-                n[x] = p;
-                slot[x] = (static_cast<int64_t>(w.x) * c.n_kv + kvh) * R + r;
-            }
-            if (f.direct && n[0] == 1) continue;  // written
+        for (int x = 0; x < 2; ++x) {
+            if (x && !f.prefix) continue;
+            const int2 w = f.where[(x ? c.tokens * a.group : 0) + tok * a.group + head % a.group];
+            const int p = w.y >> 6, r = w.y & 63;
+            // (offsets that decrease leave tokens that no item has: nothing past the slots is read)
+            if (w.x < 0 || p < 1 || r >= R || w.x >= f.slots || p > f.slots - w.x) continue;
+            n[x] = p;
+            slot[x] = (static_cast<int64_t>(w.x) * c.n_kv + kvh) * R + r;
         }
-        const int few = n[0] + n[1], all = few + a.dense;
-        float m = -INFINITY, l = 0.f;
-        float4_t v = {0.f, 0.f, 0.f, 0.f};
-        for (int i0 = lane; i0 < all; i0 += 4 * LANES) {
-            float2 t[4];
-            float4_t o[4];
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                const int i = i0 + x * LANES;
-                t[x] = make_float2(-INFINITY, 0.f);
-                o[x] = (float4_t){0.f, 0.f, 0.f, 0.f};
-                if (i < all) {
-                    const int64_t at = i < n[0] ? slot[0] + static_cast<int64_t>(i) * c.n_kv * R
-                                       : i < few ? slot[1] + static_cast<int64_t>(i - n[0]) * c.n_kv * R
-                                                 : row * a.dense + i - few;
-                    t[x] = (i < few ? f.part_ml : a.part_ml)[at];
-                    o[x] = reinterpret_cast<const float4_t *>((i < few ? f.part_o : a.part_o) + at * D)[col];
-                }
-            }
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                if (t[x].x == -INFINITY) continue;
-                const float mn = fmaxf(m, t[x].x);
-                const float fo = __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(t[x].x - mn);
-                l = l * fo + t[x].y * fn;
-                v = v * fo + o[x] * fn;
-                m = mn;
-            }
-        }
-        s_o[lane][col] = v;
-        if (col == 0) {
-            s_m[lane] = m;
-            s_l[lane] = l;
-        }
-        __syncthreads();
-        if (lane == 0) {
-#pragma unroll
-            for (int i = 0; i < LANES; ++i) m = fmaxf(m, s_m[i]);
-            l = 0.f;
-            v = (float4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-            for (int i = 0; i < LANES; ++i) {
-                if (s_m[i] == -INFINITY) continue;
-                const float fi = __builtin_amdgcn_exp2f(s_m[i] - m);
-                l += s_l[i] * fi;
-                v += s_o[i][col] * fi;
-            }
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            reinterpret_cast<u32x2_t *>(a.out + row * D)[col] =
-                (u32x2_t){pack2<DT>(v[0] * inv, v[1] * inv), pack2<DT>(v[2] * inv, v[3] * inv)};
-            if (a.lse && col == 0) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
-        }
-        __syncthreads();
+        if (f.direct && n[0] == 1) return;  // written
     }
+    const int few = n[0] + n[1], all = few + a.dense;
+    float m = -INFINITY, l = 0.f;
+    float4_t v = {0.f, 0.f, 0.f, 0.f};
+    for (int i0 = lane; i0 < all; i0 += 4 * LANES) {
+        float2 t[4];
+        float4_t o[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const int i = i0 + x * LANES;
+            t[x] = make_float2(-INFINITY, 0.f);
+            o[x] = (float4_t){0.f, 0.f, 0.f, 0.f};
+            if (i < all) {
+                const int64_t at = i < n[0] ? slot[0] + static_cast<int64_t>(i) * c.n_kv * R
+                                   : i < few ? slot[1] + static_cast<int64_t>(i - n[0]) * c.n_kv * R
+                                             : row * a.dense + i - few;
+                t[x] = (i < few ? f.part_ml : a.part_ml)[at];
+                o[x] = reinterpret_cast<const float4_t *>((i < few ? f.part_o : a.part_o) + at * D)[col];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            if (t[x].x == -INFINITY) continue;
+            const float mn = fmaxf(m, t[x].x);
+            const float fo = __builtin_amdgcn_exp2f(m - mn), fn = __builtin_amdgcn_exp2f(t[x].x - mn);
+            l = l * fo + t[x].y * fn;
+            v = v * fo + o[x] * fn;
+            m = mn;
+        }
+    }
+    s_o[lane][col] = v;
+    if (col == 0) {
+        s_m[lane] = m;
+        s_l[lane] = l;
+    }
+    __syncthreads();
+    if (lane) return;
+#pragma unroll
+    for (int i = 0; i < LANES; ++i) m = fmaxf(m, s_m[i]);
+    l = 0.f;
+    v = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < LANES; ++i) {
+        if (s_m[i] == -INFINITY) continue;
+        const float fi = __builtin_amdgcn_exp2f(s_m[i] - m);
+        l += s_l[i] * fi;
+        v += s_o[i][col] * fi;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    reinterpret_cast<u32x2_t *>(a.out + row * D)[col] =
+        (u32x2_t){pack2<DT>(v[0] * inv, v[1] * inv), pack2<DT>(v[2] * inv, v[3] * inv)};
+    if (a.lse && col == 0) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 
 // --------------------------------------------------------------------------------- host
@@ -1525,7 +1542,8 @@ int launch(const Cache &c, const Query &a, const Plan &p, hipStream_t s) {
     const int st = status_of(hipGetLastError());
     if (st != NF4_OK || p.bytes == 0) return st;
     const int64_t rows = static_cast<int64_t>(c.tokens) * a.n_heads;
-    const dim3 joins(static_cast<unsigned>(rows < (1 << 20) ? rows : 1 << 20));
+    const dim3 joins(static_cast<unsigned>(rows < (1 << kJoinShift) ? rows : 1 << kJoinShift),
+                     static_cast<unsigned>((rows + (1 << kJoinShift) - 1) >> kJoinShift));
 #define NF4_JOIN(RB)                                                                                \
     hipLaunchKernelGGL((paged_attn_join_kernel<DT, D, RB>), joins, dim3(kJoinThreads), 0, s, c, a,   \
                        p.few, rows)
