@@ -422,7 +422,8 @@ int nf4_qkv_rope_bwd(const void *dq, const void *dk, const void *dv, const float
  * head_dim values consecutive.  A table entry outside [0, pages) names no page: appends to it
  * are dropped and its keys are not seen.  lens[b] is the sequence's length with the call's own
  * tokens.  page_size is a power of two, head_dim 64 or 128, the strides multiples of 8 and k, v
- * 16-byte aligned; width * page_size at most 2^30. */
+ * 16-byte aligned; width * page_size at most 2^30, a call's
+ * tokens 2^23 and tokens times n_heads 2^30. */
 typedef struct nf4_paged_kv {
     void *k;
     void *v;
