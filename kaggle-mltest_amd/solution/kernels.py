@@ -675,7 +675,10 @@ class PagedKV:
         _check_device(k_pages, v_pages, table, lens)
         if k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.dtype != v_pages.dtype:
             raise ValueError("k_pages and v_pages are [pages, page_size, n_kv, head_dim] of one dtype")
-        if k_pages.stride() != v_pages.stride() or k_pages.stride(3) != 1:
+        # (a dimension of size one has no stride that matters)
+        strides, v_strides = ([st if n > 1 else 0 for n, st in zip(t.shape, t.stride())]
+                              for t in (k_pages, v_pages))
+        if strides != v_strides or k_pages.stride(3) != 1:
             raise ValueError("k_pages and v_pages share their strides, head_dim contiguous")
         if table.dim() != 2 or table.dtype != torch.int32 or table.stride(1) != 1:
             raise ValueError("table is an int32 [batch, width] tensor with contiguous rows")
@@ -690,18 +693,18 @@ class PagedKV:
         pages, self.page_size, self.n_kv, self.head_dim = (int(d) for d in k_pages.shape)
         ld_table = max(int(table.stride(0)), self.width)  # one row's stride says nothing
         self.desc = NF4PagedKV(
-            k_pages.data_ptr(), v_pages.data_ptr(), k_pages.stride(0), k_pages.stride(1),
-            k_pages.stride(2), table.data_ptr(), ld_table, lens.data_ptr(), pages,
+            k_pages.data_ptr(), v_pages.data_ptr(), *strides[:3], table.data_ptr(), ld_table, lens.data_ptr(), pages,
             self.page_size, self.width, self.batch, self.n_kv, self.head_dim)
         self.ref = ctypes.byref(self.desc)
+        self.index = k_pages.get_device()
 
 
 def _check_cu(cu_q, cache: PagedKV):
     if cu_q is None:
         return None
-    if not cu_q.is_cuda or cu_q.dtype != torch.int32 or tuple(cu_q.shape) != (cache.batch + 1,) \
-            or not cu_q.is_contiguous():
-        raise ValueError("cu_q is a contiguous int32 [batch + 1] device tensor")
+    if cu_q.get_device() != cache.index or cu_q.dtype != torch.int32 \
+            or tuple(cu_q.shape) != (cache.batch + 1,) or not cu_q.is_contiguous():
+        raise ValueError("cu_q is a contiguous int32 [batch + 1] tensor on the cache's device")
     return cu_q.data_ptr()
 
 
@@ -716,8 +719,8 @@ def paged_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, cache:
     if qkv.dim() != 2 or qkv.dtype != cache.dtype or qkv.stride(1) != 1:
         raise ValueError("qkv is a row-contiguous [tokens, (n_heads + 2 n_kv) head_dim] tensor of "
                          "the cache's dtype")
-    if not (qkv.is_cuda and cos.is_cuda and sin.is_cuda):
-        _check_device(qkv, cos, sin)
+    if not qkv.get_device() == cos.get_device() == sin.get_device() == cache.index:
+        raise ValueError("qkv, cos and sin are on the cache's device")
     tokens, cols = qkv.shape
     heads = cols // dim - 2 * kv
     if heads < 1 or heads % kv or cols % dim:
@@ -749,8 +752,8 @@ def _check_out(out, shape, like):
 def _attention(q, cache, shared, cu_q, scale, window, sinks, max_q, max_len, out, lse):
     if q.dim() != 3 or q.dtype != cache.dtype or q.shape[2] != cache.head_dim or q.stride(2) != 1:
         raise ValueError("q is [tokens, n_heads, head_dim] of the cache's dtype, head_dim contiguous")
-    if not q.is_cuda:
-        _check_device(q)
+    if q.get_device() != cache.index:
+        raise ValueError("q is on the cache's device")
     tokens, heads, dim = q.shape
     if heads < 1 or heads % cache.n_kv:
         raise ValueError("n_heads is a multiple of the cache's n_kv")
@@ -765,8 +768,9 @@ def _attention(q, cache, shared, cu_q, scale, window, sinks, max_q, max_len, out
     nbytes = lib.nf4_paged_attn_workspace(cache.ref, cu, tokens, heads, window, sinks, shared,
                                           max_q, max_len)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    st = lib.nf4_paged_attn(cache.ref, q.data_ptr(), q.stride(0), q.stride(1), cu, out.data_ptr(),
-                            _p(stats), tokens, heads, dim ** -0.5 if scale is None else scale,
+    st = lib.nf4_paged_attn(cache.ref, q.data_ptr(), q.stride(0) if tokens > 1 else 0,
+                            q.stride(1) if heads > 1 else 0, cu, out.data_ptr(), _p(stats),
+                            tokens, heads, dim ** -0.5 if scale is None else scale,
                             window, sinks, shared, max_q, max_len, cache.code, _p(ws), nbytes,
                             stream_of(q))
     if st:

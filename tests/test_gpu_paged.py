@@ -398,3 +398,57 @@ def test_queries_that_are_nan(cuda):
         assert o[-1, 1].isnan().all() and l[-1, 1].isnan()
         o[-1, 1], l[-1, 1] = want[0][-1, 1].to(o), want[1][-1, 1].to(l)
         _check((o, l), want, BF16)
+
+
+def test_strides_of_single_rows(cuda):
+    """A dimension of size one may have any stride: one token cut out of rows of an odd width, one
+    page, one key/value head."""
+    from solution import kernels
+
+    banner("single rows")
+    s = ref.Setup(cuda, F16, 2, 1, 64, 16, [11], [1], seed=26)
+    wide = torch.full((2, 2 * 64 + 9), math.nan, dtype=F16, device=cuda)
+    wide[0, :128] = s.q.view(-1).to(cuda)
+    page = int(s.table[0, 0])
+    k, v = (torch.as_strided(x[page].contiguous(), (1, 16, 1, 64), (n, 64, n, 1))
+            for x, n in ((s.k, 5), (s.v, 3)))
+    cache = kernels.PagedKV(k, v, torch.zeros(1, 1, dtype=torch.int32, device=cuda),
+                            torch.tensor([11], dtype=torch.int32, device=cuda))
+    q = torch.as_strided(wide, (1, 2, 64), (137, 64, 1))
+    _check(kernels.paged_attention(q, cache, lse=True), ref.attention(s), F16)
+
+
+def test_refusals(cuda):
+    """What the calls refuse, before any launch."""
+    from solution import _lib, kernels
+
+    s = ref.Setup(cuda, F16, 4, 2, 64, 16, [20], [1], seed=27)
+    cache, q = s.cache(kernels), s.q.to(cuda)
+    cos, sin = (t.to(cuda) for t in _table(32, 64))
+    qkv = s.qkv.to(cuda)
+    bad_calls = [
+        lambda: kernels.paged_attention(s.q, cache),                          # host memory
+        lambda: kernels.paged_attention(q.float(), cache),
+        lambda: kernels.paged_attention(q[:, :3], cache),                     # heads % n_kv
+        lambda: kernels.paged_attention(q[..., :32], cache),
+        lambda: kernels.paged_attention(q, cache, cu_q=s.cu),                 # host offsets
+        lambda: kernels.paged_attention(q, cache, cu_q=s.cu_d().long()),
+        lambda: kernels.paged_attention(q, cache, out=torch.empty_like(q)[:, :2]),
+        lambda: kernels.paged_append(s.qkv, cos, sin, cache),
+        lambda: kernels.paged_append(qkv[:, :-64], cos, sin, cache),
+        lambda: kernels.paged_append(qkv, cos[:, :16], sin, cache),
+        lambda: kernels.paged_append(qkv, cos.double(), sin, cache),
+        lambda: kernels.PagedKV(s.k, s.v[..., :32], cache.table, cache.lens),
+        lambda: kernels.PagedKV(s.k, s.v, cache.table.long(), cache.lens),
+        lambda: kernels.PagedKV(s.k, s.v, cache.table, cache.lens.cpu()),
+    ]
+    for call in bad_calls:
+        with pytest.raises(ValueError):
+            call()
+    for kw in (dict(window=-1), dict(sinks=-1), dict(max_len=-1)):
+        with pytest.raises(_lib.NF4LibraryError):
+            kernels.paged_attention(q, cache, **kw)
+    with pytest.raises(_lib.NF4Unsupported):  # rows of an odd width
+        wide = torch.zeros(2, 4 * 64 + 3, dtype=F16, device=cuda)
+        kernels.paged_attention(wide[:, :256].unflatten(1, (4, 64)), kernels.PagedKV(
+            s.k, s.v, cache.table.repeat(2, 1), cache.lens.repeat(2)))
