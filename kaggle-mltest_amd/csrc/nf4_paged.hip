@@ -1449,17 +1449,29 @@ struct Plan {
 // Sequences whose rows are few go to the kernel without LDS staging.  Its launch is a workgroup
 // on every CU (kFewSlots): 64 KB in flight on each are enough for the memory's rate, and more
 // workgroups mean shorter shares and more pieces (131071 keys, 64 ragged sequences: 512
-// workgroups 63.5 and 215 us, 256 60.6 and 212.7).  Where no sequence is longer than kWholeKeys and all of them fit
-// the card, a workgroup of 8 waves takes a whole sequence, and there is nothing to join.  Tiled
-// parts are cut until the launch has kTileSlots workgroups.
+// workgroups 63.5 and 215 us, 256 60.6 and 212.7).  Where no sequence is longer than kWholeKeys
+// and all of them fit the card, a workgroup of 8 waves takes a whole sequence, and there is nothing
+// to join.  Tiled parts are cut until the launch has kTileSlots workgroups.
 constexpr int kFewRows = 32, kFewSlots = 256, kTileSlots = 512, kWholeKeys = 1024;
 
-Part tile_part(bool prefix, int64_t blocks, int n_kv, int64_t keys, int slots) {
+// `rows` > 0: cutting the part is what makes a join of that many rows necessary.  A tile takes
+// 2 us, a join 4 us and 0.15 ns for each row and each of its pieces (written and read): 6 chunks of
+// 143 to 431 tokens in windows of 210 go from 34 us in 3 pieces to 18 in one, 2 chunks of 21 to 65
+// tokens behind 1500 stay at 16 us in 25 (20 in 6).
+Part tile_part(bool prefix, int64_t rows, int64_t blocks, int n_kv, int64_t keys, int slots) {
     Part p{};
     const int tiles = ceil_div(keys, 64) + 1;
     const int64_t groups = blocks * n_kv;
-    int64_t splits = slots / (groups ? groups : 1);
-    splits = splits < 1 ? 1 : splits > tiles ? tiles : splits;
+    int64_t most = slots / (groups ? groups : 1), splits = 1;
+    most = most < 1 ? 1 : most > tiles ? tiles : most;
+    double best = 2.0 * tiles;
+    for (int64_t n = most; n > 1; n /= 2) {
+        const double t = 2.0 * ceil_div(tiles, n) + (rows ? 4.0 + 1.5e-4 * rows * (n + 2) : 0.0);
+        if (t < best) {
+            best = t;
+            splits = n;
+        }
+    }
     p.prefix = prefix ? 1 : 0;
     p.min_tiles = ceil_div(tiles, splits);
     p.splits = ceil_div(tiles, p.min_tiles);
@@ -1502,10 +1514,12 @@ Plan make_plan(const Cache &c, int n_heads, int window, int sinks, int shared, i
     } else {
         const int64_t blocks = c.cu ? all_rows / kRows + seqs
                                     : static_cast<int64_t>(c.batch) * ceil_div(longest * group, kRows);
-        p.own = tile_part(false, blocks, c.n_kv, span, kTileSlots);
+        // (a row block's window, not all of a sequence's)
+        const int64_t seen = static_cast<int64_t>(window) + kRows / group + 1 + sinks;
+        p.own = tile_part(false, shared ? 0 : static_cast<int64_t>(c.tokens) * n_heads, blocks, c.n_kv, window && seen < span ? seen : span, kTileSlots);
     }
     if (shared && !few_pre)
-        p.pre = tile_part(true, ceil_div(all_rows, kRows), c.n_kv, pre_keys,
+        p.pre = tile_part(true, 0, ceil_div(all_rows, kRows), c.n_kv, pre_keys,
                           few_own ? kTileSlots / 2 : kTileSlots);
     p.own.first = p.pre.groups ? p.pre.splits : 0;
     p.dense = p.own.first + (p.own.groups ? p.own.splits : 0);
