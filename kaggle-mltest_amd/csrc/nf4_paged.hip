@@ -896,7 +896,7 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
 }
 
 template <int DT, int D, int RB, bool SMALL, int W>
-__global__ __launch_bounds__(64 * W, 2) void paged_attn_few_kernel(
+__global__ __launch_bounds__(64 * W, RB > 2 ? 1 : 2) void paged_attn_few_kernel(
     const Cache c, const Query a, const Few f) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[few_lds<D>(W, RB)];
     few_body<DT, D, RB, SMALL, W>(c, a, f, blockIdx.x, lds);
@@ -1446,13 +1446,16 @@ struct Plan {
     size_t bytes;
 };
 
-// Sequences whose rows are few go to the kernel without LDS staging.  Its launch is a workgroup
+// Sequences whose rows are few go to the kernel without LDS staging: up to 32, and up to 48 over
+// long contexts, where equal shares count more than a third row block costs (35 rows of 64
+// sequences: of 40 to 16000 keys 232 us, tiled 298; in windows of 1024 58, tiled 44; a prefix of
+// 2001 positions before 48 rows 22 us, tiled 15).  Its launch is a workgroup
 // on every CU (kFewSlots): 64 KB in flight on each are enough for the memory's rate, and more
 // workgroups mean shorter shares and more pieces (131071 keys, 64 ragged sequences: 512
 // workgroups 63.5 and 215 us, 256 60.6 and 212.7).  Where no sequence is longer than kWholeKeys
 // and all of them fit the card, a workgroup of 8 waves takes a whole sequence, and there is nothing
 // to join.  Tiled parts are cut until the launch has kTileSlots workgroups.
-constexpr int kFewRows = 32, kFewSlots = 256, kTileSlots = 512, kWholeKeys = 1024;
+constexpr int kFewRows = 32, kFewRowsLong = 48, kLongKeys = 4096, kFewSlots = 256, kTileSlots = 512, kWholeKeys = 1024;
 
 // `rows` > 0: cutting the part is what makes a join of that many rows necessary.  A tile takes
 // 2 us, a join 4 us and 0.15 ns for each row and each of its pieces (written and read): 6 chunks of
@@ -1489,11 +1492,13 @@ Plan make_plan(const Cache &c, int n_heads, int window, int sinks, int shared, i
     if (window && span > static_cast<int64_t>(window) + longest + sinks) span = window + longest + sinks;
     const int64_t pre_keys = len < shared ? len : shared;
     const int seqs = c.batch + (c.cu ? 1 : 0);  // with offsets: and the tokens past the last
-    const bool few_own = longest * group <= kFewRows, few_pre = shared && all_rows <= kFewRows;
+    const bool few_pre = shared && all_rows <= kFewRows;
+    const bool few_own = longest * group <= (!shared && span > kLongKeys ? kFewRowsLong : kFewRows);
     Plan p{};
     if (few_own) {
         Few &f = p.few;
-        p.rb = (few_pre ? all_rows : longest * group) <= 16 ? 1 : 2;
+        const int64_t rows = few_pre ? all_rows : longest * group;
+        p.rb = rows <= 16 ? 1 : rows <= 32 ? 2 : 3;
         f.seqs = seqs;
         f.prefix = few_pre ? 1 : 0;
         f.direct = shared ? 0 : 1;
@@ -1550,7 +1555,8 @@ int launch(const Cache &c, const Query &a, const Plan &p, hipStream_t s) {
         else NF4_BOTH(2);
     else if (p.few.whole) NF4_FEW(1, 8);
     else if (p.rb == 1) NF4_FEW(1, 4);
-    else NF4_FEW(2, 4);
+    else if (p.rb == 2) NF4_FEW(2, 4);
+    else NF4_FEW(3, 4);
 #undef NF4_FEW
 #undef NF4_BOTH
     const int st = status_of(hipGetLastError());
@@ -1561,7 +1567,8 @@ int launch(const Cache &c, const Query &a, const Plan &p, hipStream_t s) {
 #define NF4_JOIN(RB)                                                                                \
     hipLaunchKernelGGL((paged_attn_join_kernel<DT, D, RB>), joins, dim3(kJoinThreads), 0, s, c, a,   \
                        p.few, rows)
-    if (p.rb == 2) NF4_JOIN(2);
+    if (p.rb == 3) NF4_JOIN(3);
+    else if (p.rb == 2) NF4_JOIN(2);
     else NF4_JOIN(1);
 #undef NF4_JOIN
     return status_of(hipGetLastError());

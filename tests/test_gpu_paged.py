@@ -452,3 +452,17 @@ def test_refusals(cuda):
         wide = torch.zeros(2, 4 * 64 + 3, dtype=F16, device=cuda)
         kernels.paged_attention(wide[:, :256].unflatten(1, (4, 64)), kernels.PagedKV(
             s.k, s.v, cache.table.repeat(2, 1), cache.lens.repeat(2)))
+
+
+@pytest.mark.parametrize("heads,kv,new", [(7, 1, 5), (12, 1, 4), (6, 1, 7)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_three_row_blocks(cuda, heads, kv, new, dim):
+    """33 to 48 rows a sequence over tables long enough for the kernel of few rows, ragged, with a
+    window and without."""
+    from solution import kernels
+
+    banner("three row blocks", heads, kv, new, dim)
+    s = ref.Setup(cuda, F16, heads, kv, dim, 16, [700, 90, new, 300], [new] * 4, seed=28,
+                  extra_width=300)
+    for window, sinks in ((0, 0), (4200, 3)):
+        _check(_run(kernels, s, cuda, window, sinks), ref.attention(s, window, sinks), F16)
