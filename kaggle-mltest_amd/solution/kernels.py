@@ -691,7 +691,11 @@ class PagedKV:
         self.dtype, self.code = k_pages.dtype, _code(k_pages.dtype)
         self.batch, self.width = (int(d) for d in table.shape)
         pages, self.page_size, self.n_kv, self.head_dim = (int(d) for d in k_pages.shape)
-        ld_table = max(int(table.stride(0)), self.width)  # one row's stride says nothing
+        # (one row's stride says nothing; rows that overlap are no rows of `width` entries)
+        ld_table = int(table.stride(0)) if self.batch > 1 else self.width
+        if ld_table < self.width:
+            raise ValueError("the table's rows are at least its width apart (a row that all sequences "
+                             "share is copied for each: row.repeat(batch, 1))")
         self.desc = NF4PagedKV(
             k_pages.data_ptr(), v_pages.data_ptr(), *strides[:3], table.data_ptr(), ld_table, lens.data_ptr(), pages,
             self.page_size, self.width, self.batch, self.n_kv, self.head_dim)
