@@ -820,11 +820,13 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
 #pragma unroll 1
             for (i = rg.i0 + w; i < rg.i1; i += W) {
                 k = rg.key0(i);
+                // (full slabs, as above: their products have them already)
+                if (rg.full(a, k) && !~__ballot(good(tab[(k + (l & 31)) >> c.page_shift]))) continue;
 #pragma unroll 1
                 for (int key = k; key < k + 32; ++key) {
                     if (!rg.any(a, key)) continue;
                     const int e = sload(tab + (key >> c.page_shift));
-                    if (!good(e) || rg.full(a, k)) continue;
+                    if (!good(e)) continue;
                     const uint16_t *p = vb + e * c.page_stride + (key & page_mask) * c.slot_stride;
 #pragma unroll
                     for (int x = 0; x < 4; ++x)
@@ -1231,7 +1233,7 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
 #pragma unroll 1
         for (int i = rg.i0; i < rg.i1; ++i) {
             k = rg.key0(i);
-            if (rg.full(a, k)) continue;
+            if (rg.full(a, k) && !~__ballot(good(tab[(k + l) >> c.page_shift]))) continue;
 #pragma unroll 1
             for (int key = k; key < k + 64; ++key) {
                 if (!rg.any(a, key)) continue;

@@ -1,0 +1,62 @@
+"""The paged-cache operators where numbers are at the ends of their ranges: infinities beside
+missing pages, scores of any size, weights far below a row's largest, scales of nothing, values
+at the type's end, more output rows than a grid's first dimension."""
+
+import math
+
+import pytest
+import torch
+
+from tests import paged_ref as ref
+from tests.gpu_util import banner
+from tests.test_gpu_paged import _check, _run
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+EPS = ref.EPS
+
+
+def _one(cuda, k, v, q, page=16, prefix=0, batch=1):
+    """A Setup of `batch` sequences over the same keys k, values v [positions, dim] of one
+    key/value head (float64), queries q [tokens, heads, dim] the last tokens of each; the first
+    `prefix` positions' whole pages are shared."""
+    s = ref.Setup(cuda, q.dtype, q.shape[1], 1, q.shape[2], page, [k.shape[0]] * batch,
+                  [q.shape[0] // batch] * batch, shared=prefix)
+    j = torch.arange(k.shape[0])
+    for b in range(batch):
+        at = s.table[b].long()[j // page].to(cuda)
+        s.k[at, (j % page).to(cuda), 0] = k.to(s.k)
+        s.v[at, (j % page).to(cuda), 0] = v.to(s.v)
+    s.q = q
+    return s
+
+
+@pytest.mark.parametrize("new,page,shared", [(3, 16, 0), (40, 16, 0), (3, 8, 0), (40, 32, 0),
+                                             (40, 8, 0), (3, 16, 96), (40, 16, 96)])
+@pytest.mark.parametrize("bad", [math.inf, -math.inf, math.nan])
+def test_values_not_finite_beside_a_missing_page(cuda, new, page, shared, bad):
+    """A table entry that names no page next to the page of an infinity or NaN, all of them before
+    the new tokens: every row sees the value, in its channel and its key/value head, and nothing
+    else changes."""
+    from solution import kernels
+
+    banner("not finite beside a missing page", new, page, shared, bad)
+    lens = [200, 210]
+    s = ref.Setup(cuda, F16, 4, 2, 64, page, lens, [new] * 2, seed=30, shared=shared)
+    if shared:
+        s.table[:, 32 // page] = -1
+    else:
+        s.table[0, 32 // page] = s.table[1, 32 // page] = -1
+    want = ref.attention(s, shared=shared)
+    j = 32 + page + 1 if page < 32 else 17  # in the slab of 32 keys, or tile of 64, of the missing page
+    for b in range(2):
+        s.v[int(s.table[b, j // page]), j % page, 1, 7] = bad
+    o, l = _run(kernels, s, cuda, shared=shared)
+    hit = torch.zeros(o.shape, dtype=torch.bool)
+    hit[:, 2:, 7] = True
+    got = o.cpu()[hit]
+    assert got.isnan().all() if math.isnan(bad) else (got == bad).all()
+    o = torch.where(hit.to(cuda), torch.zeros_like(o), o)
+    want[0][hit] = 0
+    _check((o, l), want, F16)
