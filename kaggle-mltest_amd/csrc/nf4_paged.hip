@@ -1190,13 +1190,11 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         float top = sc[0][0];
 #pragma unroll
         for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
-        top = fmaxf(top, other_half(top)) * a.scale;
-        // m is a maximum of earlier tiles: probabilities up to 2^8 are let be, so that few tiles
-        // rescale (a new maximum at every tile: 3-5 % slower).  Their sums are in fp32 and their
-        // rounding to 16 bits is relative; the largest one's, which is 1 with an exact maximum,
-        // then counts too: 2.2e-3 instead of 1.9e-3 of an output in bf16, whose own is 1.6e-3
-        if (__any(top > m + 8.f)) {
-            const float mn = fmaxf(m, top), alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+        // (a maximum that may be 2^8 behind rescales less often, 3-5 % faster for prompts, but then
+        // the largest probability is rounded too: 2.2e-3 instead of 1.9e-3 of an output in bf16)
+        const float mn = fmaxf(m, fmaxf(top, other_half(top)) * a.scale);
+        if (__any(mn > m)) {
+            const float alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
             sum *= alpha;
 #pragma unroll
             for (int x = 0; x < DT32; ++x) acc[x] *= alpha;

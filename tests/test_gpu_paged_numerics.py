@@ -60,3 +60,33 @@ def test_values_not_finite_beside_a_missing_page(cuda, new, page, shared, bad):
     o = torch.where(hit.to(cuda), torch.zeros_like(o), o)
     want[0][hit] = 0
     _check((o, l), want, F16)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,prefix", [(1, 0), (40, 0), (40, 192)])
+def test_largest_weight_is_exact(cuda, dtype, new, prefix):
+    """One key ahead of the rest by 1 to 5, behind others that a running maximum met first, and the
+    only one whose value is not 0.  Its weight is 2^0 over an unrounded sum, so what is off is the
+    output's rounding, and 1e-4 for fp32's scores, exponentials and sums."""
+    from solution import kernels
+
+    banner("largest weight", dtype, new, prefix)
+    g = torch.Generator().manual_seed(36)
+    # (rows enough for 256 workgroups: the keys are not cut, one workgroup meets them in turn)
+    n, dim, heads, at, batch = 260, 64, 128, 150, 8
+    k = torch.randn(n, dim, generator=g) * 0.01
+    k[:, 0] = 0.0
+    k[at, 0] = 1.0
+    v = torch.zeros(n, dim)
+    v[at] = 1 + torch.rand(dim, generator=g)
+    q = torch.randn(batch * new, heads, dim, generator=g)
+    q[..., 0] = 1 + 4 * torch.rand(batch * new, heads, generator=g)
+    q = q.to(dtype)
+    s = _one(cuda, k, v, q, prefix=prefix, batch=batch)
+    o, _ = _run(kernels, s, cuda, shared=prefix, scale=1.0)
+    pos = n - new + torch.arange(new).repeat(batch)
+    sc = (q.double() @ k.to(dtype).double().t().contiguous()).masked_fill(
+        (torch.arange(n) > pos[:, None])[:, None], -math.inf)
+    want = torch.softmax(sc, -1)[..., at:at + 1] * v[at].to(dtype).double()
+    off = (o.double().cpu() - want).abs()
+    assert (off <= want * (EPS[dtype] + 1e-4)).all(), f"relative {(off / want).max():.3e}"
