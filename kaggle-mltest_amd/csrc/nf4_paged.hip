@@ -262,6 +262,15 @@ __device__ __forceinline__ u32x2_t bload8s(rsrc_t r, int off, int soff) {
     return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_raw_buffer_load_b64(r, off, soff, 2));
 }
 
+// A row's probabilities are formed as 2^(score - m) and rounded to the 16-bit type for the second
+// product; m lies kTop below the row's largest score, in units of log 2.  fp16 has 5 bits of
+// exponent: with a largest of 1 a probability below 2^-14 loses bits and one below 2^-25 is gone,
+// while the sum that divides them counts it (20000 keys 18 behind a first one whose value is 0,
+// as behind a sink token: an output of zeros).  With a largest of 2^15 that begins at 2^-29.  The
+// factor is in the sum as well, and by m in the joined rows and the log-sum-exp.
+template <int DT>
+constexpr float kTop = DT == NF4_BF16 ? 0.f : 15.f;
+
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // A scalar load: table entries are the same for a wave.
@@ -766,7 +775,7 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
                 for (int j = 1; j < 8; ++j) top = fmaxf(top, st[rb][j >> 2][j & 3]);
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                const float mn = fmaxf(m[rb], top * a.scale);
+                const float mn = fmaxf(m[rb], top * a.scale - kTop<DT>);
                 if (__any(mn > m[rb])) {
                     const float alpha = mn > m[rb] ? __builtin_amdgcn_exp2f(m[rb] - mn) : 1.f;
                     sum[rb] *= alpha;
@@ -1191,8 +1200,8 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
 #pragma unroll
         for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
         // (a maximum that may be 2^8 behind rescales less often, 3-5 % faster for prompts, but then
-        // the largest probability is rounded too: 2.2e-3 instead of 1.9e-3 of an output in bf16)
-        const float mn = fmaxf(m, fmaxf(top, other_half(top)) * a.scale);
+        // the largest probability, a power of two, is rounded too: 2.2e-3 instead of 1.9e-3 of an output in bf16)
+        const float mn = fmaxf(m, fmaxf(top, other_half(top)) * a.scale - kTop<DT>);
         if (__any(mn > m)) {
             const float alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
             sum *= alpha;

@@ -90,3 +90,41 @@ def test_largest_weight_is_exact(cuda, dtype, new, prefix):
     want = torch.softmax(sc, -1)[..., at:at + 1] * v[at].to(dtype).double()
     off = (o.double().cpu() - want).abs()
     assert (off <= want * (EPS[dtype] + 1e-4)).all(), f"relative {(off / want).max():.3e}"
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("new,heads,prefix", [(1, 2, 0), (40, 4, 0), (1, 2, 16000), (2, 40, 16000)])
+@pytest.mark.parametrize("lead", [12.0, 18.0])
+def test_weights_far_below_the_largest(cuda, dtype, new, heads, prefix, lead):
+    """A first key whose score leads all others by `lead`, its value 0: what is left of the output
+    is the many small weights.  Each counts with its rounding to the 16-bit type (half a step,
+    relative: exp(-18) = 2^-26 of the largest is above the type's smallest normal value where the
+    largest is 2^15), the output with its own, the scores (about 20 units, fp32 sums of 64 terms)
+    with 1e-5 of exp's relative error, the fp32 sums over 20000 weights with 1e-4."""
+    from solution import kernels
+
+    banner("small weights", dtype, new, heads, prefix, lead)
+    g = torch.Generator().manual_seed(31)
+    n, dim = 20000, 64
+    k = torch.randn(n, dim, generator=g) * 0.01
+    k[:, 0] = 0.0
+    k[0] = 0.0
+    k[0, 0] = lead / 2
+    v = 1 + torch.rand(n, dim, generator=g)
+    v[0] = 0.0
+    batch = 2 if prefix else 1
+    q = torch.randn(batch * new, heads, dim, generator=g)
+    q[..., 0] = 2.0
+    q = q.to(dtype)
+    s = _one(cuda, k, v, q, prefix=prefix, batch=batch)
+    ks, vs = k.to(dtype).double(), v.to(dtype).double()
+    o, l = _run(kernels, s, cuda, shared=prefix, scale=1.0)
+    pos = n - new + torch.arange(new).repeat(batch)
+    sc = (q.double() @ ks.t().contiguous()).masked_fill(
+        (torch.arange(n) > pos[:, None])[:, None], -math.inf)
+    lse = torch.logsumexp(sc, -1)
+    want = torch.exp(sc - lse[..., None]) @ vs
+    bound = want * (2 * EPS[dtype] + 1.2e-4)
+    off = (o.double().cpu() - want).abs()
+    assert (off <= bound).all(), f"relative {(off / want).max():.3e}"
+    torch.testing.assert_close(l.cpu().double(), lse, rtol=1e-5, atol=2e-5)
