@@ -271,6 +271,23 @@ __device__ __forceinline__ u32x2_t bload8s(rsrc_t r, int off, int soff) {
 template <int DT>
 constexpr float kTop = DT == NF4_BF16 ? 0.f : 15.f;
 
+// The exponents are fma(score, scale, -m), exact but for their own rounding, with m the rounded
+// score * scale of the largest: that one's exponent is what m's rounding left, and grows with m
+// (16 and more from 2^28 on: past fp16's range).  From kFar on the products are rounded as m is
+// and subtracted, so that the largest's exponent is 0.
+constexpr float kFar = 1 << 20;
+
+// m of a row whose largest score * scale is t
+template <int DT>
+__device__ __forceinline__ float base_of(float t) {
+    return fabsf(t) > kFar ? t : t - kTop<DT>;
+}
+// a score as its exponent at a base that is far (or -inf, of a row that saw nothing: as it is)
+__device__ __forceinline__ float far_exponent(float score, float scale, float m) {
+    return score * scale - (m == -INFINITY ? 0.f : m);
+}
+__device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && m != -INFINITY; }
+
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 
 // A scalar load: table entries are the same for a wave.
@@ -645,10 +662,12 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
         }
 
         float m[RB], sum[RB];
+        bool far[RB];  // a row's m is far (the wave's)
         float4_t acc[RB][VE];
 #pragma unroll
         for (int rb = 0; rb < RB; ++rb) {
             m[rb] = -INFINITY;
+            far[rb] = false;
             sum[rb] = 0.f;
 #pragma unroll
             for (int e = 0; e < VE; ++e) acc[rb][e] = (float4_t){0.f, 0.f, 0.f, 0.f};
@@ -775,19 +794,26 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
                 for (int j = 1; j < 8; ++j) top = fmaxf(top, st[rb][j >> 2][j & 3]);
                 top = fmaxf(top, __shfl_xor(top, 16));
                 top = fmaxf(top, __shfl_xor(top, 32));
-                const float mn = fmaxf(m[rb], top * a.scale - kTop<DT>);
+                const float mn = fmaxf(m[rb], base_of<DT>(top * a.scale));
                 if (__any(mn > m[rb])) {
                     const float alpha = mn > m[rb] ? __builtin_amdgcn_exp2f(m[rb] - mn) : 1.f;
                     sum[rb] *= alpha;
 #pragma unroll
                     for (int e = 0; e < VE; ++e) acc[rb][e] *= alpha;
                     m[rb] = mn;
+                    far[rb] = __any(is_far(mn));
                 }
-                const float base = m[rb] == -INFINITY ? 0.f : m[rb];
+                if (__builtin_expect(far[rb], 0)) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        st[rb][j >> 2][j & 3] = far_exponent(st[rb][j >> 2][j & 3], a.scale, m[rb]);
+                }
+                const float mul = far[rb] ? 1.f : a.scale;
+                const float base = far[rb] || m[rb] == -INFINITY ? 0.f : m[rb];
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    p[j] = __builtin_amdgcn_exp2f(fmaf(st[rb][j >> 2][j & 3], a.scale, -base));
+                    p[j] = __builtin_amdgcn_exp2f(fmaf(st[rb][j >> 2][j & 3], mul, -base));
                     sum[rb] += p[j];
                 }
                 // probabilities in the 16-bit type for the MFMA; their sum stays unrounded
@@ -1040,7 +1066,7 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
     rg.cut(part.splits, part.min_tiles, piece);
 
     float m = -INFINITY, sum = 0.f;
-    bool odd_seen = false;
+    bool odd_seen = false, far = false;  // far: a row's m is (the wave's)
     float16_t acc[DT32];
 #pragma unroll
     for (int x = 0; x < DT32; ++x) acc[x] = (float16_t){};
@@ -1201,22 +1227,28 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
         // (a maximum that may be 2^8 behind rescales less often, 3-5 % faster for prompts, but then
         // the largest probability, a power of two, is rounded too: 2.2e-3 instead of 1.9e-3 of an output in bf16)
-        const float mn = fmaxf(m, fmaxf(top, other_half(top)) * a.scale - kTop<DT>);
+        const float mn = fmaxf(m, base_of<DT>(fmaxf(top, other_half(top)) * a.scale));
         if (__any(mn > m)) {
             const float alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
             sum *= alpha;
 #pragma unroll
             for (int x = 0; x < DT32; ++x) acc[x] *= alpha;
             m = mn;
+            far = __any(is_far(m));
         }
-        const float base = m == -INFINITY ? 0.f : m;
+        if (__builtin_expect(far, 0)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] = far_exponent(sc[e >> 4][e & 15], a.scale, m);
+        }
+        const float mul = far ? 1.f : a.scale;
+        const float base = far || m == -INFINITY ? 0.f : m;
         u32x4_t pf[4];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             float p[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                p[e] = __builtin_amdgcn_exp2f(fmaf(sc[x >> 1][(x & 1) * 8 + e], a.scale, -base));
+                p[e] = __builtin_amdgcn_exp2f(fmaf(sc[x >> 1][(x & 1) * 8 + e], mul, -base));
                 sum += p[e];
             }
             pf[x] = (u32x4_t){pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]), pack2<DT>(p[4], p[5]),

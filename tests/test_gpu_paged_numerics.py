@@ -128,3 +128,35 @@ def test_weights_far_below_the_largest(cuda, dtype, new, heads, prefix, lead):
     off = (o.double().cpu() - want).abs()
     assert (off <= bound).all(), f"relative {(off / want).max():.3e}"
     torch.testing.assert_close(l.cpu().double(), lse, rtol=1e-5, atol=2e-5)
+
+
+@pytest.mark.parametrize("dtype,size", [(F16, 1e4), (BF16, 1e6), (BF16, 1e12)])
+@pytest.mark.parametrize("new,prefix", [(1, 0), (40, 0), (1, 160)])
+def test_scores_of_any_size(cuda, dtype, size, new, prefix):
+    """Queries and keys of 1e4 (fp16) and more: scores of 1e8 to 1e25, where one step of fp32 is
+    many units.  A key that leads by more than their rounding (1e-4 of the largest) has all the
+    weight, so the output is its value, bit for bit; every output is finite."""
+    from solution import kernels
+
+    banner("scores of any size", dtype, size, new, prefix)
+    g = torch.Generator().manual_seed(32)
+    n, dim, batch = 300, 128, 2 if prefix else 1
+    k = (torch.randn(n, dim, generator=g) * size).clamp(-6e4 if dtype == F16 else -1e30,
+                                                        6e4 if dtype == F16 else 1e30)
+    v = torch.randn(n, dim, generator=g)
+    q = (torch.randn(batch * new, 4, dim, generator=g) * size).clamp(-6e4 if dtype == F16 else -1e30,
+                                                                     6e4 if dtype == F16 else 1e30)
+    q[:, 3] = q[:, 3] / size / size  # a head of ordinary scores beside them
+    q = q.to(dtype)
+    s = _one(cuda, k, v, q, prefix=prefix, batch=batch)
+    o, l = _run(kernels, s, cuda, shared=prefix)
+    pos = n - new + torch.arange(new).repeat(batch)
+    sc = (q.double() @ k.to(dtype).double().t().contiguous()).masked_fill(
+        (torch.arange(n) > pos[:, None])[:, None], -math.inf) * dim ** -0.5
+    two = sc.topk(2, -1)
+    clear = two.values[..., 0] - two.values[..., 1] > 1e-4 * two.values[..., 0].abs() + 50
+    assert clear[:, :3].double().mean() > 0.9
+    assert torch.isfinite(o.float()).all()
+    winner = v.to(dtype)[two.indices[..., 0]]
+    assert torch.equal(o.cpu()[clear], winner[clear])
+    torch.testing.assert_close(l.cpu().double(), torch.logsumexp(sc, -1), rtol=2e-5, atol=2e-4)
