@@ -458,7 +458,8 @@ int nf4_paged_append(const nf4_paged_kv *kv, const void *qkv, int64_t ld_qkv, co
  * window == 0, j > p - window or j < sinks; with s = scale * q.k over them, out
  * [tokens, n_heads, head_dim] = sum softmax(s) v and lse [tokens, n_heads] (fp32, may be NULL)
  * = log sum exp(s).  A query that sees no key gets zeros and -inf.  Query head h reads
- * key/value head h / (n_heads / n_kv).
+ * key/value head h / (n_heads / n_kv).  scale is any number of magnitude up to 2.3e38 (NaN and
+ * infinities: NF4_ERR_ARG).
  * shared > 0: positions below it are read through sequence 0's table row for every sequence,
  * once for the whole batch (a prefix that all of them start with).
  * max_q and max_len are the longest run of new tokens and the longest length as the host knows

@@ -1674,6 +1674,8 @@ extern "C" int nf4_paged_attn(const nf4_paged_kv *kv, const void *q, int64_t ld_
     const int st = fill_cache(c, kv, cu_q, tokens, n_heads, dtype);
     if (st != NF4_OK) return st;
     if (window < 0 || sinks < 0 || shared < 0 || max_q < 0 || max_len < 0) return NF4_ERR_ARG;
+    const float scale2 = fabsf(scale) * kLog2e;
+    if (!(scale2 < INFINITY)) return NF4_ERR_ARG;  // NaN too
     if (tokens == 0) return NF4_OK;
     if (!q || !out) return NF4_ERR_ARG;
     if (ld_tok < 0 || ld_head < 0) return NF4_ERR_ARG;
@@ -1691,7 +1693,7 @@ extern "C" int nf4_paged_attn(const nf4_paged_kv *kv, const void *q, int64_t ld_
     a.sinks = cut(sinks);
     a.shared = cut(shared);
     a.flip = scale < 0.f ? 0x80008000u : 0u;
-    a.scale = fmaxf(fabsf(scale) * kLog2e, 1e-30f);  // not 0: a hidden score is -inf
+    a.scale = fmaxf(scale2, 1e-30f);  // not 0: a hidden score is -inf
     Plan p = make_plan(c, n_heads, a.window, a.sinks, a.shared, max_q, max_len, kv->head_dim);
     a.dense = p.dense;
     if (p.bytes) {
