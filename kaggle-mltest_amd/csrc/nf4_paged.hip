@@ -1693,7 +1693,7 @@ extern "C" int nf4_paged_attn(const nf4_paged_kv *kv, const void *q, int64_t ld_
     a.sinks = cut(sinks);
     a.shared = cut(shared);
     a.flip = scale < 0.f ? 0x80008000u : 0u;
-    a.scale = fmaxf(scale2, 1e-30f);  // not 0: a hidden score is -inf
+    a.scale = fmaxf(scale2, 1.2e-38f);  // not 0 (a hidden score is -inf): a normal number's least
     Plan p = make_plan(c, n_heads, a.window, a.sinks, a.shared, max_q, max_len, kv->head_dim);
     a.dense = p.dense;
     if (p.bytes) {

@@ -160,3 +160,24 @@ def test_scores_of_any_size(cuda, dtype, size, new, prefix):
     winner = v.to(dtype)[two.indices[..., 0]]
     assert torch.equal(o.cpu()[clear], winner[clear])
     torch.testing.assert_close(l.cpu().double(), torch.logsumexp(sc, -1), rtol=2e-5, atol=2e-4)
+
+
+@pytest.mark.parametrize("new", [1, 40])
+def test_scale_of_nothing(cuda, new):
+    """A scale of 0 weighs every key alike, whatever its score (1e30 here)."""
+    from solution import kernels
+
+    banner("scale 0", new)
+    g = torch.Generator().manual_seed(33)
+    k = torch.randn(90, 64, generator=g) * 1e15
+    v = torch.randn(90, 64, generator=g)
+    q = (torch.randn(new, 4, 64, generator=g) * 1e15).to(BF16)
+    s = _one(cuda, k, v, q)
+    o, l = _run(kernels, s, cuda, scale=0.0)
+    vs = v.to(BF16).double()
+    want = torch.stack([vs[:91 - new + i].mean(0) for i in range(new)])[:, None].expand(-1, 4, -1)
+    # weights of 1: no rounding but the output's, and fp32 sums
+    assert ((o.double().cpu() - want).abs() <= want.abs() * EPS[BF16] + 1e-5).all()
+    count = torch.arange(91 - new, 91).double()
+    torch.testing.assert_close(l.cpu().double(), count.log()[:, None].expand(-1, 4).contiguous(),
+                               rtol=1e-5, atol=1e-4)
