@@ -420,6 +420,19 @@ __device__ __forceinline__ float4_t mfma16(const u32x4_t &a, const u32x4_t &b, c
                                                      __builtin_bit_cast(half8_t, b), c, 0, 0, 0);
 }
 
+// Two outputs.  An output is a mean of values, so one past fp16's last number is there by the
+// roundings of its probabilities (at most one step), and is that number; an infinity that is among
+// the values stays.
+template <int DT>
+__device__ __forceinline__ uint32_t pack_out(float a, float b) {
+    if constexpr (DT == NF4_F16) {
+        constexpr float most = 65504.f;
+        a = fabsf(a) < INFINITY ? __builtin_amdgcn_fmed3f(a, -most, most) : a;
+        b = fabsf(b) < INFINITY ? __builtin_amdgcn_fmed3f(b, -most, most) : b;
+    }
+    return pack2<DT>(a, b);
+}
+
 // 8 consecutive values of a query row, its sign as the scale's.
 __device__ __forceinline__ u32x4_t load_q(const Query &a, int tok, int head, int d) {
     u32x4_t r = *reinterpret_cast<const u32x4_t *>(a.q + tok * a.ld_tok + head * a.ld_head + d);
@@ -914,7 +927,7 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
                                     kvh * a.group + (r0 + r) % a.group;
                 const float inv = ll == 0.f ? 0.f : 1.f / ll;
                 *reinterpret_cast<u32x2_t *>(a.out + row * D + d) =
-                    (u32x2_t){pack2<DT>(o[0] * inv, o[1] * inv), pack2<DT>(o[2] * inv, o[3] * inv)};
+                    (u32x2_t){pack_out<DT>(o[0] * inv, o[1] * inv), pack_out<DT>(o[2] * inv, o[3] * inv)};
                 if (a.lse && d == 0) a.lse[row] = ll == 0.f ? -INFINITY : mm * kLn2 + logf(ll);
             } else {
                 const int64_t slot = (static_cast<int64_t>(group + item) * c.n_kv + kvh) * 16 * RB + r;
@@ -1301,8 +1314,8 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
                 *reinterpret_cast<u32x2_t *>(o + x * 32 + e * 2) =
-                    (u32x2_t){pack2<DT>(acc[x][e] * inv, acc[x][e + 1] * inv),
-                              pack2<DT>(acc[x][e + 2] * inv, acc[x][e + 3] * inv)};
+                    (u32x2_t){pack_out<DT>(acc[x][e] * inv, acc[x][e + 1] * inv),
+                              pack_out<DT>(acc[x][e + 2] * inv, acc[x][e + 3] * inv)};
         if (a.lse && g == 0) a.lse[row] = sum == 0.f ? -INFINITY : m * kLn2 + logf(sum);
     } else {
         const int64_t at = row * a.dense + part.first + piece;
@@ -1428,7 +1441,7 @@ __global__ __launch_bounds__(kJoinThreads) void paged_attn_join_kernel(const Cac
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     reinterpret_cast<u32x2_t *>(a.out + row * D)[col] =
-        (u32x2_t){pack2<DT>(v[0] * inv, v[1] * inv), pack2<DT>(v[2] * inv, v[3] * inv)};
+        (u32x2_t){pack_out<DT>(v[0] * inv, v[1] * inv), pack_out<DT>(v[2] * inv, v[3] * inv)};
     if (a.lse && col == 0) a.lse[row] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
 }
 

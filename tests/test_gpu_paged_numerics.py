@@ -181,3 +181,27 @@ def test_scale_of_nothing(cuda, new):
     count = torch.arange(91 - new, 91).double()
     torch.testing.assert_close(l.cpu().double(), count.log()[:, None].expand(-1, 4).contiguous(),
                                rtol=1e-5, atol=1e-4)
+
+
+@pytest.mark.parametrize("n,new,prefix", [(32, 1, 0), (60, 40, 0), (33, 1, 32), (100, 40, 32)])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_values_at_the_end_of_the_type(cuda, n, new, prefix, dim):
+    """Values of +-65504: an output is their mean, so it is finite, and off by the rounding of the
+    weights and its own, half a step each.  All weights but a first one are just above the middle
+    between 0.5 and the next number, so that a tile's are rounded up together."""
+    from solution import kernels
+
+    banner("values of 65504", n, new, prefix, dim)
+    batch, heads = 4, 8
+    k = torch.zeros(n, dim)
+    k[1:, 0] = -1.0
+    v = torch.full((n, dim), 65504.0)
+    v[:, 1::2] = -65504.0
+    q = torch.zeros(batch * new, heads, dim, dtype=F16)
+    q[..., 0] = 1.0
+    s = _one(cuda, k, v, q, prefix=prefix, batch=batch)
+    o, _ = _run(kernels, s, cuda, shared=prefix, scale=-math.log(0.5 + 1.02 * 2.0 ** -12))
+    o = o.double().cpu()
+    assert torch.isfinite(o).all()
+    assert (o[..., 0::2] >= 65504 * (1 - 2 * EPS[F16])).all()
+    assert (o[..., 1::2] <= -65504 * (1 - 2 * EPS[F16])).all()
