@@ -1563,7 +1563,9 @@ Plan make_plan(const Cache &c, int n_heads, int window, int sinks, int shared, i
         p.waves = f.whole ? 8 : 4;
         f.min_units = 2;
         int64_t units = f.items * (span / (32 * p.waves) + 2) + pre_keys / 128 + 2;
-        int64_t groups = ceil_div(kFewSlots, c.n_kv);
+        // (three row blocks: one workgroup's registers and LDS are a CU's, one past the CUs would
+        // start when the others end: 258 of 6 heads 493 us where 252 are 316)
+        int64_t groups = p.rb < 3 ? ceil_div(kFewSlots, c.n_kv) : c.n_kv < kFewSlots ? kFewSlots / c.n_kv : 1;
         groups = groups < units / f.min_units ? groups : units / f.min_units;
         f.groups = f.whole ? (c.cu ? f.items : seqs) : static_cast<int>(groups < 1 ? 1 : groups);
         if (!f.whole) {

@@ -1,6 +1,6 @@
 """The paged-cache operators where numbers are at the ends of their ranges: infinities beside
 missing pages, scores of any size, weights far below a row's largest, scales of nothing, values
-at the type's end, more output rows than a grid's first dimension."""
+at the type's end; and launches of unusual size."""
 
 import math
 
@@ -205,3 +205,15 @@ def test_values_at_the_end_of_the_type(cuda, n, new, prefix, dim):
     assert torch.isfinite(o).all()
     assert (o[..., 0::2] >= 65504 * (1 - 2 * EPS[F16])).all()
     assert (o[..., 1::2] <= -65504 * (1 - 2 * EPS[F16])).all()
+
+
+@pytest.mark.parametrize("heads,kv,new", [(42, 6, 5), (33, 3, 4), (24, 12, 20)])
+def test_three_row_blocks_of_many_heads(cuda, heads, kv, new):
+    """33 to 48 rows a sequence, key/value heads whose number does not divide 256."""
+    from solution import kernels
+
+    banner("three row blocks of many heads", heads, kv, new)
+    s = ref.Setup(cuda, BF16, heads, kv, 64, 16, [700, 90, new, 300], [new] * 4, seed=37,
+                  extra_width=1000)
+    for window, sinks in ((0, 0), (9000, 3)):
+        _check(_run(kernels, s, cuda, window, sinks), ref.attention(s, window, sinks), BF16)

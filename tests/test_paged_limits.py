@@ -26,3 +26,21 @@ def test_scales_that_are_no_number(lib, scale):  # noqa: F811
 @pytest.mark.parametrize("scale", [0.125, -2.0, 0.0, 1e-40, 2e38])
 def test_scales_that_are(lib, scale):  # noqa: F811
     assert _attn(lib, _kv(width=1 << 16, ld_table=1 << 16), scale=scale) == WORKSPACE
+
+
+@pytest.mark.parametrize("n_kv", [1, 3, 4, 6, 12, 100])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_three_row_blocks_fit_the_card(lib, n_kv, dim):  # noqa: F811
+    """33 to 48 rows a sequence over long contexts: a workgroup fills a CU then, so there are at
+    most 256 (or one of each key/value head).  Their number is in the workspace: a slot of 48 rows
+    for each workgroup and item of a key/value head, and a pair of words for each row."""
+    batch, new, group = 32, 5, 7
+    kv = _kv(batch=batch, width=1 << 14, ld_table=1 << 14, n_kv=n_kv, head_dim=dim,
+             page_stride=1 << 20, slot_stride=n_kv * dim, head_stride=dim)
+    rows = batch * new * group
+    size = lib.nf4_paged_attn_workspace(ctypes.byref(kv), None, batch * new, group * n_kv, 0, 0, 0, 0,
+                                        1 << 18)
+    slots, left = divmod(size - rows * 8, n_kv * 48 * (4 * dim + 8))
+    assert left == 0
+    items = rows // 48 + batch
+    assert 0 < (slots - items) * n_kv <= max(256, n_kv)
