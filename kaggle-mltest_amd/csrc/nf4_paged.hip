@@ -1500,16 +1500,26 @@ struct Plan {
     size_t bytes;
 };
 
-// Sequences whose rows are few go to the kernel without LDS staging: up to 32, and up to 48 over
-// long contexts, where equal shares count more than a third row block costs (35 rows of 64
-// sequences: of 40 to 16000 keys 232 us, tiled 298; in windows of 1024 58, tiled 44; a prefix of
-// 2001 positions before 48 rows 22 us, tiled 15).  Its launch is a workgroup
-// on every CU (kFewSlots): 64 KB in flight on each are enough for the memory's rate, and more
+// Sequences whose rows are few go to the kernel without LDS staging: up to 32, and up to 48 where
+// equal shares count more than a third row block costs.  Those are sequences of different lengths,
+// which the host does not know; what it knows is the longest (max_len, or a window), and how much
+// that is over all sequences and key/value heads.  35 rows, us, this kernel and tiled:
+//   longest 16000, 64 sequences of 40 to it, 4 heads of 128    227  287   6 of 64  228  364
+//   longest 16000, 8 sequences, 4 heads 37  41, 16 of one head 31  29, 24 of one head 37  40
+//   longest 9000, 16 sequences, 4 heads 49  54, 8 sequences    31  29
+//   5000 and 6000, 8 and 16 sequences,  4 heads 30  24, 43  40; 64 of 4300 each 121 118
+//   one sequence of 9000  20  19; in windows of 1024 58  44; a prefix of 2001 22  15
+// Where all it knows is the table's width, tiles would be cut for that, and equal shares are for
+// what is there (4 heads, 16 sequences of 40 to 2000 in tables of 8192 23  46, of 5120 23  34; 64
+// of 5000 in 5120 129  135; against it 64 of 40 to 2000 of 8 heads 96  72, and one of 500 19  13).
+// Its launch is a workgroup on every CU (kFewSlots): 64 KB in flight on each are enough for the memory's rate, and more
 // workgroups mean shorter shares and more pieces (131071 keys, 64 ragged sequences: 512
 // workgroups 63.5 and 215 us, 256 60.6 and 212.7).  Where no sequence is longer than kWholeKeys
 // and all of them fit the card, a workgroup of 8 waves takes a whole sequence, and there is nothing
 // to join.  Tiled parts are cut until the launch has kTileSlots workgroups.
-constexpr int kFewRows = 32, kFewRowsLong = 48, kLongKeys = 4096, kFewSlots = 256, kTileSlots = 512, kWholeKeys = 1024;
+constexpr int kFewRows = 32, kFewRowsLong = 48, kLongKeys = 8192, kLongWidth = 4096, kFewSlots = 256,
+              kTileSlots = 512, kWholeKeys = 1024;
+constexpr int64_t kLongWork = 3 << 17;  // keys of all sequences and heads
 
 // `rows` > 0: cutting the part is what makes a join of that many rows necessary.  A tile takes
 // 2 us, a join 4 us and 0.15 ns for each row and each of its pieces (written and read): 6 chunks of
@@ -1547,7 +1557,10 @@ Plan make_plan(const Cache &c, int n_heads, int window, int sinks, int shared, i
     const int64_t pre_keys = len < shared ? len : shared;
     const int seqs = c.batch + (c.cu ? 1 : 0);  // with offsets: and the tokens past the last
     const bool few_pre = shared && all_rows <= kFewRows;
-    const bool few_own = longest * group <= (!shared && span > kLongKeys ? kFewRowsLong : kFewRows);
+    const bool told = max_len || span < c.cap;
+    const bool uneven = !shared && (told ? span > kLongKeys && span * c.batch * c.n_kv >= kLongWork
+                                         : span > kLongWidth && c.batch > 1);
+    const bool few_own = longest * group <= (uneven ? kFewRowsLong : kFewRows);
     Plan p{};
     if (few_own) {
         Few &f = p.few;

@@ -217,3 +217,12 @@ def test_three_row_blocks_of_many_heads(cuda, heads, kv, new):
                   extra_width=1000)
     for window, sinks in ((0, 0), (9000, 3)):
         _check(_run(kernels, s, cuda, window, sinks), ref.attention(s, window, sinks), BF16)
+
+
+def test_three_row_blocks_in_a_window(cuda):
+    """40 rows a sequence whose windows of 8300 keys end before some sequences begin."""
+    from solution import kernels
+
+    banner("three row blocks in a window")
+    s = ref.Setup(cuda, F16, 40, 8, 64, 16, [9100, 300, 40, 8, 8500, 100], [8] * 6, seed=38)
+    _check(_run(kernels, s, cuda, 8300, 3), ref.attention(s, 8300, 3), F16)

@@ -44,3 +44,24 @@ def test_three_row_blocks_fit_the_card(lib, n_kv, dim):  # noqa: F811
     assert left == 0
     items = rows // 48 + batch
     assert 0 < (slots - items) * n_kv <= max(256, n_kv)
+
+
+@pytest.mark.parametrize("batch,n_kv,width,max_len,window,few", [
+    (64, 4, 1 << 14, 16000, 0, True), (16, 4, 1 << 14, 9000, 0, True),
+    (8, 4, 1 << 14, 16000, 0, True), (64, 4, 1 << 14, 5000, 0, False),
+    (16, 4, 1 << 14, 6000, 0, False), (1, 4, 1 << 14, 16000, 0, False),
+    (4, 1, 1 << 14, 32000, 0, False), (64, 4, 1 << 14, 0, 1024, False),
+    (64, 4, 1 << 14, 0, 0, True), (8, 4, 512, 0, 0, True), (8, 4, 256, 0, 0, False),
+    (1, 4, 1 << 14, 0, 0, False),
+])
+def test_route_of_33_to_48_rows(lib, batch, n_kv, width, max_len, window, few):  # noqa: F811
+    """Which kernel 35 rows a sequence go to, by what the host knows of their lengths: the
+    workspace has slots of 48 rows of a key/value head for the one, whole pieces of the output for
+    the other (or nothing)."""
+    kv = _kv(batch=batch, width=width, ld_table=width, n_kv=n_kv, head_dim=64, slot_stride=n_kv * 64)
+    tokens, heads = 5 * batch, 7 * n_kv
+    size = lib.nf4_paged_attn_workspace(ctypes.byref(kv), None, tokens, heads, window, 0, 0, 0, max_len)
+    rows = 35 * batch
+    tiled = size % (tokens * heads * (4 * 64 + 8)) == 0
+    slots = size > rows * 8 and (size - rows * 8) % (n_kv * 48 * (4 * 64 + 8)) == 0
+    assert (slots and not tiled) if few else (tiled and not slots)
