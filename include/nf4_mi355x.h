@@ -422,8 +422,12 @@ int nf4_qkv_rope_bwd(const void *dq, const void *dk, const void *dv, const float
  * head_dim values consecutive.  A table entry outside [0, pages) names no page: appends to it
  * are dropped and its keys are not seen.  lens[b] is the sequence's length with the call's own
  * tokens.  page_size is a power of two, head_dim 64 or 128, the strides multiples of 8 and k, v
- * 16-byte aligned; width * page_size at most 2^30, a call's
- * tokens 2^23 and tokens times n_heads 2^30. */
+ * 16-byte aligned; rows of the table are at least width apart.
+ * At most: width * page_size 2^30, slot_stride 2^26, batch 2^20, n_heads 1024, a call's tokens
+ * 2^23 and tokens times n_heads 2^30; and for attention, where a sequence brings more than 32
+ * rows (new tokens times n_heads / n_kv), tokens * n_heads / 128 + (batch + 1) * n_kv 2^23, with a
+ * shared prefix tokens * n_heads / 64 + (batch + 2) * n_kv.  Past these the calls return
+ * NF4_ERR_UNSUPPORTED and launch nothing. */
 typedef struct nf4_paged_kv {
     void *k;
     void *v;

@@ -65,3 +65,23 @@ def test_route_of_33_to_48_rows(lib, batch, n_kv, width, max_len, window, few): 
     tiled = size % (tokens * heads * (4 * 64 + 8)) == 0
     slots = size > rows * 8 and (size - rows * 8) % (n_kv * 48 * (4 * 64 + 8)) == 0
     assert (slots and not tiled) if few else (tiled and not slots)
+
+
+# (each accepted call is one that needs a workspace, and gets none: it ends there)
+LIMITS = [  # cache, call, accepted
+    (dict(), dict(heads=1024), True), (dict(), dict(heads=1026), False),
+    (dict(batch=1 << 20), dict(tokens=1 << 20), True),
+    (dict(batch=(1 << 20) + 1), dict(tokens=(1 << 20) + 1), False),
+    (dict(slot_stride=1 << 26), dict(), True), (dict(slot_stride=(1 << 26) + 8), dict(), False),
+    (dict(batch=1), dict(tokens=1 << 23, max_q=1, cu=1 << 12), True),
+    (dict(batch=1), dict(tokens=(1 << 23) + 1, max_q=1, cu=1 << 12), False),
+    (dict(n_kv=8, batch=2), dict(tokens=1 << 23, heads=128, cu=1 << 12), False),  # > 2^23 workgroups
+    (dict(width=1 << 26, ld_table=1 << 26), dict(), True),
+    (dict(width=(1 << 26) + 1, ld_table=1 << 27), dict(), False),
+]
+
+
+@pytest.mark.parametrize("cache,call,accepted", LIMITS)
+def test_limits(lib, cache, call, accepted):  # noqa: F811
+    kv = _kv(**{**dict(width=1 << 16, ld_table=1 << 16), **cache})
+    assert _attn(lib, kv, **call) == (WORKSPACE if accepted else UNSUPPORTED)
