@@ -21,20 +21,19 @@ from . import kernels
 from .quant_state import quantize_4bit
 from .stack import Qwen2Shape
 
-EPS = 1e-6
-
 
 class DecoderLayer:
     """`weights`: {"q", "k", "v", "o", "gate", "up", "down"} -> (packed, quant_state); `norm_in`,
-    `norm_post`: fp32 RMSNorm weights; `bias`: of q|k|v, or None; `window`, `sinks`: sliding-window
-    attention (0: full)."""
+    `norm_post`: fp32 RMSNorm weights and `eps` theirs; `bias`: of q|k|v, or None; `window`,
+    `sinks`: sliding-window attention (0: full)."""
 
     def __init__(self, weights: dict, norm_in: torch.Tensor, norm_post: torch.Tensor,
-                 bias: torch.Tensor | None = None, window: int = 0, sinks: int = 0):
+                 bias: torch.Tensor | None = None, window: int = 0, sinks: int = 0,
+                 eps: float = 1e-6):
         self.qkv = [weights[n] for n in ("q", "k", "v")]
         self.o, self.gate, self.up, self.down = (weights[n] for n in ("o", "gate", "up", "down"))
         self.norm_in, self.norm_post, self.bias = norm_in, norm_post, bias
-        self.window, self.sinks = window, sinks
+        self.window, self.sinks, self.eps = window, sinks, eps
 
     @classmethod
     def synthetic(cls, shape: Qwen2Shape, device="cuda", seed: int = 0, std: float = 0.02, **kw):
@@ -50,7 +49,7 @@ class DecoderLayer:
              max_len: int = 0) -> torch.Tensor:
         """The residual stream after the layer, of the new tokens' x [tokens, hidden] (the cache's
         dtype).  `cos`, `sin`: kernels.rope_table; the rest as in kernels.paged_attention."""
-        h, _ = kernels.add_rmsnorm(x, self.norm_in, EPS)
+        h, _ = kernels.add_rmsnorm(x, self.norm_in, self.eps)
         qkv = kernels.linear_fwd(h, self.qkv, bias=self.bias)
         q = kernels.paged_append(qkv, cos, sin, cache, cu_q=cu_q)
         kw = dict(cu_q=cu_q, window=self.window, sinks=self.sinks, max_q=max_q, max_len=max_len)
@@ -59,5 +58,5 @@ class DecoderLayer:
         else:
             a = kernels.paged_attention(q, cache, **kw)
         x = x + kernels.linear_fwd(a.flatten(1), [self.o])
-        h, _ = kernels.add_rmsnorm(x, self.norm_post, EPS)
+        h, _ = kernels.add_rmsnorm(x, self.norm_post, self.eps)
         return x + kernels.linear_fwd(kernels.linear_swiglu_fwd(h, self.gate, self.up), [self.down])
