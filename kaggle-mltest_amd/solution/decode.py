@@ -32,6 +32,9 @@ class DecoderLayer:
                  eps: float = 1e-6):
         self.qkv = [weights[n] for n in ("q", "k", "v")]
         self.o, self.gate, self.up, self.down = (weights[n] for n in ("o", "gate", "up", "down"))
+        rows = sum(int(qs.shape[0]) for _, qs in self.qkv)
+        if bias is not None and tuple(bias.shape) != (rows,):
+            raise ValueError(f"the bias of q|k|v is a tensor of {rows} numbers")
         self.norm_in, self.norm_post, self.bias = norm_in, norm_post, bias
         self.window, self.sinks, self.eps = window, sinks, eps
 
@@ -50,7 +53,8 @@ class DecoderLayer:
         """The residual stream after the layer, of the new tokens' x [tokens, hidden] (the cache's
         dtype).  `cos`, `sin`: kernels.rope_table; the rest as in kernels.paged_attention."""
         h, _ = kernels.add_rmsnorm(x, self.norm_in, self.eps)
-        qkv = kernels.linear_fwd(h, self.qkv, bias=self.bias)
+        bias = None if self.bias is None else self.bias.to(h.dtype).contiguous()
+        qkv = kernels.linear_fwd(h, self.qkv, bias=bias)
         q = kernels.paged_append(qkv, cos, sin, cache, cu_q=cu_q)
         kw = dict(cu_q=cu_q, window=self.window, sinks=self.sinks, max_q=max_q, max_len=max_len)
         if shared:

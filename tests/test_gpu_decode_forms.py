@@ -114,3 +114,20 @@ def test_layer_epsilon(cuda, dtype):
     """A norm's epsilon that counts: residual streams of 0.01 (mean square 1e-4) and 1e-3."""
     banner("decoder layer epsilon", dtype)
     _run_form(cuda, dtype, 4, 2, 64, False, 1e-3, size=0.01)
+
+
+@pytest.mark.parametrize("dtype,given", [(torch.float16, torch.float32),
+                                         (torch.bfloat16, torch.float16)])
+def test_layer_bias_of_another_type(cuda, dtype, given):
+    """A bias in another type than the layer's, and one that is a view of every second number."""
+    banner("decoder layer bias", dtype, given)
+    g = torch.Generator().manual_seed(7)
+    bias = torch.randn(2 * 8 * 64, generator=g).to(dtype).to(given).to(cuda)[::2]
+    _run_form(cuda, dtype, 4, 2, 64, bias, None)
+
+
+def test_layer_bias_of_another_length(cuda):
+    """Refused: the projection would read past it."""
+    banner("decoder layer bias, short")
+    with pytest.raises(ValueError):
+        _run_form(cuda, torch.float16, 4, 2, 64, torch.zeros(8 * 64 - 64, device=cuda), None)
