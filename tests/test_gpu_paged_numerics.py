@@ -226,3 +226,25 @@ def test_three_row_blocks_in_a_window(cuda):
     banner("three row blocks in a window")
     s = ref.Setup(cuda, F16, 40, 8, 64, 16, [9100, 300, 40, 8, 8500, 100], [8] * 6, seed=38)
     _check(_run(kernels, s, cuda, 8300, 3), ref.attention(s, 8300, 3), F16)
+
+
+def test_more_rows_than_a_grid_dimension(cuda):
+    """Tokens times heads past 2^20 with pieces to join: the rows on both sides of it."""
+    from solution import kernels
+
+    banner("rows past 2^20")
+    heads, kv, dim, new, shared = 1024, 16, 64, 205, 20
+    s = ref.Setup(cuda, F16, heads, kv, dim, 16, [shared + new] * 5, [new] * 5, seed=35,
+                  shared=shared)
+    assert s.q.shape[0] * heads > 1 << 20
+    o, l = _run(kernels, s, cuda, shared=shared)
+    k, v = s.k.double().cpu(), s.v.double().cpu()
+    for t in (0, 1, 204, 205, 640, 1022, 1023, 1024):
+        b, n = t // new, shared + t % new + 1
+        j = torch.arange(n)
+        at = s.table[b].long()[j // 16]
+        ks, vs = (x[at, j % 16].repeat_interleave(heads // kv, 1) for x in (k, v))
+        sc = (ks * s.q[t].double()).sum(-1) * dim ** -0.5  # [keys, heads]
+        lse = torch.logsumexp(sc, 0)
+        want = (torch.exp(sc - lse)[..., None] * vs).sum(0)
+        _check((o[t], l[t]), (want, lse, vs.abs().amax((0, 2))), F16)
