@@ -577,8 +577,8 @@ __device__ __forceinline__ void next_units(Units &u, const Cache &c, const Query
 // results meet in LDS.
 
 //
-// Bound by memory.  bf16, 4 heads of 128: 64 ragged sequences, 1.14 GB, in 199 us (5.7 TB/s, what
-// a plain read of this card reaches); 131071 keys of one, 268 MB, in 51.5 us (5.2 TB/s) and 5 us
+// Bound by memory.  bf16, 4 heads of 128: 64 ragged sequences, 1.14 GB, in 199 us (5.7 TB/s, where
+// a plain read of this card reaches 5.6); 131071 keys of one, 268 MB, in 51.5 us (5.2 TB/s) and 5 us
 // for the join.  Up to kWholeKeys keys of a sequence it is latency: length, page entries, keys,
 // the sums over LDS, 9.4 us.  (SMALL: an address a lane, for pages under 16 slots and pages whose
 // slots span 2^31 bytes.)
@@ -829,7 +829,8 @@ __device__ __forceinline__ void few_body(const Cache &c, const Query &a, const F
                     p[j] = __builtin_amdgcn_exp2f(fmaf(st[rb][j >> 2][j & 3], mul, -base));
                     sum[rb] += p[j];
                 }
-                // probabilities in the 16-bit type for the MFMA; their sum stays unrounded
+                // probabilities in the 16-bit type for the MFMA (two products of halves would take
+                // twice the instructions); their sum stays unrounded
                 pf[rb] = (u32x4_t){pack2<DT>(p[0], p[1]), pack2<DT>(p[2], p[3]),
                                    pack2<DT>(p[4], p[5]), pack2<DT>(p[6], p[7])};
             }
@@ -961,11 +962,13 @@ __global__ __launch_bounds__(64 * W, RB > 2 ? 1 : 2) void paged_attn_few_kernel(
 // read transposed (ds_read_b64_tr_b16: 4 keys of a channel a lane) from rows whose 64-byte blocks
 // are exchanged by the key's low bits, 4 keys x 64 bytes on all banks.  No bank conflicts counted.
 //
-// 8192 new tokens, 28 heads of 128 over 4, bf16: 495-505 us, 950-970 TFLOP/s, where a library's
-// 8192^3 product reaches 1140.  The matrix pipe is in use 46 % of the cycles, and the clock falls
-// to 1.95 GHz under the load: the power cap bounds it.  Measured against it: the next tile's
-// scores formed beside this one's exponentials within a wave (fewer cycles, a lower clock: 495 us,
-// and 5-15 % slower with few tiles), the same with 256 rows a workgroup (510 us).
+// 8192 new tokens, 28 heads of 128 over 4, bf16: 500-531 us from card to card, 906-962 TFLOP/s,
+// where a library's 8192^3 product reaches 1130.  The matrix pipe is in use 42 % of the cycles,
+// and the clock falls to 1.9 GHz under the load: the power cap bounds it.  64-wide heads: 174 us,
+// 690 TFLOP/s, half the products for the same exponentials.  Measured against it (when it kept its
+// maximum 2^8 behind and took 495): the next tile's scores formed beside this one's exponentials
+// within a wave (fewer cycles, a lower clock: 495 us, and 5-15 % slower with few tiles), the same
+// with 256 rows a workgroup (510 us).
 
 typedef short v4i16_t __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) v4i16_t lds_v4i16_t;
@@ -1200,8 +1203,8 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         uint64_t ok2 = 0;
         if (i + 1 < rg.i1) ok2 = send(st ^ 1, k2);
         __builtin_amdgcn_sched_barrier(0);
-        // a wave at its products goes before one at its softmax (512 -> 494 us for the 8192-token
-        // prompt: the other has its instructions under them)
+        // a wave at its products goes before one at its softmax (4 % of the 8192-token prompt: the
+        // other has its instructions under them)
         __builtin_amdgcn_s_setprio(1);
         float16_t sc[2];
 #pragma unroll
@@ -1239,7 +1242,8 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
 #pragma unroll
         for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
         // (a maximum that may be 2^8 behind rescales less often, 3-5 % faster for prompts, but then
-        // the largest probability, a power of two, is rounded too: 2.2e-3 instead of 1.9e-3 of an output in bf16)
+        // the largest probability, a power of two here, is rounded too: 2.2e-3 instead of 1.9e-3 of
+        // an output in bf16)
         const float mn = fmaxf(m, base_of<DT>(fmaxf(top, other_half(top)) * a.scale));
         if (__any(mn > m)) {
             const float alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
@@ -1255,7 +1259,7 @@ __device__ __forceinline__ void tile_body(const Cache &c, const Query &a, const 
         }
         const float mul = far ? 1.f : a.scale;
         const float base = far || m == -INFINITY ? 0.f : m;
-        u32x4_t pf[4];
+        u32x4_t pf[4];  // (rounded as in the few-rows kernel)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
             float p[8];
@@ -1343,7 +1347,7 @@ __global__ __launch_bounds__(256, 2) void paged_attn_tile_kernel(const Cache c, 
 
 // A prefix of many rows and few rows of each sequence in one launch, their workgroups in turn, one
 // of each on a CU: the first are bound by arithmetic and latency, the second by memory.  128
-// sequences behind 16384 positions 78 us, the prefix alone as long; two launches 100 us and more
+// sequences behind 16384 positions 82 us, the prefix alone as long; two launches 100 us and more
 // (of 8 sequences 26 us instead of 14), more and shorter pieces of the prefix 99 us: they wait for
 // the other part's workgroups.
 template <int DT, int D, int RB, bool SMALL>
