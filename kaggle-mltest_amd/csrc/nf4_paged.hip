@@ -274,7 +274,7 @@ constexpr float kTop = DT == NF4_BF16 ? 0.f : 15.f;
 // The exponents are fma(score, scale, -m), exact but for their own rounding, with m the rounded
 // score * scale of the largest: that one's exponent is what m's rounding left, and grows with m
 // (16 and more from 2^28 on: past fp16's range).  From kFar on the products are rounded as m is
-// and subtracted, so that the largest's exponent is 0.
+// and subtracted (two operations: the build contracts none), so that the largest's exponent is 0.
 constexpr float kFar = 1 << 20;
 
 // m of a row whose largest score * scale is t
@@ -1516,11 +1516,11 @@ struct Plan {
 // Where all it knows is the table's width, tiles would be cut for that, and equal shares are for
 // what is there (4 heads, 16 sequences of 40 to 2000 in tables of 8192 23  46, of 5120 23  34; 64
 // of 5000 in 5120 129  135; against it 64 of 40 to 2000 of 8 heads 96  72, and one of 500 19  13).
-// Its launch is a workgroup on every CU (kFewSlots): 64 KB in flight on each are enough for the memory's rate, and more
-// workgroups mean shorter shares and more pieces (131071 keys, 64 ragged sequences: 512
-// workgroups 63.5 and 215 us, 256 60.6 and 212.7).  Where no sequence is longer than kWholeKeys
-// and all of them fit the card, a workgroup of 8 waves takes a whole sequence, and there is nothing
-// to join.  Tiled parts are cut until the launch has kTileSlots workgroups.
+// Its launch is a workgroup on every CU (kFewSlots): 64 KB in flight on each are enough for the
+// memory's rate, and more workgroups mean shorter shares and more pieces (131071 keys, 64 ragged
+// sequences: 512 workgroups 63.5 and 215 us, 256 60.6 and 212.7).  Where no sequence is longer than
+// kWholeKeys and all of them fit the card, a workgroup of 8 waves takes a whole sequence, and there
+// is nothing to join.  Tiled parts are cut until the launch has kTileSlots workgroups.
 constexpr int kFewRows = 32, kFewRowsLong = 48, kLongKeys = 8192, kLongWidth = 4096, kFewSlots = 256,
               kTileSlots = 512, kWholeKeys = 1024;
 constexpr int64_t kLongWork = 3 << 17;  // keys of all sequences and heads
