@@ -84,18 +84,23 @@ def draw(rng):
         return dict(op=op, dtype=dtype, rows=rows, cols=cols, sites=sites,
                     p=rng.choice((0.05, 0.1, 0.3, 0.5)))
     batch = _spread(rng, 1, 64)
-    hi = max(1, _spread(rng, 8, 8192) // batch)
+    # (a batch of single tokens has no gradients of q and k: they see one key each)
+    hi = max(8, _spread(rng, 8, 8192) // batch)
     case = dict(op=op, model=rng.choice(tuple(HEADS)), dtype=dtype, batch=batch,
-                len_lo=rng.choice((1, max(1, hi // 2), hi)), len_hi=hi, window=0,
+                len_lo=rng.choice((1, hi // 2, hi)), len_hi=hi, window=0,
                 pad=rng.choice((0, 0, rng.randrange(1, 200))), pick=rng.randrange(1 << 30))
     if rng.random() < 0.35:
-        case["window"] = _spread(rng, 1, 4096)
+        case["window"] = _spread(rng, 5, 4096)
+    if case["len_lo"] == 1:
+        case["batch"] = max(2, batch)
     return case
 
 
 def _lengths(case):
     rng = random.Random(case["pick"])
-    return [rng.randint(case["len_lo"], case["len_hi"]) for _ in range(case["batch"])]
+    lens = [rng.randint(case["len_lo"], case["len_hi"]) for _ in range(case["batch"])]
+    lens[-1] = case["len_hi"]  # (what the host says is the longest is there)
+    return lens
 
 
 def _inputs(case, seed):
