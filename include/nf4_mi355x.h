@@ -478,6 +478,84 @@ int nf4_paged_attn(const nf4_paged_kv *kv, const void *q, int64_t ld_tok, int64_
                    int64_t max_len, int dtype, void *workspace, size_t workspace_bytes,
                    void *stream);
 
+/* ------------------------------------------ training: attention of a packed batch, dropout */
+
+/* Attention of a packed batch: `tokens` rows of all sequences one behind the other, sequence b the
+ * rows cu[b] .. cu[b + 1] - 1 (device, [batch + 1], not decreasing; NULL with batch 1: all rows are
+ * one sequence).  Token t's query head h starts t * q_tok + h * q_head 16-bit elements after q, its
+ * head_dim values consecutive; k and v alike, with n_kv heads, of which query head h reads head
+ * h / (n_heads / n_kv).  Row i of a sequence sees its rows j <= i where window == 0 or j > i - window.
+ * max_len is the longest sequence as the host knows it (0: unknown): it chooses the launch shape
+ * only, longer sequences are still right.
+ * Supported: F16 and BF16, head_dim 64 or 128, pointers 16-byte aligned, strides multiples of 8 (a
+ * dimension of one has no stride that counts) of at most 2^23, tokens at most 2^23 and
+ * tokens * n_heads at most 2^30, n_heads at most 1024, batch at most 2^20; scale any number of
+ * magnitude up to 2.3e38 (NaN and infinities: NF4_ERR_ARG). */
+typedef struct nf4_attn {
+    const void *q;
+    const void *k;
+    const void *v;
+    int64_t q_tok, q_head;
+    int64_t k_tok, k_head;
+    int64_t v_tok, v_head;
+    const int32_t *cu; /* device, [batch + 1], or NULL */
+    int64_t tokens;
+    int64_t window;
+    int64_t max_len;
+    int32_t batch;
+    int32_t n_heads;
+    int32_t n_kv;
+    int32_t head_dim;
+    float scale;
+    int32_t dtype;
+} nf4_attn;
+
+/* out [tokens, n_heads, head_dim] = sum_j P_j v_j and stats [tokens, n_heads, 2] (fp32) = (m, l),
+ * with t_j = scale * log2(e) * q.k_j over the keys that the row sees, m = max t_j, l = sum
+ * 2^(t_j - m), P_j = 2^(t_j - m) / l (the natural log-sum-exp is m ln 2 + ln l).  A row of no
+ * sequence gets zeros and (0, 0).  Workspace: nf4_attn_fwd_workspace bytes, 16-byte aligned.
+ * Replaces: _efficient_attention_forward in _Attention (/root/reference/solution/layer.py:735-826). */
+size_t nf4_attn_fwd_workspace(const nf4_attn *a);
+int nf4_attn_fwd(const nf4_attn *a, void *out, float *stats, void *workspace,
+                 size_t workspace_bytes, void *stream);
+
+/* A gradient [tokens, heads, head_dim]: token t's head h starts t * tok + h * head elements after p,
+ * as in nf4_attn (16-byte aligned, multiples of 8). */
+typedef struct nf4_grad {
+    void *p;
+    int64_t tok, head;
+} nf4_grad;
+
+/* dq, dk, dv of the above from dout, with the forward pass's out and stats; the probabilities are
+ * formed again.  With D = dout.out and dS_j = P_j (dout.v_j - D): dq = scale sum_j dS_j k_j, and over
+ * the rows that see key j and the query heads that share it dk_j = scale sum dS_j q, dv_j = sum
+ * P_j dout, summed in a fixed order (results do not depend on timing).  Rows of no sequence get
+ * zeros.  Workspace: nf4_attn_bwd_workspace bytes, 16-byte aligned.
+ * Replaces: _efficient_attention_backward in _Attention (/root/reference/solution/layer.py:735-826). */
+size_t nf4_attn_bwd_workspace(const nf4_attn *a);
+int nf4_attn_bwd(const nf4_attn *a, const void *out, const float *stats, const nf4_grad *dout,
+                 const nf4_grad *dq, const nf4_grad *dk, const nf4_grad *dv, void *workspace,
+                 size_t workspace_bytes, void *stream);
+
+/* Dropout without a stored mask, for n sites at once (1 to 8): outs[i][r, c] = x[r, c] * s where site
+ * i keeps the element, else 0 (whatever x holds there), x and outs[i] [rows, cols] with rows ld
+ * elements apart, F16 or BF16.  seed (device) is two 64-bit numbers, the seed and the step, whose low
+ * 32 bits count.  Element (r, c) has the 16-bit number u of Philox4x32-10 (Salmon et al. 2011) with
+ * key = seed (low word first) and counter = (g, 0, step, sites[i]), g = r * ceil(cols / 8) + c / 8:
+ * the low (c even) or high half of word (c % 8) / 2 of the result.  It is kept where
+ * u >= T = floor(65536 p + 1/2), and s = 65536 / (65536 - T).  0 <= p <= 1 (p a multiple of 2^-16
+ * in effect); rows * ceil(cols / 8) below 2^31 - 256.
+ * Replaces: the dropout masks of LoRA that the reference draws and packs (layer.py:76-90, 859-870). */
+int nf4_dropout(const void *x, int64_t ld_x, void *const *outs, const int64_t *ld_outs,
+                int64_t rows, int64_t cols, double p, const int64_t *seed, const uint32_t *sites,
+                int n, int dtype, void *stream);
+
+/* Its gradient: dx = base (may be NULL: zeros) + sum_i (grads[i] * s where site i keeps the element),
+ * in fp32 in this order, rounded once.  dx may be base. */
+int nf4_dropout_bwd(const void *const *grads, const int64_t *ld_grads, const void *base,
+                    int64_t ld_base, void *dx, int64_t ld_dx, int64_t rows, int64_t cols, double p,
+                    const int64_t *seed, const uint32_t *sites, int n, int dtype, void *stream);
+
 /* -------------------------------------------------------------------------- small helpers */
 
 /* out[rows, cols] = silu(gate) * up, and its gradient (the SwiGLU step between the gate/up and

@@ -405,6 +405,59 @@ __device__ __forceinline__ void lds_dma16(uint32_t lds, int off, rsrc_t r, int s
                  : "memory", "m0");
 }
 
+// ---------------------------------------------------------------- 16-bit values, attention
+//
+// The value of 16 bits.
+template <int DT>
+__device__ __forceinline__ float f32_of(uint32_t bits) {
+    if constexpr (DT == NF4_BF16) return __uint_as_float(bits << 16);
+    else return static_cast<float>(__builtin_bit_cast(half_t, static_cast<uint16_t>(bits)));
+}
+
+template <int DT>
+__device__ __forceinline__ void unpack8(const u32x4_t &r, float (&v)[8]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        v[2 * i] = f32_of<DT>(r[i] & 0xffffu);
+        v[2 * i + 1] = f32_of<DT>(r[i] >> 16);
+    }
+}
+
+template <int DT>
+__device__ __forceinline__ u32x4_t pack8(const float (&v)[8]) {
+    u32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        r[i] = round16<DT>(v[2 * i]) | (static_cast<uint32_t>(round16<DT>(v[2 * i + 1])) << 16);
+    return r;
+}
+
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+
+// The lowest n bits.
+__device__ __forceinline__ uint64_t below(int n) {
+    return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
+}
+
+typedef short v4i16_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) v4i16_t lds_v4i16_t;
+
+// the value of lane l ^ 32
+__device__ __forceinline__ float other_half(float v) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, v);
+    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// by LDS address
+__device__ __forceinline__ u32x2_t tr_read(uint32_t at) {
+    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+        reinterpret_cast<lds_v4i16_t *>(static_cast<uintptr_t>(at))));
+}
+__device__ __forceinline__ u32x4_t lds16(uint32_t at) {
+    return *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t *>(static_cast<uintptr_t>(at));
+}
+
 static inline int status_of(hipError_t e) { return e == hipSuccess ? NF4_OK : NF4_ERR_LAUNCH; }
 
 static inline bool aligned(const void *p, uintptr_t a) {

@@ -78,30 +78,6 @@ __device__ __forceinline__ int64_t slot_of(const Cache &c, int b, int pos) {
     return page * c.page_stride + (pos & ((1 << c.page_shift) - 1)) * c.slot_stride;
 }
 
-template <int DT>
-__device__ __forceinline__ float f32_of(uint32_t bits) {
-    if constexpr (DT == NF4_BF16) return __uint_as_float(bits << 16);
-    else return static_cast<float>(__builtin_bit_cast(half_t, static_cast<uint16_t>(bits)));
-}
-
-template <int DT>
-__device__ __forceinline__ void unpack8(const u32x4_t &r, float (&v)[8]) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        v[2 * i] = f32_of<DT>(r[i] & 0xffffu);
-        v[2 * i + 1] = f32_of<DT>(r[i] >> 16);
-    }
-}
-
-template <int DT>
-__device__ __forceinline__ u32x4_t pack8(const float (&v)[8]) {
-    u32x4_t r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        r[i] = round16<DT>(v[2 * i]) | (static_cast<uint32_t>(round16<DT>(v[2 * i + 1])) << 16);
-    return r;
-}
-
 // ------------------------------------------------------------------------------- append
 
 constexpr int kAppendThreads = 256;
@@ -288,8 +264,6 @@ __device__ __forceinline__ float far_exponent(float score, float scale, float m)
 }
 __device__ __forceinline__ bool is_far(float m) { return fabsf(m) > kFar && m != -INFINITY; }
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-
 // A scalar load: table entries are the same for a wave.
 __device__ __forceinline__ int sload(const int32_t *p) {
     return *(const __attribute__((address_space(4))) int32_t *)p;
@@ -311,11 +285,6 @@ __device__ __forceinline__ int position_of(const Cache &c, int t) {
     }
     const Seq s = seq_at(c, b);
     return s.p0 + t - s.q0;
-}
-
-// The lowest n bits.
-__device__ __forceinline__ uint64_t below(int n) {
-    return n <= 0 ? 0 : n >= 64 ? ~0ull : (1ull << n) - 1;
 }
 
 // What a workgroup's rows (positions pmin .. pmax) see of a part: keys of [lo, hi) that are at
@@ -969,25 +938,6 @@ __global__ __launch_bounds__(64 * W, RB > 2 ? 1 : 2) void paged_attn_few_kernel(
 // maximum 2^8 behind and took 495): the next tile's scores formed beside this one's exponentials
 // within a wave (fewer cycles, a lower clock: 495 us, and 5-15 % slower with few tiles), the same
 // with 256 rows a workgroup (510 us).
-
-typedef short v4i16_t __attribute__((ext_vector_type(4)));
-typedef __attribute__((address_space(3))) v4i16_t lds_v4i16_t;
-
-// the value of lane l ^ 32
-__device__ __forceinline__ float other_half(float v) {
-    const uint32_t b = __builtin_bit_cast(uint32_t, v);
-    const auto r = __builtin_amdgcn_permlane32_swap(b, b, false, false);
-    return __builtin_bit_cast(float, (threadIdx.x & 32) ? r[0] : r[1]);
-}
-
-// by LDS address
-__device__ __forceinline__ u32x2_t tr_read(uint32_t at) {
-    return __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-        reinterpret_cast<lds_v4i16_t *>(static_cast<uintptr_t>(at))));
-}
-__device__ __forceinline__ u32x4_t lds16(uint32_t at) {
-    return *reinterpret_cast<const __attribute__((address_space(3))) u32x4_t *>(static_cast<uintptr_t>(at));
-}
 
 constexpr int kRows = 128;
 

@@ -64,6 +64,22 @@ class NF4PagedKV(ctypes.Structure):
     ]
 
 
+class NF4Attn(ctypes.Structure):
+    """struct nf4_attn (include/nf4_mi355x.h), 128 bytes."""
+    _fields_ = [
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("q_tok", c_int64), ("q_head", c_int64),
+        ("k_tok", c_int64), ("k_head", c_int64), ("v_tok", c_int64), ("v_head", c_int64),
+        ("cu", c_void_p), ("tokens", c_int64), ("window", c_int64), ("max_len", c_int64),
+        ("batch", c_int32), ("n_heads", c_int32), ("n_kv", c_int32), ("head_dim", c_int32),
+        ("scale", c_float), ("dtype", c_int32),
+    ]
+
+
+class NF4Grad(ctypes.Structure):
+    """struct nf4_grad (include/nf4_mi355x.h), 24 bytes."""
+    _fields_ = [("p", c_void_p), ("tok", c_int64), ("head", c_int64)]
+
+
 _SIGNATURES = {
     "nf4_abi_version": (c_int, []),
     "nf4_status_string": (ctypes.c_char_p, [c_int]),
@@ -158,6 +174,20 @@ _SIGNATURES = {
     "nf4_paged_attn": (c_int, [ctypes.POINTER(NF4PagedKV), c_void_p, c_int64, c_int64, c_void_p,
                                c_void_p, c_void_p, c_int64, c_int, c_float, c_int64, c_int64,
                                c_int64, c_int64, c_int64, c_int, c_void_p, c_size_t, c_void_p]),
+    "nf4_attn_fwd_workspace": (c_size_t, [ctypes.POINTER(NF4Attn)]),
+    "nf4_attn_fwd": (c_int, [ctypes.POINTER(NF4Attn), c_void_p, c_void_p, c_void_p, c_size_t,
+                             c_void_p]),
+    "nf4_attn_bwd_workspace": (c_size_t, [ctypes.POINTER(NF4Attn)]),
+    "nf4_attn_bwd": (c_int, [ctypes.POINTER(NF4Attn), c_void_p, c_void_p, ctypes.POINTER(NF4Grad),
+                             ctypes.POINTER(NF4Grad), ctypes.POINTER(NF4Grad),
+                             ctypes.POINTER(NF4Grad), c_void_p, c_size_t, c_void_p]),
+    "nf4_dropout": (c_int, [c_void_p, c_int64, ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64),
+                            c_int64, c_int64, ctypes.c_double, c_void_p,
+                            ctypes.POINTER(ctypes.c_uint32), c_int, c_int, c_void_p]),
+    "nf4_dropout_bwd": (c_int, [ctypes.POINTER(c_void_p), ctypes.POINTER(c_int64), c_void_p,
+                                c_int64, c_void_p, c_int64, c_int64, c_int64, ctypes.c_double,
+                                c_void_p, ctypes.POINTER(ctypes.c_uint32), c_int, c_int,
+                                c_void_p]),
 }
 
 EXPORTS = tuple(_SIGNATURES)

@@ -9,7 +9,8 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import DTYPE_CODE, NF4Lora, NF4LoraJob, NF4PagedKV, check, load, stream_of
+from ._lib import (DTYPE_CODE, NF4Attn, NF4Grad, NF4Lora, NF4LoraJob, NF4PagedKV, check, load,
+                   stream_of)
 from .quant_state import weight_array, weight_desc
 
 GEMM_DTYPES = (torch.float16, torch.bfloat16)
@@ -812,3 +813,166 @@ def rope_table(positions: int, head_dim: int, base: float, device):
     inv = base ** (-torch.arange(0, head_dim, 2, dtype=torch.float64) / head_dim)
     ang = torch.arange(positions, dtype=torch.float64)[:, None] * inv
     return ang.cos().float().to(device), ang.sin().float().to(device)
+
+
+# ------------------------------- training: attention of a packed batch, dropout without masks
+
+def _attn_desc(q, k, v, cu_seqlens, scale, window, max_len):
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] \
+            or q.shape[2] != k.shape[2]:
+        raise ValueError("q is [tokens, n_heads, head_dim], k and v [tokens, n_kv, head_dim]")
+    if not q.dtype == k.dtype == v.dtype:
+        raise ValueError("q, k and v have one dtype")
+    if q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1:
+        raise ValueError("q, k and v have head_dim contiguous")
+    dev = q.get_device()
+    if dev < 0 or not dev == k.get_device() == v.get_device():
+        raise ValueError("q, k and v are on one cuda device")
+    tokens, heads, dim = q.shape
+    n_kv = k.shape[1]
+    if heads < 1 or n_kv < 1 or heads % n_kv:
+        raise ValueError("n_heads is a multiple of n_kv")
+    cu, batch = None, 1
+    if cu_seqlens is not None:
+        if cu_seqlens.get_device() != dev or cu_seqlens.dtype != torch.int32 \
+                or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 \
+                or not cu_seqlens.is_contiguous():
+            raise ValueError("cu_seqlens is a contiguous int32 [batch + 1] tensor on q's device")
+        cu, batch = cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1
+    return NF4Attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
+                   k.stride(1), v.stride(0), v.stride(1), cu, tokens, window or 0, max_len or 0,
+                   batch, heads, n_kv, dim, dim ** -0.5 if scale is None else scale,
+                   _code(q.dtype))
+
+
+def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                  cu_seqlens: torch.Tensor | None = None, scale: float | None = None,
+                  window: int = 0, max_len: int = 0, out: torch.Tensor | None = None):
+    """Causal attention of a packed batch: (out [tokens, n_heads, head_dim], stats fp32
+    [tokens, n_heads, 2]) of q [tokens, n_heads, head_dim], k and v [tokens, n_kv, head_dim] (any
+    strides, head_dim contiguous: columns of the projection's output as they are).  `cu_seqlens`:
+    int32 offsets of the sequences on the device (None: one sequence); row i of one sees its rows
+    j <= i where window == 0 or j > i - window.  stats are (m, l): with t = scale log2(e) q.k, m =
+    max t and l = sum 2^(t - m); a row behind the last sequence gives zeros and (0, 0).  `max_len`:
+    the longest sequence as the host knows it; it only chooses the launch shape."""
+    desc = _attn_desc(q, k, v, cu_seqlens, scale, window, max_len)
+    tokens, heads, dim = q.shape
+    if out is None:
+        out = q.new_empty((tokens, heads, dim))
+    else:
+        _check_out(out, (tokens, heads, dim), q)
+    stats = torch.empty((tokens, heads, 2), dtype=torch.float32, device=q.device)
+    lib, ref = load(), ctypes.byref(desc)
+    nbytes = lib.nf4_attn_fwd_workspace(ref)
+    ws = _workspace(nbytes, q.device)
+    st = lib.nf4_attn_fwd(ref, out.data_ptr(), stats.data_ptr(), _p(ws), nbytes, stream_of(q))
+    if st:
+        check(st, "nf4_attn_fwd")
+    return out, stats
+
+
+def _grad(t, shape, like, what):
+    if tuple(t.shape) != shape or t.dtype != like.dtype or t.device != like.device \
+            or t.stride(2) != 1:
+        raise ValueError(f"{what} is a {list(shape)} tensor of q's dtype, head_dim contiguous")
+    return NF4Grad(t.data_ptr(), t.stride(0), t.stride(1))
+
+
+def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                  out: torch.Tensor, stats: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
+                  scale: float | None = None, window: int = 0, max_len: int = 0, grads=None):
+    """(dq, dk, dv) of attention_fwd from the output's gradient, with the forward pass's `out` and
+    `stats` and its other arguments.  dk and dv are summed over the query heads that share a head.
+    `grads`: (dq, dk, dv) tensors to write, of any strides (column slices of one buffer).  Rows of
+    no sequence get zeros."""
+    desc = _attn_desc(q, k, v, cu_seqlens, scale, window, max_len)
+    shape, kv_shape = tuple(q.shape), tuple(k.shape)
+    if grads is None:
+        grads = q.new_empty(shape), q.new_empty(kv_shape), q.new_empty(kv_shape)
+    _check_out(out, shape, q)
+    if tuple(stats.shape) != (*shape[:2], 2) or stats.dtype != torch.float32 \
+            or stats.device != q.device or not stats.is_contiguous():
+        raise ValueError("stats is the forward pass's fp32 [tokens, n_heads, 2] tensor")
+    args = [_grad(t, sh, q, name) for t, sh, name in
+            zip((dout, *grads), (shape, shape, kv_shape, kv_shape), ("dout", "dq", "dk", "dv"))]
+    lib, ref = load(), ctypes.byref(desc)
+    nbytes = lib.nf4_attn_bwd_workspace(ref)
+    ws = _workspace(nbytes, q.device)
+    st = lib.nf4_attn_bwd(ref, out.data_ptr(), stats.data_ptr(), *map(ctypes.byref, args), _p(ws),
+                          nbytes, stream_of(q))
+    if st:
+        check(st, "nf4_attn_bwd")
+    return tuple(grads)
+
+
+def _rows_of(t, shape, dtype, index):
+    if tuple(t.shape) != shape or t.dtype != dtype or t.get_device() != index \
+            or (t.stride(1) != 1 and shape[1] > 1):
+        raise ValueError(f"dropout's tensors are row-contiguous {list(shape)} tensors of one dtype "
+                         "and device")
+
+
+def _drop_args(tensors, seed, sites):
+    """(pointers, row strides, site numbers) as ctypes arrays."""
+    index = tensors[0].get_device()
+    if index < 0 or seed.get_device() != index or seed.dtype != torch.int64 \
+            or tuple(seed.shape) != (2,) or not seed.is_contiguous():
+        raise ValueError("seed is an int64 [2] tensor (seed, step) on the tensors' cuda device")
+    n = len(sites)
+    if not 1 <= n <= 8:
+        raise ValueError("dropout takes 1 to 8 sites")
+    if any(not 0 <= s < 1 << 32 for s in sites):
+        raise ValueError("a site is a number of 32 bits")
+    ptrs = (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
+    lds = (ctypes.c_int64 * len(tensors))(*[t.stride(0) for t in tensors])
+    return ptrs, lds, (ctypes.c_uint32 * n)(*sites)
+
+
+def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, sites, outs=None) -> list:
+    """Dropout without a stored mask: for every site a tensor like x [rows, cols] that holds
+    x * 65536 / (65536 - T) where the site keeps the element and 0 where it does not, T =
+    floor(65536 p + 1/2).  What is kept is a function of the element's place, the site's number and
+    `seed`, an int64 [2] tensor (seed, step) on the device: dropout_bwd with the same ones has the
+    same mask.  A program gives every adapter of a model its own site and every step its own `step`
+    (seed[1] += 1; a captured graph reads it at each replay)."""
+    if x.dim() != 2:
+        raise ValueError("x is [rows, cols]")
+    dt, shape, index = _code(x.dtype), tuple(x.shape), x.get_device()
+    _rows_of(x, shape, x.dtype, index)
+    if outs is None:
+        outs = [torch.empty(shape, dtype=x.dtype, device=x.device) for _ in sites]
+    if len(outs) != len(sites):
+        raise ValueError("an output for every site")
+    for t in outs:
+        _rows_of(t, shape, x.dtype, index)
+    ptrs, lds, where = _drop_args([x, *outs], seed, sites)
+    st = load().nf4_dropout(x.data_ptr(), x.stride(0), ctypes.cast(ctypes.byref(ptrs, 8), _PTRS),
+                            ctypes.cast(ctypes.byref(lds, 8), _LDS), *shape, float(p),
+                            seed.data_ptr(), where, len(sites), dt, stream_of(x))
+    if st:
+        check(st, "nf4_dropout")
+    return list(outs)
+
+
+_PTRS, _LDS = ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_int64)
+
+
+def dropout_bwd(grads, p: float, seed: torch.Tensor, sites, base: torch.Tensor | None = None,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """dx of dropout: base (None: zeros) plus every site's gradient times its mask and scale, summed
+    in fp32 in this order and rounded once.  `out` may be `base`."""
+    g = grads[0]
+    if g.dim() != 2 or len(grads) != len(sites):
+        raise ValueError("a [rows, cols] gradient for every site")
+    dt, shape, index = _code(g.dtype), tuple(g.shape), g.get_device()
+    if out is None:
+        out = torch.empty(shape, dtype=g.dtype, device=g.device)
+    for t in (*grads, out, *(() if base is None else (base,))):
+        _rows_of(t, shape, g.dtype, index)
+    ptrs, lds, where = _drop_args(list(grads), seed, sites)
+    st = load().nf4_dropout_bwd(ptrs, lds, _p(base), base.stride(0) if base is not None else 0,
+                                out.data_ptr(), out.stride(0), *shape, float(p), seed.data_ptr(),
+                                where, len(sites), dt, stream_of(g))
+    if st:
+        check(st, "nf4_dropout_bwd")
+    return out

@@ -1,0 +1,204 @@
+"""Training attention of a packed batch, forward and backward, against its 64-bit definition."""
+
+import math
+
+import pytest
+import torch
+
+from tests import train_ref as ref
+from tests.gpu_util import banner
+
+pytestmark = pytest.mark.gpu
+
+F16, BF16 = torch.float16, torch.bfloat16
+
+
+def make(dev, dtype, heads, kv, dim, lens, pad=0, seed=0, qscale=2.0, gscale=1.0, layout="qkv"):
+    """(q, k, v, dout, offsets) on the GPU; layout "qkv": columns of one buffer, "heads": one head
+    behind the other, "plain": tensors of their own."""
+    g = torch.Generator().manual_seed(seed)
+    tokens = sum(lens) + pad
+    x = torch.randn(tokens, heads + 2 * kv, dim, generator=g)
+    x[:, :heads] *= qscale
+    x = x.to(dtype)
+    parts = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+    if layout == "qkv":
+        x = x.to(dev)
+        q, k, v = x[:, :heads], x[:, heads:heads + kv], x[:, heads + kv:]
+    elif layout == "heads":
+        q, k, v = (t.transpose(0, 1).contiguous().to(dev).transpose(0, 1) for t in parts)
+    else:
+        q, k, v = (t.contiguous().to(dev) for t in parts)
+    dout = (torch.randn(tokens, heads, dim, generator=g) * gscale).to(dtype).to(dev)
+    cu = [0]
+    for n in lens:
+        cu.append(cu[-1] + n)
+    return q, k, v, dout, cu
+
+
+def run(q, k, v, dout, cu, **kw):
+    from solution import kernels
+
+    c = torch.tensor(cu, dtype=torch.int32, device=q.device) if cu is not None else None
+    out, stats = kernels.attention_fwd(q, k, v, c, **kw)
+    grads = kernels.attention_bwd(dout, q, k, v, out, stats, c, **kw)
+    torch.cuda.synchronize()
+    return dict(zip(("out", "stats", "dq", "dk", "dv"), (out, stats, *grads)))
+
+
+def check(got, q, k, v, dout, cu, **kw):
+    kw.pop("max_len", None)
+    want = ref.attention(q, k, v, cu if cu is not None else [0, q.shape[0]], dout, **kw)
+    for name in ("out", "stats", "dq", "dk", "dv"):
+        ref.assert_within(got[name], want[name], name)
+
+
+CASES = [
+    # dtype, heads, kv, dim, lens, pad, window, layout
+    (F16, 1, 1, 64, (1,), 0, 0, "plain"),
+    (BF16, 2, 1, 128, (1,), 0, 0, "qkv"),
+    (F16, 2, 2, 64, (2, 1, 3), 0, 0, "plain"),
+    (BF16, 12, 2, 128, (17,), 0, 0, "qkv"),
+    (F16, 4, 4, 64, (63, 64, 65), 0, 0, "qkv"),
+    (BF16, 4, 2, 128, (127, 1, 128, 129), 5, 0, "heads"),
+    (F16, 6, 2, 128, (200, 0, 0, 57, 300), 70, 0, "qkv"),
+    (BF16, 14, 2, 64, (333, 90), 0, 0, "qkv"),
+    (F16, 2, 1, 128, (700,), 0, 0, "plain"),
+    (BF16, 2, 1, 64, (700, 333), 140, 0, "heads"),
+    (F16, 2, 1, 128, (300, 41), 3, 1, "qkv"),
+    (BF16, 2, 1, 64, (300, 41), 3, 2, "qkv"),
+    (F16, 4, 2, 64, (500, 260), 0, 63, "qkv"),
+    (BF16, 4, 2, 128, (500, 260), 9, 64, "heads"),
+    (F16, 3, 1, 128, (450,), 0, 129, "qkv"),
+    (BF16, 3, 3, 64, (450, 450), 0, 300, "plain"),
+    (F16, 2, 2, 64, tuple([3, 1, 0, 2] * 40), 200, 0, "qkv"),
+]
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim,lens,pad,window,layout", CASES)
+def test_definition(cuda, dtype, heads, kv, dim, lens, pad, window, layout):
+    banner("attention", dtype, heads, kv, dim, lens, pad, window, layout)
+    q, k, v, dout, cu = make(cuda, dtype, heads, kv, dim, lens, pad, seed=3, layout=layout)
+    got = run(q, k, v, dout, cu, window=window, max_len=max(lens))
+    check(got, q, k, v, dout, cu, window=window)
+    tail = sum(lens)
+    for name in ("out", "stats", "dq", "dk", "dv"):  # rows of no sequence
+        assert not got[name][tail:].any(), name
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens,window", [((1500,), 0), ((1100, 900), 400)])
+def test_long(cuda, dtype, lens, window):
+    banner("long", dtype, lens, window)
+    q, k, v, dout, cu = make(cuda, dtype, 6, 2, 128, lens, 30, seed=4)
+    check(run(q, k, v, dout, cu, window=window), q, k, v, dout, cu, window=window)
+
+
+def test_one_sequence_without_offsets(cuda):
+    q, k, v, dout, _ = make(cuda, F16, 4, 2, 64, (150,), seed=5)
+    check(run(q, k, v, dout, None), q, k, v, dout, None)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("scale", [0.0, -0.125, 0.4, 1e-30])
+def test_scales(cuda, dtype, scale):
+    q, k, v, dout, cu = make(cuda, dtype, 2, 1, 64, (90, 40), seed=6)
+    check(run(q, k, v, dout, cu, scale=scale), q, k, v, dout, cu, scale=scale)
+
+
+@pytest.mark.parametrize("gscale", [1e-4, 3e3])
+def test_gradients_of_any_size_in_fp16(cuda, gscale):
+    """The scale of a loss: dS of 1e-8 and of 1e5 have their bits (a plain fp16 of them has none)."""
+    q, k, v, dout, cu = make(cuda, F16, 4, 2, 128, (300,), seed=7, gscale=gscale)
+    if gscale > 1:
+        q, k = q * 0.125, k * 0.125
+        v = v * 0.25
+    check(run(q, k, v, dout, cu), q, k, v, dout, cu)
+
+
+def test_max_len_chooses_no_result(cuda):
+    q, k, v, dout, cu = make(cuda, BF16, 4, 2, 128, (400, 130), seed=8)
+    for n in (0, 1, 400, 100000):
+        check(run(q, k, v, dout, cu, max_len=n), q, k, v, dout, cu)
+
+
+def test_results_do_not_depend_on_timing(cuda):
+    q, k, v, dout, cu = make(cuda, F16, 12, 2, 128, (900, 300), seed=9)
+    a = run(q, k, v, dout, cu)
+    for _ in range(3):
+        b = run(q, k, v, dout, cu)
+        assert all(torch.equal(a[n], b[n]) for n in a)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("what", ["v", "k", "q", "dout"])
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_not_finite_stays_with_those_who_see_it(cuda, dtype, what, value):
+    """An infinity or NaN in one sequence's row leaves the other sequences, and in k and v the rows
+    before it, as they are without it."""
+    banner("not finite", dtype, what, value)
+    q, k, v, dout, cu = make(cuda, dtype, 4, 2, 64, (50, 70, 40), seed=10, layout="plain")
+    want = ref.attention(q, k, v, cu, dout)
+    at = 50 + 33
+    {"q": q, "k": k, "v": v, "dout": dout}[what][at, -1, 5] = value
+    got = run(q, k, v, dout, cu)
+    for name in ("out", "stats", "dq", "dk", "dv"):
+        for s in (slice(0, 50), slice(120, 160)):
+            ref.assert_within(got[name][s], tuple(t[s] for t in want[name]), name)
+    # its own sequence's rows before it see none of it
+    for name in ("out", "stats", "dq"):
+        ref.assert_within(got[name][50:at], tuple(t[50:at] for t in want[name]), name)
+    # nor do the keys behind it, where it is a row's
+    if what in ("q", "dout"):
+        for name in ("dk", "dv"):
+            ref.assert_within(got[name][at + 1:120], tuple(t[at + 1:120] for t in want[name]), name)
+    # and what is touched says so
+    touched = {"v": ("out", "dq", "dk"), "k": ("out", "dq", "dk"), "q": ("out", "dq", "dk", "dv"),
+               "dout": ("dq", "dk", "dv")}[what]
+    if math.isnan(value):
+        for name in touched:
+            assert torch.isnan(got[name][50:120].float()).any(), name
+
+
+def test_gradient_against_differences(cuda):
+    """(L(x + h d) - L(x - h d)) / 2h = <gradient, d> with L = sum(out * w), by the kernel's forward
+    pass alone: fp16 outputs are off by half a step each, which the sum over them averages."""
+    q, k, v, dout, cu = make(cuda, F16, 4, 2, 64, (120, 60), seed=11, qscale=1.0, layout="plain")
+    from solution import kernels
+
+    got = run(q, k, v, dout, cu)
+    c = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    g = torch.Generator().manual_seed(12)
+    for name, x in (("dq", q), ("dk", k), ("dv", v)):
+        h = 2.0 ** -4
+        d = torch.randint(-1, 2, x.shape, generator=g).to(x)  # x +- h d: exact but for x's step
+        up, down = x + h * d, x - h * d
+        step = (up.double() - down.double())
+
+        def loss(y):
+            args = {"dq": (y, k, v), "dk": (q, y, v), "dv": (q, k, y)}[name]
+            return kernels.attention_fwd(*args, c)[0].double()
+
+        a, b = loss(up), loss(down)
+        moved = ((a - b) * dout.double()).sum()
+        told = (got[name].double() * step).sum()
+        # roundings of a and b: independent, half a step at most each (their mean square a third of
+        # that, six of the sum's deviations); the third-order term h^2 / 6 of the softmax's change
+        noise = 6 * ((2.0 ** -11 * dout.double()) ** 2 * (a ** 2 + b ** 2) / 3).sum().sqrt()
+        third = 0.02 * (got[name].double().norm() * step.norm()) / 4
+        assert (moved - told).abs() <= noise + third, (name, float(moved), float(told), float(noise))
+
+
+def test_written_views(cuda):
+    """Gradients into the columns of one buffer, beside columns that stay as they are."""
+    from solution import kernels
+
+    q, k, v, dout, cu = make(cuda, BF16, 4, 2, 64, (90, 30), pad=6, seed=13)
+    c = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    out, stats = kernels.attention_fwd(q, k, v, c)
+    big = torch.full((126, 10, 64), 7.0, dtype=BF16, device=cuda)
+    kernels.attention_bwd(dout, q, k, v, out, stats, c, grads=(big[:, 1:5], big[:, 5:7], big[:, 8:10]))
+    plain = kernels.attention_bwd(dout, q, k, v, out, stats, c)
+    assert torch.equal(big[:, 1:5], plain[0]) and torch.equal(big[:, 5:7], plain[1])
+    assert torch.equal(big[:, 8:10], plain[2])
+    assert (big[:, 0] == 7).all() and (big[:, 7] == 7).all()
