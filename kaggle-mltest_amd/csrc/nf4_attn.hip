@@ -183,50 +183,705 @@ __device__ __forceinline__ void key_backward(const Attn &a, int head, int j, int
     }
 }
 
-template <int DT, int D>
-__global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, int grad) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (i >= static_cast<int64_t>(a.tokens) * a.n_heads) return;
-    const int r = __builtin_amdgcn_readfirstlane(static_cast<int>(i / a.n_heads));
-    const int head = __builtin_amdgcn_readfirstlane(static_cast<int>(i % a.n_heads));
-    const int2 seen = keys_of(a, r);
-    float acc[D / 64], m = 0.f, l = 0.f;
-    if (grad) {
-        row_backward<DT, D>(a, head, r, seen.x, seen.y, acc);
+// --------------------------------------------------------------------------- tiles
+//
+// A workgroup of four waves owns 128 rows (or keys), 32 a wave, in registers, and goes over the keys (or
+// rows) that they see in tiles of 64, which come to LDS by DMA while the tile before is used (two
+// stages, one barrier a tile).  The first products are formed so that a lane holds one of its own
+// rows (a column of the MFMA result): what belongs to a row stays in the lane, and the probabilities
+// leave the first product in the register layout that the second takes as its operand.
+//
+// 16-byte chunk ch of a tile's row r lies at chunk ch ^ swizzle(r): the 16 lanes that LDS serves at a
+// time read one chunk of 16 rows from 16 bank groups, and 64 bytes of each of 4 consecutive rows
+// (transposed reads) from all banks.
+
+constexpr int kOwn = 128, kTile = 64;
+
+template <int D>
+__device__ __forceinline__ constexpr int swizzle(int r) {
+    return D == 128 ? (r & 3) << 2 | (r >> 2 & 3) : (r & 2) << 1 | (r >> 2 & 3);
+}
+
+template <int D>
+constexpr int kTileBytes = kTile * D * 2;
+
+// What a thread knows of a tensor's tiles: the byte of its 16 in the first pass, and its rows' pitch.
+template <int D>
+struct Stager {
+    static constexpr int CH = D / 8, RPP = 256 / CH, PASS = kTile / RPP;
+    const uint16_t *base;  // the head's first row
+    int64_t tok;
+    int off, step;
+
+    __device__ __forceinline__ void set(const Strided &x, int head) {
+        const int row = threadIdx.x / CH, ch = threadIdx.x % CH;
+        base = x.p + head * x.head;
+        tok = x.tok;
+        off = row * static_cast<int>(tok) * 2 + ((ch ^ swizzle<D>(row)) << 4);
+        step = RPP * static_cast<int>(tok) * 2;
+    }
+    // rows [t, t + 64) to LDS address `at` (the wave's); rows from `end` on are zeros, and not read
+    __device__ __forceinline__ void send(uint32_t at, int t, int end) const {
+        const int64_t bytes = t < end ? (end - t - 1) * tok * 2 + D * 2 : 0;
+        const rsrc_t r = make_rsrc(base + t * tok, bytes);
 #pragma unroll
-        for (int x = 0; x < D / 64; ++x) acc[x] *= a.scale;
-        store_row<DT, D>(a.dq.to(r, head), acc);
+        for (int x = 0; x < PASS; ++x) lds_dma16(at + x * 4096, off + x * step, r, 0);
+    }
+};
+
+// Operand addresses of a lane in a tile at LDS address 0: rows as they lie (a row a lane, 16 channels
+// a step), and transposed (a channel a lane, 16 rows a step).
+template <int D>
+__device__ __forceinline__ uint32_t row_address() {
+    const int l = threadIdx.x & 63, n = l & 31, g = l >> 5;
+    return n * D * 2 + ((g ^ swizzle<D>(n)) << 4);
+}
+template <int D>
+__device__ __forceinline__ uint32_t channel_address() {
+    const int l = threadIdx.x & 63, row = (l >> 5) * 4 + ((l & 15) >> 2);
+    const int ch = ((l >> 4) & 1) * 2 + ((l & 3) >> 1);
+    return row * D * 2 + (l & 1) * 8 + ((ch ^ swizzle<D>(row)) << 4);
+}
+// channels 16 x .. of rows 32 h .. of the tile at `at`
+template <int D>
+__device__ __forceinline__ u32x4_t rows_operand(uint32_t at, int h, int x) {
+    return lds16((at ^ (x << 5)) + h * 64 * D);
+}
+// rows 16 x .. (in the order of a result's registers) of channels 32 d ..
+template <int D>
+__device__ __forceinline__ u32x4_t channels_operand(uint32_t at, int x, int d) {
+    const uint32_t p = at ^ (d << 6);
+    const u32x2_t lo = tr_read(p + x * 32 * D), hi = tr_read((p ^ 32) + x * 32 * D + 16 * D);
+    return (u32x4_t){lo.x, lo.y, hi.x, hi.y};
+}
+
+// A lane's own row as operands: channels 16 x + 8 (l / 32) ..
+template <int D>
+__device__ __forceinline__ void own_operand(u32x4_t (&f)[D / 16], const uint16_t *row, bool live, uint32_t flip) {
+    const int g = (threadIdx.x & 63) >> 5;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) {
+        f[x] = (u32x4_t){0, 0, 0, 0};
+        if (live) f[x] = *reinterpret_cast<const u32x4_t *>(row + x * 16 + g * 8);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) f[x][i] ^= flip;
+    }
+}
+
+// The registers of a result, as 16-bit operands of the next product (x: 16 of its 32 rows).
+template <int DT>
+__device__ __forceinline__ u32x4_t operand_of(const float16_t &v, int x) {
+    u32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack2<DT>(v[x * 8 + 2 * i], v[x * 8 + 2 * i + 1]);
+    return r;
+}
+
+__device__ __forceinline__ int wave_min_i(int v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int x = __shfl_xor(v, o);
+        v = x < v ? x : v;
+    }
+    return __builtin_amdgcn_readfirstlane(v);
+}
+
+// What the rows (or keys) of a wave and of a workgroup see: [lo, hi) any of them, [full_lo, full_hi)
+// all of them (empty ones apart).
+struct Span {
+    int lo, hi, full_lo, full_hi;
+    __device__ __forceinline__ void set(int2 s) {
+        const bool some = s.x < s.y;
+        lo = wave_min_i(some ? s.x : 0x7fffffff);
+        hi = -wave_min_i(some ? -s.y : 0);
+        full_lo = -wave_min_i(some ? -s.x : 0);
+        full_hi = wave_min_i(some ? s.y : 0x7fffffff);
+    }
+    // over the four waves; `mem`: 8 words of LDS
+    __device__ __forceinline__ int2 all(int *mem) const {
+        const int w = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+            mem[w] = lo;
+            mem[4 + w] = hi;
+        }
+        __syncthreads();
+        int a = mem[0], b = mem[4];
+#pragma unroll
+        for (int i = 1; i < 4; ++i) {
+            a = mem[i] < a ? mem[i] : a;
+            b = mem[4 + i] > b ? mem[4 + i] : b;
+        }
+        return make_int2(__builtin_amdgcn_readfirstlane(a), __builtin_amdgcn_readfirstlane(b));
+    }
+    __device__ __forceinline__ bool full(int t, int n) const { return t >= full_lo && t + n <= full_hi; }
+    __device__ __forceinline__ bool none(int t, int n) const { return t >= hi || t + n <= lo; }
+};
+
+// The bits of a 64-wide tile at t that are in [s.x, s.y), for this lane's registers: register e of
+// half h is bit 32 h + 8 (e / 4) + e % 4.
+__device__ __forceinline__ uint64_t seen_bits(int2 s, int t) {
+    return (below(s.y - t) & ~below(s.x - t)) >> (((threadIdx.x >> 5) & 1) * 4);
+}
+__device__ __forceinline__ bool bit_of(uint64_t m, int h, int e) {
+    return static_cast<uint32_t>(m >> (32 * h)) >> (8 * (e >> 2) + (e & 3)) & 1;
+}
+
+// Probabilities are rounded to 16 bits for the second product; fp16's are 2^15 times as large, so that
+// those down to 2^-29 keep their bits (its least normal number is 2^-14).
+template <int DT>
+constexpr float kTop = DT == NF4_BF16 ? 0.f : 15.f;
+
+// 0 where all registers are finite, else NaN
+template <int N>
+__device__ __forceinline__ float odd_of(const float16_t (&v)[N]) {
+    float z = 0.f;
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) z = fmaf(v[x][e], 0.f, z);
+    return z;
+}
+
+// This lane's channels of its row, from a transposed result.
+template <int DT, int D>
+__device__ __forceinline__ void store_own(uint16_t *row, const float16_t (&v)[D / 32], float f) {
+    row += ((threadIdx.x & 63) >> 5) * 4;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<u32x2_t *>(row + x * 32 + e * 2) =
+                (u32x2_t){pack2<DT>(v[x][e] * f, v[x][e + 1] * f), pack2<DT>(v[x][e + 2] * f, v[x][e + 3] * f)};
+}
+
+// A row that sees nothing has zeros (its registers hold anything: no mask kept tiles from it that every
+// other row of its wave sees whole).
+template <int N>
+__device__ __forceinline__ void zero_unless(bool some, float16_t (&v)[N]) {
+    if (some) return;
+#pragma unroll
+    for (int x = 0; x < N; ++x) v[x] = (float16_t){};
+}
+
+// An output is a mean of values: one past fp16's last number is there by the roundings of its
+// probabilities (a step at most), and is that number.
+template <int DT, int N>
+__device__ __forceinline__ void keep_finite(float16_t (&v)[N], float f) {
+    if constexpr (DT == NF4_F16) {
+#pragma unroll
+        for (int x = 0; x < N; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) v[x][e] = __builtin_amdgcn_fmed3f(v[x][e] * f, -65504.f, 65504.f);
+    }
+}
+
+// ------------------------------------------------------------------------------ forward
+
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, int tiles) {
+    constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TB + 64];
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+    const int g = l >> 5, n = l & 31;
+    const int kvh = blockIdx.x % a.n_kv, y = blockIdx.x / a.n_kv;
+    const int head = kvh * a.group + y % a.group;
+    const int tile = tiles - 1 - y / a.group;  // (the last rows see most: first)
+    const int r = tile * kOwn + w * 32 + n;
+    const int2 seen = r < a.tokens ? keys_of(a, r) : make_int2(r, r);
+    Span sp;
+    sp.set(seen);
+    const int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
+
+    u32x4_t q[KS];
+    const float c = fabsf(a.c);
+    own_operand<D>(q, a.q.at(r, head), r < a.tokens, a.c < 0.f ? 0x80008000u : 0u);
+    Stager<D> sk, sv;
+    sk.set(a.k, kvh);
+    sv.set(a.v, kvh);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) uint8_t *)lds));
+    const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
+    const uint32_t ka = lds0 + row_address<D>(), va = lds0 + 2 * TB + channel_address<D>();
+
+    float m = -INFINITY, sum = 0.f;
+    bool far = false;  // a row's m is (the wave's)
+    float16_t acc[DN];
+#pragma unroll
+    for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
+    int k = all.x < all.y ? all.x & ~(kTile - 1) : all.y, st = 0;
+    if (k < all.y) {
+        sk.send(mine, k, all.y);
+        sv.send(mine + 2 * TB, k, all.y);
+    }
+    for (; k < all.y; k += kTile, st ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();  // every wave's part of this tile is there, and the one before is read
+        if (k + kTile < all.y) {
+            sk.send(mine + (st ^ 1) * TB, k + kTile, all.y);
+            sv.send(mine + (2 + (st ^ 1)) * TB, k + kTile, all.y);
+        }
+        if (sp.none(k, kTile)) continue;
+        u32x4_t kf[2][KS];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int x = 0; x < KS; ++x) kf[h][x] = rows_operand<D>(ka + st * TB, h, x);
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+        float16_t sc[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            sc[h] = (float16_t){};
+#pragma unroll
+            for (int x = 0; x < KS; ++x) sc[h] = mfma32<DT>(kf[h][x], q[x], sc[h]);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        u32x4_t vf[2][DN];
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int d = 0; d < DN; ++d) vf[x][d] = channels_operand<D>(va + st * TB, x, d);
+        __builtin_amdgcn_sched_barrier(0);
+        if (!sp.full(k, kTile)) {
+            const uint64_t see = seen_bits(seen, k);
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!bit_of(see, h, e)) sc[h][e] = -INFINITY;
+        }
+        float top = sc[0][0];
+#pragma unroll
+        for (int e = 1; e < 32; ++e) top = fmaxf(top, sc[e >> 4][e & 15]);
+        const float t = fmaxf(top, other_half(top)) * c;
+        const float mn = fmaxf(m, fabsf(t) > kFar ? t : t - kTop<DT>);
+        if (__any(mn > m)) {
+            const float alpha = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.f;
+            sum *= alpha;
+#pragma unroll
+            for (int x = 0; x < DN; ++x) acc[x] *= alpha;
+            m = mn;
+            far = __any(fabsf(m) > kFar && m != -INFINITY);
+        }
+        const float base = m == -INFINITY ? 0.f : m;
+        if (__builtin_expect(far, 0)) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] = sc[e >> 4][e & 15] * c - base;
+        }
+        const float mul = far ? 1.f : c, sub = far ? 0.f : base;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[e >> 4][e & 15], mul, -sub));
+            sum += p;
+            sc[e >> 4][e & 15] = p;
+        }
+        u32x4_t pf[4];
+#pragma unroll
+        for (int x = 0; x < 4; ++x) pf[x] = operand_of<DT>(sc[x >> 1], x & 1);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+#pragma unroll
+            for (int d = 0; d < DN; ++d) acc[d] = mfma32<DT>(vf[x & 1][d], pf[x], acc[d]);
+            if (x < 2)
+#pragma unroll
+                for (int d = 0; d < DN; ++d) vf[x][d] = channels_operand<D>(va + st * TB, x + 2, d);
+        }
+        __builtin_amdgcn_s_setprio(0);
+    }
+
+    sum += other_half(sum);
+    const bool some = seen.x < seen.y;
+    const float odd = odd_of(acc);
+    if (__any(some && !(odd == 0.f && sum > 0.f && sum < INFINITY && fabsf(m) < INFINITY))) {
+        // An infinity or NaN: a product with a probability of 0 that stands for a key that is not
+        // seen is none, and each row is formed from what it sees alone.
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+            const int row = tile * kOwn + w * 32 + i;
+            const int k0 = __builtin_amdgcn_readlane(seen.x, i), k1 = __builtin_amdgcn_readlane(seen.y, i);
+            if (row >= a.tokens) break;
+            float o[D / 64], rm, rl;
+            row_forward<DT, D>(a, head, row, k0, k1, rm, rl, o);
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) o[x] = k0 < k1 ? o[x] / rl : 0.f;
+            store_row<DT, D>(a.o.to(row, head), o);
+            if (l == 0)
+                a.stats[static_cast<int64_t>(row) * a.n_heads + head] = k0 < k1 ? make_float2(rm, rl) : make_float2(0.f, 0.f);
+        }
         return;
     }
-    row_forward<DT, D>(a, head, r, seen.x, seen.y, m, l, acc);
-    const bool none = seen.x == seen.y;
+    if (r >= a.tokens) return;
+    zero_unless(some, acc);
+    float inv = some ? 1.f / sum : 0.f;
+    keep_finite<DT>(acc, inv);
+    if constexpr (DT == NF4_F16) inv = 1.f;
+    store_own<DT, D>(a.o.to(r, head), acc, inv);
+    if (g == 0) {
+        const bool f = fabsf(m) > kFar;
+        float2 ml = make_float2(f ? m : m + kTop<DT>, f ? sum : __builtin_amdgcn_ldexpf(sum, -static_cast<int>(kTop<DT>)));
+        a.stats[static_cast<int64_t>(r) * a.n_heads + head] = some ? ml : make_float2(0.f, 0.f);
+    }
+}
+
+// ----------------------------------------------------------------------------- backward
+//
+// What the backward pass reads of a row for every key, in blocks of 64 rows, four numbers each: m,
+// log2 l and m + log2 l (in fp16 less kTop), and D.  Where |m| is below kNear a probability's exponent
+// is taken with the sum of the first two, whose rounding (2^-16) is below those that follow.
+constexpr float kNear = 256.f;
+
+struct Back {
+    float *rows;   // [n_heads][blocks][4][64]
+    float *norms;  // fp16: the largest |do| of a block's rows [n_heads][blocks], then |v| [n_kv][blocks]
+    int blocks;
+    int tiles;     // of 128
+};
+
+// One workgroup per 64 rows and head; heads from n_heads on are those of v.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back b) {
+    constexpr int CH = D / 8, RPP = 256 / CH;
+    __shared__ float most[4];
+    const int head = blockIdx.y, ch = threadIdx.x % CH;
+    const bool of_v = head >= a.n_heads;
+    float worst = 0.f;
 #pragma unroll
-    for (int x = 0; x < D / 64; ++x) acc[x] = none ? 0.f : acc[x] / l;
-    store_row<DT, D>(a.o.to(r, head), acc);
-    if ((threadIdx.x & 63) == 0) a.stats[i] = none ? make_float2(0.f, 0.f) : make_float2(m, l);
+    for (int x = 0; x < kTile; x += RPP) {
+        const int i = x + threadIdx.x / CH, r = blockIdx.x * kTile + i;
+        float d = 0.f, sq = 0.f;
+        if (r < a.tokens) {
+            float go[8], o[8];
+            unpack8<DT>(*reinterpret_cast<const u32x4_t *>((of_v ? a.v.at(r, head - a.n_heads) : a.dout.at(r, head)) + ch * 8), go);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) sq = fmaf(go[e], go[e], sq);
+            if (!of_v) {
+                unpack8<DT>(*reinterpret_cast<const u32x4_t *>(a.o.at(r, head) + ch * 8), o);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) d = fmaf(go[e], o[e], d);
+            }
+        }
+#pragma unroll
+        for (int o = 1; o < CH; o <<= 1) {
+            d += __shfl_xor(d, o);
+            sq += __shfl_xor(sq, o);
+        }
+        worst = fmaxf(worst, sq);
+        if (of_v || ch) continue;
+        float2 ml = make_float2(0.f, 0.f);
+        if (r < a.tokens) ml = a.stats[static_cast<int64_t>(r) * a.n_heads + head];
+        const float ll = (ml.y == 0.f ? 0.f : log2f(ml.y)) - kTop<DT>;
+        float *p = b.rows + (static_cast<int64_t>(head) * b.blocks + blockIdx.x) * 256 + i;
+        p[0] = ml.x;
+        p[64] = ll;
+        p[128] = ml.x + ll;
+        p[192] = d;
+    }
+    if constexpr (DT == NF4_F16) {
+        worst = wave_max(worst);
+        if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = worst;
+        __syncthreads();
+        if (threadIdx.x == 0)
+            b.norms[static_cast<int64_t>(head) * b.blocks + blockIdx.x] =
+                sqrtf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
+    }
+}
+
+// fp16's dS, of at most 2 |do| |v|, are multiplied by this power of two (beside the 2^15 of P), so that
+// the largest is near 2^15; a plain fp16 of them would be 0 for the gradients of a loss that is not scaled.
+__device__ __forceinline__ float ds_scale(float bound) {
+    int e = 0;
+    bound *= 2.02f;
+    if (bound > 0.f && bound < INFINITY) (void)frexpf(bound, &e);
+    return ldexpf(1.f, -e);
+}
+
+__device__ __forceinline__ float most_of(const float *p, int n) {
+    float v = 0.f;
+    for (int i = threadIdx.x & 63; i < n; i += 64) v = fmaxf(v, p[i]);
+    return wave_max(v);
+}
+
+// |x|^2 of a lane's row, from its operands
+template <int DT, int D>
+__device__ __forceinline__ float square_of(const u32x4_t (&f)[D / 16]) {
+    float s = 0.f;
+#pragma unroll
+    for (int x = 0; x < D / 16; ++x) {
+        float v[8];
+        unpack8<DT>(f[x], v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) s = fmaf(v[i], v[i], s);
+    }
+    return s + other_half(s);
 }
 
 template <int DT, int D>
-__global__ __launch_bounds__(256) void attn_keys_kernel(const Attn a) {
-    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (i >= static_cast<int64_t>(a.tokens) * a.n_kv) return;
-    const int j = __builtin_amdgcn_readfirstlane(static_cast<int>(i / a.n_kv));
-    const int kvh = __builtin_amdgcn_readfirstlane(static_cast<int>(i % a.n_kv));
-    const int2 seen = rows_of(a, j);
-    float dk[D / 64] = {}, dv[D / 64] = {};
-    for (int h = 0; h < a.group; ++h)
-        key_backward<DT, D>(a, kvh * a.group + h, j, seen.x, seen.y, dk, dv);
+__device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block, uint8_t *lds) {
+    constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+    const int n = l & 31;
+    const int kvh = block % a.n_kv, y = block / a.n_kv;
+    const int head = kvh * a.group + y % a.group;
+    const int tile = b.tiles - 1 - y / a.group;
+    const int r = tile * kOwn + w * 32 + n;
+    const int2 seen = r < a.tokens ? keys_of(a, r) : make_int2(r, r);
+    Span sp;
+    sp.set(seen);
+    const int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
+
+    u32x4_t q[KS], go[KS];
+    own_operand<D>(q, a.q.at(r, head), r < a.tokens, 0);
+    own_operand<D>(go, a.dout.at(r, head), r < a.tokens, 0);
+    const float *rows = b.rows + (static_cast<int64_t>(head) * b.blocks + (r < a.tokens ? r >> 6 : 0)) * 256 + (r & 63);
+    const float m = rows[0], ll = rows[64], base = rows[128], delta = rows[192];
+    const bool near = __all(!(seen.x < seen.y) || fabsf(m) < kNear);
+    float fs = 1.f;
+    if constexpr (DT == NF4_F16) {
+        const int b0 = all.x >> 6, nb = all.x < all.y ? ((all.y - 1) >> 6) - b0 + 1 : 0;
+        fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb));
+    }
+    Stager<D> sk, sv;
+    sk.set(a.k, kvh);
+    sv.set(a.v, kvh);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) uint8_t *)lds));
+    const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
+    const uint32_t ra = lds0 + row_address<D>(), ca = lds0 + channel_address<D>();
+
+    float16_t acc[DN];
 #pragma unroll
-    for (int x = 0; x < D / 64; ++x) dk[x] *= a.scale;
-    store_row<DT, D>(a.dk.to(j, kvh), dk);
-    store_row<DT, D>(a.dv.to(j, kvh), dv);
+    for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
+    int k = all.x < all.y ? all.x & ~(kTile - 1) : all.y, st = 0;
+    if (k < all.y) {
+        sk.send(mine, k, all.y);
+        sv.send(mine + 2 * TB, k, all.y);
+    }
+    for (; k < all.y; k += kTile, st ^= 1) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (k + kTile < all.y) {
+            sk.send(mine + (st ^ 1) * TB, k + kTile, all.y);
+            sv.send(mine + (2 + (st ^ 1)) * TB, k + kTile, all.y);
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (sp.none(k + 32 * h, 32)) continue;
+            float16_t sc = (float16_t){}, dp;
+#pragma unroll
+            for (int e = 0; e < 16; ++e) dp[e] = -delta;
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int x = 0; x < KS; ++x) sc = mfma32<DT>(rows_operand<D>(ra + st * TB, h, x), q[x], sc);
+#pragma unroll
+            for (int x = 0; x < KS; ++x) dp = mfma32<DT>(rows_operand<D>(ra + (2 + st) * TB, h, x), go[x], dp);
+            __builtin_amdgcn_s_setprio(0);
+            if (__builtin_expect(near, 1)) {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[e] = fmaf(sc[e], a.c, -base);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; ++e) sc[e] = exponent(sc[e], a.c, m) - ll;
+            }
+            if (!sp.full(k + 32 * h, 32)) {
+                const uint64_t see = seen_bits(seen, k);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!bit_of(see, h, e)) sc[e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[e] = __builtin_amdgcn_exp2f(sc[e]) * dp[e];
+                if constexpr (DT == NF4_F16) sc[e] *= fs;
+            }
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const u32x4_t f = operand_of<DT>(sc, x);
+#pragma unroll
+                for (int d = 0; d < DN; ++d) acc[d] = mfma32<DT>(channels_operand<D>(ca + st * TB, 2 * h + x, d), f, acc[d]);
+            }
+            __builtin_amdgcn_s_setprio(0);
+        }
+    }
+    const bool some = seen.x < seen.y;
+    if (__any(some && !(odd_of(acc) == 0.f))) {  // as in the forward pass
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+            const int row = tile * kOwn + w * 32 + i;
+            if (row >= a.tokens) break;
+            float o[D / 64];
+            row_backward<DT, D>(a, head, row, __builtin_amdgcn_readlane(seen.x, i), __builtin_amdgcn_readlane(seen.y, i), o);
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) o[x] *= a.scale;
+            store_row<DT, D>(a.dq.to(row, head), o);
+        }
+        return;
+    }
+    if (r >= a.tokens) return;
+    zero_unless(some, acc);
+    store_own<DT, D>(a.dq.to(r, head), acc, a.scale * (ldexpf(1.f, -static_cast<int>(kTop<DT>)) / fs));
+}
+
+template <int DT, int D>
+constexpr int kBackLds = 2 * (2 * kTileBytes<D> + 1024) + 64;
+
+template <int DT, int D>
+__device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block, uint8_t *lds) {
+    constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+    const int g = l >> 5, n = l & 31;
+    const int kvh = block % a.n_kv, tile = block / a.n_kv;
+    const int j = tile * kOwn + w * 32 + n;
+    const int2 seen = j < a.tokens ? rows_of(a, j) : make_int2(j, j);
+    Span sp;
+    sp.set(seen);
+    const int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB + 2048));
+
+    u32x4_t kf[KS], vf[KS];
+    own_operand<D>(kf, a.k.at(j, kvh), j < a.tokens, 0);
+    own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, 0);
+    const int t0 = all.x < all.y ? all.x >> 6 : 0, per = all.x < all.y ? ((all.y - 1) >> 6) - t0 + 1 : 0;
+    float fs = 1.f;
+    if constexpr (DT == NF4_F16) {
+        float most = 0.f;
+        for (int h = 0; h < a.group; ++h)
+            most = fmaxf(most, most_of(b.norms + static_cast<int64_t>(kvh * a.group + h) * b.blocks + t0, per));
+        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most);
+    }
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) uint8_t *)lds));
+    const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
+    const uint32_t ra = lds0 + row_address<D>(), ca = lds0 + channel_address<D>();
+    const uint32_t rows0 = lds0 + 4 * TB;
+    Stager<D> sq, sg;
+    sq.set(a.q, kvh * a.group);
+    sg.set(a.dout, kvh * a.group);
+    // unit (head of the group, row tile), the next one
+    int uh = 0, ut = 0;
+    auto send = [&](int st) {
+        const int t = (t0 + ut) * kTile;
+        sq.send(mine + st * TB, t, all.y);
+        sg.send(mine + (2 + st) * TB, t, all.y);
+        if (w == 0) {
+            const float *p = b.rows + (static_cast<int64_t>(kvh * a.group + uh) * b.blocks + t0 + ut) * 256;
+            lds_dma16(__builtin_amdgcn_readfirstlane(rows0 + st * 1024), l * 16, make_rsrc(p, 1024), 0);
+        }
+        if (++ut == per) {
+            ut = 0;
+            ++uh;
+            sq.base += a.q.head;
+            sg.base += a.dout.head;
+        }
+    };
+    float16_t dk[DN], dv[DN];
+#pragma unroll
+    for (int x = 0; x < DN; ++x) dk[x] = dv[x] = (float16_t){};
+    const int units = per * a.group;
+    int t = 0, st = 0;
+    if (units) send(0);
+    for (int u = 0; u < units; ++u, st ^= 1) {
+        const int r = (t0 + t) * kTile;
+        if (++t == per) t = 0;
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (u + 1 < units) send(st ^ 1);
+        const uint32_t rw = rows0 + st * 1024;
+        auto row4 = [&](int kind, int h, int e) {  // rows 32 h + 2 e + 4 g .. of a kind
+            return __builtin_bit_cast(float4_t, lds16(rw + kind * 256 + (32 * h + 2 * e + 4 * g) * 4));
+        };
+        const float mine_m = *reinterpret_cast<const __attribute__((address_space(3))) float *>(static_cast<uintptr_t>(rw + l * 4));
+        const bool near = __all(fabsf(mine_m) < kNear);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            if (sp.none(r + 32 * h, 32)) continue;
+            float16_t sc = (float16_t){}, dp;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const float4_t d = row4(3, h, e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) dp[e + i] = -d[i];
+            }
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int x = 0; x < KS; ++x) sc = mfma32<DT>(rows_operand<D>(ra + st * TB, h, x), kf[x], sc);
+#pragma unroll
+            for (int x = 0; x < KS; ++x) dp = mfma32<DT>(rows_operand<D>(ra + (2 + st) * TB, h, x), vf[x], dp);
+            __builtin_amdgcn_s_setprio(0);
+            if (__builtin_expect(near, 1)) {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4_t base = row4(2, h, e);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[e + i] = fmaf(sc[e + i], a.c, -base[i]);
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; e += 4) {
+                    const float4_t m = row4(0, h, e), ll = row4(1, h, e);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) sc[e + i] = exponent(sc[e + i], a.c, m[i]) - ll[i];
+                }
+            }
+            if (!sp.full(r + 32 * h, 32)) {
+                const uint64_t see = seen_bits(seen, r);
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    if (!bit_of(see, h, e)) sc[e] = -INFINITY;
+            }
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                sc[e] = __builtin_amdgcn_exp2f(sc[e]);
+                dp[e] *= sc[e];
+                if constexpr (DT == NF4_F16) dp[e] *= fs;
+            }
+            __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const u32x4_t p = operand_of<DT>(sc, x), ds = operand_of<DT>(dp, x);
+#pragma unroll
+                for (int d = 0; d < DN; ++d) {
+                    dv[d] = mfma32<DT>(channels_operand<D>(ca + (2 + st) * TB, 2 * h + x, d), p, dv[d]);
+                    dk[d] = mfma32<DT>(channels_operand<D>(ca + st * TB, 2 * h + x, d), ds, dk[d]);
+                }
+            }
+            __builtin_amdgcn_s_setprio(0);
+        }
+    }
+    const bool some = seen.x < seen.y;
+    if (__any(some && !(odd_of(dk) + odd_of(dv) == 0.f))) {  // as in the forward pass
+#pragma unroll 1
+        for (int i = 0; i < 32; ++i) {
+            const int key = tile * kOwn + w * 32 + i;
+            if (key >= a.tokens) break;
+            const int r0 = __builtin_amdgcn_readlane(seen.x, i), r1 = __builtin_amdgcn_readlane(seen.y, i);
+            float gk[D / 64] = {}, gv[D / 64] = {};
+            for (int h = 0; h < a.group; ++h) key_backward<DT, D>(a, kvh * a.group + h, key, r0, r1, gk, gv);
+#pragma unroll
+            for (int x = 0; x < D / 64; ++x) gk[x] *= a.scale;
+            store_row<DT, D>(a.dk.to(key, kvh), gk);
+            store_row<DT, D>(a.dv.to(key, kvh), gv);
+        }
+        return;
+    }
+    if (j >= a.tokens) return;
+    zero_unless(some, dk);
+    zero_unless(some, dv);
+    const float one = ldexpf(1.f, -static_cast<int>(kTop<DT>));
+    store_own<DT, D>(a.dk.to(j, kvh), dk, a.scale * (one / fs));
+    store_own<DT, D>(a.dv.to(j, kvh), dv, one);
+}
+
+// The keys' workgroups first, then the rows'.
+template <int DT, int D>
+__global__ __launch_bounds__(256, 2) void attn_bwd_kernel(const Attn a, const Back b) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBackLds<DT, D>];
+    const int keys = b.tiles * a.n_kv, i = blockIdx.x;
+    if (i < keys) dkv_body<DT, D>(a, b, i, lds);
+    else dq_body<DT, D>(a, b, i - keys, lds);
 }
 
 // ------------------------------------------------------------------------- host
-
-struct Shape {
-    int head_dim, dtype;
-};
 
 // Strides of a dimension of one do not count.
 int take(Strided &s, const void *p, int64_t tok, int64_t head, int64_t tokens, int heads) {
@@ -279,20 +934,21 @@ int fill(Attn &a, const nf4_attn *in) {
     return NF4_OK;
 }
 
-dim3 waves(int64_t n) { return dim3(static_cast<unsigned>((n + 3) / 4)); }
+int tiles_of(const nf4_attn *in, int n) { return static_cast<int>((in->tokens + n - 1) / n); }
 
 template <int DT, int D>
-int launch(const Attn &a, bool grad, hipStream_t s) {
-    const int64_t rows = static_cast<int64_t>(a.tokens) * a.n_heads, keys = static_cast<int64_t>(a.tokens) * a.n_kv;
-    hipLaunchKernelGGL((attn_rows_kernel<DT, D>), waves(rows), dim3(256), 0, s, a, grad ? 1 : 0);
-    if (grad) hipLaunchKernelGGL((attn_keys_kernel<DT, D>), waves(keys), dim3(256), 0, s, a);
+int forward(const Attn &a, const nf4_attn *in, hipStream_t s) {
+    const int tiles = tiles_of(in, kOwn);
+    hipLaunchKernelGGL((attn_fwd_kernel<DT, D>), dim3(tiles * a.n_heads), dim3(256), 0, s, a, tiles);
     return status_of(hipGetLastError());
 }
 
-int launch_of(const Attn &a, const nf4_attn *in, bool grad, hipStream_t s) {
-    if (in->dtype == NF4_BF16)
-        return in->head_dim == 128 ? launch<NF4_BF16, 128>(a, grad, s) : launch<NF4_BF16, 64>(a, grad, s);
-    return in->head_dim == 128 ? launch<NF4_F16, 128>(a, grad, s) : launch<NF4_F16, 64>(a, grad, s);
+template <int DT, int D>
+int backward(const Attn &a, const nf4_attn *in, const Back &b, hipStream_t s) {
+    const dim3 rows(b.blocks, a.n_heads + (DT == NF4_F16 ? a.n_kv : 0));
+    hipLaunchKernelGGL((attn_rows_kernel<DT, D>), rows, dim3(256), 0, s, a, b);
+    hipLaunchKernelGGL((attn_bwd_kernel<DT, D>), dim3(b.tiles * (a.n_kv + a.n_heads)), dim3(256), 0, s, a, b);
+    return status_of(hipGetLastError());
 }
 
 // out and stats as both passes have them
@@ -302,6 +958,15 @@ int take_saved(Attn &a, const nf4_attn *in, const void *out, const float *stats)
     a.o = {static_cast<const uint16_t *>(out), static_cast<int64_t>(in->n_heads) * in->head_dim, in->head_dim};
     a.stats = reinterpret_cast<float2 *>(const_cast<float *>(stats));
     return NF4_OK;
+}
+
+// The backward pass's launch, and the bytes of its workspace.
+size_t plan(Back &b, const nf4_attn *in) {
+    b.blocks = tiles_of(in, kTile);
+    b.tiles = tiles_of(in, kOwn);
+    size_t n = static_cast<size_t>(in->n_heads) * b.blocks * 256;
+    if (in->dtype == NF4_F16) n += static_cast<size_t>(in->n_heads + in->n_kv) * b.blocks;
+    return n * 4;
 }
 
 }  // namespace
@@ -314,10 +979,17 @@ extern "C" int nf4_attn_fwd(const nf4_attn *in, void *out, float *stats, void *w
     int st = fill(a, in);
     if (st != NF4_OK || in->tokens == 0) return st;
     if ((st = take_saved(a, in, out, stats)) != NF4_OK) return st;
-    return launch_of(a, in, false, static_cast<hipStream_t>(stream));
+    auto s = static_cast<hipStream_t>(stream);
+    if (in->dtype == NF4_BF16)
+        return in->head_dim == 128 ? forward<NF4_BF16, 128>(a, in, s) : forward<NF4_BF16, 64>(a, in, s);
+    return in->head_dim == 128 ? forward<NF4_F16, 128>(a, in, s) : forward<NF4_F16, 64>(a, in, s);
 }
 
-extern "C" size_t nf4_attn_bwd_workspace(const nf4_attn *in) { return 0; }
+extern "C" size_t nf4_attn_bwd_workspace(const nf4_attn *in) {
+    Attn a{};
+    Back b{};
+    return fill(a, in) != NF4_OK || in->tokens == 0 ? 0 : plan(b, in);
+}
 
 extern "C" int nf4_attn_bwd(const nf4_attn *in, const void *out, const float *stats,
                             const nf4_grad *dout, const nf4_grad *dq, const nf4_grad *dk,
@@ -332,5 +1004,14 @@ extern "C" int nf4_attn_bwd(const nf4_attn *in, const void *out, const float *st
     if ((st = take(a.dq, dq, in->tokens, in->n_heads, in->head_dim)) != NF4_OK) return st;
     if ((st = take(a.dk, dk, in->tokens, in->n_kv, in->head_dim)) != NF4_OK) return st;
     if ((st = take(a.dv, dv, in->tokens, in->n_kv, in->head_dim)) != NF4_OK) return st;
-    return launch_of(a, in, true, static_cast<hipStream_t>(stream));
+    Back b{};
+    const size_t need = plan(b, in);
+    if (!workspace || workspace_bytes < need) return NF4_ERR_WORKSPACE;
+    if (!aligned(workspace, 16)) return NF4_ERR_UNSUPPORTED;
+    b.rows = static_cast<float *>(workspace);
+    b.norms = b.rows + static_cast<int64_t>(in->n_heads) * b.blocks * 256;
+    auto s = static_cast<hipStream_t>(stream);
+    if (in->dtype == NF4_BF16)
+        return in->head_dim == 128 ? backward<NF4_BF16, 128>(a, in, b, s) : backward<NF4_BF16, 64>(a, in, b, s);
+    return in->head_dim == 128 ? backward<NF4_F16, 128>(a, in, b, s) : backward<NF4_F16, 64>(a, in, b, s);
 }
