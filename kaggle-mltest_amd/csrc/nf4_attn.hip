@@ -375,22 +375,67 @@ __device__ __forceinline__ void keep_finite(float16_t (&v)[N], float f) {
     }
 }
 
+// Pieces.  Where a launch has too few tiles to fill the card, or they are too uneven, what a tile of
+// rows (or keys) goes over is cut into pieces of `per` steps, a workgroup each; what a piece leaves is
+// fp32 in `part`, and the join launch sums a tile's pieces in their order.  A tile in one piece writes
+// its result itself.
+struct Pieces {
+    int per, most;  // steps of a piece, at least; pieces of a tile, at most
+    float *part;    // [tiles * heads][most][arrays][128][D]
+    float2 *ml;     // forward: [tiles * heads][most][128]
+    __device__ __forceinline__ int of(int n) const {
+        const int p = (n + per - 1) / per;
+        return p < 1 ? 1 : p < most ? p : most;
+    }
+};
+
+// Steps [x, y) of piece i of p.
+__device__ __forceinline__ int2 steps_of(int n, int p, int i) {
+    const int per = (n + p - 1) / p, x = i * per;
+    return make_int2(x < n ? x : n, x + per < n ? x + per : n);
+}
+
+// This lane's channels of its row, unrounded, from a transposed result.
+template <int D>
+__device__ __forceinline__ void store_part(float *row, const float16_t (&v)[D / 32]) {
+    row += ((threadIdx.x & 63) >> 5) * 4;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<float4_t *>(row + x * 32 + e * 2) = (float4_t){v[x][e], v[x][e + 1], v[x][e + 2], v[x][e + 3]};
+}
+
+template <int D>
+__device__ __forceinline__ void store_part_row(float *row, const float (&v)[D / 64]) {
+    const int l = threadIdx.x & 63;
+#pragma unroll
+    for (int x = 0; x < D / 64; ++x) row[l * (D / 64) + x] = v[x];
+}
+
 // ------------------------------------------------------------------------------ forward
 
 template <int DT, int D>
-__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, int tiles) {
+__global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pieces pc, int tiles) {
     constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
     __shared__ __attribute__((aligned(16))) uint8_t lds[4 * TB + 64];
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     const int g = l >> 5, n = l & 31;
-    const int kvh = blockIdx.x % a.n_kv, y = blockIdx.x / a.n_kv;
+    const int piece = blockIdx.x / (tiles * a.n_heads), block = blockIdx.x % (tiles * a.n_heads);
+    const int kvh = block % a.n_kv, y = block / a.n_kv;
     const int head = kvh * a.group + y % a.group;
     const int tile = tiles - 1 - y / a.group;  // (the last rows see most: first)
     const int r = tile * kOwn + w * 32 + n;
     const int2 seen = r < a.tokens ? keys_of(a, r) : make_int2(r, r);
     Span sp;
     sp.set(seen);
-    const int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
+    int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
+    const int k0 = all.x & ~(kTile - 1), steps = all.x < all.y ? (all.y - k0 + kTile - 1) / kTile : 0;
+    const int pieces = pc.of(steps);
+    if (piece >= pieces) return;
+    const int2 mine_of = steps_of(steps, pieces, piece);
+    const int k1 = k0 + mine_of.y * kTile;  // (past the last key in the last piece)
+    all.y = k1 < all.y ? k1 : all.y;
 
     u32x4_t q[KS];
     const float c = fabsf(a.c);
@@ -408,7 +453,8 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, int tile
     float16_t acc[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
-    int k = all.x < all.y ? all.x & ~(kTile - 1) : all.y, st = 0;
+    const int first = k0 + mine_of.x * kTile;
+    int k = steps ? first : all.y, st = 0;
     if (k < all.y) {
         sk.send(mine, k, all.y);
         sv.send(mine + 2 * TB, k, all.y);
@@ -491,36 +537,92 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, int tile
     }
 
     sum += other_half(sum);
-    const bool some = seen.x < seen.y;
+    const int2 part = make_int2(seen.x > first ? seen.x : first, seen.y < all.y ? seen.y : all.y);  // of this piece
+    const bool some = part.x < part.y;
     const float odd = odd_of(acc);
+    const int64_t slot = ((static_cast<int64_t>(tile) * a.n_heads + head) * pc.most + piece) * kOwn + w * 32;
     if (__any(some && !(odd == 0.f && sum > 0.f && sum < INFINITY && fabsf(m) < INFINITY))) {
         // An infinity or NaN: a product with a probability of 0 that stands for a key that is not
         // seen is none, and each row is formed from what it sees alone.
 #pragma unroll 1
         for (int i = 0; i < 32; ++i) {
             const int row = tile * kOwn + w * 32 + i;
-            const int k0 = __builtin_amdgcn_readlane(seen.x, i), k1 = __builtin_amdgcn_readlane(seen.y, i);
+            const int x0 = __builtin_amdgcn_readlane(part.x, i), x1 = __builtin_amdgcn_readlane(part.y, i);
             if (row >= a.tokens) break;
             float o[D / 64], rm, rl;
-            row_forward<DT, D>(a, head, row, k0, k1, rm, rl, o);
+            row_forward<DT, D>(a, head, row, x0, x1, rm, rl, o);
+            if (x0 >= x1) rm = rl = 0.f;
+            if (pieces > 1) {
+                store_part_row<D>(pc.part + (slot + i) * D, o);
+                if (l == 0) pc.ml[slot + i] = make_float2(rm, rl);
+                continue;
+            }
 #pragma unroll
-            for (int x = 0; x < D / 64; ++x) o[x] = k0 < k1 ? o[x] / rl : 0.f;
+            for (int x = 0; x < D / 64; ++x) o[x] = x0 < x1 ? o[x] / rl : 0.f;
             store_row<DT, D>(a.o.to(row, head), o);
-            if (l == 0)
-                a.stats[static_cast<int64_t>(row) * a.n_heads + head] = k0 < k1 ? make_float2(rm, rl) : make_float2(0.f, 0.f);
+            if (l == 0) a.stats[static_cast<int64_t>(row) * a.n_heads + head] = make_float2(rm, rl);
         }
         return;
     }
     if (r >= a.tokens) return;
     zero_unless(some, acc);
+    const bool f = fabsf(m) > kFar;
+    float2 ml = make_float2(f ? m : m + kTop<DT>, f ? sum : __builtin_amdgcn_ldexpf(sum, -static_cast<int>(kTop<DT>)));
+    if (!some) ml = make_float2(0.f, 0.f);
+    if (pieces > 1) {
+        if (!f && some)
+#pragma unroll
+            for (int x = 0; x < DN; ++x) acc[x] *= __builtin_amdgcn_ldexpf(1.f, -static_cast<int>(kTop<DT>));
+        store_part<D>(pc.part + (slot + n) * D, acc);
+        if (g == 0) pc.ml[slot + n] = ml;
+        return;
+    }
     float inv = some ? 1.f / sum : 0.f;
     keep_finite<DT>(acc, inv);
     if constexpr (DT == NF4_F16) inv = 1.f;
     store_own<DT, D>(a.o.to(r, head), acc, inv);
-    if (g == 0) {
-        const bool f = fabsf(m) > kFar;
-        float2 ml = make_float2(f ? m : m + kTop<DT>, f ? sum : __builtin_amdgcn_ldexpf(sum, -static_cast<int>(kTop<DT>)));
-        a.stats[static_cast<int64_t>(r) * a.n_heads + head] = some ? ml : make_float2(0.f, 0.f);
+    if (g == 0) a.stats[static_cast<int64_t>(r) * a.n_heads + head] = ml;
+}
+
+// A workgroup joins 32 rows of a tile that is in pieces: each a (m, l, o) of its keys.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Attn a, const Pieces pc) {
+    constexpr int PER = 1024 / D;  // rows that the workgroup takes at a time, 4 channels a thread
+    __shared__ int mem[8];
+    const int tile = blockIdx.x >> 2, head = blockIdx.y, r0 = tile * kOwn;
+    const int t = r0 + (threadIdx.x & 127);
+    Span sp;
+    sp.set(t < a.tokens ? keys_of(a, t) : make_int2(t, t));
+    const int2 all = sp.all(mem);
+    const int k0 = all.x & ~(kTile - 1), steps = all.x < all.y ? (all.y - k0 + kTile - 1) / kTile : 0;
+    const int pieces = pc.of(steps);
+    if (pieces < 2) return;
+    const int64_t slot = (static_cast<int64_t>(tile) * a.n_heads + head) * pc.most * kOwn;
+    const int ch = threadIdx.x % (D / 4) * 4;
+    for (int i = (blockIdx.x & 3) * 32 + threadIdx.x / (D / 4); i < (blockIdx.x & 3) * 32 + 32; i += PER) {
+        const int r = r0 + i;
+        if (r >= a.tokens) break;
+        float m = -INFINITY, l = 0.f;
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < pieces; ++p) {
+            const float2 x = pc.ml[slot + p * kOwn + i];
+            if (x.y != 0.f) m = fmaxf(m, x.x);
+        }
+        for (int p = 0; p < pieces; ++p) {
+            const float2 x = pc.ml[slot + p * kOwn + i];
+            if (x.y == 0.f) continue;  // (it saw nothing)
+            const float f = x.x == m ? 1.f : __builtin_amdgcn_exp2f(x.x - m);
+            l += x.y * f;
+            o += *reinterpret_cast<const float4_t *>(pc.part + (slot + p * kOwn + i) * D + ch) * f;
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        float4_t v = o * inv;
+        if constexpr (DT == NF4_F16)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[e] = fabsf(v[e]) < INFINITY ? __builtin_amdgcn_fmed3f(v[e], -65504.f, 65504.f) : v[e];
+        *reinterpret_cast<u32x2_t *>(a.o.to(r, head) + ch) = (u32x2_t){pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+        if (ch == 0) a.stats[static_cast<int64_t>(r) * a.n_heads + head] = l == 0.f ? make_float2(0.f, 0.f) : make_float2(m, l);
     }
 }
 
@@ -536,6 +638,7 @@ struct Back {
     float *norms;  // fp16: the largest |do| of a block's rows [n_heads][blocks], then |v| [n_kv][blocks]
     int blocks;
     int tiles;     // of 128
+    Pieces row, key;
 };
 
 // One workgroup per 64 rows and head; heads from n_heads on are those of v.
@@ -621,6 +724,8 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
     constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     const int n = l & 31;
+    const int piece = block / (b.tiles * a.n_heads);
+    block %= b.tiles * a.n_heads;
     const int kvh = block % a.n_kv, y = block / a.n_kv;
     const int head = kvh * a.group + y % a.group;
     const int tile = b.tiles - 1 - y / a.group;
@@ -628,7 +733,13 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
     const int2 seen = r < a.tokens ? keys_of(a, r) : make_int2(r, r);
     Span sp;
     sp.set(seen);
-    const int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
+    int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
+    const int k0 = all.x & ~(kTile - 1), steps = all.x < all.y ? (all.y - k0 + kTile - 1) / kTile : 0;
+    const int pieces = b.row.of(steps);
+    if (piece >= pieces) return;
+    const int2 mine_of = steps_of(steps, pieces, piece);
+    const int first = k0 + mine_of.x * kTile, k1 = k0 + mine_of.y * kTile;
+    all.y = k1 < all.y ? k1 : all.y;
 
     u32x4_t q[KS], go[KS];
     own_operand<D>(q, a.q.at(r, head), r < a.tokens, 0);
@@ -638,7 +749,7 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
     const bool near = __all(!(seen.x < seen.y) || fabsf(m) < kNear);
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
-        const int b0 = all.x >> 6, nb = all.x < all.y ? ((all.y - 1) >> 6) - b0 + 1 : 0;
+        const int b0 = first >> 6, nb = mine_of.y - mine_of.x;
         fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb));
     }
     Stager<D> sk, sv;
@@ -652,7 +763,7 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
     float16_t acc[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
-    int k = all.x < all.y ? all.x & ~(kTile - 1) : all.y, st = 0;
+    int k = steps ? first : all.y, st = 0;
     if (k < all.y) {
         sk.send(mine, k, all.y);
         sv.send(mine + 2 * TB, k, all.y);
@@ -704,23 +815,33 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
             __builtin_amdgcn_s_setprio(0);
         }
     }
-    const bool some = seen.x < seen.y;
+    const int2 part = make_int2(seen.x > first ? seen.x : first, seen.y < all.y ? seen.y : all.y);  // of this piece
+    const bool some = part.x < part.y;
+    const int64_t slot = ((static_cast<int64_t>(tile) * a.n_heads + head) * b.row.most + piece) * kOwn + w * 32;
     if (__any(some && !(odd_of(acc) == 0.f))) {  // as in the forward pass
 #pragma unroll 1
         for (int i = 0; i < 32; ++i) {
             const int row = tile * kOwn + w * 32 + i;
             if (row >= a.tokens) break;
             float o[D / 64];
-            row_backward<DT, D>(a, head, row, __builtin_amdgcn_readlane(seen.x, i), __builtin_amdgcn_readlane(seen.y, i), o);
+            row_backward<DT, D>(a, head, row, __builtin_amdgcn_readlane(part.x, i), __builtin_amdgcn_readlane(part.y, i), o);
 #pragma unroll
             for (int x = 0; x < D / 64; ++x) o[x] *= a.scale;
-            store_row<DT, D>(a.dq.to(row, head), o);
+            if (pieces > 1) store_part_row<D>(b.row.part + (slot + i) * D, o);
+            else store_row<DT, D>(a.dq.to(row, head), o);
         }
         return;
     }
     if (r >= a.tokens) return;
     zero_unless(some, acc);
-    store_own<DT, D>(a.dq.to(r, head), acc, a.scale * (ldexpf(1.f, -static_cast<int>(kTop<DT>)) / fs));
+    const float f = a.scale * (ldexpf(1.f, -static_cast<int>(kTop<DT>)) / fs);
+    if (pieces > 1) {
+#pragma unroll
+        for (int x = 0; x < DN; ++x) acc[x] *= f;
+        store_part<D>(b.row.part + (slot + n) * D, acc);
+    } else {
+        store_own<DT, D>(a.dq.to(r, head), acc, f);
+    }
 }
 
 template <int DT, int D>
@@ -731,6 +852,8 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
     constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     const int g = l >> 5, n = l & 31;
+    const int piece = block / (b.tiles * a.n_kv);
+    block %= b.tiles * a.n_kv;
     const int kvh = block % a.n_kv, tile = block / a.n_kv;
     const int j = tile * kOwn + w * 32 + n;
     const int2 seen = j < a.tokens ? rows_of(a, j) : make_int2(j, j);
@@ -738,10 +861,14 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
     sp.set(seen);
     const int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB + 2048));
 
+    const int t0 = all.x < all.y ? all.x >> 6 : 0, per = all.x < all.y ? ((all.y - 1) >> 6) - t0 + 1 : 0;
+    const int pieces = b.key.of(per * a.group);
+    if (piece >= pieces) return;
+    const int2 units = steps_of(per * a.group, pieces, piece);
+
     u32x4_t kf[KS], vf[KS];
     own_operand<D>(kf, a.k.at(j, kvh), j < a.tokens, 0);
     own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, 0);
-    const int t0 = all.x < all.y ? all.x >> 6 : 0, per = all.x < all.y ? ((all.y - 1) >> 6) - t0 + 1 : 0;
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
         float most = 0.f;
@@ -758,7 +885,10 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
     sq.set(a.q, kvh * a.group);
     sg.set(a.dout, kvh * a.group);
     // unit (head of the group, row tile), the next one
-    int uh = 0, ut = 0;
+    int uh = per ? units.x / per : 0, ut = units.x - uh * per;
+    sq.base += uh * a.q.head;
+    sg.base += uh * a.dout.head;
+    int t = ut, st = 0;
     auto send = [&](int st) {
         const int t = (t0 + ut) * kTile;
         sq.send(mine + st * TB, t, all.y);
@@ -777,15 +907,13 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
     float16_t dk[DN], dv[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) dk[x] = dv[x] = (float16_t){};
-    const int units = per * a.group;
-    int t = 0, st = 0;
-    if (units) send(0);
-    for (int u = 0; u < units; ++u, st ^= 1) {
+    if (units.x < units.y) send(0);
+    for (int u = units.x; u < units.y; ++u, st ^= 1) {
         const int r = (t0 + t) * kTile;
         if (++t == per) t = 0;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (u + 1 < units) send(st ^ 1);
+        if (u + 1 < units.y) send(st ^ 1);
         const uint32_t rw = rows0 + st * 1024;
         auto row4 = [&](int kind, int h, int e) {  // rows 32 h + 2 e + 4 g .. of a kind
             return __builtin_bit_cast(float4_t, lds16(rw + kind * 256 + (32 * h + 2 * e + 4 * g) * 4));
@@ -849,6 +977,7 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
         }
     }
     const bool some = seen.x < seen.y;
+    const int64_t slot = ((static_cast<int64_t>(tile) * a.n_kv + kvh) * b.key.most + piece) * 2 * kOwn + w * 32;
     if (__any(some && !(odd_of(dk) + odd_of(dv) == 0.f))) {  // as in the forward pass
 #pragma unroll 1
         for (int i = 0; i < 32; ++i) {
@@ -856,9 +985,18 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
             if (key >= a.tokens) break;
             const int r0 = __builtin_amdgcn_readlane(seen.x, i), r1 = __builtin_amdgcn_readlane(seen.y, i);
             float gk[D / 64] = {}, gv[D / 64] = {};
-            for (int h = 0; h < a.group; ++h) key_backward<DT, D>(a, kvh * a.group + h, key, r0, r1, gk, gv);
+            for (int h = units.x / per; h * per < units.y; ++h) {  // the piece's rows of each head
+                const int u0 = h * per > units.x ? h * per : units.x, u1 = (h + 1) * per < units.y ? (h + 1) * per : units.y;
+                const int x0 = (t0 + u0 - h * per) * kTile, x1 = (t0 + u1 - h * per) * kTile;
+                key_backward<DT, D>(a, kvh * a.group + h, key, r0 > x0 ? r0 : x0, r1 < x1 ? r1 : x1, gk, gv);
+            }
 #pragma unroll
             for (int x = 0; x < D / 64; ++x) gk[x] *= a.scale;
+            if (pieces > 1) {
+                store_part_row<D>(b.key.part + (slot + i) * D, gk);
+                store_part_row<D>(b.key.part + (slot + kOwn + i) * D, gv);
+                continue;
+            }
             store_row<DT, D>(a.dk.to(key, kvh), gk);
             store_row<DT, D>(a.dv.to(key, kvh), gv);
         }
@@ -867,8 +1005,18 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
     if (j >= a.tokens) return;
     zero_unless(some, dk);
     zero_unless(some, dv);
-    const float one = ldexpf(1.f, -static_cast<int>(kTop<DT>));
-    store_own<DT, D>(a.dk.to(j, kvh), dk, a.scale * (one / fs));
+    const float one = ldexpf(1.f, -static_cast<int>(kTop<DT>)), f = a.scale * (one / fs);
+    if (pieces > 1) {
+#pragma unroll
+        for (int x = 0; x < DN; ++x) {
+            dk[x] *= f;
+            dv[x] *= one;
+        }
+        store_part<D>(b.key.part + (slot + n) * D, dk);
+        store_part<D>(b.key.part + (slot + kOwn + n) * D, dv);
+        return;
+    }
+    store_own<DT, D>(a.dk.to(j, kvh), dk, f);
     store_own<DT, D>(a.dv.to(j, kvh), dv, one);
 }
 
@@ -876,9 +1024,43 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_bwd_kernel(const Attn a, const Back b) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBackLds<DT, D>];
-    const int keys = b.tiles * a.n_kv, i = blockIdx.x;
+    const int keys = b.tiles * a.n_kv * b.key.most, i = blockIdx.x;
     if (i < keys) dkv_body<DT, D>(a, b, i, lds);
     else dq_body<DT, D>(a, b, i - keys, lds);
+}
+
+// A workgroup sums the pieces of 32 rows of dq, or of 32 keys of dk or dv: grid x = tiles of 128 times
+// 4, y = heads of dq, then of dk, then of dv.
+template <int DT, int D>
+__global__ __launch_bounds__(256) void attn_bwd_join_kernel(const Attn a, const Back b) {
+    constexpr int PER = 1024 / D;  // rows that the workgroup takes at a time, 4 channels a thread
+    __shared__ int mem[8];
+    const int tile = blockIdx.x >> 2, r0 = tile * kOwn, t = r0 + (threadIdx.x & 127);
+    int head = blockIdx.y, array = 0;
+    const bool of_keys = head >= a.n_heads;
+    if (of_keys) {
+        array = head >= a.n_heads + a.n_kv;
+        head -= a.n_heads + array * a.n_kv;
+    }
+    Span sp;
+    sp.set(t < a.tokens ? (of_keys ? rows_of(a, t) : keys_of(a, t)) : make_int2(t, t));
+    const int2 all = sp.all(mem);
+    const int t0 = all.x >> 6, steps = all.x < all.y ? ((all.y - 1) >> 6) - t0 + 1 : 0;
+    const Pieces &pc = of_keys ? b.key : b.row;
+    const int pieces = pc.of(of_keys ? steps * a.group : steps), arrays = of_keys ? 2 : 1;
+    if (pieces < 2) return;
+    const Strided &out = !of_keys ? a.dq : array ? a.dv : a.dk;
+    const float *part = pc.part + ((static_cast<int64_t>(tile) * (of_keys ? a.n_kv : a.n_heads) + head) * pc.most * arrays + array) * kOwn * D;
+    const int ch = threadIdx.x % (D / 4) * 4;
+#pragma unroll
+    for (int x = 0; x < 32; x += PER) {
+        const int i = (blockIdx.x & 3) * 32 + x + threadIdx.x / (D / 4);
+        if (r0 + i >= a.tokens) break;
+        float4_t v = {0.f, 0.f, 0.f, 0.f};
+        for (int p = 0; p < pieces; ++p)
+            v += *reinterpret_cast<const float4_t *>(part + (static_cast<int64_t>(p) * arrays * kOwn + i) * D + ch);
+        *reinterpret_cast<u32x2_t *>(out.to(r0 + i, head) + ch) = (u32x2_t){pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+    }
 }
 
 // ------------------------------------------------------------------------- host
@@ -937,17 +1119,20 @@ int fill(Attn &a, const nf4_attn *in) {
 int tiles_of(const nf4_attn *in, int n) { return static_cast<int>((in->tokens + n - 1) / n); }
 
 template <int DT, int D>
-int forward(const Attn &a, const nf4_attn *in, hipStream_t s) {
-    const int tiles = tiles_of(in, kOwn);
-    hipLaunchKernelGGL((attn_fwd_kernel<DT, D>), dim3(tiles * a.n_heads), dim3(256), 0, s, a, tiles);
+int forward(const Attn &a, const Pieces &pc, int tiles, hipStream_t s) {
+    hipLaunchKernelGGL((attn_fwd_kernel<DT, D>), dim3(tiles * a.n_heads * pc.most), dim3(256), 0, s, a, pc, tiles);
+    if (pc.most > 1) hipLaunchKernelGGL((attn_fwd_join_kernel<DT, D>), dim3(tiles * 4, a.n_heads), dim3(256), 0, s, a, pc);
     return status_of(hipGetLastError());
 }
 
 template <int DT, int D>
-int backward(const Attn &a, const nf4_attn *in, const Back &b, hipStream_t s) {
+int backward(const Attn &a, const Back &b, hipStream_t s) {
     const dim3 rows(b.blocks, a.n_heads + (DT == NF4_F16 ? a.n_kv : 0));
+    const dim3 join(b.tiles * 4, a.n_heads + 2 * a.n_kv);
     hipLaunchKernelGGL((attn_rows_kernel<DT, D>), rows, dim3(256), 0, s, a, b);
-    hipLaunchKernelGGL((attn_bwd_kernel<DT, D>), dim3(b.tiles * (a.n_kv + a.n_heads)), dim3(256), 0, s, a, b);
+    hipLaunchKernelGGL((attn_bwd_kernel<DT, D>), dim3(b.tiles * (a.n_kv * b.key.most + a.n_heads * b.row.most)), dim3(256), 0, s, a, b);
+    if (b.row.most > 1 || b.key.most > 1)
+        hipLaunchKernelGGL((attn_bwd_join_kernel<DT, D>), join, dim3(256), 0, s, a, b);
     return status_of(hipGetLastError());
 }
 
@@ -960,18 +1145,74 @@ int take_saved(Attn &a, const nf4_attn *in, const void *out, const float *stats)
     return NF4_OK;
 }
 
-// The backward pass's launch, and the bytes of its workspace.
+constexpr int kPlaces = 512;  // workgroups that the card holds: two a CU
+
+// What a row of the longest sequence sees, as the host knows it.
+int64_t span_of(const nf4_attn *in) {
+    return in->max_len && in->max_len < in->tokens ? in->max_len : in->tokens;
+}
+
+// Steps of 64 of a tile of 128 rows (or keys): on average, and at most.
+struct Steps {
+    double mean;
+    int64_t most;
+};
+Steps steps_of(const nf4_attn *in) {
+    const int64_t span = span_of(in), w = in->window && in->window < span ? in->window : span;
+    // (a tile's rows see w + 127 keys of a long sequence's middle, and half as many on average where
+    // the window is all of it)
+    const double seen = w < span ? static_cast<double>(w) : 0.5 * span;
+    return {seen / kTile + 1.5, (w + kOwn - 1) / kTile + 2};
+}
+
+Pieces cut(double total, int64_t most, int per_least) {
+    Pieces p{};
+    int64_t per = static_cast<int64_t>(total / kPlaces) + 1;
+    if (per < per_least) per = per_least;
+    p.per = static_cast<int>(per);
+    p.most = static_cast<int>((most + per - 1) / per);
+    if (p.most > 64) p.most = 64;
+    return p;
+}
+
+// The forward pass's launch, and the bytes of its workspace.
+size_t plan(Pieces &p, const nf4_attn *in) {
+    const int64_t items = static_cast<int64_t>(tiles_of(in, kOwn)) * in->n_heads;
+    const Steps n = steps_of(in);
+    p = cut(items * n.mean, n.most, 6);
+    if (items >= 2 * kPlaces || p.most < 2) p = {1 << 30, 1, nullptr, nullptr};
+    return p.most > 1 ? items * p.most * kOwn * (in->head_dim * 4 + 8) : 0;
+}
+
+// The backward pass's, in 4-byte words after each other: rows, norms, rows' parts, keys' parts.
 size_t plan(Back &b, const nf4_attn *in) {
     b.blocks = tiles_of(in, kTile);
     b.tiles = tiles_of(in, kOwn);
-    size_t n = static_cast<size_t>(in->n_heads) * b.blocks * 256;
-    if (in->dtype == NF4_F16) n += static_cast<size_t>(in->n_heads + in->n_kv) * b.blocks;
-    return n * 4;
+    const int64_t rows = static_cast<int64_t>(b.tiles) * in->n_heads, keys = static_cast<int64_t>(b.tiles) * in->n_kv;
+    const Steps n = steps_of(in);
+    const int group = in->n_heads / in->n_kv;
+    b.row = cut(rows * n.mean, n.most, 8);
+    if (rows >= 2 * kPlaces || b.row.most < 2) b.row = {1 << 30, 1, nullptr, nullptr};
+    b.key = cut(rows * n.mean, n.most * group, static_cast<int>(sqrt(rows * n.mean) / 5));
+    int64_t at = static_cast<int64_t>(in->n_heads) * b.blocks * 256;
+    auto next = [&](int64_t words) {
+        float *p = reinterpret_cast<float *>(at * 4);
+        at += (words + 3) / 4 * 4;
+        return p;
+    };
+    b.norms = next(in->dtype == NF4_F16 ? static_cast<int64_t>(in->n_heads + in->n_kv) * b.blocks : 0);
+    b.row.part = next(b.row.most > 1 ? rows * b.row.most * kOwn * in->head_dim : 0);
+    b.key.part = next(b.key.most > 1 ? keys * b.key.most * 2 * kOwn * in->head_dim : 0);
+    return at * 4;
 }
 
 }  // namespace
 
-extern "C" size_t nf4_attn_fwd_workspace(const nf4_attn *in) { return 0; }
+extern "C" size_t nf4_attn_fwd_workspace(const nf4_attn *in) {
+    Attn a{};
+    Pieces p{};
+    return fill(a, in) != NF4_OK || in->tokens == 0 ? 0 : plan(p, in);
+}
 
 extern "C" int nf4_attn_fwd(const nf4_attn *in, void *out, float *stats, void *workspace,
                             size_t workspace_bytes, void *stream) {
@@ -979,10 +1220,19 @@ extern "C" int nf4_attn_fwd(const nf4_attn *in, void *out, float *stats, void *w
     int st = fill(a, in);
     if (st != NF4_OK || in->tokens == 0) return st;
     if ((st = take_saved(a, in, out, stats)) != NF4_OK) return st;
+    Pieces p{};
+    const size_t need = plan(p, in);
+    const int tiles = tiles_of(in, kOwn);
+    if (need) {
+        if (!workspace || workspace_bytes < need) return NF4_ERR_WORKSPACE;
+        if (!aligned(workspace, 16)) return NF4_ERR_UNSUPPORTED;
+        p.part = static_cast<float *>(workspace);
+        p.ml = reinterpret_cast<float2 *>(p.part + static_cast<int64_t>(tiles) * in->n_heads * p.most * kOwn * in->head_dim);
+    }
     auto s = static_cast<hipStream_t>(stream);
     if (in->dtype == NF4_BF16)
-        return in->head_dim == 128 ? forward<NF4_BF16, 128>(a, in, s) : forward<NF4_BF16, 64>(a, in, s);
-    return in->head_dim == 128 ? forward<NF4_F16, 128>(a, in, s) : forward<NF4_F16, 64>(a, in, s);
+        return in->head_dim == 128 ? forward<NF4_BF16, 128>(a, p, tiles, s) : forward<NF4_BF16, 64>(a, p, tiles, s);
+    return in->head_dim == 128 ? forward<NF4_F16, 128>(a, p, tiles, s) : forward<NF4_F16, 64>(a, p, tiles, s);
 }
 
 extern "C" size_t nf4_attn_bwd_workspace(const nf4_attn *in) {
@@ -1008,10 +1258,11 @@ extern "C" int nf4_attn_bwd(const nf4_attn *in, const void *out, const float *st
     const size_t need = plan(b, in);
     if (!workspace || workspace_bytes < need) return NF4_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return NF4_ERR_UNSUPPORTED;
+    char *ws = static_cast<char *>(workspace);
     b.rows = static_cast<float *>(workspace);
-    b.norms = b.rows + static_cast<int64_t>(in->n_heads) * b.blocks * 256;
+    for (float **p : {&b.norms, &b.row.part, &b.key.part}) *p = reinterpret_cast<float *>(ws + reinterpret_cast<uintptr_t>(*p));
     auto s = static_cast<hipStream_t>(stream);
     if (in->dtype == NF4_BF16)
-        return in->head_dim == 128 ? backward<NF4_BF16, 128>(a, in, b, s) : backward<NF4_BF16, 64>(a, in, b, s);
-    return in->head_dim == 128 ? backward<NF4_F16, 128>(a, in, b, s) : backward<NF4_F16, 64>(a, in, b, s);
+        return in->head_dim == 128 ? backward<NF4_BF16, 128>(a, b, s) : backward<NF4_BF16, 64>(a, b, s);
+    return in->head_dim == 128 ? backward<NF4_F16, 128>(a, b, s) : backward<NF4_F16, 64>(a, b, s);
 }
