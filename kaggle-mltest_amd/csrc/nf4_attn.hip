@@ -11,6 +11,8 @@
 
 #include "nf4_common.h"
 
+#include <math.h>
+
 namespace {
 
 struct Strided {  // [tokens, heads, D]: offsets in elements
@@ -29,28 +31,62 @@ struct Attn {
     float scale;
 };
 
-// The rows [s, e) of row t's sequence, or [t, t) of a row that belongs to none.
+// How many offsets are at or before t (the wave's), 64 at a time: a load's latency for every factor of
+// 64 of the batch.
+__device__ __forceinline__ int offsets_upto(const Attn &a, int t) {
+    const int l = threadIdx.x & 63;
+    int lo = 0, n = a.batch + 1;
+    while (n > 64) {
+        const int step = (n + 63) >> 6, i = l * step;
+        const int c = __popcll(__ballot(i < n && a.cu[lo + i] <= t));
+        if (c == 0) return lo;
+        const int past = (c - 1) * step + 1;  // the offset c - 1 steps on is at or before t
+        lo += past;
+        n = n - past < step - 1 ? n - past : step - 1;
+    }
+    return lo + __popcll(__ballot(l < n && a.cu[lo + l] <= t));
+}
+
+// The rows [s, e) of the sequence of row t, or [t, t) of a row that belongs to none.  Every lane of the
+// wave calls it, with rows of at most 32 from the first lane's on.
 __device__ __forceinline__ int2 sequence_of(const Attn &a, int t) {
     if (!a.cu) return make_int2(0, a.tokens);
-    int lo = 0, hi = a.batch + 1;  // the first offset past t
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= t) lo = mid + 1;
-        else hi = mid;
+    // the next 64 offsets, a lane each, from the first row's sequence on
+    const int i0 = offsets_upto(a, __builtin_amdgcn_readfirstlane(t)) - 1, l = threadIdx.x & 63;
+    const int at = i0 + l < 0 ? 0 : i0 + l;
+    const int next = at <= a.batch ? a.cu[at] : 0x7fffffff;
+    int s = i0 < 0 ? 0x7fffffff : __builtin_amdgcn_readlane(next, 0), e = __builtin_amdgcn_readlane(next, 1);
+    int k = 1;
+    for (; k < 63 && __any(t >= e); ++k) {
+        const int x = __builtin_amdgcn_readlane(next, k + 1);
+        if (t >= e) {
+            s = e;
+            e = x;
+        }
     }
-    if (lo == 0 || lo > a.batch) return make_int2(t, t);
-    const int s = a.cu[lo - 1], e = a.cu[lo];
+    if (__any(t >= e)) {  // (more than 62 sequences in 32 rows: empty ones)
+        int lo = 0, hi = a.batch + 1;  // the first offset past t
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (a.cu[mid] <= t) lo = mid + 1;
+            else hi = mid;
+        }
+        s = lo == 0 ? 0x7fffffff : a.cu[lo - 1];
+        e = lo > a.batch ? 0x7fffffff : a.cu[lo];
+    }
+    if (s > t || e <= t || e == 0x7fffffff) return make_int2(t, t);
     return make_int2(s < 0 ? 0 : s, e > a.tokens ? a.tokens : e);
 }
 
-// The keys [lo, hi) that row t sees, and the rows [t, hi) that see key t.
+// The keys [lo, hi) that row t sees, and the rows [t, hi) that see key t (t as above, or past the last
+// row: none).
 __device__ __forceinline__ int2 keys_of(const Attn &a, int t) {
-    const int2 s = sequence_of(a, t);
+    const int2 s = sequence_of(a, t < a.tokens ? t : a.tokens - 1);
     if (s.y <= t) return make_int2(t, t);
     return make_int2(a.window && t - a.window + 1 > s.x ? t - a.window + 1 : s.x, t + 1);
 }
 __device__ __forceinline__ int2 rows_of(const Attn &a, int t) {
-    const int2 s = sequence_of(a, t);
+    const int2 s = sequence_of(a, t < a.tokens ? t : a.tokens - 1);
     if (s.y <= t) return make_int2(t, t);
     return make_int2(t, a.window && t + a.window < s.y ? t + a.window : s.y);
 }
@@ -206,9 +242,9 @@ template <int D>
 constexpr int kTileBytes = kTile * D * 2;
 
 // What a thread knows of a tensor's tiles: the byte of its 16 in the first pass, and its rows' pitch.
-template <int D>
+template <int D, int ROWS>
 struct Stager {
-    static constexpr int CH = D / 8, RPP = 256 / CH, PASS = kTile / RPP;
+    static constexpr int CH = D / 8, RPP = 256 / CH;
     const uint16_t *base;  // the head's first row
     int64_t tok;
     int off, step;
@@ -220,12 +256,12 @@ struct Stager {
         off = row * static_cast<int>(tok) * 2 + ((ch ^ swizzle<D>(row)) << 4);
         step = RPP * static_cast<int>(tok) * 2;
     }
-    // rows [t, t + 64) to LDS address `at` (the wave's); rows from `end` on are zeros, and not read
+    // rows [t, t + ROWS) to LDS address `at` (the wave's); rows from `end` on are zeros, and not read
     __device__ __forceinline__ void send(uint32_t at, int t, int end) const {
         const int64_t bytes = t < end ? (end - t - 1) * tok * 2 + D * 2 : 0;
         const rsrc_t r = make_rsrc(base + t * tok, bytes);
 #pragma unroll
-        for (int x = 0; x < PASS; ++x) lds_dma16(at + x * 4096, off + x * step, r, 0);
+        for (int x = 0; x < ROWS / RPP; ++x) lds_dma16(at + x * 4096, off + x * step, r, 0);
     }
 };
 
@@ -277,25 +313,19 @@ __device__ __forceinline__ u32x4_t operand_of(const float16_t &v, int x) {
     return r;
 }
 
-__device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int x = __shfl_xor(v, o);
-        v = x < v ? x : v;
-    }
-    return __builtin_amdgcn_readfirstlane(v);
-}
-
 // What the rows (or keys) of a wave and of a workgroup see: [lo, hi) any of them, [full_lo, full_hi)
-// all of them (empty ones apart).
+// all of them (empty ones apart).  Both ends grow with the row, so the first and the last that see
+// anything tell; with offsets that decrease some see less than they would, and nothing out of range.
 struct Span {
     int lo, hi, full_lo, full_hi;
     __device__ __forceinline__ void set(int2 s) {
-        const bool some = s.x < s.y;
-        lo = wave_min_i(some ? s.x : 0x7fffffff);
-        hi = -wave_min_i(some ? -s.y : 0);
-        full_lo = -wave_min_i(some ? -s.x : 0);
-        full_hi = wave_min_i(some ? s.y : 0x7fffffff);
+        const uint64_t some = __ballot(s.x < s.y);
+        const int first = some ? __builtin_ctzll(some) : 0;
+        const int last = (some & 0xffffffffull) ? 31 - __builtin_clz(static_cast<uint32_t>(some)) : 0;
+        lo = some ? __builtin_amdgcn_readlane(s.x, first) : 0x7fffffff;
+        hi = some ? __builtin_amdgcn_readlane(s.y, last) : 0;
+        full_lo = __builtin_amdgcn_readlane(s.x, last);
+        full_hi = __builtin_amdgcn_readlane(s.y, first);
     }
     // over the four waves; `mem`: 8 words of LDS
     __device__ __forceinline__ int2 all(int *mem) const {
@@ -381,7 +411,7 @@ __device__ __forceinline__ void keep_finite(float16_t (&v)[N], float f) {
 // its result itself.
 struct Pieces {
     int per, most;  // steps of a piece, at least; pieces of a tile, at most
-    float *part;    // [tiles * heads][most][arrays][128][D]
+    float *part;    // [tiles * heads][most][arrays][4 waves][32 D]
     float2 *ml;     // forward: [tiles * heads][most][128]
     __device__ __forceinline__ int of(int n) const {
         const int p = (n + per - 1) / per;
@@ -389,28 +419,58 @@ struct Pieces {
     }
 };
 
+// Steps of UNIT that a tile's rows (or keys) go over, found by four waves of 32 of its rows.
+template <int UNIT>
+__device__ __forceinline__ int steps_of_tile(const Attn &a, int tile, bool of_rows, int *mem) {
+    const int t = tile * kOwn + (threadIdx.x >> 6) * 32 + (threadIdx.x & 31);
+    Span sp;
+    sp.set(of_rows ? keys_of(a, t) : rows_of(a, t));
+    const int2 all = sp.all(mem);
+    return all.x < all.y ? (all.y - 1) / UNIT - all.x / UNIT + 1 : 0;
+}
+
 // Steps [x, y) of piece i of p.
 __device__ __forceinline__ int2 steps_of(int n, int p, int i) {
     const int per = (n + p - 1) / p, x = i * per;
     return make_int2(x < n ? x : n, x + per < n ? x + per : n);
 }
 
-// This lane's channels of its row, unrounded, from a transposed result.
+// The 32 rows of a wave in `part`: its registers as they are, 16 bytes a lane one behind the other
+// (as rows of D, 64 lanes write 64 lines at a time: a join of 280 pieces 23 us instead of 16).
 template <int D>
-__device__ __forceinline__ void store_part(float *row, const float16_t (&v)[D / 32]) {
-    row += ((threadIdx.x & 63) >> 5) * 4;
+__device__ __forceinline__ void store_part(float *part, const float16_t (&v)[D / 32]) {
+    part += (threadIdx.x & 63) * 4;
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<float4_t *>(row + x * 32 + e * 2) = (float4_t){v[x][e], v[x][e + 1], v[x][e + 2], v[x][e + 3]};
+            *reinterpret_cast<float4_t *>(part + (x * 4 + e / 4) * 256) = (float4_t){v[x][e], v[x][e + 1], v[x][e + 2], v[x][e + 3]};
 }
-
+// row i of them, VE channels a lane
 template <int D>
-__device__ __forceinline__ void store_part_row(float *row, const float (&v)[D / 64]) {
-    const int l = threadIdx.x & 63;
+__device__ __forceinline__ void store_part_row(float *part, int i, const float (&v)[D / 64]) {
 #pragma unroll
-    for (int x = 0; x < D / 64; ++x) row[l * (D / 64) + x] = v[x];
+    for (int x = 0; x < D / 64; ++x) {
+        const int c = (threadIdx.x & 63) * (D / 64) + x;
+        part[(c >> 3) * 256 + ((c >> 2 & 1) * 32 + i) * 4 + (c & 3)] = v[x];
+    }
+}
+// The sums of the pieces' rows go to memory through LDS ([32][D + 8]), a row's 16 bytes a thread.
+template <int DT, int D>
+__device__ __forceinline__ void join_put(uint16_t *lds, int i, const float4_t &v) {  // float4 i of a wave's
+    const int lane = i & 63;
+    *reinterpret_cast<u32x2_t *>(lds + (lane & 31) * (D + 8) + (i >> 6) * 8 + (lane >> 5) * 4) =
+        (u32x2_t){pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
+}
+template <int D>
+__device__ __forceinline__ void join_write(const Strided &out, int head, int r0, int tokens, const uint16_t *lds) {
+    __syncthreads();
+#pragma unroll
+    for (int x = threadIdx.x; x < 4 * D; x += 256) {
+        const int i = x / (D / 8), ch = x % (D / 8) * 8;
+        if (r0 + i < tokens)
+            *reinterpret_cast<u32x4_t *>(out.to(r0 + i, head) + ch) = *reinterpret_cast<const u32x4_t *>(lds + i * (D + 8) + ch);
+    }
 }
 
 // ------------------------------------------------------------------------------ forward
@@ -426,7 +486,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     const int head = kvh * a.group + y % a.group;
     const int tile = tiles - 1 - y / a.group;  // (the last rows see most: first)
     const int r = tile * kOwn + w * 32 + n;
-    const int2 seen = r < a.tokens ? keys_of(a, r) : make_int2(r, r);
+    const int2 seen = keys_of(a, r);
     Span sp;
     sp.set(seen);
     int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
@@ -440,7 +500,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     u32x4_t q[KS];
     const float c = fabsf(a.c);
     own_operand<D>(q, a.q.at(r, head), r < a.tokens, a.c < 0.f ? 0x80008000u : 0u);
-    Stager<D> sk, sv;
+    Stager<D, kTile> sk, sv;
     sk.set(a.k, kvh);
     sv.set(a.v, kvh);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
@@ -548,12 +608,12 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
         for (int i = 0; i < 32; ++i) {
             const int row = tile * kOwn + w * 32 + i;
             const int x0 = __builtin_amdgcn_readlane(part.x, i), x1 = __builtin_amdgcn_readlane(part.y, i);
-            if (row >= a.tokens) break;
+            if (row >= a.tokens) break;  // (parts of rows that are not there are not read)
             float o[D / 64], rm, rl;
             row_forward<DT, D>(a, head, row, x0, x1, rm, rl, o);
             if (x0 >= x1) rm = rl = 0.f;
             if (pieces > 1) {
-                store_part_row<D>(pc.part + (slot + i) * D, o);
+                store_part_row<D>(pc.part + slot * D, i, o);
                 if (l == 0) pc.ml[slot + i] = make_float2(rm, rl);
                 continue;
             }
@@ -564,7 +624,6 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
         }
         return;
     }
-    if (r >= a.tokens) return;
     zero_unless(some, acc);
     const bool f = fabsf(m) > kFar;
     float2 ml = make_float2(f ? m : m + kTop<DT>, f ? sum : __builtin_amdgcn_ldexpf(sum, -static_cast<int>(kTop<DT>)));
@@ -573,10 +632,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
         if (!f && some)
 #pragma unroll
             for (int x = 0; x < DN; ++x) acc[x] *= __builtin_amdgcn_ldexpf(1.f, -static_cast<int>(kTop<DT>));
-        store_part<D>(pc.part + (slot + n) * D, acc);
+        store_part<D>(pc.part + slot * D, acc);
         if (g == 0) pc.ml[slot + n] = ml;
         return;
     }
+    if (r >= a.tokens) return;
     float inv = some ? 1.f / sum : 0.f;
     keep_finite<DT>(acc, inv);
     if constexpr (DT == NF4_F16) inv = 1.f;
@@ -587,54 +647,59 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
 // A workgroup joins 32 rows of a tile that is in pieces: each a (m, l, o) of its keys.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Attn a, const Pieces pc) {
-    constexpr int PER = 1024 / D;  // rows that the workgroup takes at a time, 4 channels a thread
+    __shared__ __attribute__((aligned(16))) uint16_t lds[32 * (D + 8)];
     __shared__ int mem[8];
-    const int tile = blockIdx.x >> 2, head = blockIdx.y, r0 = tile * kOwn;
-    const int t = r0 + (threadIdx.x & 127);
-    Span sp;
-    sp.set(t < a.tokens ? keys_of(a, t) : make_int2(t, t));
-    const int2 all = sp.all(mem);
-    const int k0 = all.x & ~(kTile - 1), steps = all.x < all.y ? (all.y - k0 + kTile - 1) / kTile : 0;
-    const int pieces = pc.of(steps);
+    const int tile = blockIdx.x >> 2, w = blockIdx.x & 3, head = blockIdx.y;
+    const int pieces = pc.of(steps_of_tile<kTile>(a, tile, true, mem));
     if (pieces < 2) return;
-    const int64_t slot = (static_cast<int64_t>(tile) * a.n_heads + head) * pc.most * kOwn;
-    const int ch = threadIdx.x % (D / 4) * 4;
-    for (int i = (blockIdx.x & 3) * 32 + threadIdx.x / (D / 4); i < (blockIdx.x & 3) * 32 + 32; i += PER) {
-        const int r = r0 + i;
-        if (r >= a.tokens) break;
-        float m = -INFINITY, l = 0.f;
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
+    const int64_t slot = (static_cast<int64_t>(tile) * a.n_heads + head) * pc.most * kOwn + w * 32;
+    const int n = threadIdx.x & 31, r = tile * kOwn + w * 32 + n;
+    float m = -INFINITY, l = 0.f;
+    if (r < a.tokens) {
         for (int p = 0; p < pieces; ++p) {
-            const float2 x = pc.ml[slot + p * kOwn + i];
-            if (x.y != 0.f) m = fmaxf(m, x.x);
+            const float2 x = pc.ml[slot + p * kOwn + n];
+            if (x.y != 0.f) m = fmaxf(m, x.x);  // (0: it saw nothing)
         }
         for (int p = 0; p < pieces; ++p) {
-            const float2 x = pc.ml[slot + p * kOwn + i];
-            if (x.y == 0.f) continue;  // (it saw nothing)
-            const float f = x.x == m ? 1.f : __builtin_amdgcn_exp2f(x.x - m);
-            l += x.y * f;
-            o += *reinterpret_cast<const float4_t *>(pc.part + (slot + p * kOwn + i) * D + ch) * f;
+            const float2 x = pc.ml[slot + p * kOwn + n];
+            if (x.y != 0.f) l += x.y * (x.x == m ? 1.f : __builtin_amdgcn_exp2f(x.x - m));
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        float4_t v = o * inv;
+        if (threadIdx.x < 32)
+            a.stats[static_cast<int64_t>(r) * a.n_heads + head] = l == 0.f ? make_float2(0.f, 0.f) : make_float2(m, l);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float4_t o[D / 32];
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) o[x] = (float4_t){0.f, 0.f, 0.f, 0.f};
+    if (r < a.tokens)
+        for (int p = 0; p < pieces; ++p) {
+            const float2 x = pc.ml[slot + p * kOwn + n];
+            if (x.y == 0.f) continue;
+            const float f = (x.x == m ? 1.f : __builtin_amdgcn_exp2f(x.x - m)) * inv;
+            const float *part = pc.part + (slot + p * kOwn) * D + threadIdx.x * 4;
+#pragma unroll
+            for (int y = 0; y < D / 32; ++y) o[y] += *reinterpret_cast<const float4_t *>(part + y * 1024) * f;
+        }
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) {
         if constexpr (DT == NF4_F16)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-                v[e] = fabsf(v[e]) < INFINITY ? __builtin_amdgcn_fmed3f(v[e], -65504.f, 65504.f) : v[e];
-        *reinterpret_cast<u32x2_t *>(a.o.to(r, head) + ch) = (u32x2_t){pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
-        if (ch == 0) a.stats[static_cast<int64_t>(r) * a.n_heads + head] = l == 0.f ? make_float2(0.f, 0.f) : make_float2(m, l);
+                o[x][e] = fabsf(o[x][e]) < INFINITY ? __builtin_amdgcn_fmed3f(o[x][e], -65504.f, 65504.f) : o[x][e];
+        join_put<DT, D>(lds, x * 256 + threadIdx.x, o[x]);
     }
+    join_write<D>(a.o, head, tile * kOwn + w * 32, a.tokens, lds);
 }
 
 // ----------------------------------------------------------------------------- backward
 //
-// What the backward pass reads of a row for every key, in blocks of 64 rows, four numbers each: m,
-// log2 l and m + log2 l (in fp16 less kTop), and D.  Where |m| is below kNear a probability's exponent
+// What the backward pass reads of a row for every key, in blocks of 32 rows, four numbers each: m,
+// log2 l and m + log2 l (in fp16 less kTop), and -D.  Where |m| is below kNear a probability's exponent
 // is taken with the sum of the first two, whose rounding (2^-16) is below those that follow.
 constexpr float kNear = 256.f;
 
 struct Back {
-    float *rows;   // [n_heads][blocks][4][64]
+    float *rows;   // [n_heads][2 blocks][4][32]
     float *norms;  // fp16: the largest |do| of a block's rows [n_heads][blocks], then |v| [n_kv][blocks]
     int blocks;
     int tiles;     // of 128
@@ -674,11 +739,11 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back
         float2 ml = make_float2(0.f, 0.f);
         if (r < a.tokens) ml = a.stats[static_cast<int64_t>(r) * a.n_heads + head];
         const float ll = (ml.y == 0.f ? 0.f : log2f(ml.y)) - kTop<DT>;
-        float *p = b.rows + (static_cast<int64_t>(head) * b.blocks + blockIdx.x) * 256 + i;
+        float *p = b.rows + (static_cast<int64_t>(head) * b.blocks + blockIdx.x) * 256 + (i >> 5) * 128 + (i & 31);
         p[0] = ml.x;
-        p[64] = ll;
-        p[128] = ml.x + ll;
-        p[192] = d;
+        p[32] = ll;
+        p[64] = ml.x + ll;
+        p[96] = -d;
     }
     if constexpr (DT == NF4_F16) {
         worst = wave_max(worst);
@@ -730,7 +795,7 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
     const int head = kvh * a.group + y % a.group;
     const int tile = b.tiles - 1 - y / a.group;
     const int r = tile * kOwn + w * 32 + n;
-    const int2 seen = r < a.tokens ? keys_of(a, r) : make_int2(r, r);
+    const int2 seen = keys_of(a, r);
     Span sp;
     sp.set(seen);
     int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
@@ -744,15 +809,16 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
     u32x4_t q[KS], go[KS];
     own_operand<D>(q, a.q.at(r, head), r < a.tokens, 0);
     own_operand<D>(go, a.dout.at(r, head), r < a.tokens, 0);
-    const float *rows = b.rows + (static_cast<int64_t>(head) * b.blocks + (r < a.tokens ? r >> 6 : 0)) * 256 + (r & 63);
-    const float m = rows[0], ll = rows[64], base = rows[128], delta = rows[192];
+    const float *rows = b.rows + (static_cast<int64_t>(head) * b.blocks * 2 + (r < a.tokens ? r >> 5 : 0)) * 128 + (r & 31);
+    const float m = rows[0], ll = rows[32], base = rows[64], delta = rows[96];
     const bool near = __all(!(seen.x < seen.y) || fabsf(m) < kNear);
+    const float mul = near ? a.c : 1.f, sub = near ? base : 0.f;
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
         const int b0 = first >> 6, nb = mine_of.y - mine_of.x;
         fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb));
     }
-    Stager<D> sk, sv;
+    Stager<D, kTile> sk, sv;
     sk.set(a.k, kvh);
     sv.set(a.v, kvh);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
@@ -775,22 +841,40 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
             sk.send(mine + (st ^ 1) * TB, k + kTile, all.y);
             sv.send(mine + (2 + (st ^ 1)) * TB, k + kTile, all.y);
         }
+        const uint32_t ka = ra + st * TB, va = ra + (2 + st) * TB, kt = ca + st * TB;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (sp.none(k + 32 * h, 32)) continue;
+            constexpr int AHEAD = 4;  // steps of k's and v's operands under way
+            u32x4_t kf[AHEAD], vf[AHEAD];
+#pragma unroll
+            for (int x = 0; x < AHEAD; ++x) {
+                kf[x] = rows_operand<D>(ka, h, x);
+                vf[x] = rows_operand<D>(va, h, x);
+            }
             float16_t sc = (float16_t){}, dp;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) dp[e] = -delta;
+            for (int e = 0; e < 16; ++e) dp[e] = delta;
+            __builtin_amdgcn_sched_barrier(0);
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int x = 0; x < KS; ++x) sc = mfma32<DT>(rows_operand<D>(ra + st * TB, h, x), q[x], sc);
-#pragma unroll
-            for (int x = 0; x < KS; ++x) dp = mfma32<DT>(rows_operand<D>(ra + (2 + st) * TB, h, x), go[x], dp);
+            for (int x = 0; x < KS; ++x) {
+                sc = mfma32<DT>(kf[x % AHEAD], q[x], sc);
+                dp = mfma32<DT>(vf[x % AHEAD], go[x], dp);
+                if (x + AHEAD < KS) {
+                    kf[x % AHEAD] = rows_operand<D>(ka, h, x + AHEAD);
+                    vf[x % AHEAD] = rows_operand<D>(va, h, x + AHEAD);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
             __builtin_amdgcn_s_setprio(0);
-            if (__builtin_expect(near, 1)) {
+            u32x4_t tf[2][DN];
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[e] = fmaf(sc[e], a.c, -base);
-            } else {
+            for (int x = 0; x < 2; ++x)
+#pragma unroll
+                for (int d = 0; d < DN; ++d) tf[x][d] = channels_operand<D>(kt, 2 * h + x, d);
+            __builtin_amdgcn_sched_barrier(0);
+            if (__builtin_expect(!near, 0)) {
 #pragma unroll
                 for (int e = 0; e < 16; ++e) sc[e] = exponent(sc[e], a.c, m) - ll;
             }
@@ -798,20 +882,19 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
                 const uint64_t see = seen_bits(seen, k);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (!bit_of(see, h, e)) sc[e] = -INFINITY;
+                    if (!bit_of(see, h, e)) sc[e] = a.c < 0.f && near ? INFINITY : -INFINITY;
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) {
-                sc[e] = __builtin_amdgcn_exp2f(sc[e]) * dp[e];
+                sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], mul, -sub)) * dp[e];
                 if constexpr (DT == NF4_F16) sc[e] *= fs;
             }
+            const u32x4_t pf[2] = {operand_of<DT>(sc, 0), operand_of<DT>(sc, 1)};
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const u32x4_t f = operand_of<DT>(sc, x);
+            for (int x = 0; x < 2; ++x)
 #pragma unroll
-                for (int d = 0; d < DN; ++d) acc[d] = mfma32<DT>(channels_operand<D>(ca + st * TB, 2 * h + x, d), f, acc[d]);
-            }
+                for (int d = 0; d < DN; ++d) acc[d] = mfma32<DT>(tf[x][d], pf[x], acc[d]);
             __builtin_amdgcn_s_setprio(0);
         }
     }
@@ -827,75 +910,83 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
             row_backward<DT, D>(a, head, row, __builtin_amdgcn_readlane(part.x, i), __builtin_amdgcn_readlane(part.y, i), o);
 #pragma unroll
             for (int x = 0; x < D / 64; ++x) o[x] *= a.scale;
-            if (pieces > 1) store_part_row<D>(b.row.part + (slot + i) * D, o);
+            if (pieces > 1) store_part_row<D>(b.row.part + slot * D, i, o);
             else store_row<DT, D>(a.dq.to(row, head), o);
         }
         return;
     }
-    if (r >= a.tokens) return;
     zero_unless(some, acc);
     const float f = a.scale * (ldexpf(1.f, -static_cast<int>(kTop<DT>)) / fs);
     if (pieces > 1) {
 #pragma unroll
         for (int x = 0; x < DN; ++x) acc[x] *= f;
-        store_part<D>(b.row.part + (slot + n) * D, acc);
-    } else {
+        store_part<D>(b.row.part + slot * D, acc);
+    } else if (r < a.tokens) {
         store_own<DT, D>(a.dq.to(r, head), acc, f);
     }
 }
 
-template <int DT, int D>
-constexpr int kBackLds = 2 * (2 * kTileBytes<D> + 1024) + 64;
+// The keys' workgroup holds its k and its sums in registers (160 of the 256 that two waves a SIMD leave)
+// and its v in LDS: with v in registers too, the operands of each product were waited for one at a time
+// (8192 tokens of
+// 28 heads, the whole backward pass: 2200 us instead of 1660), and tiles are of 32 rows, so that two workgroups' LDS fits a CU.
+constexpr int kRows = 32;
+
+template <int D>
+constexpr int kKeyLds = kOwn * D * 2 + 4 * kRows * D * 2 + 2 * 1024;  // v; q and do, two stages; their rows' numbers
+template <int D>
+constexpr int kBackLds = (kKeyLds<D> > 4 * kTileBytes<D> ? kKeyLds<D> : 4 * kTileBytes<D>) + 64;
 
 template <int DT, int D>
 __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block, uint8_t *lds) {
-    constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
+    constexpr int KS = D / 16, DN = D / 32, RB = kRows * D * 2, VB = kOwn * D * 2;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
     const int g = l >> 5, n = l & 31;
     const int piece = block / (b.tiles * a.n_kv);
     block %= b.tiles * a.n_kv;
     const int kvh = block % a.n_kv, tile = block / a.n_kv;
     const int j = tile * kOwn + w * 32 + n;
-    const int2 seen = j < a.tokens ? rows_of(a, j) : make_int2(j, j);
+    const int2 seen = rows_of(a, j);
     Span sp;
     sp.set(seen);
-    const int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB + 2048));
-
-    const int t0 = all.x < all.y ? all.x >> 6 : 0, per = all.x < all.y ? ((all.y - 1) >> 6) - t0 + 1 : 0;
+    const int2 all = sp.all(reinterpret_cast<int *>(lds + kKeyLds<D>));
+    const int t0 = all.x < all.y ? all.x / kRows : 0, per = all.x < all.y ? (all.y - 1) / kRows - t0 + 1 : 0;
     const int pieces = b.key.of(per * a.group);
     if (piece >= pieces) return;
     const int2 units = steps_of(per * a.group, pieces, piece);
 
-    u32x4_t kf[KS], vf[KS];
-    own_operand<D>(kf, a.k.at(j, kvh), j < a.tokens, 0);
-    own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, 0);
-    float fs = 1.f;
-    if constexpr (DT == NF4_F16) {
-        float most = 0.f;
-        for (int h = 0; h < a.group; ++h)
-            most = fmaxf(most, most_of(b.norms + static_cast<int64_t>(kvh * a.group + h) * b.blocks + t0, per));
-        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most);
-    }
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) uint8_t *)lds));
     const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
-    const uint32_t ra = lds0 + row_address<D>(), ca = lds0 + channel_address<D>();
-    const uint32_t rows0 = lds0 + 4 * TB;
-    Stager<D> sq, sg;
-    sq.set(a.q, kvh * a.group);
-    sg.set(a.dout, kvh * a.group);
-    // unit (head of the group, row tile), the next one
+    const uint32_t tiles0 = mine + VB, rows0 = __builtin_amdgcn_readfirstlane(lds0 + VB + 4 * RB);
+    Stager<D, kOwn> sv;
+    Stager<D, kRows> sq, sg;
+    sv.set(a.v, kvh);
+    sv.send(mine, tile * kOwn, a.tokens);
+    u32x4_t kf[KS];
+    own_operand<D>(kf, a.k.at(j, kvh), j < a.tokens, 0);
+    float fs = 1.f;
+    if constexpr (DT == NF4_F16) {
+        u32x4_t vf[KS];
+        own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, 0);
+        const int b0 = t0 * kRows / kTile, nb = per ? (all.y - 1) / kTile - b0 + 1 : 0;
+        float most = 0.f;
+        for (int h = 0; h < a.group; ++h)
+            most = fmaxf(most, most_of(b.norms + static_cast<int64_t>(kvh * a.group + h) * b.blocks + b0, nb));
+        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most);
+    }
+    // unit (head of the group, tile of rows), the next one
     int uh = per ? units.x / per : 0, ut = units.x - uh * per;
-    sq.base += uh * a.q.head;
-    sg.base += uh * a.dout.head;
+    sq.set(a.q, kvh * a.group + uh);
+    sg.set(a.dout, kvh * a.group + uh);
     int t = ut, st = 0;
     auto send = [&](int st) {
-        const int t = (t0 + ut) * kTile;
-        sq.send(mine + st * TB, t, all.y);
-        sg.send(mine + (2 + st) * TB, t, all.y);
-        if (w == 0) {
-            const float *p = b.rows + (static_cast<int64_t>(kvh * a.group + uh) * b.blocks + t0 + ut) * 256;
-            lds_dma16(__builtin_amdgcn_readfirstlane(rows0 + st * 1024), l * 16, make_rsrc(p, 1024), 0);
+        const int r = (t0 + ut) * kRows;
+        sq.send(tiles0 + st * RB, r, all.y);
+        sg.send(tiles0 + (2 + st) * RB, r, all.y);
+        if (w == 0) {  // (512 bytes: the upper lanes' are past the end, zeros)
+            const float *p = b.rows + (static_cast<int64_t>(kvh * a.group + uh) * b.blocks * 2 + t0 + ut) * 128;
+            lds_dma16(__builtin_amdgcn_readfirstlane(rows0 + st * 1024), l * 16, make_rsrc(p, 512), 0);
         }
         if (++ut == per) {
             ut = 0;
@@ -904,77 +995,100 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
             sg.base += a.dout.head;
         }
     };
+    const uint32_t va = lds0 + w * 32 * D * 2 + row_address<D>();
+    const uint32_t ra = lds0 + VB + row_address<D>(), ca = lds0 + VB + channel_address<D>();
     float16_t dk[DN], dv[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) dk[x] = dv[x] = (float16_t){};
     if (units.x < units.y) send(0);
+#pragma unroll 1
     for (int u = units.x; u < units.y; ++u, st ^= 1) {
-        const int r = (t0 + t) * kTile;
+        const int r = (t0 + t) * kRows;
         if (++t == per) t = 0;
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (u + 1 < units.y) send(st ^ 1);
-        const uint32_t rw = rows0 + st * 1024;
-        auto row4 = [&](int kind, int h, int e) {  // rows 32 h + 2 e + 4 g .. of a kind
-            return __builtin_bit_cast(float4_t, lds16(rw + kind * 256 + (32 * h + 2 * e + 4 * g) * 4));
+        if (sp.none(r, kRows)) continue;
+        const uint32_t qa = ra + st * RB, ga = ra + (2 + st) * RB, rw = rows0 + st * 1024 + g * 16;
+        auto row4 = [&](int kind, int e) {  // rows 2 e + 4 g .. of a kind
+            return __builtin_bit_cast(float4_t, lds16(rw + kind * 128 + e * 8));
         };
-        const float mine_m = *reinterpret_cast<const __attribute__((address_space(3))) float *>(static_cast<uintptr_t>(rw + l * 4));
-        const bool near = __all(fabsf(mine_m) < kNear);
+        constexpr int AHEAD = 2;  // steps of the operands of q, do and v under way
+        u32x4_t qf[AHEAD], gf[AHEAD], vf[AHEAD];
+        auto read = [&](int x) {
+            qf[x % AHEAD] = rows_operand<D>(qa, 0, x);
+            gf[x % AHEAD] = rows_operand<D>(ga, 0, x);
+            vf[x % AHEAD] = rows_operand<D>(va, 0, x);
+        };
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            if (sp.none(r + 32 * h, 32)) continue;
-            float16_t sc = (float16_t){}, dp;
+        for (int x = 0; x < AHEAD; ++x) read(x);
+        float16_t sc = (float16_t){}, dp;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const float4_t d = row4(3, e);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) dp[e + i] = d[i];
+        }
+        const float row_m = *reinterpret_cast<const __attribute__((address_space(3))) float *>(static_cast<uintptr_t>(rw - g * 16 + n * 4));
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int x = 0; x < KS; ++x) {
+            sc = mfma32<DT>(qf[x % AHEAD], kf[x], sc);
+            dp = mfma32<DT>(gf[x % AHEAD], vf[x % AHEAD], dp);
+            if (x + AHEAD < KS) read(x + AHEAD);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
+        const bool near = __all(fabsf(row_m) < kNear);
+        u32x4_t tf[2][DN];
+        auto read_t = [&](int i) {  // operands of the last products' i-th quarter: do and q in turn
+#pragma unroll
+            for (int d = 0; d < DN; ++d)
+                tf[i & 1][d] = channels_operand<D>(ca + ((i & 1 ? 0 : 2) + st) * RB, i >> 1, d);
+        };
+        if (__builtin_expect(near, 1)) {
 #pragma unroll
             for (int e = 0; e < 16; e += 4) {
-                const float4_t d = row4(3, h, e);
+                const float4_t base = row4(2, e);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) dp[e + i] = -d[i];
+                for (int i = 0; i < 4; ++i) sc[e + i] = fmaf(sc[e + i], a.c, -base[i]);
             }
-            __builtin_amdgcn_s_setprio(1);
+        } else {
 #pragma unroll
-            for (int x = 0; x < KS; ++x) sc = mfma32<DT>(rows_operand<D>(ra + st * TB, h, x), kf[x], sc);
+            for (int e = 0; e < 16; e += 4) {
+                const float4_t m = row4(0, e), ll = row4(1, e);
 #pragma unroll
-            for (int x = 0; x < KS; ++x) dp = mfma32<DT>(rows_operand<D>(ra + (2 + st) * TB, h, x), vf[x], dp);
-            __builtin_amdgcn_s_setprio(0);
-            if (__builtin_expect(near, 1)) {
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const float4_t base = row4(2, h, e);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[e + i] = fmaf(sc[e + i], a.c, -base[i]);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 16; e += 4) {
-                    const float4_t m = row4(0, h, e), ll = row4(1, h, e);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) sc[e + i] = exponent(sc[e + i], a.c, m[i]) - ll[i];
-                }
+                for (int i = 0; i < 4; ++i) sc[e + i] = exponent(sc[e + i], a.c, m[i]) - ll[i];
             }
-            if (!sp.full(r + 32 * h, 32)) {
-                const uint64_t see = seen_bits(seen, r);
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    if (!bit_of(see, h, e)) sc[e] = -INFINITY;
-            }
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sc[e] = __builtin_amdgcn_exp2f(sc[e]);
-                dp[e] *= sc[e];
-                if constexpr (DT == NF4_F16) dp[e] *= fs;
-            }
-            __builtin_amdgcn_s_setprio(1);
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                const u32x4_t p = operand_of<DT>(sc, x), ds = operand_of<DT>(dp, x);
-#pragma unroll
-                for (int d = 0; d < DN; ++d) {
-                    dv[d] = mfma32<DT>(channels_operand<D>(ca + (2 + st) * TB, 2 * h + x, d), p, dv[d]);
-                    dk[d] = mfma32<DT>(channels_operand<D>(ca + st * TB, 2 * h + x, d), ds, dk[d]);
-                }
-            }
-            __builtin_amdgcn_s_setprio(0);
         }
+        if (!sp.full(r, kRows)) {
+            const uint64_t see = seen_bits(seen, r);
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+                if (!bit_of(see, 0, e)) sc[e] = -INFINITY;
+        }
+        read_t(0);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            sc[e] = __builtin_amdgcn_exp2f(sc[e]);
+            dp[e] *= sc[e];
+            if constexpr (DT == NF4_F16) dp[e] *= fs;
+        }
+        const u32x4_t pf[4] = {operand_of<DT>(sc, 0), operand_of<DT>(dp, 0), operand_of<DT>(sc, 1), operand_of<DT>(dp, 1)};
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (i < 3) read_t(i + 1);
+#pragma unroll
+            for (int d = 0; d < DN; ++d) {
+                if (i & 1) dk[d] = mfma32<DT>(tf[1][d], pf[i], dk[d]);
+                else dv[d] = mfma32<DT>(tf[0][d], pf[i], dv[d]);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        __builtin_amdgcn_s_setprio(0);
     }
     const bool some = seen.x < seen.y;
     const int64_t slot = ((static_cast<int64_t>(tile) * a.n_kv + kvh) * b.key.most + piece) * 2 * kOwn + w * 32;
@@ -987,14 +1101,14 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
             float gk[D / 64] = {}, gv[D / 64] = {};
             for (int h = units.x / per; h * per < units.y; ++h) {  // the piece's rows of each head
                 const int u0 = h * per > units.x ? h * per : units.x, u1 = (h + 1) * per < units.y ? (h + 1) * per : units.y;
-                const int x0 = (t0 + u0 - h * per) * kTile, x1 = (t0 + u1 - h * per) * kTile;
+                const int x0 = (t0 + u0 - h * per) * kRows, x1 = (t0 + u1 - h * per) * kRows;
                 key_backward<DT, D>(a, kvh * a.group + h, key, r0 > x0 ? r0 : x0, r1 < x1 ? r1 : x1, gk, gv);
             }
 #pragma unroll
             for (int x = 0; x < D / 64; ++x) gk[x] *= a.scale;
             if (pieces > 1) {
-                store_part_row<D>(b.key.part + (slot + i) * D, gk);
-                store_part_row<D>(b.key.part + (slot + kOwn + i) * D, gv);
+                store_part_row<D>(b.key.part + slot * D, i, gk);
+                store_part_row<D>(b.key.part + (slot + kOwn) * D, i, gv);
                 continue;
             }
             store_row<DT, D>(a.dk.to(key, kvh), gk);
@@ -1002,7 +1116,6 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
         }
         return;
     }
-    if (j >= a.tokens) return;
     zero_unless(some, dk);
     zero_unless(some, dv);
     const float one = ldexpf(1.f, -static_cast<int>(kTop<DT>)), f = a.scale * (one / fs);
@@ -1012,10 +1125,11 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
             dk[x] *= f;
             dv[x] *= one;
         }
-        store_part<D>(b.key.part + (slot + n) * D, dk);
-        store_part<D>(b.key.part + (slot + kOwn + n) * D, dv);
+        store_part<D>(b.key.part + slot * D, dk);
+        store_part<D>(b.key.part + (slot + kOwn) * D, dv);
         return;
     }
+    if (j >= a.tokens) return;
     store_own<DT, D>(a.dk.to(j, kvh), dk, f);
     store_own<DT, D>(a.dv.to(j, kvh), dv, one);
 }
@@ -1023,7 +1137,7 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
 // The keys' workgroups first, then the rows'.
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_bwd_kernel(const Attn a, const Back b) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[kBackLds<DT, D>];
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kBackLds<D>];
     const int keys = b.tiles * a.n_kv * b.key.most, i = blockIdx.x;
     if (i < keys) dkv_body<DT, D>(a, b, i, lds);
     else dq_body<DT, D>(a, b, i - keys, lds);
@@ -1033,34 +1147,33 @@ __global__ __launch_bounds__(256, 2) void attn_bwd_kernel(const Attn a, const Ba
 // 4, y = heads of dq, then of dk, then of dv.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_bwd_join_kernel(const Attn a, const Back b) {
-    constexpr int PER = 1024 / D;  // rows that the workgroup takes at a time, 4 channels a thread
+    __shared__ __attribute__((aligned(16))) uint16_t lds[32 * (D + 8)];
     __shared__ int mem[8];
-    const int tile = blockIdx.x >> 2, r0 = tile * kOwn, t = r0 + (threadIdx.x & 127);
+    const int tile = blockIdx.x >> 2, w = blockIdx.x & 3;
     int head = blockIdx.y, array = 0;
     const bool of_keys = head >= a.n_heads;
     if (of_keys) {
         array = head >= a.n_heads + a.n_kv;
         head -= a.n_heads + array * a.n_kv;
     }
-    Span sp;
-    sp.set(t < a.tokens ? (of_keys ? rows_of(a, t) : keys_of(a, t)) : make_int2(t, t));
-    const int2 all = sp.all(mem);
-    const int t0 = all.x >> 6, steps = all.x < all.y ? ((all.y - 1) >> 6) - t0 + 1 : 0;
     const Pieces &pc = of_keys ? b.key : b.row;
-    const int pieces = pc.of(of_keys ? steps * a.group : steps), arrays = of_keys ? 2 : 1;
+    if (pc.most < 2) return;
+    const int pieces = pc.of(of_keys ? steps_of_tile<kRows>(a, tile, false, mem) * a.group : steps_of_tile<kTile>(a, tile, true, mem));
+    const int arrays = of_keys ? 2 : 1;
     if (pieces < 2) return;
-    const Strided &out = !of_keys ? a.dq : array ? a.dv : a.dk;
-    const float *part = pc.part + ((static_cast<int64_t>(tile) * (of_keys ? a.n_kv : a.n_heads) + head) * pc.most * arrays + array) * kOwn * D;
-    const int ch = threadIdx.x % (D / 4) * 4;
+    const float *part = pc.part + threadIdx.x * 4 +
+        (((static_cast<int64_t>(tile) * (of_keys ? a.n_kv : a.n_heads) + head) * pc.most * arrays + array) * kOwn + w * 32) * D;
+    float4_t v[D / 32];
 #pragma unroll
-    for (int x = 0; x < 32; x += PER) {
-        const int i = (blockIdx.x & 3) * 32 + x + threadIdx.x / (D / 4);
-        if (r0 + i >= a.tokens) break;
-        float4_t v = {0.f, 0.f, 0.f, 0.f};
-        for (int p = 0; p < pieces; ++p)
-            v += *reinterpret_cast<const float4_t *>(part + (static_cast<int64_t>(p) * arrays * kOwn + i) * D + ch);
-        *reinterpret_cast<u32x2_t *>(out.to(r0 + i, head) + ch) = (u32x2_t){pack2<DT>(v[0], v[1]), pack2<DT>(v[2], v[3])};
-    }
+    for (int x = 0; x < D / 32; ++x) v[x] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int p = 0; p < pieces; ++p)
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x)
+            v[x] += *reinterpret_cast<const float4_t *>(part + static_cast<int64_t>(p) * arrays * kOwn * D + x * 1024);
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x) join_put<DT, D>(lds, x * 256 + threadIdx.x, v[x]);
+    join_write<D>(!of_keys ? a.dq : array ? a.dv : a.dk, head, tile * kOwn + w * 32, a.tokens, lds);
 }
 
 // ------------------------------------------------------------------------- host
@@ -1145,8 +1258,6 @@ int take_saved(Attn &a, const nf4_attn *in, const void *out, const float *stats)
     return NF4_OK;
 }
 
-constexpr int kPlaces = 512;  // workgroups that the card holds: two a CU
-
 // What a row of the longest sequence sees, as the host knows it.
 int64_t span_of(const nf4_attn *in) {
     return in->max_len && in->max_len < in->tokens ? in->max_len : in->tokens;
@@ -1165,23 +1276,68 @@ Steps steps_of(const nf4_attn *in) {
     return {seen / kTile + 1.5, (w + kOwn - 1) / kTile + 2};
 }
 
-Pieces cut(double total, int64_t most, int per_least) {
+// A launch's time by measured constants (us, heads of 128, two workgroups on every CU; alone on a CU a
+// workgroup takes half as long): a step of the forward pass, of a tile of keys and of a tile of rows,
+// a workgroup's beginning and end, a launch that joins, and 64 KB written and read again.
+constexpr double kFwdStep = 2.2, kKeyStep = 2.1, kRowStep = 3.1, kBegin = 9., kJoin = 5., kPart = 0.03;
+constexpr int kPlaces = 512;
+
+struct Group {      // tiles of one kind
+    int64_t items;
+    double mean;    // steps of one
+    int64_t most;
+    double step;    // us
+    int arrays;     // parts of 64 KB that a piece leaves
+};
+
+Pieces cut(const Group &g, double us) {  // pieces of about so long
     Pieces p{};
-    int64_t per = static_cast<int64_t>(total / kPlaces) + 1;
-    if (per < per_least) per = per_least;
-    p.per = static_cast<int>(per);
-    p.most = static_cast<int>((most + per - 1) / per);
-    if (p.most > 64) p.most = 64;
+    const double per = us / g.step;
+    p.per = per < 1. ? 1 : per < g.most ? static_cast<int>(per) : static_cast<int>(g.most);
+    const int64_t n = (g.most + p.per - 1) / p.per;
+    p.most = static_cast<int>(n < 64 ? n : 64);
     return p;
 }
 
+// Cuts the tiles of one launch: the length of a piece that takes least by the constants above.
+void cut(const Group *g, int n, Pieces *out) {
+    double best = INFINITY;
+    for (double us = 6.; us < 4e5; us *= 1.19) {
+        Pieces p[2];
+        double groups = 0., work = 0., longest = 0., more = 0.;
+        bool whole = true;
+        for (int i = 0; i < n; ++i) {
+            p[i] = cut(g[i], us);
+            // (a tile's last piece is half a one on average)
+            const double pieces = p[i].most > 1 ? fmax(1., g[i].mean / p[i].per + 0.5) : 1.;
+            const double len = fmin(p[i].per, g[i].most) * g[i].step;
+            groups += g[i].items * pieces;
+            work += g[i].items * g[i].mean * g[i].step;
+            longest = fmax(longest, len);
+            if (p[i].most > 1) more += g[i].items * pieces * g[i].arrays * kPart;
+            whole = whole && p[i].most == 1;
+        }
+        work += groups * kBegin;
+        const double alone = groups < kPlaces / 2 ? 0.5 : groups < kPlaces ? groups / kPlaces : 1.;
+        double t = groups <= kPlaces ? (kBegin + longest) * alone : work / kPlaces + longest / 2;
+        if (!whole) t += kJoin + more;
+        if (t < best * 0.97) {
+            best = t;
+            for (int i = 0; i < n; ++i) out[i] = p[i];
+        }
+        if (whole) break;
+    }
+}
+
+// (heads of 64: half the products for the same exponentials)
+double step_us(const nf4_attn *in, double us) { return in->head_dim == 128 ? us : 0.6 * us; }
+
 // The forward pass's launch, and the bytes of its workspace.
 size_t plan(Pieces &p, const nf4_attn *in) {
-    const int64_t items = static_cast<int64_t>(tiles_of(in, kOwn)) * in->n_heads;
     const Steps n = steps_of(in);
-    p = cut(items * n.mean, n.most, 6);
-    if (items >= 2 * kPlaces || p.most < 2) p = {1 << 30, 1, nullptr, nullptr};
-    return p.most > 1 ? items * p.most * kOwn * (in->head_dim * 4 + 8) : 0;
+    const Group g = {static_cast<int64_t>(tiles_of(in, kOwn)) * in->n_heads, n.mean, n.most, step_us(in, kFwdStep), 1};
+    cut(&g, 1, &p);
+    return p.most > 1 ? g.items * p.most * kOwn * (in->head_dim * 4 + 8) : 0;
 }
 
 // The backward pass's, in 4-byte words after each other: rows, norms, rows' parts, keys' parts.
@@ -1190,15 +1346,18 @@ size_t plan(Back &b, const nf4_attn *in) {
     b.tiles = tiles_of(in, kOwn);
     const int64_t rows = static_cast<int64_t>(b.tiles) * in->n_heads, keys = static_cast<int64_t>(b.tiles) * in->n_kv;
     const Steps n = steps_of(in);
-    const int group = in->n_heads / in->n_kv;
-    b.row = cut(rows * n.mean, n.most, 8);
-    if (rows >= 2 * kPlaces || b.row.most < 2) b.row = {1 << 30, 1, nullptr, nullptr};
-    b.key = cut(rows * n.mean, n.most * group, static_cast<int>(sqrt(rows * n.mean) / 5));
+    const int units = in->n_heads / in->n_kv * (kTile / kRows);
+    const Group g[2] = {{rows, n.mean, n.most, step_us(in, kRowStep), 1},
+                        {keys, n.mean * units, n.most * units, step_us(in, kKeyStep), 2}};
+    Pieces p[2];
+    cut(g, 2, p);
+    b.row = p[0];
+    b.key = p[1];
     int64_t at = static_cast<int64_t>(in->n_heads) * b.blocks * 256;
     auto next = [&](int64_t words) {
-        float *p = reinterpret_cast<float *>(at * 4);
+        float *x = reinterpret_cast<float *>(at * 4);
         at += (words + 3) / 4 * 4;
-        return p;
+        return x;
     };
     b.norms = next(in->dtype == NF4_F16 ? static_cast<int64_t>(in->n_heads + in->n_kv) * b.blocks : 0);
     b.row.part = next(b.row.most > 1 ? rows * b.row.most * kOwn * in->head_dim : 0);
