@@ -812,12 +812,13 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
     const float *rows = b.rows + (static_cast<int64_t>(head) * b.blocks * 2 + (r < a.tokens ? r >> 5 : 0)) * 128 + (r & 31);
     const float m = rows[0], ll = rows[32], base = rows[64], delta = rows[96];
     const bool near = __all(!(seen.x < seen.y) || fabsf(m) < kNear);
-    const float mul = near ? a.c : 1.f, sub = near ? base : 0.f;
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
         const int b0 = first >> 6, nb = mine_of.y - mine_of.x;
         fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb));
     }
+    // (the probabilities are used for dS only: their scale goes into the exponent)
+    const float mul = near ? a.c : 1.f, sub = (near ? base : 0.f) - log2f(fs);
     Stager<D, kTile> sk, sv;
     sk.set(a.k, kvh);
     sv.set(a.v, kvh);
@@ -885,10 +886,7 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
                     if (!bit_of(see, h, e)) sc[e] = a.c < 0.f && near ? INFINITY : -INFINITY;
             }
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], mul, -sub)) * dp[e];
-                if constexpr (DT == NF4_F16) sc[e] *= fs;
-            }
+            for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], mul, -sub)) * dp[e];
             const u32x4_t pf[2] = {operand_of<DT>(sc, 0), operand_of<DT>(sc, 1)};
             __builtin_amdgcn_s_setprio(1);
 #pragma unroll
@@ -1136,7 +1134,7 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
 
 // The keys' workgroups first, then the rows'.
 template <int DT, int D>
-__global__ __launch_bounds__(256, 2) void attn_bwd_kernel(const Attn a, const Back b) {
+__global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_bwd_kernel(const Attn a, const Back b) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBackLds<D>];
     const int keys = b.tiles * a.n_kv * b.key.most, i = blockIdx.x;
     if (i < keys) dkv_body<DT, D>(a, b, i, lds);
