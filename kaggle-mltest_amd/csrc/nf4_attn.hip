@@ -13,6 +13,8 @@
 
 #include <math.h>
 
+#include <type_traits>
+
 namespace {
 
 struct Strided {  // [tokens, heads, D]: offsets in elements
@@ -31,10 +33,18 @@ struct Attn {
     float scale;
 };
 
+// threadIdx.x, as the compiler does not know it: what is computed of it in a loop over tiles stays in there
+// (ahead of the loop for two kinds of tiles at once, it took the registers that their own loops need).
+__device__ __forceinline__ int thread_here() {
+    int t = threadIdx.x;
+    asm volatile("" : "+v"(t));
+    return t;
+}
+
 // How many offsets are at or before t (the wave's), 64 at a time: a load's latency for every factor of
 // 64 of the batch.
 __device__ __forceinline__ int offsets_upto(const Attn &a, int t) {
-    const int l = threadIdx.x & 63;
+    const int l = thread_here() & 63;
     int lo = 0, n = a.batch + 1;
     while (n > 64) {
         const int step = (n + 63) >> 6, i = l * step;
@@ -52,7 +62,7 @@ __device__ __forceinline__ int offsets_upto(const Attn &a, int t) {
 __device__ __forceinline__ int2 sequence_of(const Attn &a, int t) {
     if (!a.cu) return make_int2(0, a.tokens);
     // the next 64 offsets, a lane each, from the first row's sequence on
-    const int i0 = offsets_upto(a, __builtin_amdgcn_readfirstlane(t)) - 1, l = threadIdx.x & 63;
+    const int i0 = offsets_upto(a, __builtin_amdgcn_readfirstlane(t)) - 1, l = thread_here() & 63;
     const int at = i0 + l < 0 ? 0 : i0 + l;
     const int next = at <= a.batch ? a.cu[at] : 0x7fffffff;
     int s = i0 < 0 ? 0x7fffffff : __builtin_amdgcn_readlane(next, 0), e = __builtin_amdgcn_readlane(next, 1);
@@ -128,7 +138,7 @@ __device__ __forceinline__ float lane_value(float v, int l) {
 // acc += f * this lane's channels of a row
 template <int DT, int D>
 __device__ __forceinline__ void add_row(float (&acc)[D / 64], float f, const uint16_t *row) {
-    const int l = threadIdx.x & 63;
+    const int l = thread_here() & 63;
     if constexpr (D == 128) {
         const uint32_t w = *reinterpret_cast<const uint32_t *>(row + 2 * l);
         acc[0] = fmaf(f, f32_of<DT>(w & 0xffffu), acc[0]);
@@ -140,7 +150,7 @@ __device__ __forceinline__ void add_row(float (&acc)[D / 64], float f, const uin
 
 template <int DT, int D>
 __device__ __forceinline__ void store_row(uint16_t *row, const float (&v)[D / 64]) {
-    const int l = threadIdx.x & 63;
+    const int l = thread_here() & 63;
     if constexpr (D == 128)
         *reinterpret_cast<uint32_t *>(row + 2 * l) = round16<DT>(v[0]) | static_cast<uint32_t>(round16<DT>(v[1])) << 16;
     else row[l] = round16<DT>(v[0]);
@@ -156,7 +166,7 @@ __device__ __forceinline__ float wave_max(float v) {
 template <int DT, int D>
 __device__ __forceinline__ void row_forward(const Attn &a, int head, int r, int k0, int k1, float &m,
                                             float &l, float (&acc)[D / 64]) {
-    const int lane = threadIdx.x & 63, kvh = head / a.group;
+    const int lane = thread_here() & 63, kvh = head / a.group;
     const uint16_t *q = a.q.at(r, head);
     m = -INFINITY;
     for (int k = k0; k < k1; k += 64)
@@ -180,7 +190,7 @@ __device__ __forceinline__ void row_forward(const Attn &a, int head, int r, int 
 template <int DT, int D>
 __device__ __forceinline__ void row_backward(const Attn &a, int head, int r, int k0, int k1,
                                              float (&acc)[D / 64]) {
-    const int lane = threadIdx.x & 63, kvh = head / a.group;
+    const int lane = thread_here() & 63, kvh = head / a.group;
     const uint16_t *q = a.q.at(r, head), *go = a.dout.at(r, head);
     const float2 ml = a.stats[static_cast<int64_t>(r) * a.n_heads + head];
     const float delta = dot_of<DT, D>(go, a.o.at(r, head)), inv = 1.f / ml.y;
@@ -201,7 +211,7 @@ __device__ __forceinline__ void row_backward(const Attn &a, int head, int r, int
 template <int DT, int D>
 __device__ __forceinline__ void key_backward(const Attn &a, int head, int j, int r0, int r1,
                                              float (&dk)[D / 64], float (&dv)[D / 64]) {
-    const int lane = threadIdx.x & 63, kvh = head / a.group;
+    const int lane = thread_here() & 63, kvh = head / a.group;
     const uint16_t *kj = a.k.at(j, kvh), *vj = a.v.at(j, kvh);
     for (int r = r0; r < r1; r += 64) {
         float p = 0.f, ds = 0.f;
@@ -231,7 +241,7 @@ __device__ __forceinline__ void key_backward(const Attn &a, int head, int j, int
 // time read one chunk of 16 rows from 16 bank groups, and 64 bytes of each of 4 consecutive rows
 // (transposed reads) from all banks.
 
-constexpr int kOwn = 128, kTile = 64;
+constexpr int kOwn = 128, kTile = 64, kRows = 32;  // (kRows: a tile of rows in the backward pass)
 
 template <int D>
 __device__ __forceinline__ constexpr int swizzle(int r) {
@@ -249,8 +259,8 @@ struct Stager {
     int64_t tok;
     int off, step;
 
-    __device__ __forceinline__ void set(const Strided &x, int head) {
-        const int row = threadIdx.x / CH, ch = threadIdx.x % CH;
+    __device__ __forceinline__ void set(const Strided &x, int head, int tid) {
+        const int row = tid / CH, ch = tid % CH;
         base = x.p + head * x.head;
         tok = x.tok;
         off = row * static_cast<int>(tok) * 2 + ((ch ^ swizzle<D>(row)) << 4);
@@ -268,13 +278,13 @@ struct Stager {
 // Operand addresses of a lane in a tile at LDS address 0: rows as they lie (a row a lane, 16 channels
 // a step), and transposed (a channel a lane, 16 rows a step).
 template <int D>
-__device__ __forceinline__ uint32_t row_address() {
-    const int l = threadIdx.x & 63, n = l & 31, g = l >> 5;
+__device__ __forceinline__ uint32_t row_address(int l) {
+    const int n = l & 31, g = l >> 5;
     return n * D * 2 + ((g ^ swizzle<D>(n)) << 4);
 }
 template <int D>
-__device__ __forceinline__ uint32_t channel_address() {
-    const int l = threadIdx.x & 63, row = (l >> 5) * 4 + ((l & 15) >> 2);
+__device__ __forceinline__ uint32_t channel_address(int l) {
+    const int row = (l >> 5) * 4 + ((l & 15) >> 2);
     const int ch = ((l >> 4) & 1) * 2 + ((l & 3) >> 1);
     return row * D * 2 + (l & 1) * 8 + ((ch ^ swizzle<D>(row)) << 4);
 }
@@ -293,8 +303,9 @@ __device__ __forceinline__ u32x4_t channels_operand(uint32_t at, int x, int d) {
 
 // A lane's own row as operands: channels 16 x + 8 (l / 32) ..
 template <int D>
-__device__ __forceinline__ void own_operand(u32x4_t (&f)[D / 16], const uint16_t *row, bool live, uint32_t flip) {
-    const int g = (threadIdx.x & 63) >> 5;
+__device__ __forceinline__ void own_operand(u32x4_t (&f)[D / 16], const uint16_t *row, bool live, int l,
+                                            uint32_t flip = 0) {
+    const int g = l >> 5;
 #pragma unroll
     for (int x = 0; x < D / 16; ++x) {
         f[x] = (u32x4_t){0, 0, 0, 0};
@@ -330,7 +341,7 @@ struct Span {
     // over the four waves; `mem`: 8 words of LDS
     __device__ __forceinline__ int2 all(int *mem) const {
         const int w = threadIdx.x >> 6;
-        if ((threadIdx.x & 63) == 0) {
+        if ((thread_here() & 63) == 0) {
             mem[w] = lo;
             mem[4 + w] = hi;
         }
@@ -350,7 +361,7 @@ struct Span {
 // The bits of a 64-wide tile at t that are in [s.x, s.y), for this lane's registers: register e of
 // half h is bit 32 h + 8 (e / 4) + e % 4.
 __device__ __forceinline__ uint64_t seen_bits(int2 s, int t) {
-    return (below(s.y - t) & ~below(s.x - t)) >> (((threadIdx.x >> 5) & 1) * 4);
+    return (below(s.y - t) & ~below(s.x - t)) >> (((thread_here() >> 5) & 1) * 4);
 }
 __device__ __forceinline__ bool bit_of(uint64_t m, int h, int e) {
     return static_cast<uint32_t>(m >> (32 * h)) >> (8 * (e >> 2) + (e & 3)) & 1;
@@ -375,7 +386,7 @@ __device__ __forceinline__ float odd_of(const float16_t (&v)[N]) {
 // This lane's channels of its row, from a transposed result.
 template <int DT, int D>
 __device__ __forceinline__ void store_own(uint16_t *row, const float16_t (&v)[D / 32], float f) {
-    row += ((threadIdx.x & 63) >> 5) * 4;
+    row += ((thread_here() & 63) >> 5) * 4;
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
@@ -439,7 +450,7 @@ __device__ __forceinline__ int2 steps_of(int n, int p, int i) {
 // (as rows of D, 64 lanes write 64 lines at a time: a join of 280 pieces 23 us instead of 16).
 template <int D>
 __device__ __forceinline__ void store_part(float *part, const float16_t (&v)[D / 32]) {
-    part += (threadIdx.x & 63) * 4;
+    part += (thread_here() & 63) * 4;
 #pragma unroll
     for (int x = 0; x < D / 32; ++x)
 #pragma unroll
@@ -451,7 +462,7 @@ template <int D>
 __device__ __forceinline__ void store_part_row(float *part, int i, const float (&v)[D / 64]) {
 #pragma unroll
     for (int x = 0; x < D / 64; ++x) {
-        const int c = (threadIdx.x & 63) * (D / 64) + x;
+        const int c = (thread_here() & 63) * (D / 64) + x;
         part[(c >> 3) * 256 + ((c >> 2 & 1) * 32 + i) * 4 + (c & 3)] = v[x];
     }
 }
@@ -499,14 +510,14 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
 
     u32x4_t q[KS];
     const float c = fabsf(a.c);
-    own_operand<D>(q, a.q.at(r, head), r < a.tokens, a.c < 0.f ? 0x80008000u : 0u);
+    own_operand<D>(q, a.q.at(r, head), r < a.tokens, l, a.c < 0.f ? 0x80008000u : 0u);
     Stager<D, kTile> sk, sv;
-    sk.set(a.k, kvh);
-    sv.set(a.v, kvh);
+    sk.set(a.k, kvh, threadIdx.x);
+    sv.set(a.v, kvh, threadIdx.x);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) uint8_t *)lds));
     const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
-    const uint32_t ka = lds0 + row_address<D>(), va = lds0 + 2 * TB + channel_address<D>();
+    const uint32_t ka = lds0 + row_address<D>(l), va = lds0 + 2 * TB + channel_address<D>(l);
 
     float m = -INFINITY, sum = 0.f;
     bool far = false;  // a row's m is (the wave's)
@@ -698,20 +709,137 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Attn a, const 
 // is taken with the sum of the first two, whose rounding (2^-16) is below those that follow.
 constexpr float kNear = 256.f;
 
+//
+// Tiles or shares.  Where all tiles are short, each has a workgroup.  Else that is uneven, and a
+// key/value head's work is a line: its tiles of keys one behind the other, then the tiles of rows of its
+// query heads, each as long as its steps cost and its beginning.  `groups` workgroups take an equal share
+// of the line each, which may begin and end inside a tile: all are on the card at once and end together,
+// whatever the lengths of the sequences are (device data).  A step belongs to the share in which it
+// begins; a tile whose steps are in several leaves a part for each, and the join launch sums a tile's
+// parts in their order.  (Heads of 128, bf16, the whole pass: one sequence of 2048, 12 heads over 2: 82 us,
+// with pieces of equal length instead 98; of 4096: 239 and 306; of 8192, 28 over 4: 1740 both; 30
+// sequences of 200, 16 heads of 64: 71, and 52 with a workgroup a tile.)
+constexpr int kKeyCost = 20, kRowCost = 30, kItemCost = 80;  // a step of keys, of rows; a tile
+constexpr int kLeast = 160;                                  // a share
+
 struct Back {
-    float *rows;   // [n_heads][2 blocks][4][32]
-    float *norms;  // fp16: the largest |do| of a block's rows [n_heads][blocks], then |v| [n_kv][blocks]
+    float *rows;    // [n_heads][2 blocks][4][32]
+    float *norms;   // fp16: the largest |do| of a block's rows [n_heads][blocks], then |v| [n_kv][blocks]
+    int4 *tab;      // a tile's keys [x, y) and rows [z, w): what its rows see, what sees its keys
+    int64_t *line;  // [2 tiles + 1]: where the tiles of keys begin, then those of rows (of all heads)
+    int *inside;    // [n_kv * groups]: the tile (of all heads) that a share begins inside of, or -1
+    float *part;    // [n_kv * groups][2][arrays][4 waves][32 D]
     int blocks;
-    int tiles;     // of 128
-    Pieces row, key;
+    int tiles;      // of 128
+    int groups;     // shares of a key/value head, at most; 0: tiles
 };
 
-// One workgroup per 64 rows and head; heads from n_heads on are those of v.
+struct Line {
+    int64_t total;
+    int groups;
+    __device__ __forceinline__ void set(const Back &b) {
+        total = uniform64(b.line[2 * b.tiles]);
+        const int64_t n = total / kLeast;
+        groups = n < 1 ? 1 : n < b.groups ? static_cast<int>(n) : b.groups;
+    }
+    // share g's first place: a quotient by way of 64-bit floats, then put right (a division of 64-bit
+    // whole numbers is a hundred instructions)
+    __device__ __forceinline__ int64_t begin(int g) const { return quotient(total * g, groups); }
+    __device__ __forceinline__ static int64_t quotient(int64_t a, int64_t b) {
+        int64_t q = static_cast<int64_t>(static_cast<double>(a) / static_cast<double>(b));
+        if (q * b > a) --q;
+        else if ((q + 1) * b <= a) ++q;
+        return uniform64(q);
+    }
+};
+
+// Steps of `cost` that begin in the share [s0, s1), of n (a tile without any counts as one) of a tile
+// that begins at c.
+__device__ __forceinline__ int2 steps_in(int64_t s0, int64_t s1, int64_t c, int n, int cost) {
+    const int64_t m = n < 1 ? 1 : n;
+    const int64_t x = s0 > c ? (s0 - c + cost - 1) / cost : 0, y = s1 > c ? (s1 - c + cost - 1) / cost : 0;
+    return make_int2(static_cast<int>(x < m ? x : m), static_cast<int>(y < m ? y : m));
+}
+
+// Steps of `unit` positions over [x, y), whole ones.
+__device__ __forceinline__ int steps_over(int x, int y, int unit) { return x < y ? (y - 1) / unit - x / unit + 1 : 0; }
+
+// A lane's own search: the rows of row t's sequence, or [t, t).
+__device__ __forceinline__ int2 sequence_of_lane(const Attn &a, int t) {
+    if (!a.cu) return make_int2(0, a.tokens);
+    int lo = 0, hi = a.batch + 1;  // the first offset past t
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (a.cu[mid] <= t) lo = mid + 1;
+        else hi = mid;
+    }
+    if (lo == 0 || lo > a.batch) return make_int2(t, t);
+    const int s = a.cu[lo - 1], e = a.cu[lo];
+    return make_int2(s < 0 ? 0 : s, e > a.tokens ? a.tokens : e);
+}
+
+// The table and the line, by one workgroup: a tile a thread, 256 at a time.
+__device__ __forceinline__ void make_line(const Attn &a, const Back &b) {
+    __shared__ int64_t sum[2][4];
+    int64_t done[2] = {0, 0};
+    const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
+    const int begin = a.cu ? a.cu[0] : 0, end = a.cu ? a.cu[a.batch] : a.tokens;
+#pragma unroll 1
+    for (int pass = 0; pass < 2; ++pass) {  // (rows' tiles begin behind all keys')
+        int64_t at = done[0];
+#pragma unroll 1
+        for (int t0 = 0; t0 < b.tiles; t0 += 256) {
+            const int t = t0 + threadIdx.x;
+            int64_t cost = 0;
+            if (t < b.tiles) {
+                int4 r;
+                if (pass == 0) {
+                    const int first = t * kOwn > begin ? t * kOwn : begin;
+                    int last = t * kOwn + kOwn < a.tokens ? t * kOwn + kOwn - 1 : a.tokens - 1;
+                    last = last < end ? last : end - 1;
+                    r = make_int4(0, 0, 0, 0);
+                    if (first <= last) {
+                        const int2 x = sequence_of_lane(a, first), y = sequence_of_lane(a, last);
+                        r.x = a.window && first - a.window + 1 > x.x ? first - a.window + 1 : x.x;
+                        r.y = last + 1;
+                        r.z = first;
+                        r.w = a.window && last + a.window < y.y ? last + a.window : y.y;
+                    }
+                    b.tab[t] = r;
+                } else {
+                    r = b.tab[t];
+                }
+                cost = pass == 0 ? static_cast<int64_t>(steps_over(r.z, r.w, kRows)) * a.group * kKeyCost + kItemCost
+                                 : static_cast<int64_t>(steps_over(r.x, r.y, kTile) * kRowCost + kItemCost) * a.group;
+            }
+            int64_t upto = cost;
+#pragma unroll
+            for (int o = 1; o < 64; o <<= 1) {
+                const int64_t x = __shfl_up(upto, o);
+                if (l >= o) upto += x;
+            }
+            if (l == 63) sum[pass][w] = upto;
+            __syncthreads();
+            for (int i = 0; i < w; ++i) upto += sum[pass][i];
+            if (t < b.tiles) b.line[pass * b.tiles + t] = at + upto - cost;
+            at += sum[pass][0] + sum[pass][1] + sum[pass][2] + sum[pass][3];
+            __syncthreads();
+        }
+        done[0] = at;
+    }
+    if (threadIdx.x == 0) b.line[2 * b.tiles] = done[0];
+}
+
+// One workgroup per 64 rows and head; heads from n_heads on are those of v, the last makes the line.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back b) {
     constexpr int CH = D / 8, RPP = 256 / CH;
     __shared__ float most[4];
     const int head = blockIdx.y, ch = threadIdx.x % CH;
+    if (head == static_cast<int>(gridDim.y) - 1) {
+        if (blockIdx.x == 0) make_line(a, b);
+        return;
+    }
     const bool of_v = head >= a.n_heads;
     float worst = 0.f;
 #pragma unroll
@@ -766,7 +894,7 @@ __device__ __forceinline__ float ds_scale(float bound) {
 
 __device__ __forceinline__ float most_of(const float *p, int n) {
     float v = 0.f;
-    for (int i = threadIdx.x & 63; i < n; i += 64) v = fmaxf(v, p[i]);
+    for (int i = thread_here() & 63; i < n; i += 64) v = fmaxf(v, p[i]);
     return wave_max(v);
 }
 
@@ -784,69 +912,63 @@ __device__ __forceinline__ float square_of(const u32x4_t (&f)[D / 16]) {
     return s + other_half(s);
 }
 
+// A tile of rows: keys [x, y) are seen, steps [u.x, u.y) are this share's; `part` where they are not all.
 template <int DT, int D>
-__device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block, uint8_t *lds) {
+__device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, int tile, int2 keys, int2 u,
+                                        float *part, uint8_t *lds) {
     constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
-    const int n = l & 31;
-    const int piece = block / (b.tiles * a.n_heads);
-    block %= b.tiles * a.n_heads;
-    const int kvh = block % a.n_kv, y = block / a.n_kv;
-    const int head = kvh * a.group + y % a.group;
-    const int tile = b.tiles - 1 - y / a.group;
+    const int tid = thread_here(), w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
+    const int n = l & 31, kvh = head / a.group;
     const int r = tile * kOwn + w * 32 + n;
     const int2 seen = keys_of(a, r);
     Span sp;
     sp.set(seen);
-    int2 all = sp.all(reinterpret_cast<int *>(lds + 4 * TB));
-    const int k0 = all.x & ~(kTile - 1), steps = all.x < all.y ? (all.y - k0 + kTile - 1) / kTile : 0;
-    const int pieces = b.row.of(steps);
-    if (piece >= pieces) return;
-    const int2 mine_of = steps_of(steps, pieces, piece);
-    const int first = k0 + mine_of.x * kTile, k1 = k0 + mine_of.y * kTile;
-    all.y = k1 < all.y ? k1 : all.y;
+    const int first = (keys.x & ~(kTile - 1)) + u.x * kTile;
+    int last = (keys.x & ~(kTile - 1)) + u.y * kTile;
+    last = last < keys.y ? last : keys.y;
 
     u32x4_t q[KS], go[KS];
-    own_operand<D>(q, a.q.at(r, head), r < a.tokens, 0);
-    own_operand<D>(go, a.dout.at(r, head), r < a.tokens, 0);
+    own_operand<D>(q, a.q.at(r, head), r < a.tokens, l);
+    own_operand<D>(go, a.dout.at(r, head), r < a.tokens, l);
     const float *rows = b.rows + (static_cast<int64_t>(head) * b.blocks * 2 + (r < a.tokens ? r >> 5 : 0)) * 128 + (r & 31);
     const float m = rows[0], ll = rows[32], base = rows[64], delta = rows[96];
     const bool near = __all(!(seen.x < seen.y) || fabsf(m) < kNear);
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
-        const int b0 = first >> 6, nb = mine_of.y - mine_of.x;
+        const int b0 = first >> 6, nb = u.y - u.x;
         fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb));
     }
     // (the probabilities are used for dS only: their scale goes into the exponent)
     const float mul = near ? a.c : 1.f, sub = (near ? base : 0.f) - log2f(fs);
     Stager<D, kTile> sk, sv;
-    sk.set(a.k, kvh);
-    sv.set(a.v, kvh);
+    sk.set(a.k, kvh, tid);
+    sv.set(a.v, kvh, tid);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) uint8_t *)lds));
     const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
-    const uint32_t ra = lds0 + row_address<D>(), ca = lds0 + channel_address<D>();
+    const uint32_t ra = lds0 + row_address<D>(l), ca = lds0 + channel_address<D>(l);
 
     float16_t acc[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
-    int k = steps ? first : all.y, st = 0;
-    if (k < all.y) {
-        sk.send(mine, k, all.y);
-        sv.send(mine + 2 * TB, k, all.y);
+    int k = u.x < u.y ? first : last, st = 0;
+    if (k < last) {
+        sk.send(mine, k, last);
+        sv.send(mine + 2 * TB, k, last);
     }
-    for (; k < all.y; k += kTile, st ^= 1) {
+#pragma unroll 1
+    for (; k < last; k += kTile, st ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
-        if (k + kTile < all.y) {
-            sk.send(mine + (st ^ 1) * TB, k + kTile, all.y);
-            sv.send(mine + (2 + (st ^ 1)) * TB, k + kTile, all.y);
+        if (k + kTile < last) {
+            sk.send(mine + (st ^ 1) * TB, k + kTile, last);
+            sv.send(mine + (2 + (st ^ 1)) * TB, k + kTile, last);
         }
         const uint32_t ka = ra + st * TB, va = ra + (2 + st) * TB, kt = ca + st * TB;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
             if (sp.none(k + 32 * h, 32)) continue;
-            constexpr int AHEAD = 4;  // steps of k's and v's operands under way
+            constexpr int AHEAD = D == 128 ? 4 : 2;  // steps of k's and v's operands under way
             u32x4_t kf[AHEAD], vf[AHEAD];
 #pragma unroll
             for (int x = 0; x < AHEAD; ++x) {
@@ -896,29 +1018,29 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
             __builtin_amdgcn_s_setprio(0);
         }
     }
-    const int2 part = make_int2(seen.x > first ? seen.x : first, seen.y < all.y ? seen.y : all.y);  // of this piece
-    const bool some = part.x < part.y;
-    const int64_t slot = ((static_cast<int64_t>(tile) * a.n_heads + head) * b.row.most + piece) * kOwn + w * 32;
+    const int2 own = make_int2(seen.x > first ? seen.x : first, seen.y < last ? seen.y : last);  // of this share
+    const bool some = own.x < own.y;
+    if (part) part += w * 32 * D;
     if (__any(some && !(odd_of(acc) == 0.f))) {  // as in the forward pass
 #pragma unroll 1
         for (int i = 0; i < 32; ++i) {
             const int row = tile * kOwn + w * 32 + i;
             if (row >= a.tokens) break;
             float o[D / 64];
-            row_backward<DT, D>(a, head, row, __builtin_amdgcn_readlane(part.x, i), __builtin_amdgcn_readlane(part.y, i), o);
+            row_backward<DT, D>(a, head, row, __builtin_amdgcn_readlane(own.x, i), __builtin_amdgcn_readlane(own.y, i), o);
 #pragma unroll
             for (int x = 0; x < D / 64; ++x) o[x] *= a.scale;
-            if (pieces > 1) store_part_row<D>(b.row.part + slot * D, i, o);
+            if (part) store_part_row<D>(part, i, o);
             else store_row<DT, D>(a.dq.to(row, head), o);
         }
         return;
     }
     zero_unless(some, acc);
     const float f = a.scale * (ldexpf(1.f, -static_cast<int>(kTop<DT>)) / fs);
-    if (pieces > 1) {
+    if (part) {
 #pragma unroll
         for (int x = 0; x < DN; ++x) acc[x] *= f;
-        store_part<D>(b.row.part + slot * D, acc);
+        store_part<D>(part, acc);
     } else if (r < a.tokens) {
         store_own<DT, D>(a.dq.to(r, head), acc, f);
     }
@@ -928,30 +1050,23 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int block,
 // and its v in LDS: with v in registers too, the operands of each product were waited for one at a time
 // (8192 tokens of
 // 28 heads, the whole backward pass: 2200 us instead of 1660), and tiles are of 32 rows, so that two workgroups' LDS fits a CU.
-constexpr int kRows = 32;
-
 template <int D>
 constexpr int kKeyLds = kOwn * D * 2 + 4 * kRows * D * 2 + 2 * 1024;  // v; q and do, two stages; their rows' numbers
 template <int D>
 constexpr int kBackLds = (kKeyLds<D> > 4 * kTileBytes<D> ? kKeyLds<D> : 4 * kTileBytes<D>) + 64;
 
+// A tile of keys: rows [x, y) see them, steps [u.x, u.y) are this share's; `part` where they are not all.
 template <int DT, int D>
-__device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block, uint8_t *lds) {
+__device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, int tile, int2 rows, int2 units,
+                                         float *part, uint8_t *lds) {
     constexpr int KS = D / 16, DN = D / 32, RB = kRows * D * 2, VB = kOwn * D * 2;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), l = threadIdx.x & 63;
+    const int tid = thread_here(), w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
     const int g = l >> 5, n = l & 31;
-    const int piece = block / (b.tiles * a.n_kv);
-    block %= b.tiles * a.n_kv;
-    const int kvh = block % a.n_kv, tile = block / a.n_kv;
     const int j = tile * kOwn + w * 32 + n;
     const int2 seen = rows_of(a, j);
     Span sp;
     sp.set(seen);
-    const int2 all = sp.all(reinterpret_cast<int *>(lds + kKeyLds<D>));
-    const int t0 = all.x < all.y ? all.x / kRows : 0, per = all.x < all.y ? (all.y - 1) / kRows - t0 + 1 : 0;
-    const int pieces = b.key.of(per * a.group);
-    if (piece >= pieces) return;
-    const int2 units = steps_of(per * a.group, pieces, piece);
+    const int t0 = rows.x / kRows, per = steps_over(rows.x, rows.y, kRows);
 
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) uint8_t *)lds));
@@ -959,15 +1074,15 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
     const uint32_t tiles0 = mine + VB, rows0 = __builtin_amdgcn_readfirstlane(lds0 + VB + 4 * RB);
     Stager<D, kOwn> sv;
     Stager<D, kRows> sq, sg;
-    sv.set(a.v, kvh);
-    sv.send(mine, tile * kOwn, a.tokens);
+    sv.set(a.v, kvh, tid);
+    if (units.x < units.y) sv.send(mine, tile * kOwn, a.tokens);
     u32x4_t kf[KS];
-    own_operand<D>(kf, a.k.at(j, kvh), j < a.tokens, 0);
+    own_operand<D>(kf, a.k.at(j, kvh), j < a.tokens, l);
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
         u32x4_t vf[KS];
-        own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, 0);
-        const int b0 = t0 * kRows / kTile, nb = per ? (all.y - 1) / kTile - b0 + 1 : 0;
+        own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, l);
+        const int b0 = t0 * kRows / kTile, nb = per ? (rows.y - 1) / kTile - b0 + 1 : 0;
         float most = 0.f;
         for (int h = 0; h < a.group; ++h)
             most = fmaxf(most, most_of(b.norms + static_cast<int64_t>(kvh * a.group + h) * b.blocks + b0, nb));
@@ -975,13 +1090,13 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
     }
     // unit (head of the group, tile of rows), the next one
     int uh = per ? units.x / per : 0, ut = units.x - uh * per;
-    sq.set(a.q, kvh * a.group + uh);
-    sg.set(a.dout, kvh * a.group + uh);
+    sq.set(a.q, kvh * a.group + uh, tid);
+    sg.set(a.dout, kvh * a.group + uh, tid);
     int t = ut, st = 0;
     auto send = [&](int st) {
         const int r = (t0 + ut) * kRows;
-        sq.send(tiles0 + st * RB, r, all.y);
-        sg.send(tiles0 + (2 + st) * RB, r, all.y);
+        sq.send(tiles0 + st * RB, r, rows.y);
+        sg.send(tiles0 + (2 + st) * RB, r, rows.y);
         if (w == 0) {  // (512 bytes: the upper lanes' are past the end, zeros)
             const float *p = b.rows + (static_cast<int64_t>(kvh * a.group + uh) * b.blocks * 2 + t0 + ut) * 128;
             lds_dma16(__builtin_amdgcn_readfirstlane(rows0 + st * 1024), l * 16, make_rsrc(p, 512), 0);
@@ -993,8 +1108,8 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
             sg.base += a.dout.head;
         }
     };
-    const uint32_t va = lds0 + w * 32 * D * 2 + row_address<D>();
-    const uint32_t ra = lds0 + VB + row_address<D>(), ca = lds0 + VB + channel_address<D>();
+    const uint32_t va = lds0 + w * 32 * D * 2 + row_address<D>(l);
+    const uint32_t ra = lds0 + VB + row_address<D>(l), ca = lds0 + VB + channel_address<D>(l);
     float16_t dk[DN], dv[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) dk[x] = dv[x] = (float16_t){};
@@ -1089,7 +1204,7 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
         __builtin_amdgcn_s_setprio(0);
     }
     const bool some = seen.x < seen.y;
-    const int64_t slot = ((static_cast<int64_t>(tile) * a.n_kv + kvh) * b.key.most + piece) * 2 * kOwn + w * 32;
+    if (part) part += w * 32 * D;
     if (__any(some && !(odd_of(dk) + odd_of(dv) == 0.f))) {  // as in the forward pass
 #pragma unroll 1
         for (int i = 0; i < 32; ++i) {
@@ -1097,16 +1212,16 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
             if (key >= a.tokens) break;
             const int r0 = __builtin_amdgcn_readlane(seen.x, i), r1 = __builtin_amdgcn_readlane(seen.y, i);
             float gk[D / 64] = {}, gv[D / 64] = {};
-            for (int h = units.x / per; h * per < units.y; ++h) {  // the piece's rows of each head
+            for (int h = units.x / per; h * per < units.y; ++h) {  // the share's rows of each head
                 const int u0 = h * per > units.x ? h * per : units.x, u1 = (h + 1) * per < units.y ? (h + 1) * per : units.y;
                 const int x0 = (t0 + u0 - h * per) * kRows, x1 = (t0 + u1 - h * per) * kRows;
                 key_backward<DT, D>(a, kvh * a.group + h, key, r0 > x0 ? r0 : x0, r1 < x1 ? r1 : x1, gk, gv);
             }
 #pragma unroll
             for (int x = 0; x < D / 64; ++x) gk[x] *= a.scale;
-            if (pieces > 1) {
-                store_part_row<D>(b.key.part + slot * D, i, gk);
-                store_part_row<D>(b.key.part + (slot + kOwn) * D, i, gv);
+            if (part) {
+                store_part_row<D>(part, i, gk);
+                store_part_row<D>(part + kOwn * D, i, gv);
                 continue;
             }
             store_row<DT, D>(a.dk.to(key, kvh), gk);
@@ -1117,58 +1232,146 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int block
     zero_unless(some, dk);
     zero_unless(some, dv);
     const float one = ldexpf(1.f, -static_cast<int>(kTop<DT>)), f = a.scale * (one / fs);
-    if (pieces > 1) {
+    if (part) {
 #pragma unroll
         for (int x = 0; x < DN; ++x) {
             dk[x] *= f;
             dv[x] *= one;
         }
-        store_part<D>(b.key.part + slot * D, dk);
-        store_part<D>(b.key.part + (slot + kOwn) * D, dv);
-        return;
+        store_part<D>(part, dk);
+        store_part<D>(part + kOwn * D, dv);
+    } else if (j < a.tokens) {
+        store_own<DT, D>(a.dk.to(j, kvh), dk, f);
+        store_own<DT, D>(a.dv.to(j, kvh), dv, one);
     }
-    if (j >= a.tokens) return;
-    store_own<DT, D>(a.dk.to(j, kvh), dk, f);
-    store_own<DT, D>(a.dv.to(j, kvh), dv, one);
 }
 
-// The keys' workgroups first, then the rows'.
+// A share's slot of parts: 0 of the tile that it begins inside of, 1 of the one that it begins.
+template <int D>
+__device__ __forceinline__ float *slot_of(const Back &b, int kvh, int g, int i) {
+    return b.part + ((static_cast<int64_t>(kvh) * b.groups + g) * 2 + i) * 2 * kOwn * D;
+}
+
 template <int DT, int D>
 __global__ __launch_bounds__(256, D == 64 ? 3 : 2) void attn_bwd_kernel(const Attn a, const Back b) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[kBackLds<D>];
-    const int keys = b.tiles * a.n_kv * b.key.most, i = blockIdx.x;
-    if (i < keys) dkv_body<DT, D>(a, b, i, lds);
-    else dq_body<DT, D>(a, b, i - keys, lds);
+    __shared__ int cursor[2];  // shares: the next tile of the line and head of the group
+    if (b.groups) {
+        const int g = blockIdx.x / a.n_kv, kvh0 = blockIdx.x % a.n_kv, l = threadIdx.x & 63;
+        Line line;
+        line.set(b);
+        int *inside = b.inside + kvh0 * b.groups + g;
+        if (threadIdx.x == 0) *inside = -1;
+        if (g >= line.groups) return;
+        const int64_t s0 = line.begin(g);
+        // the last tile (of all heads) that begins at or before the share
+        int e = 0;
+        for (int n = 2 * b.tiles; n > 1;) {
+            const int step = (n + 63) >> 6, i = l * step;
+            const int c = __popcll(__ballot(i < n && b.line[e + i] <= s0));  // (at least 1)
+            e += (c - 1) * step;
+            n = n - (c - 1) * step < step ? n - (c - 1) * step : step;
+        }
+        if (threadIdx.x == 0) {
+            int h = 0;
+            if (e >= b.tiles) {
+                const int4 r = b.tab[e - b.tiles];
+                h = static_cast<int>((s0 - b.line[e]) / (steps_over(r.x, r.y, kTile) * kRowCost + kItemCost));
+            }
+            cursor[0] = e;
+            cursor[1] = h;
+        }
+    }
+    // (what a tile needs to know is read again for each: kept over the tiles' work, it took registers that
+    // their loops spilled)
+    for (;;) {
+        __syncthreads();  // the cursor is there, and the tile before is read
+        int kvh = blockIdx.x % a.n_kv, e, h;
+        if (b.groups) {
+            e = __builtin_amdgcn_readfirstlane(cursor[0]);
+            h = __builtin_amdgcn_readfirstlane(cursor[1]);
+            if (e >= 2 * b.tiles) return;
+        } else {
+            const int i = blockIdx.x / a.n_kv - b.tiles;
+            e = i < 0 ? i + b.tiles : 2 * b.tiles - 1 - i / a.group;  // (the last rows see most: first)
+            h = i < 0 ? 0 : i % a.group;
+        }
+        const bool of_keys = e < b.tiles;
+        const int tile = of_keys ? e : e - b.tiles;
+        const int4 r = b.tab[tile];
+        const int x = __builtin_amdgcn_readfirstlane(of_keys ? r.z : r.x), y = __builtin_amdgcn_readfirstlane(of_keys ? r.w : r.y);
+        const int n = of_keys ? steps_over(x, y, kRows) * a.group : steps_over(x, y, kTile);
+        int2 u = make_int2(0, n);
+        float *part = nullptr;
+        if (b.groups) {
+            const int g = blockIdx.x / a.n_kv, cost = of_keys ? kKeyCost : kRowCost;
+            Line line;
+            line.set(b);
+            const int64_t c = uniform64(b.line[e]) + static_cast<int64_t>(h) * (n * cost + kItemCost);
+            const int64_t s1 = line.begin(g + 1);
+            if (c >= s1) return;
+            u = steps_in(line.begin(g), s1, c, n, cost);
+            u.x = __builtin_amdgcn_readfirstlane(u.x);
+            u.y = __builtin_amdgcn_readfirstlane(u.y);
+            __syncthreads();
+            if (threadIdx.x == 0) {
+                const bool on = of_keys || h + 1 == a.group;
+                cursor[0] = on ? e + 1 : e;
+                cursor[1] = on ? 0 : h + 1;
+            }
+            if (u.x >= u.y) continue;
+            if (u.x > 0 && threadIdx.x == 0)
+                b.inside[kvh * b.groups + g] = of_keys ? tile : b.tiles + tile * a.group + h;
+            if (u.x > 0 || u.y < n) part = slot_of<D>(b, kvh, g, u.x == 0);
+            if (n == 0) u.y = 0;
+        }
+        if (of_keys) dkv_body<DT, D>(a, b, kvh, tile, make_int2(x, y), u, part, lds);
+        else dq_body<DT, D>(a, b, kvh * a.group + h, tile, make_int2(x, y), u, part, lds);
+        if (!b.groups) return;
+    }
 }
 
-// A workgroup sums the pieces of 32 rows of dq, or of 32 keys of dk or dv: grid x = tiles of 128 times
-// 4, y = heads of dq, then of dk, then of dv.
+// The tile that a share begins inside of, where it is the first one to: 32 of its rows (or keys) a
+// workgroup, whose parts are summed in the shares' order.  Grid x = rows / 32 of dq or dk, then of dv,
+// y = shares of all heads.
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_bwd_join_kernel(const Attn a, const Back b) {
     __shared__ __attribute__((aligned(16))) uint16_t lds[32 * (D + 8)];
-    __shared__ int mem[8];
-    const int tile = blockIdx.x >> 2, w = blockIdx.x & 3;
-    int head = blockIdx.y, array = 0;
-    const bool of_keys = head >= a.n_heads;
-    if (of_keys) {
-        array = head >= a.n_heads + a.n_kv;
-        head -= a.n_heads + array * a.n_kv;
+    const int kvh = blockIdx.y / b.groups, w = blockIdx.x & 3, array = blockIdx.x >> 2;
+    int g = blockIdx.y % b.groups;
+    const int *inside = b.inside + kvh * b.groups;
+    const int e = inside[g];
+    if (e < 0 || (array && e >= b.tiles) || (g > 0 && inside[g - 1] == e)) return;
+    int end = g;  // the first share that is not inside of it
+    for (;;) {
+        const int i = end + (threadIdx.x & 63);
+        const uint64_t same = __ballot(i < b.groups && inside[i < b.groups ? i : 0] == e);
+        end += ~same ? __builtin_ctzll(~same) : 64;
+        if (~same) break;
     }
-    const Pieces &pc = of_keys ? b.key : b.row;
-    if (pc.most < 2) return;
-    const int pieces = pc.of(of_keys ? steps_of_tile<kRows>(a, tile, false, mem) * a.group : steps_of_tile<kTile>(a, tile, true, mem));
-    const int arrays = of_keys ? 2 : 1;
-    if (pieces < 2) return;
-    const float *part = pc.part + threadIdx.x * 4 +
-        (((static_cast<int64_t>(tile) * (of_keys ? a.n_kv : a.n_heads) + head) * pc.most * arrays + array) * kOwn + w * 32) * D;
+    const int at = (array * kOwn + w * 32) * D + threadIdx.x * 4;
     float4_t v[D / 32];
+    const float *part = slot_of<D>(b, kvh, g - 1, 1) + at;
 #pragma unroll
-    for (int x = 0; x < D / 32; ++x) v[x] = (float4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-    for (int p = 0; p < pieces; ++p)
+    for (int x = 0; x < D / 32; ++x) v[x] = *reinterpret_cast<const float4_t *>(part + x * 1024);
+    part = slot_of<D>(b, kvh, g, 0) + at;
+    constexpr int64_t NEXT = 4 * kOwn * D;  // the next share's slot 0
+    for (; g < end; g += 4, part += 4 * NEXT) {  // (four parts' loads under way: their latency counts)
+        float4_t f[4][D / 32];
 #pragma unroll
-        for (int x = 0; x < D / 32; ++x)
-            v[x] += *reinterpret_cast<const float4_t *>(part + static_cast<int64_t>(p) * arrays * kOwn * D + x * 1024);
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) {
+                f[i][x] = (float4_t){0.f, 0.f, 0.f, 0.f};
+                if (g + i < end) f[i][x] = *reinterpret_cast<const float4_t *>(part + i * NEXT + x * 1024);
+            }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int x = 0; x < D / 32; ++x) v[x] += f[i][x];
+    }
+    const bool of_keys = e < b.tiles;
+    const int tile = of_keys ? e : (e - b.tiles) / a.group, head = of_keys ? kvh : kvh * a.group + (e - b.tiles) % a.group;
 #pragma unroll
     for (int x = 0; x < D / 32; ++x) join_put<DT, D>(lds, x * 256 + threadIdx.x, v[x]);
     join_write<D>(!of_keys ? a.dq : array ? a.dv : a.dk, head, tile * kOwn + w * 32, a.tokens, lds);
@@ -1238,12 +1441,12 @@ int forward(const Attn &a, const Pieces &pc, int tiles, hipStream_t s) {
 
 template <int DT, int D>
 int backward(const Attn &a, const Back &b, hipStream_t s) {
-    const dim3 rows(b.blocks, a.n_heads + (DT == NF4_F16 ? a.n_kv : 0));
-    const dim3 join(b.tiles * 4, a.n_heads + 2 * a.n_kv);
+    const dim3 rows(b.blocks, a.n_heads + (DT == NF4_F16 ? a.n_kv : 0) + 1);
+    const int groups = b.groups ? b.groups : b.tiles * (1 + a.group);
     hipLaunchKernelGGL((attn_rows_kernel<DT, D>), rows, dim3(256), 0, s, a, b);
-    hipLaunchKernelGGL((attn_bwd_kernel<DT, D>), dim3(b.tiles * (a.n_kv * b.key.most + a.n_heads * b.row.most)), dim3(256), 0, s, a, b);
-    if (b.row.most > 1 || b.key.most > 1)
-        hipLaunchKernelGGL((attn_bwd_join_kernel<DT, D>), join, dim3(256), 0, s, a, b);
+    hipLaunchKernelGGL((attn_bwd_kernel<DT, D>), dim3(groups * a.n_kv), dim3(256), 0, s, a, b);
+    if (b.groups > 1)
+        hipLaunchKernelGGL((attn_bwd_join_kernel<DT, D>), dim3(8, b.groups * a.n_kv), dim3(256), 0, s, a, b);
     return status_of(hipGetLastError());
 }
 
@@ -1271,96 +1474,79 @@ Steps steps_of(const nf4_attn *in) {
     // (a tile's rows see w + 127 keys of a long sequence's middle, and half as many on average where
     // the window is all of it)
     const double seen = w < span ? static_cast<double>(w) : 0.5 * span;
-    return {seen / kTile + 1.5, (w + kOwn - 1) / kTile + 2};
+    const int64_t all = tiles_of(in, kTile), most = (w + kOwn - 1) / kTile + 2;
+    return {fmin(seen / kTile + 1.5, all), most < all ? most : all};
 }
 
 // A launch's time by measured constants (us, heads of 128, two workgroups on every CU; alone on a CU a
 // workgroup takes half as long): a step of the forward pass, of a tile of keys and of a tile of rows,
 // a workgroup's beginning and end, a launch that joins, and 64 KB written and read again.
-constexpr double kFwdStep = 2.2, kKeyStep = 2.1, kRowStep = 3.1, kBegin = 9., kJoin = 5., kPart = 0.03;
-constexpr int kPlaces = 512;
+constexpr double kFwdStep = 2.2, kKeyStep = 2.1, kRowStep = 3.1, kBegin = 9., kJoin = 5., kPart = 0.015;
 
-struct Group {      // tiles of one kind
-    int64_t items;
-    double mean;    // steps of one
-    int64_t most;
-    double step;    // us
-    int arrays;     // parts of 64 KB that a piece leaves
-};
-
-Pieces cut(const Group &g, double us) {  // pieces of about so long
-    Pieces p{};
-    const double per = us / g.step;
-    p.per = per < 1. ? 1 : per < g.most ? static_cast<int>(per) : static_cast<int>(g.most);
-    const int64_t n = (g.most + p.per - 1) / p.per;
-    p.most = static_cast<int>(n < 64 ? n : 64);
-    return p;
-}
-
-// Cuts the tiles of one launch: the length of a piece that takes least by the constants above.
-void cut(const Group *g, int n, Pieces *out) {
-    double best = INFINITY;
-    for (double us = 6.; us < 4e5; us *= 1.19) {
-        Pieces p[2];
-        double groups = 0., work = 0., longest = 0., more = 0.;
-        bool whole = true;
-        for (int i = 0; i < n; ++i) {
-            p[i] = cut(g[i], us);
-            // (a tile's last piece is half a one on average)
-            const double pieces = p[i].most > 1 ? fmax(1., g[i].mean / p[i].per + 0.5) : 1.;
-            const double len = fmin(p[i].per, g[i].most) * g[i].step;
-            groups += g[i].items * pieces;
-            work += g[i].items * g[i].mean * g[i].step;
-            longest = fmax(longest, len);
-            if (p[i].most > 1) more += g[i].items * pieces * g[i].arrays * kPart;
-            whole = whole && p[i].most == 1;
-        }
-        work += groups * kBegin;
-        const double alone = groups < kPlaces / 2 ? 0.5 : groups < kPlaces ? groups / kPlaces : 1.;
-        double t = groups <= kPlaces ? (kBegin + longest) * alone : work / kPlaces + longest / 2;
-        if (!whole) t += kJoin + more;
-        if (t < best * 0.97) {
-            best = t;
-            for (int i = 0; i < n; ++i) out[i] = p[i];
-        }
-        if (whole) break;
-    }
-}
-
-// (heads of 64: half the products for the same exponentials)
+// (heads of 64: half the products for the same exponentials, and three workgroups a CU)
 double step_us(const nf4_attn *in, double us) { return in->head_dim == 128 ? us : 0.6 * us; }
+int places_of(const nf4_attn *in) { return in->head_dim == 128 ? 512 : 768; }
+
+// Time of a launch of `groups` workgroups that take `work` together and `longest` each at most.
+double launch_us(const nf4_attn *in, double groups, double work, double longest) {
+    const double begin = step_us(in, kBegin), places = places_of(in);
+    // (the last to end find the card half empty, the less so the more there are)
+    return groups <= places ? (begin + longest) * fmax(groups / places, 0.5)
+                            : (work + groups * begin) / places + longest * places / groups / 2;
+}
 
 // The forward pass's launch, and the bytes of its workspace.
 size_t plan(Pieces &p, const nf4_attn *in) {
+    const int64_t items = static_cast<int64_t>(tiles_of(in, kOwn)) * in->n_heads;
     const Steps n = steps_of(in);
-    const Group g = {static_cast<int64_t>(tiles_of(in, kOwn)) * in->n_heads, n.mean, n.most, step_us(in, kFwdStep), 1};
-    cut(&g, 1, &p);
-    return p.most > 1 ? g.items * p.most * kOwn * (in->head_dim * 4 + 8) : 0;
+    const double step = step_us(in, kFwdStep);
+    double best = INFINITY;
+    for (double per = 4.; ; per *= 1.25) {
+        const bool whole = per >= n.most;
+        const double most = whole ? 1. : fmin(ceil(n.most / floor(per)), 64.), pieces = whole ? 1. : fmax(1., n.mean / per + 0.5);
+        double t = launch_us(in, items * pieces, items * n.mean * step, fmin(per, n.most) * step);
+        if (!whole) t += kJoin + items * pieces * kPart;
+        if (t < best) {
+            best = t;
+            p.per = static_cast<int>(fmin(per, n.most));
+            p.most = static_cast<int>(most);
+        }
+        if (whole) break;
+    }
+    return p.most > 1 ? items * p.most * kOwn * (in->head_dim * 4 + 8) : 0;
 }
 
-// The backward pass's, in 4-byte words after each other: rows, norms, rows' parts, keys' parts.
+// The backward pass's launch, and its workspace, in bytes one behind the other from 0 on.
 size_t plan(Back &b, const nf4_attn *in) {
     b.blocks = tiles_of(in, kTile);
     b.tiles = tiles_of(in, kOwn);
-    const int64_t rows = static_cast<int64_t>(b.tiles) * in->n_heads, keys = static_cast<int64_t>(b.tiles) * in->n_kv;
     const Steps n = steps_of(in);
-    const int units = in->n_heads / in->n_kv * (kTile / kRows);
-    const Group g[2] = {{rows, n.mean, n.most, step_us(in, kRowStep), 1},
-                        {keys, n.mean * units, n.most * units, step_us(in, kKeyStep), 2}};
-    Pieces p[2];
-    cut(g, 2, p);
-    b.row = p[0];
-    b.key = p[1];
-    int64_t at = static_cast<int64_t>(in->n_heads) * b.blocks * 256;
-    auto next = [&](int64_t words) {
-        float *x = reinterpret_cast<float *>(at * 4);
-        at += (words + 3) / 4 * 4;
-        return x;
+    const int64_t rows = static_cast<int64_t>(b.tiles) * in->n_heads, keys = static_cast<int64_t>(b.tiles) * in->n_kv;
+    const int64_t units = in->n_heads / in->n_kv * (kTile / kRows);  // steps of keys where rows have one
+    const int places = places_of(in);
+    const double key = step_us(in, kKeyStep), row = step_us(in, kRowStep);
+    const double work = rows * n.mean * row + keys * n.mean * units * key;
+    const double line = rows * n.mean * (kTile / kRows * kKeyCost + kRowCost) + (rows + keys) * kItemCost;
+    const double groups = fmin(floor(line / kLeast), places);
+    const double shares = (work + (rows + keys + groups) * step_us(in, kBegin)) / groups * fmax(groups / places, 0.5) +
+                          kJoin + groups * kPart * in->head_dim / 64;
+    const double most_keys = fmin(n.most * (kTile / kRows), tiles_of(in, kRows)) * (in->n_heads / in->n_kv);
+    const double tiles = launch_us(in, rows + keys, work, fmax(n.most * row, most_keys * key));
+    b.groups = shares < 1.1 * tiles ? static_cast<int>(fmax(groups / in->n_kv, 1.)) : 0;
+    size_t at = 0;
+    auto next = [&](size_t bytes) {
+        char *p = reinterpret_cast<char *>(at);
+        at += (bytes + 15) / 16 * 16;
+        return p;
     };
-    b.norms = next(in->dtype == NF4_F16 ? static_cast<int64_t>(in->n_heads + in->n_kv) * b.blocks : 0);
-    b.row.part = next(b.row.most > 1 ? rows * b.row.most * kOwn * in->head_dim : 0);
-    b.key.part = next(b.key.most > 1 ? keys * b.key.most * 2 * kOwn * in->head_dim : 0);
-    return at * 4;
+    b.rows = reinterpret_cast<float *>(next(static_cast<size_t>(in->n_heads) * b.blocks * 1024));
+    b.norms = reinterpret_cast<float *>(next(in->dtype == NF4_F16 ? static_cast<size_t>(in->n_heads + in->n_kv) * b.blocks * 4 : 0));
+    b.tab = reinterpret_cast<int4 *>(next(static_cast<size_t>(b.tiles) * 16));
+    b.line = reinterpret_cast<int64_t *>(next((2 * static_cast<size_t>(b.tiles) + 1) * 8));
+    b.inside = reinterpret_cast<int *>(next(static_cast<size_t>(b.groups) * in->n_kv * 4));
+    const size_t slots = b.groups > 1 ? 2 * static_cast<size_t>(b.groups) * in->n_kv : 0;
+    b.part = reinterpret_cast<float *>(next(slots * 2 * kOwn * in->head_dim * 4));
+    return at;
 }
 
 }  // namespace
@@ -1415,9 +1601,15 @@ extern "C" int nf4_attn_bwd(const nf4_attn *in, const void *out, const float *st
     const size_t need = plan(b, in);
     if (!workspace || workspace_bytes < need) return NF4_ERR_WORKSPACE;
     if (!aligned(workspace, 16)) return NF4_ERR_UNSUPPORTED;
-    char *ws = static_cast<char *>(workspace);
-    b.rows = static_cast<float *>(workspace);
-    for (float **p : {&b.norms, &b.row.part, &b.key.part}) *p = reinterpret_cast<float *>(ws + reinterpret_cast<uintptr_t>(*p));
+    auto moved = [&](auto *&p) {
+        p = reinterpret_cast<std::remove_reference_t<decltype(p)>>(static_cast<char *>(workspace) + reinterpret_cast<uintptr_t>(p));
+    };
+    moved(b.rows);
+    moved(b.norms);
+    moved(b.tab);
+    moved(b.line);
+    moved(b.inside);
+    moved(b.part);
     auto s = static_cast<hipStream_t>(stream);
     if (in->dtype == NF4_BF16)
         return in->head_dim == 128 ? backward<NF4_BF16, 128>(a, b, s) : backward<NF4_BF16, 64>(a, b, s);
