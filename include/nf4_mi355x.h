@@ -414,6 +414,13 @@ int nf4_qkv_rope_bwd(const void *dq, const void *dk, const void *dv, const float
                      const float *sin_t, void *dqkv, int64_t ld_dqkv, int64_t tokens, int n_heads,
                      int n_kv, int head_dim, int dtype, void *stream);
 
+/* The rotation alone, or its transpose (inverse != 0: the gradient's): the `heads` heads of every row
+ * of x (rows ld_x elements apart) into y, per pair as above (cos, sin fp32 [tokens, head_dim]); y may be
+ * x.  Heads as they lie: of a q|k|v row, q's and k's at once, shared key heads once.  head_dim a multiple
+ * of 8 up to 512, 8-byte aligned rows, 16-byte aligned tables. */
+int nf4_rope(const void *x, int64_t ld_x, const float *cos_t, const float *sin_t, void *y, int64_t ld_y,
+             int64_t tokens, int heads, int head_dim, int inverse, int dtype, void *stream);
+
 /* ------------------------------------------ serving: a paged cache and attention over it */
 
 /* A paged key/value cache and one step's sequences.  Position j of sequence b lies in page

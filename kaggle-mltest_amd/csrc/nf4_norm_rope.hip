@@ -491,6 +491,37 @@ __global__ __launch_bounds__(64) void qkv_rope_bwd_vec_kernel(
     }
 }
 
+// One thread per 4 rotary pairs of a head: the forward rotation of qkv_rope_vec_kernel or the transposed
+// one of qkv_rope_bwd_vec_kernel, on heads as they lie (shared key heads are not expanded).  Bound by
+// memory: 8192 tokens of 28 + 4 heads of 128, 134 MB, ROPE_US.
+template <int DT>
+__global__ __launch_bounds__(256) void rope_heads_kernel(const uint16_t *x, int64_t ld_x, const float *cs,
+                                                         const float *sn, uint16_t *y, int64_t ld_y,
+                                                         int heads, int head_dim, int inverse) {
+    const int64_t t = blockIdx.x;
+    const int half = head_dim / 2, per = half / 4;
+    for (int u = blockIdx.y * 256 + threadIdx.x; u < heads * per; u += 256 * gridDim.y) {
+        const int head = u / per, i = (u - head * per) * 4;
+        const uint16_t *src = x + t * ld_x + head * head_dim + i;
+        uint16_t *dst = y + t * ld_y + head * head_dim + i;
+        float c_lo[4], c_hi[4], s_lo[4], s_hi[4], lo[4], hi[4];
+        ldf4(cs + t * head_dim + i, c_lo);
+        ldf4(cs + t * head_dim + half + i, c_hi);
+        ldf4(sn + t * head_dim + i, s_lo);
+        ldf4(sn + t * head_dim + half + i, s_hi);
+        ld4<DT>(src, lo);
+        ld4<DT>(src + half, hi);
+        uint16_t a[4], b[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            a[j] = st1<DT>(inverse ? lo[j] * c_lo[j] + hi[j] * s_hi[j] : lo[j] * c_lo[j] - hi[j] * s_lo[j]);
+            b[j] = st1<DT>(inverse ? hi[j] * c_hi[j] - lo[j] * s_lo[j] : hi[j] * c_hi[j] + lo[j] * s_hi[j]);
+        }
+        *reinterpret_cast<u32x2_t *>(dst) = pack4(a);
+        *reinterpret_cast<u32x2_t *>(dst + half) = pack4(b);
+    }
+}
+
 int norm_shape_ok(int64_t rows, int64_t cols, int dtype) {
     if (dtype != NF4_F16 && dtype != NF4_BF16) return NF4_ERR_ARG;
     if (rows < 0 || cols <= 0) return NF4_ERR_ARG;
@@ -657,5 +688,29 @@ extern "C" int nf4_qkv_rope_bwd(const void *dq, const void *dk, const void *dv, 
         hipLaunchKernelGGL(qkv_rope_bwd_kernel<NF4_F16>, grid, dim3(64), 0, s, P(dq), P(dk), P(dv),
                            cos_t, sin_t, static_cast<uint16_t *>(dqkv), ld_dqkv, n_heads, n_kv,
                            head_dim);
+    return status_of(hipGetLastError());
+}
+
+extern "C" int nf4_rope(const void *x, int64_t ld_x, const float *cos_t, const float *sin_t, void *y,
+                        int64_t ld_y, int64_t tokens, int heads, int head_dim, int inverse, int dtype,
+                        void *stream) {
+    const int st = rope_shape_ok(tokens, heads, 1, head_dim, dtype);
+    if (st != NF4_OK) return st;
+    const int64_t cols = static_cast<int64_t>(heads) * head_dim;
+    if (tokens > 1 && (ld_x < cols || ld_y < cols)) return NF4_ERR_ARG;
+    if (tokens == 0) return NF4_OK;
+    if (!x || !y || !cos_t || !sin_t) return NF4_ERR_ARG;
+    if (!rope_vec_ok(head_dim, ld_x, {x, y}, cos_t, sin_t) || ld_y % 4 != 0) return NF4_ERR_UNSUPPORTED;
+    auto s = static_cast<hipStream_t>(stream);
+    const int work = heads * (head_dim / 8);
+    const dim3 grid(static_cast<unsigned>(tokens), static_cast<unsigned>(work < 256 * 64 ? (work + 255) / 256 : 64));
+    auto X = static_cast<const uint16_t *>(x);
+    auto Y = static_cast<uint16_t *>(y);
+    if (dtype == NF4_BF16)
+        hipLaunchKernelGGL(rope_heads_kernel<NF4_BF16>, grid, dim3(256), 0, s, X, ld_x, cos_t, sin_t, Y,
+                           ld_y, heads, head_dim, inverse);
+    else
+        hipLaunchKernelGGL(rope_heads_kernel<NF4_F16>, grid, dim3(256), 0, s, X, ld_x, cos_t, sin_t, Y,
+                           ld_y, heads, head_dim, inverse);
     return status_of(hipGetLastError());
 }

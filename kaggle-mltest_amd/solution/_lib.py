@@ -166,6 +166,8 @@ _SIGNATURES = {
                              c_void_p, c_void_p, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
     "nf4_qkv_rope_bwd": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                  c_int64, c_int64, c_int, c_int, c_int, c_int, c_void_p]),
+    "nf4_rope": (c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_int,
+                         c_int, c_int, c_int, c_void_p]),
     "nf4_paged_append": (c_int, [ctypes.POINTER(NF4PagedKV), c_void_p, c_int64, c_void_p,
                                  c_void_p, c_int64, c_void_p, c_void_p, c_int64, c_int, c_int,
                                  c_void_p]),

@@ -485,6 +485,31 @@ def qkv_rope_bwd(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, cos: torc
     return out
 
 
+def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int, head_dim: int,
+         inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+    """The first `heads` heads of every row of x [tokens, *] rotated as qkv_rope does (cos, sin
+    [tokens, head_dim]), or by the transposed rotation (`inverse`: gradients), into `out`
+    [tokens, >= heads head_dim] (a new [tokens, heads head_dim] tensor; may be x itself)."""
+    _check_device(x, cos, sin, out)
+    tokens, cols = x.shape[0], heads * head_dim
+    if out is None:
+        out = torch.empty((tokens, cols), dtype=x.dtype, device=x.device)
+    for t in (x, out):
+        if t.dim() != 2 or t.shape[0] != tokens or t.shape[1] < cols or t.stride(1) != 1 \
+                or t.dtype != x.dtype or t.device != x.device:
+            raise ValueError("x and out are row-contiguous [tokens, >= heads * head_dim] tensors of "
+                             "one dtype and device")
+    if tuple(cos.shape) != (tokens, head_dim) or cos.shape != sin.shape or \
+            not x.device == cos.device == sin.device:
+        raise ValueError("cos and sin are [tokens, head_dim] on x's device")
+    cos, sin = cos.to(torch.float32).contiguous(), sin.to(torch.float32).contiguous()
+    st = load().nf4_rope(x.data_ptr(), x.stride(0), cos.data_ptr(), sin.data_ptr(), out.data_ptr(),
+                         out.stride(0), tokens, heads, head_dim, int(inverse), _code(x.dtype),
+                         stream_of(x))
+    check(st, "nf4_rope")
+    return out
+
+
 def make_lora(seg: int, rank: int, scale: float, t=None, b=None, a=None, da=None) -> NF4Lora:
     """The adapter struct of segment `seg`.  It holds raw pointers, so it also keeps references
     to its tensors: a temporary passed here (t=lora_xa(...)) stays allocated while the struct

@@ -13,7 +13,10 @@ its segments:
 
 The LoRA input xd of an adapter is x itself (dropout p = 0), or its own tensor: LoRA's
 dropout output, which the reference's norm kernel writes (drop_q, drop_v; layer.py:859-878)
-and whose gradient its norm backward masks (layer.py:1072-1090, 135-164: dd_q = da_q A_q).
+and whose gradient its norm backward masks (layer.py:1072-1090, 135-164: dd_q = da_q A_q),
+or x's dropout by the adapter's own `dropout` and `site` (kernels.dropout): the mask is a function of
+the element's place and ProjectionSpec.seed, so neither it nor xd is kept, and the backward pass forms
+both again and adds d(xd)'s masked sum to dX in one launch.
 The LoRA product is folded into the same GEMM launch as the weight product (one extra rank-r
 reduction slab), instead of the reference's separate mm's and fp32 add in the RoPE kernel; for
 an adapter on x its down-projection t = x A^T is left to the projection call too (inside the
@@ -97,12 +100,15 @@ class LoraAdapter:
     seg: int                  # index of the segment the adapter adds to
     scale: float              # alpha / r
     own_input: bool = False   # the adapter reads its own input xd (LoRA dropout) instead of x
+    dropout: float = 0.0      # of x, by the generator of kernels.dropout, at `site` with the spec's seed
+    site: int = 0
 
 
 @dataclass
 class ProjectionSpec:
     weights: list             # [(packed, quant_state)] stacked along the output dim
     loras: list = field(default_factory=list)   # [LoraAdapter]
+    seed: torch.Tensor | None = None            # int64 [2] (seed, step) of adapters with dropout
 
     def offsets(self):
         offs, o = [], 0
@@ -127,6 +133,25 @@ def _run_jobs(fn, jobs, like):
     for r, js in by_rank.items():
         for k in range(0, len(js), 4):
             fn(js[k:k + 4], like.shape[0], r, like.dtype, like)
+
+
+def _dropped(x, spec):
+    """{adapter index: its dropped x}, one launch for the adapters of one probability."""
+    by_p = {}
+    for i, ad in enumerate(spec.loras):
+        if ad.dropout:
+            if ad.own_input:
+                raise ValueError("an adapter's own input comes dropped: no `dropout` beside own_input")
+            if spec.seed is None:
+                raise ValueError("adapters with dropout need the spec's seed")
+            by_p.setdefault(ad.dropout, []).append(i)
+    out = {}
+    for p, where in by_p.items():
+        for k in range(0, len(where), 8):
+            part = where[k:k + 8]
+            sites = [spec.loras[i].site for i in part]
+            out.update(zip(part, kernels.dropout(x, p, spec.seed, sites)))
+    return out
 
 
 def _xd_slots(spec):
@@ -164,7 +189,8 @@ class NF4Projection(torch.autograd.Function):
         dtype = x.dtype
         x = _aligned_rows(x)
         structs, saved, jobs, xd_dtypes = [], [], [], []
-        for ad, a, b, xd in _adapter_params(spec, lora_params):
+        dropped = _dropped(x, spec)
+        for i, (ad, a, b, xd) in enumerate(_adapter_params(spec, lora_params)):
             a16 = a.detach().to(dtype).contiguous()
             b16 = b.detach().to(dtype).contiguous()
             xin = x
@@ -173,8 +199,10 @@ class NF4Projection(torch.autograd.Function):
                     raise ValueError("a LoRA input has the projection input's shape")
                 xd_dtypes.append(xd.dtype)
                 xin = _aligned_rows(xd.detach().to(dtype))
+            elif i in dropped:
+                xin = dropped[i]
             t = torch.empty((x.shape[0], a16.shape[0]), dtype=dtype, device=x.device)
-            if xd is None:  # t = x A^T: the projection's own call computes it
+            if xin is x:  # t = x A^T: the projection's own call computes it
                 if a16.data_ptr() % 16:
                     a16 = a16.clone()
                 structs.append(kernels.make_lora(ad.seg, a16.shape[0], ad.scale, t=t, b=b16, a=a16))
@@ -189,13 +217,15 @@ class NF4Projection(torch.autograd.Function):
         ctx.has_bias = bias is not None
         ctx.param_dtypes = [p.dtype for p in lora_params]
         ctx.xd_dtypes = xd_dtypes
-        ctx.save_for_backward(x, *saved)
+        # (the seed too: writing to it before the backward pass, which needs the same, is an error)
+        ctx.save_for_backward(x, spec.seed if dropped else None, *saved)
         return y
 
     @staticmethod
     def backward(ctx, dy):
-        x, *saved = ctx.saved_tensors
+        x, _, *saved = ctx.saved_tensors
         spec = ctx.spec
+        dropped, drop_grads = _dropped(x, spec), []
         dy = _aligned_rows(dy.to(x.dtype))
         offs = spec.offsets()
         # `live` holds every tensor the launches below reach only through raw pointers in
@@ -204,13 +234,15 @@ class NF4Projection(torch.autograd.Function):
         # while a queued kernel still reads it
         structs, da_jobs, wg_jobs, ax_jobs, per_ad, live = [], [], [], [], [], []
         k = 0
-        for ad in spec.loras:
+        for i, ad in enumerate(spec.loras):
             t, a16, b16 = saved[k: k + 3]
             k += 3
             xin = x
             if ad.own_input:
                 xin = saved[k]
                 k += 1
+            elif i in dropped:
+                xin = dropped[i]
             r = a16.shape[0]
             rows = int(spec.weights[ad.seg][1].shape[0])
             dy_s = dy[:, offs[ad.seg]: offs[ad.seg] + rows]
@@ -227,6 +259,10 @@ class NF4Projection(torch.autograd.Function):
             if ad.own_input:
                 dxd = torch.empty_like(xin)
                 ax_jobs.append((r, kernels.lora_ax_job(da, a16, dxd)))
+            elif i in dropped:
+                if ctx.needs_input_grad[0]:
+                    drop_grads.append((ad, torch.empty_like(xin)))
+                    ax_jobs.append((r, kernels.lora_ax_job(da, a16, drop_grads[-1][1])))
             else:
                 structs.append(kernels.make_lora(ad.seg, r, ad.scale, a=a16, da=da))
             per_ad.append((grad_a, grad_b, dxd))
@@ -242,6 +278,13 @@ class NF4Projection(torch.autograd.Function):
                 p += 1
                 q += 1
         dx = kernels.linear_dx(dy, spec.weights, structs) if ctx.needs_input_grad[0] else None
+        by_p = {}
+        for ad, g in drop_grads:
+            by_p.setdefault(ad.dropout, []).append((ad.site, g))
+        for p, parts in by_p.items():
+            for k in range(0, len(parts), 8):
+                sites, gs = zip(*parts[k:k + 8])
+                kernels.dropout_bwd(gs, p, spec.seed, sites, base=dx, out=dx)
         dbias = kernels.bias_grad(dy) if ctx.has_bias and ctx.needs_input_grad[1] else None
         return (dx, dbias, None, *grads)
 
@@ -253,3 +296,74 @@ def project(x, spec: ProjectionSpec, bias=None, lora_params=()):
             for t, a in zip(lora_params, _xd_slots(spec))]
     y = NF4Projection.apply(x.reshape(-1, shape[-1]), bias, spec, *flat)
     return y.view(*shape[:-1], y.shape[-1])
+
+
+def _rows3(t):
+    """A [tokens, heads, head_dim] tensor as the attention kernels take it (rows 16-byte aligned)."""
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
+        return t.contiguous()
+    return t
+
+
+class Attention(torch.autograd.Function):
+    """Causal attention of a packed batch (the reference's varlen _Attention, layer.py:735-826):
+    apply(q, k, v, cu_seqlens, scale, window, max_len) -> out, as kernels.attention_fwd takes them; the
+    backward pass forms the probabilities again."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, scale, window, max_len):
+        q, k, v = _rows3(q), _rows3(k), _rows3(v)
+        out, stats = kernels.attention_fwd(q, k, v, cu_seqlens, scale, window, max_len)
+        ctx.save_for_backward(q, k, v, out, stats, cu_seqlens)
+        ctx.how = scale, window, max_len
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        *saved, cu = ctx.saved_tensors
+        grads = kernels.attention_bwd(_rows3(dout), *saved, cu, *ctx.how)
+        return *grads, None, None, None, None
+
+
+def attention(q, k, v, cu_seqlens=None, scale=None, window=0, max_len=0):
+    """Attention.apply with kernels.attention_fwd's defaults."""
+    return Attention.apply(q, k, v, cu_seqlens, scale, window, max_len)
+
+
+class RopeAttention(torch.autograd.Function):
+    """Rotation and attention of a projection's q|k|v rows (layer.py:880-898): apply(qkv [tokens,
+    (n_heads + 2 n_kv) head_dim], cos, sin [tokens, head_dim], n_heads, n_kv, cu_seqlens, scale, window,
+    max_len) -> [tokens, n_heads, head_dim].  v is read where the projection wrote it, shared key heads
+    are rotated once, and the three gradients are written into one d(q|k|v)."""
+
+    @staticmethod
+    def forward(ctx, qkv, cos, sin, n_heads, n_kv, cu_seqlens, scale, window, max_len):
+        qkv = _aligned_rows(qkv)
+        tokens, cols = qkv.shape
+        if n_heads < 1 or n_kv < 1 or cols % (n_heads + 2 * n_kv):
+            raise ValueError("qkv has (n_heads + 2 n_kv) head_dim columns")
+        dim = cols // (n_heads + 2 * n_kv)
+        qk = kernels.rope(qkv, cos, sin, n_heads + n_kv, dim).view(tokens, n_heads + n_kv, dim)
+        v = qkv.view(tokens, n_heads + 2 * n_kv, dim)[:, n_heads + n_kv:]
+        out, stats = kernels.attention_fwd(qk[:, :n_heads], qk[:, n_heads:], v, cu_seqlens, scale,
+                                           window, max_len)
+        ctx.save_for_backward(qk, v, out, stats, cu_seqlens, cos, sin)
+        ctx.how = n_heads, (scale, window, max_len)
+        return out
+
+    @staticmethod
+    def backward(ctx, dout):
+        qk, v, out, stats, cu, cos, sin = ctx.saved_tensors
+        n_heads, how = ctx.how
+        tokens, both, dim = qk.shape
+        dqkv = torch.empty((tokens, both + v.shape[1], dim), dtype=qk.dtype, device=qk.device)
+        kernels.attention_bwd(_rows3(dout), qk[:, :n_heads], qk[:, n_heads:], v, out, stats, cu, *how,
+                              grads=(dqkv[:, :n_heads], dqkv[:, n_heads:both], dqkv[:, both:]))
+        dqkv = dqkv.view(tokens, -1)
+        kernels.rope(dqkv, cos, sin, both, dim, inverse=True, out=dqkv)
+        return dqkv, *[None] * 8
+
+
+def rope_attention(qkv, cos, sin, n_heads, n_kv, cu_seqlens=None, scale=None, window=0, max_len=0):
+    """RopeAttention.apply with kernels.attention_fwd's defaults."""
+    return RopeAttention.apply(qkv, cos, sin, n_heads, n_kv, cu_seqlens, scale, window, max_len)

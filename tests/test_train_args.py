@@ -147,3 +147,16 @@ def test_python_refusals():
         kernels.dropout(x.float(), 0.5, seed, [0])
     with pytest.raises(ValueError):
         kernels.dropout_bwd([x, x], 0.5, seed, [0])
+
+
+def test_rope_refusals(lib):
+    def rope(x=P, ld=128, cos=P, sin=P, y=P, ldy=128, tokens=3, heads=2, dim=64, inverse=0, dtype=0):
+        return lib.nf4_rope(x, ld, cos, sin, y, ldy, tokens, heads, dim, inverse, dtype, None)
+
+    assert rope(x=None) == ARG and rope(y=None) == ARG and rope(cos=None) == ARG and rope(sin=None) == ARG
+    assert rope(tokens=-1) == ARG and rope(heads=0) == ARG and rope(dtype=2) == ARG and rope(dim=7) == ARG
+    assert rope(ld=120) == ARG and rope(ldy=120) == ARG
+    assert rope(dim=4, heads=2) == UNSUPPORTED and rope(dim=520, ld=2080, ldy=2080) == UNSUPPORTED
+    assert rope(x=P + 4) == UNSUPPORTED and rope(y=P + 2) == UNSUPPORTED and rope(cos=P + 8) == UNSUPPORTED
+    assert rope(ld=130) == UNSUPPORTED and rope(ldy=130) == UNSUPPORTED
+    assert rope(tokens=0, x=None) == OK
