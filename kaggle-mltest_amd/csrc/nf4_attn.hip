@@ -251,27 +251,31 @@ __device__ __forceinline__ constexpr int swizzle(int r) {
 template <int D>
 constexpr int kTileBytes = kTile * D * 2;
 
-// What a thread knows of a tensor's tiles: the byte of its 16 in the first pass, and its rows' pitch.
+// A tensor's tiles of ROWS rows of a head, one after the other: where the next begins, and what a thread
+// knows of them: the byte of its 16 in the first pass, and the passes' distance.
 template <int D, int ROWS>
 struct Stager {
     static constexpr int CH = D / 8, RPP = 256 / CH;
-    const uint16_t *base;  // the head's first row
-    int64_t tok;
-    int off, step;
+    const uint16_t *next;
+    int pitch, off;  // bytes
 
-    __device__ __forceinline__ void set(const Strided &x, int head, int tid) {
-        const int row = tid / CH, ch = tid % CH;
-        base = x.p + head * x.head;
-        tok = x.tok;
-        off = row * static_cast<int>(tok) * 2 + ((ch ^ swizzle<D>(row)) << 4);
-        step = RPP * static_cast<int>(tok) * 2;
+    __device__ __forceinline__ void begin(const Strided &x, int head, int t) {
+        next = reinterpret_cast<const uint16_t *>(uniform64(reinterpret_cast<int64_t>(x.p + head * x.head + t * x.tok)));
     }
-    // rows [t, t + ROWS) to LDS address `at` (the wave's); rows from `end` on are zeros, and not read
-    __device__ __forceinline__ void send(uint32_t at, int t, int end) const {
-        const int64_t bytes = t < end ? (end - t - 1) * tok * 2 + D * 2 : 0;
-        const rsrc_t r = make_rsrc(base + t * tok, bytes);
+    __device__ __forceinline__ void set(const Strided &x, int head, int t, int tid) {
+        const int row = tid / CH, ch = tid % CH;
+        begin(x, head, t);
+        pitch = static_cast<int>(x.tok) * 2;
+        off = row * pitch + ((ch ^ swizzle<D>(row)) << 4);
+    }
+    // the next tile to LDS address `at` (the wave's); rows from `rows` on are zeros, and not read
+    __device__ __forceinline__ void send(uint32_t at, int rows) {
+        const int n = rows < ROWS ? rows : ROWS;
+        const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(next), static_cast<short>(0),
+                                                           n > 0 ? (n - 1) * pitch + D * 2 : 0, 0x00020000);
 #pragma unroll
-        for (int x = 0; x < ROWS / RPP; ++x) lds_dma16(at + x * 4096, off + x * step, r, 0);
+        for (int x = 0; x < ROWS / RPP; ++x) lds_dma16(at + x * 4096, off + x * RPP * pitch, r, 0);
+        next = reinterpret_cast<const uint16_t *>(reinterpret_cast<const char *>(next) + static_cast<int64_t>(ROWS) * pitch);
     }
 };
 
@@ -512,8 +516,9 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     const float c = fabsf(a.c);
     own_operand<D>(q, a.q.at(r, head), r < a.tokens, l, a.c < 0.f ? 0x80008000u : 0u);
     Stager<D, kTile> sk, sv;
-    sk.set(a.k, kvh, threadIdx.x);
-    sv.set(a.v, kvh, threadIdx.x);
+    const int first = k0 + mine_of.x * kTile;
+    sk.set(a.k, kvh, first, threadIdx.x);
+    sv.set(a.v, kvh, first, threadIdx.x);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) uint8_t *)lds));
     const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
@@ -524,18 +529,17 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     float16_t acc[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
-    const int first = k0 + mine_of.x * kTile;
     int k = steps ? first : all.y, st = 0;
     if (k < all.y) {
-        sk.send(mine, k, all.y);
-        sv.send(mine + 2 * TB, k, all.y);
+        sk.send(mine, all.y - k);
+        sv.send(mine + 2 * TB, all.y - k);
     }
     for (; k < all.y; k += kTile, st ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();  // every wave's part of this tile is there, and the one before is read
         if (k + kTile < all.y) {
-            sk.send(mine + (st ^ 1) * TB, k + kTile, all.y);
-            sv.send(mine + (2 + (st ^ 1)) * TB, k + kTile, all.y);
+            sk.send(mine + (st ^ 1) * TB, all.y - k - kTile);
+            sv.send(mine + (2 + (st ^ 1)) * TB, all.y - k - kTile);
         }
         if (sp.none(k, kTile)) continue;
         u32x4_t kf[2][KS];
@@ -941,8 +945,8 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     // (the probabilities are used for dS only: their scale goes into the exponent)
     const float mul = near ? a.c : 1.f, sub = (near ? base : 0.f) - log2f(fs);
     Stager<D, kTile> sk, sv;
-    sk.set(a.k, kvh, tid);
-    sv.set(a.v, kvh, tid);
+    sk.set(a.k, kvh, first, tid);
+    sv.set(a.v, kvh, first, tid);
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
         (__attribute__((address_space(3))) uint8_t *)lds));
     const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
@@ -953,16 +957,16 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
     int k = u.x < u.y ? first : last, st = 0;
     if (k < last) {
-        sk.send(mine, k, last);
-        sv.send(mine + 2 * TB, k, last);
+        sk.send(mine, last - k);
+        sv.send(mine + 2 * TB, last - k);
     }
 #pragma unroll 1
     for (; k < last; k += kTile, st ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __syncthreads();
         if (k + kTile < last) {
-            sk.send(mine + (st ^ 1) * TB, k + kTile, last);
-            sv.send(mine + (2 + (st ^ 1)) * TB, k + kTile, last);
+            sk.send(mine + (st ^ 1) * TB, last - k - kTile);
+            sv.send(mine + (2 + (st ^ 1)) * TB, last - k - kTile);
         }
         const uint32_t ka = ra + st * TB, va = ra + (2 + st) * TB, kt = ca + st * TB;
 #pragma unroll
@@ -1074,8 +1078,8 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
     const uint32_t tiles0 = mine + VB, rows0 = __builtin_amdgcn_readfirstlane(lds0 + VB + 4 * RB);
     Stager<D, kOwn> sv;
     Stager<D, kRows> sq, sg;
-    sv.set(a.v, kvh, tid);
-    if (units.x < units.y) sv.send(mine, tile * kOwn, a.tokens);
+    sv.set(a.v, kvh, tile * kOwn, tid);
+    if (units.x < units.y) sv.send(mine, a.tokens - tile * kOwn);
     u32x4_t kf[KS];
     own_operand<D>(kf, a.k.at(j, kvh), j < a.tokens, l);
     float fs = 1.f;
@@ -1090,22 +1094,26 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
     }
     // unit (head of the group, tile of rows), the next one
     int uh = per ? units.x / per : 0, ut = units.x - uh * per;
-    sq.set(a.q, kvh * a.group + uh, tid);
-    sg.set(a.dout, kvh * a.group + uh, tid);
+    sq.set(a.q, kvh * a.group + uh, (t0 + ut) * kRows, tid);
+    sg.set(a.dout, kvh * a.group + uh, (t0 + ut) * kRows, tid);
     int t = ut, st = 0;
+    auto numbers = [&](int h) {  // of the rows of tile t0 of a head
+        return b.rows + (static_cast<int64_t>(kvh * a.group + h) * b.blocks * 2 + t0) * 128;
+    };
+    const float *rw_next = numbers(uh) + ut * 128;
     auto send = [&](int st) {
-        const int r = (t0 + ut) * kRows;
-        sq.send(tiles0 + st * RB, r, rows.y);
-        sg.send(tiles0 + (2 + st) * RB, r, rows.y);
-        if (w == 0) {  // (512 bytes: the upper lanes' are past the end, zeros)
-            const float *p = b.rows + (static_cast<int64_t>(kvh * a.group + uh) * b.blocks * 2 + t0 + ut) * 128;
-            lds_dma16(__builtin_amdgcn_readfirstlane(rows0 + st * 1024), l * 16, make_rsrc(p, 512), 0);
-        }
+        const int left = rows.y - (t0 + ut) * kRows;
+        sq.send(tiles0 + st * RB, left);
+        sg.send(tiles0 + (2 + st) * RB, left);
+        if (w == 0)  // (512 bytes: the upper lanes' are past the end, zeros)
+            lds_dma16(rows0 + st * 1024, l * 16, make_rsrc(reinterpret_cast<const float *>(uniform64(reinterpret_cast<int64_t>(rw_next))), 512), 0);
+        rw_next += 128;
         if (++ut == per) {
             ut = 0;
             ++uh;
-            sq.base += a.q.head;
-            sg.base += a.dout.head;
+            sq.begin(a.q, kvh * a.group + uh, t0 * kRows);
+            sg.begin(a.dout, kvh * a.group + uh, t0 * kRows);
+            rw_next = numbers(uh);
         }
     };
     const uint32_t va = lds0 + w * 32 * D * 2 + row_address<D>(l);
