@@ -1348,15 +1348,13 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(const Attn a, const 
     const int kvh = blockIdx.y / b.groups, w = blockIdx.x & 3, array = blockIdx.x >> 2;
     int g = blockIdx.y % b.groups;
     const int *inside = b.inside + kvh * b.groups;
-    const int e = inside[g];
-    if (e < 0 || (array && e >= b.tiles) || (g > 0 && inside[g - 1] == e)) return;
-    int end = g;  // the first share that is not inside of it
-    for (;;) {
-        const int i = end + (threadIdx.x & 63);
-        const uint64_t same = __ballot(i < b.groups && inside[i < b.groups ? i : 0] == e);
-        end += ~same ? __builtin_ctzll(~same) : 64;
-        if (~same) break;
-    }
+    const int i = g - 1 + (threadIdx.x & 63);  // the share before, this one and those behind it
+    const int near = i >= 0 && i < b.groups ? inside[i] : -1;
+    const int e = __builtin_amdgcn_readlane(near, 1);
+    if (e < 0 || (array && e >= b.tiles) || __builtin_amdgcn_readlane(near, 0) == e) return;
+    int end = g + __builtin_ctzll(~(__ballot(near == e) >> 1));  // the first share that is not inside of it
+    if (end == g + 63)
+        while (end < b.groups && inside[end] == e) ++end;
     const int at = (array * kOwn + w * 32) * D + threadIdx.x * 4;
     float4_t v[D / 32];
     const float *part = slot_of<D>(b, kvh, g - 1, 1) + at;
@@ -1364,17 +1362,18 @@ __global__ __launch_bounds__(256) void attn_bwd_join_kernel(const Attn a, const 
     for (int x = 0; x < D / 32; ++x) v[x] = *reinterpret_cast<const float4_t *>(part + x * 1024);
     part = slot_of<D>(b, kvh, g, 0) + at;
     constexpr int64_t NEXT = 4 * kOwn * D;  // the next share's slot 0
-    for (; g < end; g += 4, part += 4 * NEXT) {  // (four parts' loads under way: their latency counts)
-        float4_t f[4][D / 32];
+    constexpr int BATCH = 4;                // parts whose loads are under way: it is their latency that counts
+    for (; g < end; g += BATCH, part += BATCH * NEXT) {
+        float4_t f[BATCH][D / 32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < BATCH; ++i)
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) {
                 f[i][x] = (float4_t){0.f, 0.f, 0.f, 0.f};
                 if (g + i < end) f[i][x] = *reinterpret_cast<const float4_t *>(part + i * NEXT + x * 1024);
             }
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < BATCH; ++i)
 #pragma unroll
             for (int x = 0; x < D / 32; ++x) v[x] += f[i][x];
     }
