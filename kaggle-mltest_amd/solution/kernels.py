@@ -931,26 +931,30 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
 
 
 def _rows_of(t, shape, dtype, index):
-    if tuple(t.shape) != shape or t.dtype != dtype or t.get_device() != index \
+    if t.shape != shape or t.dtype != dtype or t.get_device() != index \
             or (t.stride(1) != 1 and shape[1] > 1):
         raise ValueError(f"dropout's tensors are row-contiguous {list(shape)} tensors of one dtype "
                          "and device")
 
 
-def _drop_args(tensors, seed, sites):
-    """(pointers, row strides, site numbers) as ctypes arrays."""
-    index = tensors[0].get_device()
+_SITES = range(9)  # (array types are made once: ctypes looks them up by name otherwise)
+_PTR_ARRAYS = [ctypes.c_void_p * n for n in _SITES]
+_LD_ARRAYS = [ctypes.c_int64 * n for n in _SITES]
+_SITE_ARRAYS = [ctypes.c_uint32 * n for n in _SITES]
+
+
+def _drop_args(tensors, seed, sites, index):
+    """(pointers, row strides, site numbers) of the sites' tensors as ctypes arrays, n."""
     if index < 0 or seed.get_device() != index or seed.dtype != torch.int64 \
-            or tuple(seed.shape) != (2,) or not seed.is_contiguous():
+            or seed.shape != (2,) or not seed.is_contiguous():
         raise ValueError("seed is an int64 [2] tensor (seed, step) on the tensors' cuda device")
     n = len(sites)
     if not 1 <= n <= 8:
         raise ValueError("dropout takes 1 to 8 sites")
-    if any(not 0 <= s < 1 << 32 for s in sites):
+    if min(sites) < 0 or max(sites) >> 32:
         raise ValueError("a site is a number of 32 bits")
-    ptrs = (ctypes.c_void_p * len(tensors))(*[t.data_ptr() for t in tensors])
-    lds = (ctypes.c_int64 * len(tensors))(*[t.stride(0) for t in tensors])
-    return ptrs, lds, (ctypes.c_uint32 * n)(*sites)
+    return (_PTR_ARRAYS[n](*[t.data_ptr() for t in tensors]),
+            _LD_ARRAYS[n](*[t.stride(0) for t in tensors]), _SITE_ARRAYS[n](*sites), n)
 
 
 def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, sites, outs=None) -> list:
@@ -962,24 +966,22 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, sites, outs=None) -> 
     (seed[1] += 1; a captured graph reads it at each replay)."""
     if x.dim() != 2:
         raise ValueError("x is [rows, cols]")
-    dt, shape, index = _code(x.dtype), tuple(x.shape), x.get_device()
-    _rows_of(x, shape, x.dtype, index)
+    shape, dtype, index = x.shape, x.dtype, x.get_device()
+    dt = _code(dtype)
+    _rows_of(x, shape, dtype, index)
     if outs is None:
-        outs = [torch.empty(shape, dtype=x.dtype, device=x.device) for _ in sites]
-    if len(outs) != len(sites):
-        raise ValueError("an output for every site")
-    for t in outs:
-        _rows_of(t, shape, x.dtype, index)
-    ptrs, lds, where = _drop_args([x, *outs], seed, sites)
-    st = load().nf4_dropout(x.data_ptr(), x.stride(0), ctypes.cast(ctypes.byref(ptrs, 8), _PTRS),
-                            ctypes.cast(ctypes.byref(lds, 8), _LDS), *shape, float(p),
-                            seed.data_ptr(), where, len(sites), dt, stream_of(x))
+        outs = [x.new_empty(shape) for _ in sites]
+    else:
+        if len(outs) != len(sites):
+            raise ValueError("an output for every site")
+        for t in outs:
+            _rows_of(t, shape, dtype, index)
+    ptrs, lds, where, n = _drop_args(outs, seed, sites, index)
+    st = load().nf4_dropout(x.data_ptr(), x.stride(0), ptrs, lds, shape[0], shape[1], p,
+                            seed.data_ptr(), where, n, dt, stream_of(x))
     if st:
         check(st, "nf4_dropout")
-    return list(outs)
-
-
-_PTRS, _LDS = ctypes.POINTER(ctypes.c_void_p), ctypes.POINTER(ctypes.c_int64)
+    return outs
 
 
 def dropout_bwd(grads, p: float, seed: torch.Tensor, sites, base: torch.Tensor | None = None,
@@ -989,15 +991,20 @@ def dropout_bwd(grads, p: float, seed: torch.Tensor, sites, base: torch.Tensor |
     g = grads[0]
     if g.dim() != 2 or len(grads) != len(sites):
         raise ValueError("a [rows, cols] gradient for every site")
-    dt, shape, index = _code(g.dtype), tuple(g.shape), g.get_device()
+    shape, dtype, index = g.shape, g.dtype, g.get_device()
+    dt = _code(dtype)
+    for t in grads:
+        _rows_of(t, shape, dtype, index)
+    if base is not None:
+        _rows_of(base, shape, dtype, index)
     if out is None:
-        out = torch.empty(shape, dtype=g.dtype, device=g.device)
-    for t in (*grads, out, *(() if base is None else (base,))):
-        _rows_of(t, shape, g.dtype, index)
-    ptrs, lds, where = _drop_args(list(grads), seed, sites)
-    st = load().nf4_dropout_bwd(ptrs, lds, _p(base), base.stride(0) if base is not None else 0,
-                                out.data_ptr(), out.stride(0), *shape, float(p), seed.data_ptr(),
-                                where, len(sites), dt, stream_of(g))
+        out = g.new_empty(shape)
+    elif out is not base:
+        _rows_of(out, shape, dtype, index)
+    ptrs, lds, where, n = _drop_args(grads, seed, sites, index)
+    st = load().nf4_dropout_bwd(ptrs, lds, _p(base), 0 if base is None else base.stride(0),
+                                out.data_ptr(), out.stride(0), shape[0], shape[1], p,
+                                seed.data_ptr(), where, n, dt, stream_of(g))
     if st:
         check(st, "nf4_dropout_bwd")
     return out
