@@ -103,12 +103,13 @@ __device__ __forceinline__ int2 rows_of(const Attn &a, int t) {
 
 // A score's exponent: fma(score, c, -m), exact but for its own rounding; where m is far from 0 the
 // rounding of m itself would show in that (16 and more from 2^28 on), so there the product is rounded
-// as m was.  Never above 0, where m is the largest: sums in another order could be.
+// as m was.  It is above 0 by as much as m was rounded, which the row's sum has in it as well; a
+// probability is at most 1 also where sums in another order would make more of it (`capped`).
 constexpr float kFar = 1 << 20;
 __device__ __forceinline__ float exponent(float s, float c, float m) {
-    const float x = fabsf(m) > kFar ? s * c - m : fmaf(s, c, -m);
-    return x > 0.f ? 0.f : x;  // (a NaN stays)
+    return fabsf(m) > kFar ? s * c - m : fmaf(s, c, -m);
 }
+__device__ __forceinline__ float capped(float x, float most) { return x > most ? most : x; }  // (a NaN stays)
 
 // ------------------------------------------------------------------- one row, one key
 //
@@ -199,7 +200,7 @@ __device__ __forceinline__ void row_backward(const Attn &a, int head, int r, int
     for (int k = k0; k < k1; k += 64) {
         float ds = 0.f;
         if (k + lane < k1) {
-            const float p = __builtin_amdgcn_exp2f(exponent(dot_of<DT, D>(q, a.k.at(k + lane, kvh)), a.c, ml.x)) * inv;
+            const float p = capped(__builtin_amdgcn_exp2f(exponent(dot_of<DT, D>(q, a.k.at(k + lane, kvh)), a.c, ml.x)) * inv, 1.f);
             ds = p * (dot_of<DT, D>(go, a.v.at(k + lane, kvh)) - delta);
         }
         const int n = k1 - k < 64 ? k1 - k : 64;
@@ -218,7 +219,7 @@ __device__ __forceinline__ void key_backward(const Attn &a, int head, int j, int
         if (r + lane < r1) {
             const float2 ml = a.stats[static_cast<int64_t>(r + lane) * a.n_heads + head];
             const uint16_t *go = a.dout.at(r + lane, head);
-            p = __builtin_amdgcn_exp2f(exponent(dot_of<DT, D>(kj, a.q.at(r + lane, head)), a.c, ml.x)) / ml.y;
+            p = capped(__builtin_amdgcn_exp2f(exponent(dot_of<DT, D>(kj, a.q.at(r + lane, head)), a.c, ml.x)) / ml.y, 1.f);
             ds = p * (dot_of<DT, D>(vj, go) - dot_of<DT, D>(go, a.o.at(r + lane, head)));
         }
         const int n = r1 - r < 64 ? r1 - r : 64;
@@ -376,15 +377,36 @@ __device__ __forceinline__ bool bit_of(uint64_t m, int h, int e) {
 template <int DT>
 constexpr float kTop = DT == NF4_BF16 ? 0.f : 15.f;
 
-// 0 where all registers are finite, else NaN
+// Infinities and NaN.  A probability of 0 that stands for a key that is not seen makes NaN of an infinity
+// or NaN beside it in the tile.  So a row (or key) whose sums hold a NaN is formed again from what it
+// sees alone, by the functions above, unless what it sees says that it is NaN.
 template <int N>
-__device__ __forceinline__ float odd_of(const float16_t (&v)[N]) {
-    float z = 0.f;
+__device__ __forceinline__ bool any_nan(const float16_t (&v)[N]) {
+    float odd = 0.f;
 #pragma unroll
     for (int x = 0; x < N; ++x)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) z = fmaf(v[x][e], 0.f, z);
+        for (int e = 0; e < 16; ++e) odd = fmaf(v[x][e], 0.f, odd);
+    bool z = false;
+    if (__any(odd != 0.f)) {  // (one instruction a register, where all are finite)
+#pragma unroll
+        for (int x = 0; x < N; ++x)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) z |= v[x][e] != v[x][e];
+    }
     return z;
+}
+// the rows of a wave (bit n: lanes n and n + 32) for which `which` is true of a lane
+__device__ __forceinline__ uint32_t rows_where(bool which) {
+    const uint64_t m = __ballot(which);
+    return static_cast<uint32_t>(m) | static_cast<uint32_t>(m >> 32);
+}
+template <int N>
+__device__ __forceinline__ void fill_of(float16_t (&v)[N], float f) {
+#pragma unroll
+    for (int x = 0; x < N; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) v[x][e] = f;
 }
 
 // This lane's channels of its row, from a transposed result.
@@ -399,15 +421,6 @@ __device__ __forceinline__ void store_own(uint16_t *row, const float16_t (&v)[D 
                 (u32x2_t){pack2<DT>(v[x][e] * f, v[x][e + 1] * f), pack2<DT>(v[x][e + 2] * f, v[x][e + 3] * f)};
 }
 
-// A row that sees nothing has zeros (its registers hold anything: no mask kept tiles from it that every
-// other row of its wave sees whole).
-template <int N>
-__device__ __forceinline__ void zero_unless(bool some, float16_t (&v)[N]) {
-    if (some) return;
-#pragma unroll
-    for (int x = 0; x < N; ++x) v[x] = (float16_t){};
-}
-
 // An output is a mean of values: one past fp16's last number is there by the roundings of its
 // probabilities (a step at most), and is that number.
 template <int DT, int N>
@@ -416,7 +429,10 @@ __device__ __forceinline__ void keep_finite(float16_t (&v)[N], float f) {
 #pragma unroll
         for (int x = 0; x < N; ++x)
 #pragma unroll
-            for (int e = 0; e < 16; ++e) v[x][e] = __builtin_amdgcn_fmed3f(v[x][e] * f, -65504.f, 65504.f);
+            for (int e = 0; e < 16; ++e) {
+                v[x][e] *= f;
+                v[x][e] = fabsf(v[x][e]) < INFINITY ? __builtin_amdgcn_fmed3f(v[x][e], -65504.f, 65504.f) : v[x][e];
+            }
     }
 }
 
@@ -525,7 +541,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     const uint32_t ka = lds0 + row_address<D>(l), va = lds0 + 2 * TB + channel_address<D>(l);
 
     float m = -INFINITY, sum = 0.f;
-    bool far = false;  // a row's m is (the wave's)
+    bool far = false;  // a row's m is (of the wave's; each row by its own, as in the backward pass)
     float16_t acc[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
@@ -587,7 +603,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
         const float base = m == -INFINITY ? 0.f : m;
         if (__builtin_expect(far, 0)) {
 #pragma unroll
-            for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] = sc[e >> 4][e & 15] * c - base;
+            for (int e = 0; e < 32; ++e) sc[e >> 4][e & 15] = exponent(sc[e >> 4][e & 15], c, base);
         }
         const float mul = far ? 1.f : c, sub = far ? 0.f : base;
 #pragma unroll
@@ -614,49 +630,48 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     sum += other_half(sum);
     const int2 part = make_int2(seen.x > first ? seen.x : first, seen.y < all.y ? seen.y : all.y);  // of this piece
     const bool some = part.x < part.y;
-    const float odd = odd_of(acc);
     const int64_t slot = ((static_cast<int64_t>(tile) * a.n_heads + head) * pc.most + piece) * kOwn + w * 32;
-    if (__any(some && !(odd == 0.f && sum > 0.f && sum < INFINITY && fabsf(m) < INFINITY))) {
-        // An infinity or NaN: a product with a probability of 0 that stands for a key that is not
-        // seen is none, and each row is formed from what it sees alone.
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-            const int row = tile * kOwn + w * 32 + i;
-            const int x0 = __builtin_amdgcn_readlane(part.x, i), x1 = __builtin_amdgcn_readlane(part.y, i);
-            if (row >= a.tokens) break;  // (parts of rows that are not there are not read)
-            float o[D / 64], rm, rl;
-            row_forward<DT, D>(a, head, row, x0, x1, rm, rl, o);
-            if (x0 >= x1) rm = rl = 0.f;
-            if (pieces > 1) {
-                store_part_row<D>(pc.part + slot * D, i, o);
-                if (l == 0) pc.ml[slot + i] = make_float2(rm, rl);
-                continue;
-            }
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) o[x] = x0 < x1 ? o[x] / rl : 0.f;
-            store_row<DT, D>(a.o.to(row, head), o);
-            if (l == 0) a.stats[static_cast<int64_t>(row) * a.n_heads + head] = make_float2(rm, rl);
-        }
-        return;
-    }
-    zero_unless(some, acc);
+    const bool nan = some && !(sum > 0.f && fabsf(m) < INFINITY);  // a score is NaN or +inf, or all are -inf
+    const bool none = nan && pieces > 1 && m == -INFINITY && sum == 0.f;  // (here: other pieces may have more)
+    const uint32_t again = rows_where(some && !nan && any_nan(acc));
+    // a row that sees nothing has zeros (its registers hold anything: no mask kept tiles from it that every
+    // other row of its wave sees whole)
+    if (!some || none) fill_of(acc, 0.f);
+    else if (nan) fill_of(acc, NAN);
     const bool f = fabsf(m) > kFar;
     float2 ml = make_float2(f ? m : m + kTop<DT>, f ? sum : __builtin_amdgcn_ldexpf(sum, -static_cast<int>(kTop<DT>)));
+    if (nan) ml.y = none ? 0.f : NAN;
     if (!some) ml = make_float2(0.f, 0.f);
+    const bool mine_now = r < a.tokens && !(again >> n & 1);
     if (pieces > 1) {
         if (!f && some)
 #pragma unroll
             for (int x = 0; x < DN; ++x) acc[x] *= __builtin_amdgcn_ldexpf(1.f, -static_cast<int>(kTop<DT>));
-        store_part<D>(pc.part + slot * D, acc);
+        store_part<D>(pc.part + slot * D, acc);  // (rows that follow below or are not there, too)
         if (g == 0) pc.ml[slot + n] = ml;
-        return;
+    } else if (mine_now) {
+        const float inv = some ? 1.f / sum : 0.f;
+        keep_finite<DT>(acc, inv);
+        store_own<DT, D>(a.o.to(r, head), acc, DT == NF4_F16 ? 1.f : inv);
+        if (g == 0) a.stats[static_cast<int64_t>(r) * a.n_heads + head] = ml;
     }
-    if (r >= a.tokens) return;
-    float inv = some ? 1.f / sum : 0.f;
-    keep_finite<DT>(acc, inv);
-    if constexpr (DT == NF4_F16) inv = 1.f;
-    store_own<DT, D>(a.o.to(r, head), acc, inv);
-    if (g == 0) a.stats[static_cast<int64_t>(r) * a.n_heads + head] = ml;
+    if (!again) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (parts are there before their rows are written again)
+#pragma unroll 1
+    for (uint32_t left = again; left; left &= left - 1) {
+        const int i = __builtin_ctz(left), row = tile * kOwn + w * 32 + i;
+        float o[D / 64], rm, rl;
+        row_forward<DT, D>(a, head, row, __builtin_amdgcn_readlane(part.x, i), __builtin_amdgcn_readlane(part.y, i), rm, rl, o);
+        if (pieces > 1) {
+            store_part_row<D>(pc.part + slot * D, i, o);
+            if (l == 0) pc.ml[slot + i] = make_float2(rm, rl);
+            continue;
+        }
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) o[x] /= rl;
+        store_row<DT, D>(a.o.to(row, head), o);
+        if (l == 0) a.stats[static_cast<int64_t>(row) * a.n_heads + head] = make_float2(rm, rl);
+    }
 }
 
 // A workgroup joins 32 rows of a tile that is in pieces: each a (m, l, o) of its keys.
@@ -671,14 +686,17 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Attn a, const 
     const int n = threadIdx.x & 31, r = tile * kOwn + w * 32 + n;
     float m = -INFINITY, l = 0.f;
     if (r < a.tokens) {
+        bool all_low = false;  // a piece saw scores of -inf only
         for (int p = 0; p < pieces; ++p) {
             const float2 x = pc.ml[slot + p * kOwn + n];
             if (x.y != 0.f) m = fmaxf(m, x.x);  // (0: it saw nothing)
+            else all_low |= x.x == -INFINITY;
         }
         for (int p = 0; p < pieces; ++p) {
             const float2 x = pc.ml[slot + p * kOwn + n];
             if (x.y != 0.f) l += x.y * (x.x == m ? 1.f : __builtin_amdgcn_exp2f(x.x - m));
         }
+        if (l == 0.f && all_low) l = NAN;
         if (threadIdx.x < 32)
             a.stats[static_cast<int64_t>(r) * a.n_heads + head] = l == 0.f ? make_float2(0.f, 0.f) : make_float2(m, l);
     }
@@ -701,6 +719,7 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Attn a, const 
 #pragma unroll
             for (int e = 0; e < 4; ++e)
                 o[x][e] = fabsf(o[x][e]) < INFINITY ? __builtin_amdgcn_fmed3f(o[x][e], -65504.f, 65504.f) : o[x][e];
+        if (l != l) o[x] = (float4_t){NAN, NAN, NAN, NAN};
         join_put<DT, D>(lds, x * 256 + threadIdx.x, o[x]);
     }
     join_write<D>(a.o, head, tile * kOwn + w * 32, a.tokens, lds);
@@ -709,7 +728,10 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Attn a, const 
 // ----------------------------------------------------------------------------- backward
 //
 // What the backward pass reads of a row for every key, in blocks of 32 rows, four numbers each: m,
-// log2 l and m + log2 l (in fp16 less kTop), and -D.  Where |m| is below kNear a probability's exponent
+// log2 l and m + log2 l (in fp16 less kTop), and -D; zeros of a row of no sequence, and NaN of a row whose
+// do, statistics or D hold an infinity or NaN: its dq is NaN then, and the dk and dv of every key that it
+// sees (elementwise some would be infinite or finite; that costs what forming them one by one does, and a
+// loss whose scale was too high has such rows everywhere).  Where |m| is below kNear a probability's exponent
 // is taken with the sum of the first two, whose rounding (2^-16) is below those that follow.
 constexpr float kNear = 256.f;
 
@@ -850,6 +872,8 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back
     for (int x = 0; x < kTile; x += RPP) {
         const int i = x + threadIdx.x / CH, r = blockIdx.x * kTile + i;
         float d = 0.f, sq = 0.f;
+        float2 ml = make_float2(0.f, 0.f);
+        if (r < a.tokens) ml = a.stats[static_cast<int64_t>(r) * a.n_heads + (of_v ? 0 : head)];
         if (r < a.tokens) {
             float go[8], o[8];
             unpack8<DT>(*reinterpret_cast<const u32x4_t *>((of_v ? a.v.at(r, head - a.n_heads) : a.dout.at(r, head)) + ch * 8), go);
@@ -866,10 +890,11 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back
             d += __shfl_xor(d, o);
             sq += __shfl_xor(sq, o);
         }
-        worst = fmaxf(worst, sq);
+        const bool none = ml.y == 0.f;  // a row of no sequence, whatever lies there
+        if (!none && sq < INFINITY) worst = fmaxf(worst, sq);  // (what sees an odd one is NaN)
         if (of_v || ch) continue;
-        float2 ml = make_float2(0.f, 0.f);
-        if (r < a.tokens) ml = a.stats[static_cast<int64_t>(r) * a.n_heads + head];
+        if (none) d = 0.f;
+        else if (!(fabsf(d) < INFINITY && fabsf(ml.x) < INFINITY)) ml = make_float2(NAN, NAN);  // (an odd do or out: an odd d)
         const float ll = (ml.y == 0.f ? 0.f : log2f(ml.y)) - kTop<DT>;
         float *p = b.rows + (static_cast<int64_t>(head) * b.blocks + blockIdx.x) * 256 + (i >> 5) * 128 + (i & 31);
         p[0] = ml.x;
@@ -1003,7 +1028,7 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
             __builtin_amdgcn_sched_barrier(0);
             if (__builtin_expect(!near, 0)) {
 #pragma unroll
-                for (int e = 0; e < 16; ++e) sc[e] = exponent(sc[e], a.c, m) - ll;
+                for (int e = 0; e < 16; ++e) sc[e] = capped(exponent(sc[e], a.c, m) - ll, kTop<DT>);
             }
             if (!sp.full(k + 32 * h, 32)) {
                 const uint64_t see = seen_bits(seen, k);
@@ -1025,28 +1050,29 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     const int2 own = make_int2(seen.x > first ? seen.x : first, seen.y < last ? seen.y : last);  // of this share
     const bool some = own.x < own.y;
     if (part) part += w * 32 * D;
-    if (__any(some && !(odd_of(acc) == 0.f))) {  // as in the forward pass
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-            const int row = tile * kOwn + w * 32 + i;
-            if (row >= a.tokens) break;
-            float o[D / 64];
-            row_backward<DT, D>(a, head, row, __builtin_amdgcn_readlane(own.x, i), __builtin_amdgcn_readlane(own.y, i), o);
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) o[x] *= a.scale;
-            if (part) store_part_row<D>(part, i, o);
-            else store_row<DT, D>(a.dq.to(row, head), o);
-        }
-        return;
-    }
-    zero_unless(some, acc);
+    const bool nan = some && base != base;
+    const uint32_t again = rows_where(some && !nan && any_nan(acc));
+    if (!some) fill_of(acc, 0.f);
+    else if (nan) fill_of(acc, NAN);
     const float f = a.scale * (ldexpf(1.f, -static_cast<int>(kTop<DT>)) / fs);
     if (part) {
 #pragma unroll
         for (int x = 0; x < DN; ++x) acc[x] *= f;
         store_part<D>(part, acc);
-    } else if (r < a.tokens) {
+    } else if (r < a.tokens && !(again >> n & 1)) {
         store_own<DT, D>(a.dq.to(r, head), acc, f);
+    }
+    if (!again) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (as in the forward pass)
+#pragma unroll 1
+    for (uint32_t left = again; left; left &= left - 1) {
+        const int i = __builtin_ctz(left), row = tile * kOwn + w * 32 + i;
+        float o[D / 64];
+        row_backward<DT, D>(a, head, row, __builtin_amdgcn_readlane(own.x, i), __builtin_amdgcn_readlane(own.y, i), o);
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) o[x] *= a.scale;
+        if (part) store_part_row<D>(part, i, o);
+        else store_row<DT, D>(a.dq.to(row, head), o);
     }
 }
 
@@ -1180,7 +1206,7 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
             for (int e = 0; e < 16; e += 4) {
                 const float4_t m = row4(0, e), ll = row4(1, e);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sc[e + i] = exponent(sc[e + i], a.c, m[i]) - ll[i];
+                for (int i = 0; i < 4; ++i) sc[e + i] = capped(exponent(sc[e + i], a.c, m[i]) - ll[i], kTop<DT>);
             }
         }
         if (!sp.full(r, kRows)) {
@@ -1213,32 +1239,38 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
     }
     const bool some = seen.x < seen.y;
     if (part) part += w * 32 * D;
-    if (__any(some && !(odd_of(dk) + odd_of(dv) == 0.f))) {  // as in the forward pass
-#pragma unroll 1
-        for (int i = 0; i < 32; ++i) {
-            const int key = tile * kOwn + w * 32 + i;
-            if (key >= a.tokens) break;
-            const int r0 = __builtin_amdgcn_readlane(seen.x, i), r1 = __builtin_amdgcn_readlane(seen.y, i);
-            float gk[D / 64] = {}, gv[D / 64] = {};
-            for (int h = units.x / per; h * per < units.y; ++h) {  // the share's rows of each head
-                const int u0 = h * per > units.x ? h * per : units.x, u1 = (h + 1) * per < units.y ? (h + 1) * per : units.y;
-                const int x0 = (t0 + u0 - h * per) * kRows, x1 = (t0 + u1 - h * per) * kRows;
-                key_backward<DT, D>(a, kvh * a.group + h, key, r0 > x0 ? r0 : x0, r1 < x1 ? r1 : x1, gk, gv);
-            }
-#pragma unroll
-            for (int x = 0; x < D / 64; ++x) gk[x] *= a.scale;
-            if (part) {
-                store_part_row<D>(part, i, gk);
-                store_part_row<D>(part + kOwn * D, i, gv);
-                continue;
-            }
-            store_row<DT, D>(a.dk.to(key, kvh), gk);
-            store_row<DT, D>(a.dv.to(key, kvh), gv);
-        }
-        return;
+    uint32_t again = rows_where(some && (any_nan(dk) || any_nan(dv)));
+    if (!some) {
+        fill_of(dk, 0.f);
+        fill_of(dv, 0.f);
     }
-    zero_unless(some, dk);
-    zero_unless(some, dv);
+    // rows of this share's heads [x0, x1), the last head first
+    int h = per ? (units.y - 1) / per : -1;
+    auto span = [&](int &x0, int &x1) {
+        x0 = (t0 + (units.x > h * per ? units.x - h * per : 0)) * kRows;
+        x1 = (t0 + (units.y < (h + 1) * per ? units.y - h * per : per)) * kRows;
+    };
+    if (again) {
+        // a key that sees a row whose numbers are NaN has NaN: the last rows first, which most keys see
+        bool nan = false;
+#pragma unroll 1
+        for (; h >= 0 && h * per + per > units.x && (again & ~rows_where(nan)); --h) {
+            int x0, x1;
+            span(x0, x1);
+            for (int x = x1 - 64; x > x0 - 64 && (again & ~rows_where(nan)); x -= 64) {
+                const int row = x + l;
+                float base = 0.f;
+                if (row >= x0) base = numbers(h)[(row / kRows - t0) * 128 + 64 + row % kRows];
+                nan |= (__ballot(base != base) & below(seen.y - x) & ~below(seen.x - x)) != 0;
+            }
+        }
+        nan = nan && some;
+        if (nan) {
+            fill_of(dk, NAN);
+            fill_of(dv, NAN);
+        }
+        again &= ~rows_where(nan);
+    }
     const float one = ldexpf(1.f, -static_cast<int>(kTop<DT>)), f = a.scale * (one / fs);
     if (part) {
 #pragma unroll
@@ -1248,9 +1280,31 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
         }
         store_part<D>(part, dk);
         store_part<D>(part + kOwn * D, dv);
-    } else if (j < a.tokens) {
+    } else if (j < a.tokens && !(again >> n & 1)) {
         store_own<DT, D>(a.dk.to(j, kvh), dk, f);
         store_own<DT, D>(a.dv.to(j, kvh), dv, one);
+    }
+    if (!again) return;
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (as in the forward pass)
+#pragma unroll 1
+    for (uint32_t left = again; left; left &= left - 1) {
+        const int i = __builtin_ctz(left), key = tile * kOwn + w * 32 + i;
+        const int r0 = __builtin_amdgcn_readlane(seen.x, i), r1 = __builtin_amdgcn_readlane(seen.y, i);
+        float gk[D / 64] = {}, gv[D / 64] = {};
+        for (h = units.x / per; h * per < units.y; ++h) {
+            int x0, x1;
+            span(x0, x1);
+            key_backward<DT, D>(a, kvh * a.group + h, key, r0 > x0 ? r0 : x0, r1 < x1 ? r1 : x1, gk, gv);
+        }
+#pragma unroll
+        for (int x = 0; x < D / 64; ++x) gk[x] *= a.scale;
+        if (part) {
+            store_part_row<D>(part, i, gk);
+            store_part_row<D>(part + kOwn * D, i, gv);
+        } else {
+            store_row<DT, D>(a.dk.to(key, kvh), gk);
+            store_row<DT, D>(a.dv.to(key, kvh), gv);
+        }
     }
 }
 
@@ -1539,7 +1593,7 @@ size_t plan(Back &b, const nf4_attn *in) {
                           kJoin + groups * kPart * in->head_dim / 64;
     const double most_keys = fmin(n.most * (kTile / kRows), tiles_of(in, kRows)) * (in->n_heads / in->n_kv);
     const double tiles = launch_us(in, rows + keys, work, fmax(n.most * row, most_keys * key));
-    b.groups = shares < 1.1 * tiles ? static_cast<int>(fmax(groups / in->n_kv, 1.)) : 0;
+    b.groups = shares < 1.1 * tiles || rows + keys > (1 << 23) ? static_cast<int>(fmax(groups / in->n_kv, 1.)) : 0;
     size_t at = 0;
     auto next = [&](size_t bytes) {
         char *p = reinterpret_cast<char *>(at);

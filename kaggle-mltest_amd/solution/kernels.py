@@ -5,6 +5,7 @@ nonzero status.  No arithmetic happens here."""
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -842,6 +843,20 @@ def rope_table(positions: int, head_dim: int, base: float, device):
 
 # ------------------------------- training: attention of a packed batch, dropout without masks
 
+def _on_its_device(fn):
+    """Runs a call with its first tensor's device as the current one: launches go to the current device,
+    and the handle of another's default stream is none of its own."""
+    @functools.wraps(fn)
+    def call(first, *args, **kw):
+        t = first[0] if isinstance(first, (list, tuple)) else first
+        if t.is_cuda and t.get_device() != torch.cuda.current_device():
+            with torch.cuda.device(t.get_device()):
+                return fn(first, *args, **kw)
+        return fn(first, *args, **kw)
+
+    return call
+
+
 def _attn_desc(q, k, v, cu_seqlens, scale, window, max_len):
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] \
             or q.shape[2] != k.shape[2]:
@@ -870,6 +885,7 @@ def _attn_desc(q, k, v, cu_seqlens, scale, window, max_len):
                    _code(q.dtype))
 
 
+@_on_its_device
 def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                   cu_seqlens: torch.Tensor | None = None, scale: float | None = None,
                   window: int = 0, max_len: int = 0, out: torch.Tensor | None = None):
@@ -903,6 +919,7 @@ def _grad(t, shape, like, what):
     return NF4Grad(t.data_ptr(), t.stride(0), t.stride(1))
 
 
+@_on_its_device
 def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                   out: torch.Tensor, stats: torch.Tensor, cu_seqlens: torch.Tensor | None = None,
                   scale: float | None = None, window: int = 0, max_len: int = 0, grads=None):
@@ -957,6 +974,7 @@ def _drop_args(tensors, seed, sites, index):
             _LD_ARRAYS[n](*[t.stride(0) for t in tensors]), _SITE_ARRAYS[n](*sites), n)
 
 
+@_on_its_device
 def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, sites, outs=None) -> list:
     """Dropout without a stored mask: for every site a tensor like x [rows, cols] that holds
     x * 65536 / (65536 - T) where the site keeps the element and 0 where it does not, T =
@@ -984,6 +1002,7 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, sites, outs=None) -> 
     return outs
 
 
+@_on_its_device
 def dropout_bwd(grads, p: float, seed: torch.Tensor, sites, base: torch.Tensor | None = None,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """dx of dropout: base (None: zeros) plus every site's gradient times its mask and scale, summed

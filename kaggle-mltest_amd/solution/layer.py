@@ -30,6 +30,7 @@ from __future__ import annotations
 from dataclasses import dataclass, field
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels
 
@@ -319,6 +320,7 @@ class Attention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         *saved, cu = ctx.saved_tensors
         grads = kernels.attention_bwd(_rows3(dout), *saved, cu, *ctx.how)
@@ -352,6 +354,7 @@ class RopeAttention(torch.autograd.Function):
         return out
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dout):
         qk, v, out, stats, cu, cos, sin = ctx.saved_tensors
         n_heads, how = ctx.how

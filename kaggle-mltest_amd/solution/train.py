@@ -11,6 +11,7 @@ the backward pass forms them again (`layer.RopeAttention`, `mlp.RecomputedMLP`, 
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import kernels
 from .layer import LoraAdapter, ProjectionSpec, project, rope_attention
@@ -29,6 +30,7 @@ class AddNorm(torch.autograd.Function):
         return x.view_as(x) if d is None else x + d.to(x.dtype), y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dres, dy):
         x, d, weight, rstd = ctx.saved_tensors
         dx = kernels.rmsnorm_bwd(x, weight, rstd, dy=dy.contiguous(), d=d, dres=dres.contiguous(),

@@ -202,3 +202,131 @@ def test_written_views(cuda):
     assert torch.equal(big[:, 1:5], plain[0]) and torch.equal(big[:, 5:7], plain[1])
     assert torch.equal(big[:, 8:10], plain[2])
     assert (big[:, 0] == 7).all() and (big[:, 7] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("value", [math.nan, math.inf, 6e4])
+def test_what_lies_in_rows_of_no_sequence_does_not_matter(cuda, dtype, value):
+    """Rows of padding that hold NaN, infinities or large numbers, as memory that nothing wrote does."""
+    banner("padding", dtype, value)
+    q, k, v, dout, cu = make(cuda, dtype, 4, 2, 64, (150, 40), pad=60, seed=14, layout="plain")
+    clean = run(q, k, v, dout, cu)
+    for t in (q, k, v, dout):
+        t[190:] = value
+    got = run(q, k, v, dout, cu)
+    assert all(torch.equal(got[n], clean[n]) for n in clean)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_gradients_that_are_not_finite(cuda, dtype):
+    """A loss whose scale was too high: a row whose dout holds an infinity or NaN has NaN for its dq, and so
+    have all dk and dv that it sees; nothing else has."""
+    q, k, v, dout, cu = make(cuda, dtype, 4, 2, 64, (200, 90), seed=15, layout="plain")
+    want = ref.attention(q, k, v, cu, dout)
+    for value in (math.inf, math.nan):
+        d = dout.clone()
+        d[120, 1, 7] = value  # head 1 reads key head 0
+        got = run(q, k, v, d, cu)
+        assert torch.isnan(got["dq"][120, 1]).all()
+        for name in ("dk", "dv"):
+            assert torch.isnan(got[name][:121, 0]).all()
+            ref.assert_within(got[name][121:], tuple(t[121:] for t in want[name]), name)
+            ref.assert_within(got[name][:, 1], tuple(t[:, 1] for t in want[name]), name)
+        rest = torch.ones(290, 4, dtype=torch.bool)
+        rest[120, 1] = False
+        ref.assert_within(got["dq"].cpu()[rest], tuple(t[rest] for t in want["dq"]), "dq")
+    got = run(q, k, v, torch.full_like(dout, math.nan), cu)
+    assert all(torch.isnan(got[n]).all() for n in ("dq", "dk", "dv"))
+
+
+def test_scores_that_are_not_finite(cuda):
+    """Keys with a score of -inf have no weight beside others; a row with such keys only, or with one of
+    +inf, is NaN, as the formula is."""
+    q, k, v, dout, cu = make(cuda, BF16, 1, 1, 64, (300,), seed=16, layout="plain")
+    q[:, 0, 0], k[:, 0, 0] = -1.0, 0.0
+    k[0, 0, 0] = math.inf
+    out = run(q, k, v, dout, cu)
+    q1 = q[1:], k[1:], v[1:]
+    want = ref.attention(*q1, [0, 299])
+    assert torch.isnan(out["out"][0]).all()
+    for name in ("out", "stats"):
+        ref.assert_within(out[name][1:], want[name], name)
+    q[150, 0, 0] = 1.0
+    out = run(q, k, v, dout, cu)
+    assert torch.isnan(out["out"][150]).all() and not torch.isnan(out["out"][149]).any()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_scores_of_any_size(cuda, dtype):
+    """Scores of 1e5 and more, whose statistics no float holds to a step of 1: rows that see one key have a
+    probability of 1, whatever its score."""
+    q, k, v, dout, cu = make(cuda, dtype, 2, 1, 64, (1,) * 40, seed=17, qscale=60.0, layout="plain")
+    for scale in (1e3, 1e9, -1e9, 1e30):
+        got = run(q, k, v, dout, cu, scale=scale)
+        # The maximum as a float is off by up to 2^-5 where it is near 2^20, the row's sum 2^that, and so is its
+        # one probability before the division; that is rounded to the type, the sum is not, and the quotient
+        # is rounded again: two half steps.
+        away = (got["out"].double() - v.double()).abs()
+        assert (away <= 2.01 * ref.HALF[dtype] * v.double().abs()).all()
+        sums = dout.double().sum(1, keepdim=True)
+        off = (got["dv"].double() - sums).abs()
+        assert (off <= ref.HALF[dtype] * sums.abs() + 2.0 ** -20).all()
+        # (dS is 0 but for the saved output's half step: up to 2^-11 of sum |do v|, 0.03 here; with a scale of
+        # 1e9 and q of 60 that is 2e9, beyond fp16's largest number: infinite there, but no NaN)
+        assert not torch.isnan(got["dq"]).any() and not torch.isnan(got["dk"]).any()
+
+
+def test_nothing_to_do(cuda):
+    from solution import kernels
+
+    e = torch.empty(0, 4, 64, dtype=F16, device=cuda)
+    k = torch.empty(0, 2, 64, dtype=F16, device=cuda)
+    cu = torch.zeros(1, dtype=torch.int32, device=cuda)
+    for c in (None, cu):
+        out, stats = kernels.attention_fwd(e, k, k, c)
+        assert out.shape == (0, 4, 64) and stats.shape == (0, 4, 2)
+        assert [t.shape[0] for t in kernels.attention_bwd(out, e, k, k, out, stats, c)] == [0, 0, 0]
+    q, k, v, dout, _ = make(cuda, F16, 4, 2, 64, (), pad=70, seed=18)
+    got = run(q, k, v, dout, [0])  # rows, and no sequence
+    assert not any(t.any() for t in got.values())
+
+
+def test_offsets_past_32_bits(cuda):
+    """Heads 2^31 + 64 elements apart."""
+    q, k, v, dout, cu = make(cuda, F16, 2, 2, 64, (100, 29), seed=19, layout="plain")
+    far = (1 << 31) + 64
+    big = torch.empty(far + 129 * 64, dtype=F16, device=cuda)
+
+    def place(t):
+        x = torch.as_strided(big, t.shape, (64, far, 1))
+        x.copy_(t)
+        return x
+
+    clean = run(q, k, v, dout, cu)
+    for i in range(4):  # (one at a time: they share the memory)
+        args = [q, k, v, dout]
+        args[i] = place(args[i])
+        got = run(*args, cu)
+        assert all(torch.equal(got[n], clean[n]) for n in clean)
+    from solution import kernels
+
+    c = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    grads = torch.as_strided(big, (129, 2, 64), (64, far, 1)), torch.empty_like(k), torch.empty_like(v)
+    got = kernels.attention_bwd(dout, q, k, v, clean["out"], clean["stats"], c, grads=grads)
+    assert torch.equal(got[0], clean["dq"])
+
+
+def test_many_sequences_and_one_among_empty_ones(cuda):
+    """More offsets than a wave holds, and more empty sequences in a row than it looks through."""
+    lens = [0] * 70 + [5] + [0] * 5000 + [3, 0, 90] + [1] * 300 + [0] * 64 + [20]
+    q, k, v, dout, cu = make(cuda, F16, 2, 1, 64, lens, pad=3, seed=20)
+    check(run(q, k, v, dout, cu, max_len=90), q, k, v, dout, cu)
+
+
+@pytest.mark.parametrize("window", [0, 700])
+def test_shares_and_tiles_agree(cuda, window):
+    """A wrong `max_len` changes how the work is cut (few long tiles, or each its own): the same sums in
+    another order."""
+    q, k, v, dout, cu = make(cuda, BF16, 8, 2, 64, (2000, 64, 64), seed=21)
+    for n in (64, 2000):
+        check(run(q, k, v, dout, cu, max_len=n, window=window), q, k, v, dout, cu, window=window)
