@@ -493,7 +493,7 @@ __global__ __launch_bounds__(64) void qkv_rope_bwd_vec_kernel(
 
 // One thread per 4 rotary pairs of a head: the forward rotation of qkv_rope_vec_kernel or the transposed
 // one of qkv_rope_bwd_vec_kernel, on heads as they lie (shared key heads are not expanded).  Bound by
-// memory: 8192 tokens of 28 + 4 heads of 128, 134 MB, ROPE_US.
+// memory: 8192 tokens of 28 + 4 heads of 128, 134 MB, 23 us, 6 TB/s.
 template <int DT>
 __global__ __launch_bounds__(256) void rope_heads_kernel(const uint16_t *x, int64_t ld_x, const float *cs,
                                                          const float *sn, uint16_t *y, int64_t ld_y,

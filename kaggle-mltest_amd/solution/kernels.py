@@ -486,6 +486,29 @@ def qkv_rope_bwd(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, cos: torc
     return out
 
 
+def _on_its_device(fn):
+    """Runs a call with its first tensor's device as the current one: launches go to the current device,
+    and the handle of another's default stream is none of its own."""
+    @functools.wraps(fn)
+    def call(*args, **kw):
+        if _devices() < 2:
+            return fn(*args, **kw)
+        t = args[0] if args else next(iter(kw.values()))
+        t = t[0] if isinstance(t, (list, tuple)) else t
+        if not t.is_cuda or t.get_device() == torch.cuda.current_device():
+            return fn(*args, **kw)
+        with torch.cuda.device(t.get_device()):
+            return fn(*args, **kw)
+
+    return call
+
+
+@functools.lru_cache(maxsize=None)
+def _devices() -> int:
+    return torch.cuda.device_count()
+
+
+@_on_its_device
 def rope(x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, heads: int, head_dim: int,
          inverse: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """The first `heads` heads of every row of x [tokens, *] rotated as qkv_rope does (cos, sin
@@ -843,20 +866,6 @@ def rope_table(positions: int, head_dim: int, base: float, device):
 
 # ------------------------------- training: attention of a packed batch, dropout without masks
 
-def _on_its_device(fn):
-    """Runs a call with its first tensor's device as the current one: launches go to the current device,
-    and the handle of another's default stream is none of its own."""
-    @functools.wraps(fn)
-    def call(first, *args, **kw):
-        t = first[0] if isinstance(first, (list, tuple)) else first
-        if t.is_cuda and t.get_device() != torch.cuda.current_device():
-            with torch.cuda.device(t.get_device()):
-                return fn(first, *args, **kw)
-        return fn(first, *args, **kw)
-
-    return call
-
-
 def _attn_desc(q, k, v, cu_seqlens, scale, window, max_len):
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] \
             or q.shape[2] != k.shape[2]:
@@ -902,10 +911,10 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
         out = q.new_empty((tokens, heads, dim))
     else:
         _check_out(out, (tokens, heads, dim), q)
-    stats = torch.empty((tokens, heads, 2), dtype=torch.float32, device=q.device)
+    stats = q.new_empty((tokens, heads, 2), dtype=torch.float32)
     lib, ref = load(), ctypes.byref(desc)
     nbytes = lib.nf4_attn_fwd_workspace(ref)
-    ws = _workspace(nbytes, q.device)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     st = lib.nf4_attn_fwd(ref, out.data_ptr(), stats.data_ptr(), _p(ws), nbytes, stream_of(q))
     if st:
         check(st, "nf4_attn_fwd")
@@ -913,7 +922,7 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 
 def _grad(t, shape, like, what):
-    if tuple(t.shape) != shape or t.dtype != like.dtype or t.device != like.device \
+    if t.shape != shape or t.dtype != like.dtype or t.get_device() != like.get_device() \
             or t.stride(2) != 1:
         raise ValueError(f"{what} is a {list(shape)} tensor of q's dtype, head_dim contiguous")
     return NF4Grad(t.data_ptr(), t.stride(0), t.stride(1))
@@ -928,18 +937,18 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     `grads`: (dq, dk, dv) tensors to write, of any strides (column slices of one buffer).  Rows of
     no sequence get zeros."""
     desc = _attn_desc(q, k, v, cu_seqlens, scale, window, max_len)
-    shape, kv_shape = tuple(q.shape), tuple(k.shape)
+    shape, kv_shape = q.shape, k.shape
     if grads is None:
         grads = q.new_empty(shape), q.new_empty(kv_shape), q.new_empty(kv_shape)
     _check_out(out, shape, q)
-    if tuple(stats.shape) != (*shape[:2], 2) or stats.dtype != torch.float32 \
-            or stats.device != q.device or not stats.is_contiguous():
+    if stats.shape != (*shape[:2], 2) or stats.dtype != torch.float32 \
+            or stats.get_device() != q.get_device() or not stats.is_contiguous():
         raise ValueError("stats is the forward pass's fp32 [tokens, n_heads, 2] tensor")
     args = [_grad(t, sh, q, name) for t, sh, name in
             zip((dout, *grads), (shape, shape, kv_shape, kv_shape), ("dout", "dq", "dk", "dv"))]
     lib, ref = load(), ctypes.byref(desc)
     nbytes = lib.nf4_attn_bwd_workspace(ref)
-    ws = _workspace(nbytes, q.device)
+    ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
     st = lib.nf4_attn_bwd(ref, out.data_ptr(), stats.data_ptr(), *map(ctypes.byref, args), _p(ws),
                           nbytes, stream_of(q))
     if st:
