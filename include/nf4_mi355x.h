@@ -520,7 +520,11 @@ typedef struct nf4_attn {
 /* out [tokens, n_heads, head_dim] = sum_j P_j v_j and stats [tokens, n_heads, 2] (fp32) = (m, l),
  * with t_j = scale * log2(e) * q.k_j over the keys that the row sees, m = max t_j, l = sum
  * 2^(t_j - m), P_j = 2^(t_j - m) / l (the natural log-sum-exp is m ln 2 + ln l).  A row of no
- * sequence gets zeros and (0, 0).  Workspace: nf4_attn_fwd_workspace bytes, 16-byte aligned.
+ * sequence gets zeros and (0, 0).  What a row does not see has no part in its result, whatever lies
+ * there; a row that sees a score of NaN or +inf, or scores of -inf only, is NaN, stats too.  Offsets that
+ * are not as above (decreasing, outside of the rows) are no error: rows get what some of them say, and
+ * nothing outside of the rows is read or written.  out and stats overlap no input.  Workspace:
+ * nf4_attn_fwd_workspace bytes, 16-byte aligned, the call's own until it has run.
  * Replaces: _efficient_attention_forward in _Attention (/root/reference/solution/layer.py:735-826). */
 size_t nf4_attn_fwd_workspace(const nf4_attn *a);
 int nf4_attn_fwd(const nf4_attn *a, void *out, float *stats, void *workspace,
@@ -537,7 +541,9 @@ typedef struct nf4_grad {
  * formed again.  With D = dout.out and dS_j = P_j (dout.v_j - D): dq = scale sum_j dS_j k_j, and over
  * the rows that see key j and the query heads that share it dk_j = scale sum dS_j q, dv_j = sum
  * P_j dout, summed in a fixed order (results do not depend on timing).  Rows of no sequence get
- * zeros.  Workspace: nf4_attn_bwd_workspace bytes, 16-byte aligned.
+ * zeros.  A row whose dout, out or stats hold an infinity or NaN that shows in D or m has NaN for its dq, and
+ * so have all dk and dv that it sees.  dq, dk and dv overlap neither each other nor what is read; they may be
+ * columns of one buffer.  Workspace: nf4_attn_bwd_workspace bytes, as above.
  * Replaces: _efficient_attention_backward in _Attention (/root/reference/solution/layer.py:735-826). */
 size_t nf4_attn_bwd_workspace(const nf4_attn *a);
 int nf4_attn_bwd(const nf4_attn *a, const void *out, const float *stats, const nf4_grad *dout,

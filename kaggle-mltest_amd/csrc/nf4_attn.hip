@@ -750,7 +750,7 @@ constexpr int kLeast = 160;                                  // a share
 
 struct Back {
     float *rows;    // [n_heads][2 blocks][4][32]
-    float *norms;   // fp16: the largest |do| of a block's rows [n_heads][blocks], then |v| [n_kv][blocks]
+    float *norms;   // fp16: the largest |do| of a block's rows [n_heads][blocks], |v| [n_kv][blocks], |D| [n_heads][blocks]
     int4 *tab;      // a tile's keys [x, y) and rows [z, w): what its rows see, what sees its keys
     int64_t *line;  // [2 tiles + 1]: where the tiles of keys begin, then those of rows (of all heads)
     int *inside;    // [n_kv * groups]: the tile (of all heads) that a share begins inside of, or -1
@@ -860,14 +860,14 @@ __device__ __forceinline__ void make_line(const Attn &a, const Back &b) {
 template <int DT, int D>
 __global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back b) {
     constexpr int CH = D / 8, RPP = 256 / CH;
-    __shared__ float most[4];
+    __shared__ float most[2][4];
     const int head = blockIdx.y, ch = threadIdx.x % CH;
     if (head == static_cast<int>(gridDim.y) - 1) {
         if (blockIdx.x == 0) make_line(a, b);
         return;
     }
     const bool of_v = head >= a.n_heads;
-    float worst = 0.f;
+    float worst = 0.f, worst_d = 0.f;
 #pragma unroll
     for (int x = 0; x < kTile; x += RPP) {
         const int i = x + threadIdx.x / CH, r = blockIdx.x * kTile + i;
@@ -895,6 +895,7 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back
         if (of_v || ch) continue;
         if (none) d = 0.f;
         else if (!(fabsf(d) < INFINITY && fabsf(ml.x) < INFINITY)) ml = make_float2(NAN, NAN);  // (an odd do or out: an odd d)
+        else worst_d = fmaxf(worst_d, fabsf(d));
         const float ll = (ml.y == 0.f ? 0.f : log2f(ml.y)) - kTop<DT>;
         float *p = b.rows + (static_cast<int64_t>(head) * b.blocks + blockIdx.x) * 256 + (i >> 5) * 128 + (i & 31);
         p[0] = ml.x;
@@ -904,26 +905,36 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back
     }
     if constexpr (DT == NF4_F16) {
         worst = wave_max(worst);
-        if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = worst;
+        worst_d = wave_max(worst_d);
+        if ((threadIdx.x & 63) == 0) {
+            most[0][threadIdx.x >> 6] = worst;
+            most[1][threadIdx.x >> 6] = worst_d;
+        }
         __syncthreads();
-        if (threadIdx.x == 0)
-            b.norms[static_cast<int64_t>(head) * b.blocks + blockIdx.x] =
-                sqrtf(fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
+        if (threadIdx.x < 2 && !(of_v && threadIdx.x)) {
+            const float *m = most[threadIdx.x];
+            const float x = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+            b.norms[static_cast<int64_t>(head + (threadIdx.x ? a.n_heads + a.n_kv : 0)) * b.blocks + blockIdx.x] = threadIdx.x ? x : sqrtf(x);
+        }
     }
 }
 
-// fp16's dS, of at most 2 |do| |v|, are multiplied by this power of two (beside the 2^15 of P), so that
-// the largest is near 2^15; a plain fp16 of them would be 0 for the gradients of a loss that is not scaled.
+// fp16's dS, of at most `bound` = |do| |v| + |D|, are multiplied by this power of two (beside the 2^15 of P),
+// so that the largest is near 2^15; a plain fp16 of them would be 0 for the gradients of a loss that is not
+// scaled.  (D by itself: it has the v of every key that the row sees in it, which can be far larger than
+// those at hand.)
 __device__ __forceinline__ float ds_scale(float bound) {
     int e = 0;
-    bound *= 2.02f;
+    bound *= 1.01f;
     if (bound > 0.f && bound < INFINITY) (void)frexpf(bound, &e);
     return ldexpf(1.f, -e);
 }
 
-__device__ __forceinline__ float most_of(const float *p, int n) {
+// the largest of n numbers of `heads` heads each, `blocks` apart
+__device__ __forceinline__ float most_of(const float *p, int n, int heads, int64_t blocks) {
     float v = 0.f;
-    for (int i = thread_here() & 63; i < n; i += 64) v = fmaxf(v, p[i]);
+    for (int h = 0; h < heads; ++h, p += blocks)
+        for (int i = thread_here() & 63; i < n; i += 64) v = fmaxf(v, p[i]);
     return wave_max(v);
 }
 
@@ -965,7 +976,7 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
         const int b0 = first >> 6, nb = u.y - u.x;
-        fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb));
+        fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb, 1, 0) + fabsf(delta));
     }
     // (the probabilities are used for dS only: their scale goes into the exponent)
     const float mul = near ? a.c : 1.f, sub = (near ? base : 0.f) - log2f(fs);
@@ -1113,10 +1124,10 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
         u32x4_t vf[KS];
         own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, l);
         const int b0 = t0 * kRows / kTile, nb = per ? (rows.y - 1) / kTile - b0 + 1 : 0;
-        float most = 0.f;
-        for (int h = 0; h < a.group; ++h)
-            most = fmaxf(most, most_of(b.norms + static_cast<int64_t>(kvh * a.group + h) * b.blocks + b0, nb));
-        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most);
+        const float *norms = b.norms + static_cast<int64_t>(kvh * a.group) * b.blocks + b0;
+        const float most = most_of(norms, nb, a.group, b.blocks);
+        const float most_d = most_of(norms + static_cast<int64_t>(a.n_heads + a.n_kv) * b.blocks, nb, a.group, b.blocks);
+        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most + most_d);
     }
     // unit (head of the group, tile of rows), the next one
     int uh = per ? units.x / per : 0, ut = units.x - uh * per;
@@ -1601,7 +1612,7 @@ size_t plan(Back &b, const nf4_attn *in) {
         return p;
     };
     b.rows = reinterpret_cast<float *>(next(static_cast<size_t>(in->n_heads) * b.blocks * 1024));
-    b.norms = reinterpret_cast<float *>(next(in->dtype == NF4_F16 ? static_cast<size_t>(in->n_heads + in->n_kv) * b.blocks * 4 : 0));
+    b.norms = reinterpret_cast<float *>(next(in->dtype == NF4_F16 ? static_cast<size_t>(2 * in->n_heads + in->n_kv) * b.blocks * 4 : 0));
     b.tab = reinterpret_cast<int4 *>(next(static_cast<size_t>(b.tiles) * 16));
     b.line = reinterpret_cast<int64_t *>(next((2 * static_cast<size_t>(b.tiles) + 1) * 8));
     b.inside = reinterpret_cast<int *>(next(static_cast<size_t>(b.groups) * in->n_kv * 4));

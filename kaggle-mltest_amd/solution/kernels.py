@@ -934,8 +934,8 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
                   scale: float | None = None, window: int = 0, max_len: int = 0, grads=None):
     """(dq, dk, dv) of attention_fwd from the output's gradient, with the forward pass's `out` and
     `stats` and its other arguments.  dk and dv are summed over the query heads that share a head.
-    `grads`: (dq, dk, dv) tensors to write, of any strides (column slices of one buffer).  Rows of
-    no sequence get zeros."""
+    `grads`: (dq, dk, dv) tensors to write, of any strides (column slices of one buffer), none of
+    them an input.  Rows of no sequence get zeros."""
     desc = _attn_desc(q, k, v, cu_seqlens, scale, window, max_len)
     shape, kv_shape = q.shape, k.shape
     if grads is None:

@@ -330,3 +330,18 @@ def test_shares_and_tiles_agree(cuda, window):
     q, k, v, dout, cu = make(cuda, BF16, 8, 2, 64, (2000, 64, 64), seed=21)
     for n in (64, 2000):
         check(run(q, k, v, dout, cu, max_len=n, window=window), q, k, v, dout, cu, window=window)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("lens, window", [((70,), 0), ((700, 40), 0), ((900,), 130)])
+def test_values_of_unequal_size(cuda, dtype, lens, window):
+    """Keys whose v is small or 0 beside others' (dS is as large as the others make it)."""
+    q, k, v, dout, cu = make(cuda, dtype, 4, 2, 64, lens, seed=22, qscale=0.5, gscale=8.0, layout="plain")
+    small = torch.arange(sum(lens)) % 3
+    v[small == 0] *= 2.0 ** -12
+    v[small == 1] = 0.0
+    v[small == 2] *= 8.0
+    dout[100:] *= 2.0 ** -8
+    check(run(q, k, v, dout, cu, window=window), q, k, v, dout, cu, window=window)
+    v[: sum(lens) // 2] *= 2.0 ** -6  # (what one share of the work sees is small, and not what its rows see)
+    check(run(q, k, v, dout, cu, window=window), q, k, v, dout, cu, window=window)
