@@ -345,3 +345,76 @@ def test_values_of_unequal_size(cuda, dtype, lens, window):
     check(run(q, k, v, dout, cu, window=window), q, k, v, dout, cu, window=window)
     v[: sum(lens) // 2] *= 2.0 ** -6  # (what one share of the work sees is small, and not what its rows see)
     check(run(q, k, v, dout, cu, window=window), q, k, v, dout, cu, window=window)
+
+
+@pytest.mark.parametrize("dtype, window", [(BF16, 500), (F16, 129)])
+def test_long_with_a_window(cuda, dtype, window):
+    """70001 rows; a stretch of 2000 in the middle and the last ones as sequences of their own are the same
+    for rows whose keys, and keys whose rows, lie in the stretch."""
+    q, k, v, dout, cu = make(cuda, dtype, 2, 1, 64, (70001,), seed=23, layout="plain")
+    got = run(q, k, v, dout, cu, window=window)
+    for a, b in ((33000, 35000), (68001, 70001)):
+        s = slice(a, b)
+        want = ref.attention(q[s], k[s], v[s], [0, b - a], dout[s], window=window)
+        hi = b - a if b == 70001 else 1000
+        for name in ("out", "stats", "dq", "dk", "dv"):
+            ref.assert_within(got[name][s][500:hi], tuple(t[500:hi] for t in want[name]), name)
+
+
+def test_one_long_sequence(cuda):
+    """40000 rows of one sequence: the last rows, and the last keys, by the formulas alone."""
+    n, last = 40000, 70
+    q, k, v, dout, cu = make(cuda, BF16, 1, 1, 128, (n,), seed=24, layout="plain")
+    got = run(q, k, v, dout, cu)
+    q64, k64, v64, do = (t.double().cpu()[:, 0] for t in (q, k, v, dout))
+    s = q64[-last:] @ k64.t() * 128 ** -0.5
+    rows = torch.arange(n - last, n)[:, None]
+    s = s.masked_fill(torch.arange(n)[None] > rows, -math.inf)
+    p = torch.softmax(s, -1)
+    o = p @ v64
+    # a probability's error as in train_ref: a score's (twice), 8 half steps, and n of the sum
+    es = (q64[-last:].abs() @ k64.abs().t()).amax(-1, keepdim=True) * 128 ** -0.5 * 136 * ref.U32
+    half, ep = ref.HALF[BF16], 2 * es + (8 + n) * ref.U32
+    oa = p @ v64.abs()
+    off = (got["out"][-last:, 0].double().cpu() - o).abs()
+    eo = half * o.abs() + (half + ep + n * ref.U32) * oa
+    assert (off <= 1.01 * eo).all()
+    # dS = P (dP - D): P's error of all, dP's and D's own (D's by the saved output's, too)
+    dp, d = do[-last:] @ v64.t(), (do[-last:] * o).sum(-1, keepdim=True)
+    ed = 136 * ref.U32 * (do[-last:].abs() @ v64.abs().t()) + (do[-last:].abs() * (1.01 * eo)).sum(-1, keepdim=True) \
+        + 136 * ref.U32 * (do[-last:].abs() * o.abs()).sum(-1, keepdim=True)
+    ds = p * (dp - d)
+    eds = (ep + half) * ds.abs() + p * ed
+    dq = ds @ k64 * 128 ** -0.5
+    edq = 128 ** -0.5 * ((eds + n * ref.U32 * ds.abs()) @ k64.abs()) + half * dq.abs()
+    assert ((got["dq"][-last:, 0].double().cpu() - dq).abs() <= 1.02 * edq).all()
+    sl = slice(n - last, n)  # keys that only the last rows see
+    dk, dv = ds[:, sl].t() @ q64[-last:] * 128 ** -0.5, p[:, sl].t() @ do[-last:]
+    edk = 128 ** -0.5 * ((eds + n * ref.U32 * ds.abs())[:, sl].t() @ q64[-last:].abs()) + half * dk.abs()
+    edv = ((half + ep + n * ref.U32) * p)[:, sl].t() @ do[-last:].abs() + half * dv.abs()
+    assert ((got["dk"][-last:, 0].double().cpu() - dk).abs() <= 1.02 * edk).all()
+    assert ((got["dv"][-last:, 0].double().cpu() - dv).abs() <= 1.02 * edv).all()
+
+
+@pytest.mark.parametrize("heads, kv", [(40, 1), (40, 8), (9, 9), (66, 33)])
+def test_head_groups(cuda, heads, kv):
+    q, k, v, dout, cu = make(cuda, F16, heads, kv, 64, (130, 20), seed=25)
+    check(run(q, k, v, dout, cu), q, k, v, dout, cu)
+
+
+def test_strides_of_views(cuda):
+    """Key heads that are one tensor's, expanded (a stride of 0), and gradients that come transposed."""
+    from solution.layer import attention
+
+    q, k, v, dout, cu = make(cuda, BF16, 4, 1, 64, (150, 9), seed=26, layout="plain")
+    k4, v4 = k.expand(-1, 4, -1), v.expand(-1, 4, -1)
+    check(run(q, k4, v4, dout, cu), q, k4, v4, dout, cu)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v)]
+    c = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    out = attention(leaves[0], leaves[1].expand(-1, 4, -1), leaves[2].expand(-1, 4, -1), c)
+    out.transpose(1, 2).backward(dout.transpose(1, 2).contiguous())
+    got = run(q, k4, v4, dout, cu)
+    assert torch.equal(leaves[0].grad, got["dq"])
+    for x, name in zip(leaves[1:], ("dk", "dv")):  # (the sum over the expanded heads is autograd's)
+        want = got[name].double().sum(1, keepdim=True)
+        assert ((x.grad.double() - want).abs() <= 4 * ref.HALF[BF16] * got[name].double().abs().sum(1, keepdim=True)).all()

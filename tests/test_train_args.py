@@ -160,3 +160,74 @@ def test_rope_refusals(lib):
     assert rope(x=P + 4) == UNSUPPORTED and rope(y=P + 2) == UNSUPPORTED and rope(cos=P + 8) == UNSUPPORTED
     assert rope(ld=130) == UNSUPPORTED and rope(ldy=130) == UNSUPPORTED
     assert rope(tokens=0, x=None) == OK
+
+
+def test_workspaces(lib):
+    a = desc(tokens=4096, batch=1)
+    for call, need in ((fwd, lib.nf4_attn_fwd_workspace(ctypes.byref(a))),
+                       (bwd, lib.nf4_attn_bwd_workspace(ctypes.byref(a)))):
+        assert need > 0
+        assert call(lib, a) == WORKSPACE
+        assert call(lib, a, ws=P, nws=need - 1) == WORKSPACE
+        assert call(lib, a, ws=P + 8, nws=need) == UNSUPPORTED
+    for bad in (desc(tokens=-1), desc(head_dim=96), desc(tokens=0)):
+        assert lib.nf4_attn_fwd_workspace(ctypes.byref(bad)) == 0
+        assert lib.nf4_attn_bwd_workspace(ctypes.byref(bad)) == 0
+    assert lib.nf4_attn_fwd_workspace(None) == 0 and lib.nf4_attn_bwd_workspace(None) == 0
+
+
+@pytest.mark.parametrize("kw", [
+    dict(tokens=1 << 23, n_heads=128, n_kv=128, head_dim=128),  # the largest calls
+    dict(tokens=1 << 23, n_heads=128, n_kv=1, head_dim=64),
+    dict(tokens=1 << 20, n_heads=1024, n_kv=1024, head_dim=64, batch=1 << 20),
+    dict(tokens=1 << 20, n_heads=1024, n_kv=1, head_dim=128, window=1),
+    dict(tokens=1, n_heads=1024, n_kv=1, head_dim=128), dict(tokens=8192, n_heads=28, n_kv=4, head_dim=128),
+])
+def test_workspace_of_the_largest_calls(lib, kw):
+    """Whole numbers of 64 bits on the way, and a workspace that a call of that size can have: the rows'
+    numbers (16 bytes a row and head) and at most 300 MB of parts."""
+    for dtype in (0, 1):
+        for max_len in (0, 100):
+            a = desc(dtype=dtype, max_len=max_len, **kw)
+            rows = (kw["tokens"] + 127) // 128 * 128 * kw["n_heads"]
+            assert 16 * rows <= lib.nf4_attn_bwd_workspace(ctypes.byref(a)) <= 18 * rows + kw["tokens"] + (300 << 20)
+            assert lib.nf4_attn_fwd_workspace(ctypes.byref(a)) <= 300 << 20
+
+
+def test_structs_as_the_header_has_them():
+    from solution._lib import NF4Attn, NF4Grad
+
+    assert ctypes.sizeof(NF4Attn) == 128 and NF4Attn.scale.offset == 120
+    assert ctypes.sizeof(NF4Grad) == 24
+
+
+def test_calls_run_on_their_tensors_device(monkeypatch):
+    import contextlib
+
+    import torch
+
+    from solution import kernels
+
+    class Tensor:
+        is_cuda = True
+
+        def __init__(self, index):
+            self.index = index
+
+        def get_device(self):
+            return self.index
+
+    at = [0]
+
+    @contextlib.contextmanager
+    def device(index):
+        old, at[0] = at[0], index
+        yield
+        at[0] = old
+
+    monkeypatch.setattr(kernels, "_devices", lambda: 2)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    seen = kernels._on_its_device(lambda x, y=None: at[0])
+    assert seen(Tensor(1)) == 1 and seen(Tensor(0)) == 0 and seen([Tensor(1)]) == 1
+    assert seen(x=Tensor(1), y=3) == 1 and at == [0]
