@@ -960,9 +960,6 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     const int tid = thread_here(), w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
     const int n = l & 31, kvh = head / a.group;
     const int r = tile * kOwn + w * 32 + n;
-    const int2 seen = keys_of(a, r);
-    Span sp;
-    sp.set(seen);
     const int first = (keys.x & ~(kTile - 1)) + u.x * kTile;
     int last = (keys.x & ~(kTile - 1)) + u.y * kTile;
     last = last < keys.y ? last : keys.y;
@@ -972,6 +969,21 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     own_operand<D>(go, a.dout.at(r, head), r < a.tokens, l);
     const float *rows = b.rows + (static_cast<int64_t>(head) * b.blocks * 2 + (r < a.tokens ? r >> 5 : 0)) * 128 + (r & 31);
     const float m = rows[0], ll = rows[32], base = rows[64], delta = rows[96];
+    Stager<D, kTile> sk, sv;
+    sk.set(a.k, kvh, first, tid);
+    sv.set(a.v, kvh, first, tid);
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
+        (__attribute__((address_space(3))) uint8_t *)lds));
+    const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
+    int k = u.x < u.y ? first : last, st = 0;
+    if (k < last) {
+        sk.send(mine, last - k);
+        sv.send(mine + 2 * TB, last - k);
+    }
+    // (what the rows see is found while all that is on its way)
+    const int2 seen = keys_of(a, r);
+    Span sp;
+    sp.set(seen);
     const bool near = __all(!(seen.x < seen.y) || fabsf(m) < kNear);
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
@@ -980,22 +992,11 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     }
     // (the probabilities are used for dS only: their scale goes into the exponent)
     const float mul = near ? a.c : 1.f, sub = (near ? base : 0.f) - log2f(fs);
-    Stager<D, kTile> sk, sv;
-    sk.set(a.k, kvh, first, tid);
-    sv.set(a.v, kvh, first, tid);
-    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
-        (__attribute__((address_space(3))) uint8_t *)lds));
-    const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
     const uint32_t ra = lds0 + row_address<D>(l), ca = lds0 + channel_address<D>(l);
 
     float16_t acc[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
-    int k = u.x < u.y ? first : last, st = 0;
-    if (k < last) {
-        sk.send(mine, last - k);
-        sv.send(mine + 2 * TB, last - k);
-    }
 #pragma unroll 1
     for (; k < last; k += kTile, st ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1104,9 +1105,6 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
     const int tid = thread_here(), w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63;
     const int g = l >> 5, n = l & 31;
     const int j = tile * kOwn + w * 32 + n;
-    const int2 seen = rows_of(a, j);
-    Span sp;
-    sp.set(seen);
     const int t0 = rows.x / kRows, per = steps_over(rows.x, rows.y, kRows);
 
     const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(
@@ -1119,16 +1117,6 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
     if (units.x < units.y) sv.send(mine, a.tokens - tile * kOwn);
     u32x4_t kf[KS];
     own_operand<D>(kf, a.k.at(j, kvh), j < a.tokens, l);
-    float fs = 1.f;
-    if constexpr (DT == NF4_F16) {
-        u32x4_t vf[KS];
-        own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, l);
-        const int b0 = t0 * kRows / kTile, nb = per ? (rows.y - 1) / kTile - b0 + 1 : 0;
-        const float *norms = b.norms + static_cast<int64_t>(kvh * a.group) * b.blocks + b0;
-        const float most = most_of(norms, nb, a.group, b.blocks);
-        const float most_d = most_of(norms + static_cast<int64_t>(a.n_heads + a.n_kv) * b.blocks, nb, a.group, b.blocks);
-        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most + most_d);
-    }
     // unit (head of the group, tile of rows), the next one
     int uh = per ? units.x / per : 0, ut = units.x - uh * per;
     sq.set(a.q, kvh * a.group + uh, (t0 + ut) * kRows, tid);
@@ -1155,10 +1143,24 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
     };
     const uint32_t va = lds0 + w * 32 * D * 2 + row_address<D>(l);
     const uint32_t ra = lds0 + VB + row_address<D>(l), ca = lds0 + VB + channel_address<D>(l);
+    if (units.x < units.y) send(0);
+    // (what sees the keys is found while all that is on its way)
+    const int2 seen = rows_of(a, j);
+    Span sp;
+    sp.set(seen);
+    float fs = 1.f;
+    if constexpr (DT == NF4_F16) {
+        u32x4_t vf[KS];
+        own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, l);
+        const int b0 = t0 * kRows / kTile, nb = per ? (rows.y - 1) / kTile - b0 + 1 : 0;
+        const float *norms = b.norms + static_cast<int64_t>(kvh * a.group) * b.blocks + b0;
+        const float most = most_of(norms, nb, a.group, b.blocks);
+        const float most_d = most_of(norms + static_cast<int64_t>(a.n_heads + a.n_kv) * b.blocks, nb, a.group, b.blocks);
+        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most + most_d);
+    }
     float16_t dk[DN], dv[DN];
 #pragma unroll
     for (int x = 0; x < DN; ++x) dk[x] = dv[x] = (float16_t){};
-    if (units.x < units.y) send(0);
 #pragma unroll 1
     for (int u = units.x; u < units.y; ++u, st ^= 1) {
         const int r = (t0 + t) * kRows;
