@@ -505,7 +505,13 @@ __device__ __forceinline__ void join_write(const Strided &out, int head, int r0,
 }
 
 // ------------------------------------------------------------------------------ forward
-
+//
+// The running maximum and sum of a row stay in its lane; a wave whose rows' maxima all hold does not
+// rescale.  8192 tokens of 28 heads of 128 over 4, bf16: 495 us, 972 TFLOP/s.  A step of 64 keys for 128 rows
+// takes two workgroups on a CU 2.2 us: its matrix instructions alone, on values as these are, 1.27 at the
+// clock that the power cap leaves (0.93 on zeros), the exponentials, maxima and sums 0.24 more, reading k and v
+// out of LDS 0.26, barrier and DMA 0.2.  (The next step's scores formed between this one's exponentials, in the
+// same wave: 20 % slower, and not faster without its spills, in steps of 32 keys.)
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pieces pc, int tiles) {
     constexpr int KS = D / 16, DN = D / 32, TB = kTileBytes<D>;
@@ -735,16 +741,23 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Attn a, const 
 // is taken with the sum of the first two, whose rounding (2^-16) is below those that follow.
 constexpr float kNear = 256.f;
 
-//
 // Tiles or shares.  Where all tiles are short, each has a workgroup.  Else that is uneven, and a
 // key/value head's work is a line: its tiles of keys one behind the other, then the tiles of rows of its
 // query heads, each as long as its steps cost and its beginning.  `groups` workgroups take an equal share
 // of the line each, which may begin and end inside a tile: all are on the card at once and end together,
 // whatever the lengths of the sequences are (device data).  A step belongs to the share in which it
 // begins; a tile whose steps are in several leaves a part for each, and the join launch sums a tile's
-// parts in their order.  (Heads of 128, bf16, the whole pass: one sequence of 2048, 12 heads over 2: 82 us,
-// with pieces of equal length instead 98; of 4096: 239 and 306; of 8192, 28 over 4: 1740 both; 30
-// sequences of 200, 16 heads of 64: 71, and 52 with a workgroup a tile.)
+// parts in their order.  (Heads of 128, bf16, the whole pass: one sequence of 2048, 12 heads over 2: 81 us,
+// a fifth more with pieces of equal length; of 4096: 234, 28 % more; of 8192, 28 over 4: 1620, the same; 30
+// sequences of 200, 16 heads of 64: 50 with a workgroup a tile, 40 % more with shares.  Half as many shares,
+// one a CU: 2048 100 us, 8192 2270.)
+//
+// What bounds it, bf16, 8192 tokens of 28 heads of 128 over 4: the rows' launch 22 us, this one 1600, the join
+// 22.  It does 7 products where a formula's 5 would do (the scores and do.v are formed for the keys and for the
+// rows again, since a sum of dq over the keys' workgroups would need atomics, whose order changes results):
+// 1.04 PFLOP/s of them, where a large matrix product by the library reaches 1.35.  The matrix pipe is busy 51 % of the
+// cycles, at 1.64 GHz: the power cap.  At 2048 tokens of 12 heads (66 us, the join 15) a workgroup has about 17
+// steps, and 55 MB of parts are written and read again.
 constexpr int kKeyCost = 20, kRowCost = 30, kItemCost = 80;  // a step of keys, of rows; a tile
 constexpr int kLeast = 160;                                  // a share
 
@@ -930,12 +943,17 @@ __device__ __forceinline__ float ds_scale(float bound) {
     return ldexpf(1.f, -e);
 }
 
-// the largest of n numbers of `heads` heads each, `blocks` apart
-__device__ __forceinline__ float most_of(const float *p, int n, int heads, int64_t blocks) {
-    float v = 0.f;
+// The largest of n numbers of `heads` heads each, `blocks` apart, and of those `other` behind them: of both at a
+// time, since it is the loads' latency that counts.
+__device__ __forceinline__ float2 most_of(const float *p, int n, int heads, int64_t blocks, int64_t other) {
+    float2 v = make_float2(0.f, 0.f);
     for (int h = 0; h < heads; ++h, p += blocks)
-        for (int i = thread_here() & 63; i < n; i += 64) v = fmaxf(v, p[i]);
-    return wave_max(v);
+        for (int i = thread_here() & 63; i < n; i += 64) {
+            const float x = p[i], y = p[i + other];
+            v.x = fmaxf(v.x, x);
+            v.y = fmaxf(v.y, y);
+        }
+    return make_float2(wave_max(v.x), wave_max(v.y));
 }
 
 // |x|^2 of a lane's row, from its operands
@@ -988,7 +1006,7 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     float fs = 1.f;
     if constexpr (DT == NF4_F16) {
         const int b0 = first >> 6, nb = u.y - u.x;
-        fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb, 1, 0) + fabsf(delta));
+        fs = ds_scale(sqrtf(square_of<DT, D>(go)) * most_of(b.norms + static_cast<int64_t>(a.n_heads + kvh) * b.blocks + b0, nb, 1, 0, 0).x + fabsf(delta));
     }
     // (the probabilities are used for dS only: their scale goes into the exponent)
     const float mul = near ? a.c : 1.f, sub = (near ? base : 0.f) - log2f(fs);
@@ -1090,8 +1108,8 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
 
 // The keys' workgroup holds its k and its sums in registers (160 of the 256 that two waves a SIMD leave)
 // and its v in LDS: with v in registers too, the operands of each product were waited for one at a time
-// (8192 tokens of
-// 28 heads, the whole backward pass: 2200 us instead of 1660), and tiles are of 32 rows, so that two workgroups' LDS fits a CU.
+// (8192 tokens of 28 heads, the whole backward pass: a third longer), and tiles are of 32 rows, so that two
+// workgroups' LDS fits a CU.
 template <int D>
 constexpr int kKeyLds = kOwn * D * 2 + 4 * kRows * D * 2 + 2 * 1024;  // v; q and do, two stages; their rows' numbers
 template <int D>
@@ -1153,10 +1171,9 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
         u32x4_t vf[KS];
         own_operand<D>(vf, a.v.at(j, kvh), j < a.tokens, l);
         const int b0 = t0 * kRows / kTile, nb = per ? (rows.y - 1) / kTile - b0 + 1 : 0;
-        const float *norms = b.norms + static_cast<int64_t>(kvh * a.group) * b.blocks + b0;
-        const float most = most_of(norms, nb, a.group, b.blocks);
-        const float most_d = most_of(norms + static_cast<int64_t>(a.n_heads + a.n_kv) * b.blocks, nb, a.group, b.blocks);
-        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most + most_d);
+        const float2 most = most_of(b.norms + static_cast<int64_t>(kvh * a.group) * b.blocks + b0, nb, a.group, b.blocks,
+                                    static_cast<int64_t>(a.n_heads + a.n_kv) * b.blocks);
+        fs = ds_scale(sqrtf(square_of<DT, D>(vf)) * most.x + most.y);
     }
     float16_t dk[DN], dv[DN];
 #pragma unroll
