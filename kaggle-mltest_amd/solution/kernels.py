@@ -867,31 +867,31 @@ def rope_table(positions: int, head_dim: int, base: float, device):
 # ------------------------------- training: attention of a packed batch, dropout without masks
 
 def _attn_desc(q, k, v, cu_seqlens, scale, window, max_len):
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] \
-            or q.shape[2] != k.shape[2]:
+    shape, kv_shape, dtype, dev = q.shape, k.shape, q.dtype, q.get_device()
+    if len(shape) != 3 or len(kv_shape) != 3 or kv_shape != v.shape or shape[0] != kv_shape[0] \
+            or shape[2] != kv_shape[2]:
         raise ValueError("q is [tokens, n_heads, head_dim], k and v [tokens, n_kv, head_dim]")
-    if not q.dtype == k.dtype == v.dtype:
+    if not dtype == k.dtype == v.dtype:
         raise ValueError("q, k and v have one dtype")
-    if q.stride(2) != 1 or k.stride(2) != 1 or v.stride(2) != 1:
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if not qs[2] == ks[2] == vs[2] == 1:
         raise ValueError("q, k and v have head_dim contiguous")
-    dev = q.get_device()
     if dev < 0 or not dev == k.get_device() == v.get_device():
         raise ValueError("q, k and v are on one cuda device")
-    tokens, heads, dim = q.shape
-    n_kv = k.shape[1]
+    tokens, heads, dim = shape
+    n_kv = kv_shape[1]
     if heads < 1 or n_kv < 1 or heads % n_kv:
         raise ValueError("n_heads is a multiple of n_kv")
     cu, batch = None, 1
     if cu_seqlens is not None:
+        offsets = cu_seqlens.shape
         if cu_seqlens.get_device() != dev or cu_seqlens.dtype != torch.int32 \
-                or cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 1 \
-                or not cu_seqlens.is_contiguous():
+                or len(offsets) != 1 or offsets[0] < 1 or not cu_seqlens.is_contiguous():
             raise ValueError("cu_seqlens is a contiguous int32 [batch + 1] tensor on q's device")
-        cu, batch = cu_seqlens.data_ptr(), cu_seqlens.shape[0] - 1
-    return NF4Attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), q.stride(0), q.stride(1), k.stride(0),
-                   k.stride(1), v.stride(0), v.stride(1), cu, tokens, window or 0, max_len or 0,
-                   batch, heads, n_kv, dim, dim ** -0.5 if scale is None else scale,
-                   _code(q.dtype))
+        cu, batch = cu_seqlens.data_ptr(), offsets[0] - 1
+    return NF4Attn(q.data_ptr(), k.data_ptr(), v.data_ptr(), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+                   cu, tokens, window or 0, max_len or 0, batch, heads, n_kv, dim,
+                   dim ** -0.5 if scale is None else scale, _code(dtype))
 
 
 @_on_its_device
@@ -922,10 +922,12 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
 
 
 def _grad(t, shape, like, what):
-    if t.shape != shape or t.dtype != like.dtype or t.get_device() != like.get_device() \
-            or t.stride(2) != 1:
+    if t.shape != shape or t.dtype != like.dtype or t.get_device() != like.get_device():
         raise ValueError(f"{what} is a {list(shape)} tensor of q's dtype, head_dim contiguous")
-    return NF4Grad(t.data_ptr(), t.stride(0), t.stride(1))
+    tok, head, one = t.stride()
+    if one != 1:
+        raise ValueError(f"{what} is a {list(shape)} tensor of q's dtype, head_dim contiguous")
+    return NF4Grad(t.data_ptr(), tok, head)
 
 
 @_on_its_device
@@ -938,14 +940,18 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     them an input.  Rows of no sequence get zeros."""
     desc = _attn_desc(q, k, v, cu_seqlens, scale, window, max_len)
     shape, kv_shape = q.shape, k.shape
+    args = [_grad(dout, shape, q, "dout")]
     if grads is None:
         grads = q.new_empty(shape), q.new_empty(kv_shape), q.new_empty(kv_shape)
+        args += [NF4Grad(t.data_ptr(), h * shape[2], shape[2])
+                 for t, h in zip(grads, (shape[1], kv_shape[1], kv_shape[1]))]
+    else:
+        args += [_grad(t, sh, q, name) for t, sh, name in
+                 zip(grads, (shape, kv_shape, kv_shape), ("dq", "dk", "dv"))]
     _check_out(out, shape, q)
     if stats.shape != (*shape[:2], 2) or stats.dtype != torch.float32 \
             or stats.get_device() != q.get_device() or not stats.is_contiguous():
         raise ValueError("stats is the forward pass's fp32 [tokens, n_heads, 2] tensor")
-    args = [_grad(t, sh, q, name) for t, sh, name in
-            zip((dout, *grads), (shape, shape, kv_shape, kv_shape), ("dout", "dq", "dk", "dv"))]
     lib, ref = load(), ctypes.byref(desc)
     nbytes = lib.nf4_attn_bwd_workspace(ref)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
@@ -995,7 +1001,8 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, sites, outs=None) -> 
         raise ValueError("x is [rows, cols]")
     shape, dtype, index = x.shape, x.dtype, x.get_device()
     dt = _code(dtype)
-    _rows_of(x, shape, dtype, index)
+    if x.stride(1) != 1 and shape[1] > 1:
+        _rows_of(x, shape, dtype, index)  # (refuses)
     if outs is None:
         outs = [x.new_empty(shape) for _ in sites]
     else:
