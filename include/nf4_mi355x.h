@@ -521,9 +521,10 @@ typedef struct nf4_attn {
  * with t_j = scale * log2(e) * q.k_j over the keys that the row sees, m = max t_j, l = sum
  * 2^(t_j - m), P_j = 2^(t_j - m) / l (the natural log-sum-exp is m ln 2 + ln l).  A row of no
  * sequence gets zeros and (0, 0).  What a row does not see has no part in its result, whatever lies
- * there; a row that sees a score of NaN or +inf, or scores of -inf only, is NaN, stats too.  Offsets that
- * are not as above (decreasing, outside of the rows) are no error: rows get what some of them say, and
- * nothing outside of the rows is read or written.  out and stats overlap no input.  Workspace:
+ * there; a row that sees a score of NaN or +inf, or scores of -inf only, is NaN, stats too.  Offsets count
+ * as far as there are rows (what lies before 0 or behind tokens is left out); of offsets that decrease the
+ * results are not defined, but nothing outside of the rows is read or written.  out and stats overlap no
+ * input.  Workspace:
  * nf4_attn_fwd_workspace bytes, 16-byte aligned, the call's own until it has run.
  * Replaces: _efficient_attention_forward in _Attention (/root/reference/solution/layer.py:735-826). */
 size_t nf4_attn_fwd_workspace(const nf4_attn *a);

@@ -418,3 +418,38 @@ def test_strides_of_views(cuda):
     for x, name in zip(leaves[1:], ("dk", "dv")):  # (the sum over the expanded heads is autograd's)
         want = got[name].double().sum(1, keepdim=True)
         assert ((x.grad.double() - want).abs() <= 4 * ref.HALF[BF16] * got[name].double().abs().sum(1, keepdim=True)).all()
+
+
+@pytest.mark.parametrize("cu", [[5, 60, 100], [-7, 40, 130], [100, 100], [0, 50, 20, 90], [70, 10], [0, 1 << 30]])
+@pytest.mark.parametrize("window", [0, 9])
+def test_offsets_that_leave_rows_out_or_make_no_sense(cuda, cu, window):
+    """Rows before the first sequence and offsets outside of the rows: rows of no sequence are 0.  Offsets that
+    decrease: nothing is defined but that what lies around the gradients stays as it is."""
+    q, k, v, dout, _ = make(cuda, F16, 4, 2, 64, (100,), seed=27, layout="plain")
+    c = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    from solution import kernels
+
+    out, stats = kernels.attention_fwd(q, k, v, c, window=window)
+    around = [torch.full((104, *t.shape[1:]), 7.0, dtype=F16, device=cuda) for t in (q, k, v)]
+    grads = kernels.attention_bwd(dout, q, k, v, out, stats, c, window=window, grads=[t[2:102] for t in around])
+    assert all((t[:2] == 7).all() and (t[102:] == 7).all() for t in around)
+    if all(a <= b for a, b in zip(cu, cu[1:])):
+        inside = [min(max(x, 0), 100) for x in cu]
+        want = ref.attention(q, k, v, inside, dout, window=window)
+        for name, t in zip(("out", "stats", "dq", "dk", "dv"), (out, stats, *grads)):
+            ref.assert_within(t, want[name], name)
+
+
+def test_a_second_derivative_raises(cuda):
+    from solution.layer import attention, rope_attention
+
+    q, k, v, dout, cu = make(cuda, F16, 4, 2, 64, (20,), seed=28, layout="plain")
+    q.requires_grad_()
+    g, = torch.autograd.grad(attention(q, k, v), q, dout.requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().sum().backward()
+    x = torch.cat([t.detach().flatten(1) for t in (q, k, v)], 1).requires_grad_()
+    cos = sin = torch.ones(20, 64, device=cuda)
+    g, = torch.autograd.grad(rope_attention(x, cos, sin, 4, 2), x, dout, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().sum().backward()
