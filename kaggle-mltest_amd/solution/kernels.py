@@ -866,6 +866,11 @@ def rope_table(positions: int, head_dim: int, base: float, device):
 
 # ------------------------------- training: attention of a packed batch, dropout without masks
 
+def _empty(like):
+    """A contiguous tensor like this one (1.2 us of the host's; new_empty 1.6, torch.empty 2.1)."""
+    return torch.empty_like(like, memory_format=torch.contiguous_format)
+
+
 def _attn_desc(q, k, v, cu_seqlens, scale, window, max_len):
     shape, kv_shape, dtype, dev = q.shape, k.shape, q.dtype, q.get_device()
     if len(shape) != 3 or len(kv_shape) != 3 or kv_shape != v.shape or shape[0] != kv_shape[0] \
@@ -908,10 +913,10 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     desc = _attn_desc(q, k, v, cu_seqlens, scale, window, max_len)
     tokens, heads, dim = q.shape
     if out is None:
-        out = q.new_empty((tokens, heads, dim))
+        out = _empty(q)
     else:
         _check_out(out, (tokens, heads, dim), q)
-    stats = q.new_empty((tokens, heads, 2), dtype=torch.float32)
+    stats = q.new_empty(tokens, heads, 2, dtype=torch.float32)
     lib, ref = load(), ctypes.byref(desc)
     nbytes = lib.nf4_attn_fwd_workspace(ref)
     ws = q.new_empty(nbytes, dtype=torch.uint8) if nbytes else None
@@ -942,9 +947,10 @@ def attention_bwd(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch
     shape, kv_shape = q.shape, k.shape
     args = [_grad(dout, shape, q, "dout")]
     if grads is None:
-        grads = q.new_empty(shape), q.new_empty(kv_shape), q.new_empty(kv_shape)
-        args += [NF4Grad(t.data_ptr(), h * shape[2], shape[2])
-                 for t, h in zip(grads, (shape[1], kv_shape[1], kv_shape[1]))]
+        dq, dk, dv = grads = _empty(q), _empty(k), _empty(v)
+        dim, row = shape[2], kv_shape[1] * shape[2]
+        args += (NF4Grad(dq.data_ptr(), shape[1] * dim, dim), NF4Grad(dk.data_ptr(), row, dim),
+                 NF4Grad(dv.data_ptr(), row, dim))
     else:
         args += [_grad(t, sh, q, name) for t, sh, name in
                  zip(grads, (shape, kv_shape, kv_shape), ("dq", "dk", "dv"))]
@@ -1004,7 +1010,7 @@ def dropout(x: torch.Tensor, p: float, seed: torch.Tensor, sites, outs=None) -> 
     if x.stride(1) != 1 and shape[1] > 1:
         _rows_of(x, shape, dtype, index)  # (refuses)
     if outs is None:
-        outs = [x.new_empty(shape) for _ in sites]
+        outs = [_empty(x) for _ in sites]
     else:
         if len(outs) != len(sites):
             raise ValueError("an output for every site")
@@ -1033,7 +1039,7 @@ def dropout_bwd(grads, p: float, seed: torch.Tensor, sites, base: torch.Tensor |
     if base is not None:
         _rows_of(base, shape, dtype, index)
     if out is None:
-        out = g.new_empty(shape)
+        out = _empty(g)
     elif out is not base:
         _rows_of(out, shape, dtype, index)
     ptrs, lds, where, n = _drop_args(grads, seed, sites, index)
