@@ -803,70 +803,88 @@ __device__ __forceinline__ int2 steps_in(int64_t s0, int64_t s1, int64_t c, int 
 // Steps of `unit` positions over [x, y), whole ones.
 __device__ __forceinline__ int steps_over(int x, int y, int unit) { return x < y ? (y - 1) / unit - x / unit + 1 : 0; }
 
-// A lane's own search: the rows of row t's sequence, or [t, t).
-__device__ __forceinline__ int2 sequence_of_lane(const Attn &a, int t) {
-    if (!a.cu) return make_int2(0, a.tokens);
+// A lane's own search in offsets `cu` (in LDS or not): the rows of row t's sequence, or [t, t).
+template <typename Offsets>
+__device__ __forceinline__ int2 sequence_of_lane(const Attn &a, Offsets cu, int t) {
     int lo = 0, hi = a.batch + 1;  // the first offset past t
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (a.cu[mid] <= t) lo = mid + 1;
+        if (cu[mid] <= t) lo = mid + 1;
         else hi = mid;
     }
     if (lo == 0 || lo > a.batch) return make_int2(t, t);
-    const int s = a.cu[lo - 1], e = a.cu[lo];
+    const int s = cu[lo - 1], e = cu[lo];
     return make_int2(s < 0 ? 0 : s, e > a.tokens ? a.tokens : e);
 }
 
-// The table and the line, by one workgroup: a tile a thread, 256 at a time.
+// The table and the line, by one workgroup: a tile a thread, 256 at a time.  It is the latency of what it waits for
+// that counts: the offsets come to LDS at once where they fit, and what a thread has found stays with it.
 __device__ __forceinline__ void make_line(const Attn &a, const Back &b) {
+    constexpr int LDS_OFFSETS = 1024;
     __shared__ int64_t sum[2][4];
-    int64_t done[2] = {0, 0};
+    __shared__ int offsets[LDS_OFFSETS];
     const int w = threadIdx.x >> 6, l = threadIdx.x & 63;
-    const int begin = a.cu ? a.cu[0] : 0, end = a.cu ? a.cu[a.batch] : a.tokens;
+    const bool fit = a.cu && a.batch < LDS_OFFSETS;
+    if (fit) {
+#pragma unroll
+        for (int x = 0; x < LDS_OFFSETS; x += 256)
+            if (x + static_cast<int>(threadIdx.x) <= a.batch) offsets[x + threadIdx.x] = a.cu[x + threadIdx.x];
+        __syncthreads();
+    }
+    const int begin = !a.cu ? 0 : fit ? offsets[0] : a.cu[0], end = !a.cu ? a.tokens : fit ? offsets[a.batch] : a.cu[a.batch];
+    auto sequence = [&](int t) {
+        return !a.cu ? make_int2(0, a.tokens) : fit ? sequence_of_lane(a, offsets, t) : sequence_of_lane(a, a.cu, t);
+    };
+    int64_t at[2] = {0, 0}, of_rows = 0;  // (rows' tiles begin behind all keys')
 #pragma unroll 1
-    for (int pass = 0; pass < 2; ++pass) {  // (rows' tiles begin behind all keys')
-        int64_t at = done[0];
-#pragma unroll 1
-        for (int t0 = 0; t0 < b.tiles; t0 += 256) {
-            const int t = t0 + threadIdx.x;
-            int64_t cost = 0;
-            if (t < b.tiles) {
-                int4 r;
-                if (pass == 0) {
-                    const int first = t * kOwn > begin ? t * kOwn : begin;
-                    int last = t * kOwn + kOwn < a.tokens ? t * kOwn + kOwn - 1 : a.tokens - 1;
-                    last = last < end ? last : end - 1;
-                    r = make_int4(0, 0, 0, 0);
-                    if (first <= last) {
-                        const int2 x = sequence_of_lane(a, first), y = sequence_of_lane(a, last);
-                        r.x = a.window && first - a.window + 1 > x.x ? first - a.window + 1 : x.x;
-                        r.y = last + 1;
-                        r.z = first;
-                        r.w = a.window && last + a.window < y.y ? last + a.window : y.y;
-                    }
-                    b.tab[t] = r;
-                } else {
-                    r = b.tab[t];
-                }
-                cost = pass == 0 ? static_cast<int64_t>(steps_over(r.z, r.w, kRows)) * a.group * kKeyCost + kItemCost
-                                 : static_cast<int64_t>(steps_over(r.x, r.y, kTile) * kRowCost + kItemCost) * a.group;
+    for (int t0 = 0; t0 < b.tiles; t0 += 256) {
+        const int t = t0 + threadIdx.x;
+        int64_t cost[2] = {0, 0}, upto[2];
+        if (t < b.tiles) {
+            const int first = t * kOwn > begin ? t * kOwn : begin;
+            int last = t * kOwn + kOwn < a.tokens ? t * kOwn + kOwn - 1 : a.tokens - 1;
+            last = last < end ? last : end - 1;
+            int4 r = make_int4(0, 0, 0, 0);
+            if (first <= last) {
+                const int2 x = sequence(first), y = sequence(last);
+                r.x = a.window && first - a.window + 1 > x.x ? first - a.window + 1 : x.x;
+                r.y = last + 1;
+                r.z = first;
+                r.w = a.window && last + a.window < y.y ? last + a.window : y.y;
             }
-            int64_t upto = cost;
+            b.tab[t] = r;
+            cost[0] = static_cast<int64_t>(steps_over(r.z, r.w, kRows)) * a.group * kKeyCost + kItemCost;
+            cost[1] = static_cast<int64_t>(steps_over(r.x, r.y, kTile) * kRowCost + kItemCost) * a.group;
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            upto[k] = cost[k];
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
-                const int64_t x = __shfl_up(upto, o);
-                if (l >= o) upto += x;
+                const int64_t x = __shfl_up(upto[k], o);
+                if (l >= o) upto[k] += x;
             }
-            if (l == 63) sum[pass][w] = upto;
-            __syncthreads();
-            for (int i = 0; i < w; ++i) upto += sum[pass][i];
-            if (t < b.tiles) b.line[pass * b.tiles + t] = at + upto - cost;
-            at += sum[pass][0] + sum[pass][1] + sum[pass][2] + sum[pass][3];
-            __syncthreads();
+            if (l == 63) sum[k][w] = upto[k];
         }
-        done[0] = at;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            for (int i = 0; i < w; ++i) upto[k] += sum[k][i];
+            upto[k] += at[k] - cost[k];
+            at[k] += sum[k][0] + sum[k][1] + sum[k][2] + sum[k][3];
+        }
+        if (t < b.tiles) {
+            b.line[t] = upto[0];
+            of_rows = upto[1];
+            if (b.tiles > 256) b.line[b.tiles + t] = of_rows;
+        }
+        __syncthreads();
     }
-    if (threadIdx.x == 0) b.line[2 * b.tiles] = done[0];
+    for (int t = threadIdx.x; t < b.tiles; t += 256) {
+        if (b.tiles > 256) of_rows = b.line[b.tiles + t];
+        b.line[b.tiles + t] = at[0] + of_rows;
+    }
+    if (threadIdx.x == 0) b.line[2 * b.tiles] = at[0] + at[1];
 }
 
 // One workgroup per 64 rows and head; heads from n_heads on are those of v, the last makes the line.
@@ -881,22 +899,29 @@ __global__ __launch_bounds__(256) void attn_rows_kernel(const Attn a, const Back
     }
     const bool of_v = head >= a.n_heads;
     float worst = 0.f, worst_d = 0.f;
+    constexpr int N = kTile / RPP;
+    u32x4_t go[N], out[N];
+    float2 stats[N];
 #pragma unroll
-    for (int x = 0; x < kTile; x += RPP) {
-        const int i = x + threadIdx.x / CH, r = blockIdx.x * kTile + i;
-        float d = 0.f, sq = 0.f;
-        float2 ml = make_float2(0.f, 0.f);
-        if (r < a.tokens) ml = a.stats[static_cast<int64_t>(r) * a.n_heads + (of_v ? 0 : head)];
-        if (r < a.tokens) {
-            float go[8], o[8];
-            unpack8<DT>(*reinterpret_cast<const u32x4_t *>((of_v ? a.v.at(r, head - a.n_heads) : a.dout.at(r, head)) + ch * 8), go);
+    for (int x = 0; x < N; ++x) {  // (all are asked for at once; rows that are not there: the last one)
+        int r = blockIdx.x * kTile + x * RPP + threadIdx.x / CH;
+        r = r < a.tokens ? r : a.tokens - 1;
+        stats[x] = a.stats[static_cast<int64_t>(r) * a.n_heads + (of_v ? 0 : head)];
+        go[x] = *reinterpret_cast<const u32x4_t *>((of_v ? a.v.at(r, head - a.n_heads) : a.dout.at(r, head)) + ch * 8);
+        out[x] = go[x];
+        if (!of_v) out[x] = *reinterpret_cast<const u32x4_t *>(a.o.at(r, head) + ch * 8);
+    }
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sq = fmaf(go[e], go[e], sq);
-            if (!of_v) {
-                unpack8<DT>(*reinterpret_cast<const u32x4_t *>(a.o.at(r, head) + ch * 8), o);
+    for (int x = 0; x < N; ++x) {
+        const int i = x * RPP + threadIdx.x / CH, r = blockIdx.x * kTile + i;
+        float2 ml = r < a.tokens ? stats[x] : make_float2(0.f, 0.f);
+        float f[8], o[8], d = 0.f, sq = 0.f;
+        unpack8<DT>(go[x], f);
+        unpack8<DT>(out[x], o);
 #pragma unroll
-                for (int e = 0; e < 8; ++e) d = fmaf(go[e], o[e], d);
-            }
+        for (int e = 0; e < 8; ++e) {
+            sq = fmaf(f[e], f[e], sq);
+            d = fmaf(f[e], o[e], d);
         }
 #pragma unroll
         for (int o = 1; o < CH; o <<= 1) {
