@@ -756,7 +756,7 @@ constexpr float kNear = 256.f;
 // 22.  It does 7 products where a formula's 5 would do (the scores and do.v are formed for the keys and for the
 // rows again, since a sum of dq over the keys' workgroups would need atomics, whose order changes results):
 // 1.04 PFLOP/s of them, where a large matrix product by the library reaches 1.35.  The matrix pipe is busy 51 % of the
-// cycles, at 1.64 GHz: the power cap.  At 2048 tokens of 12 heads (66 us, the join 15) a workgroup has about 17
+// cycles, at 1.64 GHz: the power cap.  At 2048 tokens of 12 heads (65 us, the join 15) a workgroup has about 17
 // steps, and 55 MB of parts are written and read again.
 constexpr int kKeyCost = 20, kRowCost = 30, kItemCost = 80;  // a step of keys, of rows; a tile
 constexpr int kLeast = 160;                                  // a share
