@@ -27,6 +27,7 @@ d(xd) unfolded (nf4_lora_ax_multi) for the norm backward.
 
 from __future__ import annotations
 
+import copy
 from dataclasses import dataclass, field
 
 import torch
@@ -136,14 +137,19 @@ def _run_jobs(fn, jobs, like):
             fn(js[k:k + 4], like.shape[0], r, like.dtype, like)
 
 
-def _dropped(x, spec):
+def _as_it_is(spec):
+    """The spec of one forward pass and its backward pass: a program may change its own between them."""
+    return ProjectionSpec(list(spec.weights), [copy.copy(ad) for ad in spec.loras], spec.seed)
+
+
+def _dropped(x, spec, seed):
     """{adapter index: its dropped x}, one launch for the adapters of one probability."""
     by_p = {}
     for i, ad in enumerate(spec.loras):
         if ad.dropout:
             if ad.own_input:
                 raise ValueError("an adapter's own input comes dropped: no `dropout` beside own_input")
-            if spec.seed is None:
+            if seed is None:
                 raise ValueError("adapters with dropout need the spec's seed")
             by_p.setdefault(ad.dropout, []).append(i)
     out = {}
@@ -151,7 +157,7 @@ def _dropped(x, spec):
         for k in range(0, len(where), 8):
             part = where[k:k + 8]
             sites = [spec.loras[i].site for i in part]
-            out.update(zip(part, kernels.dropout(x, p, spec.seed, sites)))
+            out.update(zip(part, kernels.dropout(x, p, seed, sites)))
     return out
 
 
@@ -189,8 +195,9 @@ class NF4Projection(torch.autograd.Function):
     def forward(ctx, x, bias, spec, *lora_params):
         dtype = x.dtype
         x = _aligned_rows(x)
+        spec = _as_it_is(spec)
         structs, saved, jobs, xd_dtypes = [], [], [], []
-        dropped = _dropped(x, spec)
+        dropped = _dropped(x, spec, spec.seed)
         for i, (ad, a, b, xd) in enumerate(_adapter_params(spec, lora_params)):
             a16 = a.detach().to(dtype).contiguous()
             b16 = b.detach().to(dtype).contiguous()
@@ -224,9 +231,9 @@ class NF4Projection(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dy):
-        x, _, *saved = ctx.saved_tensors
+        x, seed, *saved = ctx.saved_tensors
         spec = ctx.spec
-        dropped, drop_grads = _dropped(x, spec), []
+        dropped, drop_grads = _dropped(x, spec, seed), []
         dy = _aligned_rows(dy.to(x.dtype))
         offs = spec.offsets()
         # `live` holds every tensor the launches below reach only through raw pointers in
@@ -285,7 +292,7 @@ class NF4Projection(torch.autograd.Function):
         for p, parts in by_p.items():
             for k in range(0, len(parts), 8):
                 sites, gs = zip(*parts[k:k + 8])
-                kernels.dropout_bwd(gs, p, spec.seed, sites, base=dx, out=dx)
+                kernels.dropout_bwd(gs, p, seed, sites, base=dx, out=dx)
         dbias = kernels.bias_grad(dy) if ctx.has_bias and ctx.needs_input_grad[1] else None
         return (dx, dbias, None, *grads)
 
