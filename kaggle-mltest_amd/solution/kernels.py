@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import inspect
 
 import torch
 
@@ -487,15 +488,19 @@ def qkv_rope_bwd(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, cos: torc
 
 
 def _on_its_device(fn):
-    """Runs a call with its first tensor's device as the current one: launches go to the current device,
-    and the handle of another's default stream is none of its own."""
+    """Runs a call with the device of its first parameter (a tensor, or a list of them) as the current
+    one: launches go to the current device, and the handle of another's default stream is none of its
+    own.  Calls without such a tensor are refused by `fn` itself."""
+    first = next(iter(inspect.signature(fn).parameters))
+
     @functools.wraps(fn)
     def call(*args, **kw):
         if _devices() < 2:
             return fn(*args, **kw)
-        t = args[0] if args else next(iter(kw.values()))
-        t = t[0] if isinstance(t, (list, tuple)) else t
-        if not t.is_cuda or t.get_device() == torch.cuda.current_device():
+        t = args[0] if args else kw.get(first)
+        if isinstance(t, (list, tuple)):
+            t = t[0] if t else None
+        if not getattr(t, "is_cuda", False) or t.get_device() == torch.cuda.current_device():
             return fn(*args, **kw)
         with torch.cuda.device(t.get_device()):
             return fn(*args, **kw)

@@ -1,0 +1,59 @@
+"""How the training operators' calls find their tensors' device, with two devices (no GPU needed)."""
+
+import contextlib
+
+import pytest
+import torch
+
+
+class Tensor:
+    def __init__(self, index, is_cuda=True):
+        self.index, self.is_cuda = index, is_cuda
+
+    def get_device(self):
+        return self.index
+
+
+@pytest.fixture()
+def two_devices(monkeypatch):
+    """Two GPUs as the calls see them; [the current one]."""
+    from solution import kernels
+
+    at = [0]
+
+    @contextlib.contextmanager
+    def device(index):
+        old, at[0] = at[0], index
+        yield
+        at[0] = old
+
+    monkeypatch.setattr(kernels, "_devices", lambda: 2)
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
+    monkeypatch.setattr(torch.cuda, "device", device)
+    return at
+
+
+def test_keywords_in_any_order(two_devices):
+    """The first parameter's tensor decides, wherever the call names it."""
+    from solution import kernels
+
+    seen = kernels._on_its_device(lambda x, p=0.5, other=None: two_devices[0])
+    assert seen(p=0.1, x=Tensor(1)) == 1 and seen(other=None, x=Tensor(1)) == 1
+    assert seen(other=Tensor(0), x=Tensor(1)) == 1 and seen(p=[], x=[Tensor(1)]) == 1
+    assert seen(p=0.1, x=Tensor(1, is_cuda=False)) == 0 and two_devices == [0]
+    with pytest.raises(TypeError):
+        seen(p=0.1)
+
+
+def test_refusals_by_keyword_are_the_calls_own(two_devices):
+    """What a call refuses it refuses with two devices as with one."""
+    from solution import kernels
+
+    x, seed = torch.zeros(3, 8).half(), torch.zeros(2, dtype=torch.int64)
+    q = torch.zeros(4, 4, 64).half()
+    with pytest.raises(ValueError, match="cuda"):
+        kernels.dropout(p=0.5, seed=seed, sites=[0], x=x)
+    with pytest.raises(ValueError, match="cuda"):
+        kernels.attention_fwd(cu_seqlens=None, k=q, v=q, q=q)
+    with pytest.raises(TypeError):
+        kernels.attention_fwd(k=q, v=q)
