@@ -1034,9 +1034,9 @@ def dropout_bwd(grads, p: float, seed: torch.Tensor, sites, base: torch.Tensor |
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """dx of dropout: base (None: zeros) plus every site's gradient times its mask and scale, summed
     in fp32 in this order and rounded once.  `out` may be `base`."""
-    g = grads[0]
-    if g.dim() != 2 or len(grads) != len(sites):
+    if not grads or len(grads) != len(sites) or grads[0].dim() != 2:
         raise ValueError("a [rows, cols] gradient for every site")
+    g = grads[0]
     shape, dtype, index = g.shape, g.dtype, g.get_device()
     dt = _code(dtype)
     for t in grads:

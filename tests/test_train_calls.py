@@ -1,4 +1,4 @@
-"""How the training operators' calls find their tensors' device, with two devices (no GPU needed)."""
+"""How the training operators' calls find their tensors' device, and what they refuse (no GPU needed)."""
 
 import contextlib
 
@@ -57,3 +57,14 @@ def test_refusals_by_keyword_are_the_calls_own(two_devices):
         kernels.attention_fwd(cu_seqlens=None, k=q, v=q, q=q)
     with pytest.raises(TypeError):
         kernels.attention_fwd(k=q, v=q)
+
+
+@pytest.mark.parametrize("devices", [1, 2])
+def test_no_gradients_are_refused(monkeypatch, devices):
+    from solution import kernels
+
+    monkeypatch.setattr(kernels, "_devices", lambda: devices)
+    seed = torch.zeros(2, dtype=torch.int64)
+    for grads, sites in (([], []), ([], [0])):
+        with pytest.raises(ValueError, match="gradient"):
+            kernels.dropout_bwd(grads, 0.5, seed, sites)
