@@ -24,6 +24,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib, kernels
+from .layer import _aligned_rows
 from .quant_state import nf4_state_ok
 
 # int8 input gradients (int8_mlp.mlp_input_grad_int8) in RecomputedMLP.backward
@@ -46,9 +47,7 @@ class RecomputedMLP(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, gate_w, gate_qs, up_w, up_qs, down_w, down_qs):
         shape = x.shape
-        x2 = x.reshape(-1, shape[-1])
-        if x2.stride(0) % 8 or x2.data_ptr() % 16:
-            x2 = x2.contiguous()
+        x2 = _aligned_rows(x.reshape(-1, shape[-1]))
         gate_w, up_w, down_w = gate_w.reshape(-1), up_w.reshape(-1), down_w.reshape(-1)
         inter = int(gate_qs.shape[0])
         if INT8_FORWARD and _int8_ok(gate_qs, down_qs):
@@ -72,9 +71,7 @@ class RecomputedMLP(torch.autograd.Function):
         x2, gate_w, up_w, down_w = ctx.saved_tensors
         gate_qs, up_qs, down_qs = ctx.qs
         inter = int(gate_qs.shape[0])
-        grad = grad.reshape(-1, grad.shape[-1]).to(x2.dtype)
-        if grad.stride(0) % 8 or grad.data_ptr() % 16:
-            grad = grad.contiguous()
+        grad = _aligned_rows(grad.reshape(-1, grad.shape[-1]).to(x2.dtype))
         if INT8_BACKWARD and _int8_ok(gate_qs, down_qs):
             from .int8_mlp import mlp_input_grad_int8
 

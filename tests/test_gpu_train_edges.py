@@ -58,3 +58,22 @@ def test_a_spec_changed_before_the_backward_pass(cuda, change):
         assert not torch.equal(want[0][1], want[1][1])
     for a, b in zip(got, want):
         assert all(torch.equal(s, t) for s, t in zip(a, b))
+
+
+# -------------------------------------------------------------- views at any address
+
+@pytest.mark.parametrize("m", [20, 100])
+def test_mlp_of_expanded_and_strided_tensors(cuda, m):
+    """The gradient of a sum (one value, expanded), and every second column of a wider tensor."""
+    from solution.mlp import RecomputedMLP
+
+    w = [random_weight(*s, seed=87 + i, dev=cuda) for i, s in enumerate(((256, 128), (256, 128), (128, 256)))]
+    x = torch.randn(m, 256, generator=torch.Generator().manual_seed(88)).half().to(cuda)[:, ::2]
+    got = []
+    for dense in (True, False):
+        leaf = (x.clone(memory_format=torch.contiguous_format) if dense else x.detach()).requires_grad_()
+        y = RecomputedMLP.apply(leaf, *w[0], *w[1], *w[2])
+        one = torch.ones((), dtype=F16, device=cuda).expand(m, 128)
+        y.backward(one.contiguous() if dense else one)
+        got.append((y, leaf.grad))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])

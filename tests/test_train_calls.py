@@ -68,3 +68,35 @@ def test_no_gradients_are_refused(monkeypatch, devices):
     for grads, sites in (([], []), ([], [0])):
         with pytest.raises(ValueError, match="gradient"):
             kernels.dropout_bwd(grads, 0.5, seed, sites)
+
+
+def test_the_mlp_hands_on_rows(monkeypatch):
+    """An expanded gradient (a sum's: one value, strides of 0) and every second column of a wider tensor
+    reach the products as rows of consecutive values, in memory of their own."""
+    from solution import kernels, mlp
+
+    class Stop(Exception):
+        pass
+
+    def product(t, *args, **kw):
+        assert t.stride(1) == 1 and t.stride(0) == t.shape[1]
+        assert t.untyped_storage().nbytes() == 2 * t.numel()
+        raise Stop
+
+    class State:
+        shape = (256, 128)
+
+    class Ctx:
+        saved_tensors = (torch.zeros(100, 128).half(),) * 4
+        qs, shape = (State,) * 3, (100, 128)
+
+    for name in ("linear_fwd", "linear_swiglu_fwd", "linear_dx"):
+        monkeypatch.setattr(kernels, name, product)
+    w = torch.zeros(8, dtype=torch.uint8)
+    for rows in (20, 100):
+        wide = torch.zeros(rows, 256).half()[:, ::2]
+        with pytest.raises(Stop):
+            mlp.RecomputedMLP.forward(Ctx(), wide, w, State, w, State, w, State)
+        for grad in (torch.ones((), dtype=torch.half).expand(rows, 128), wide):
+            with pytest.raises(Stop):
+                mlp.RecomputedMLP.backward(Ctx(), grad)
