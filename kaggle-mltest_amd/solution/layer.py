@@ -120,9 +120,14 @@ class ProjectionSpec:
         return offs
 
 
+_FAR = 1 << 23  # elements from a token's row to the next: the attention kernels' most
+
+
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    if t.stride(-1) != 1 or t.stride(0) % 8 or t.data_ptr() % 16:
-        return t.contiguous()
+    """t [rows, cols] as the kernels take it: rows 16-byte aligned.  (A copy by clone: contiguous() gives
+    back a contiguous tensor that starts at another address as it is.)"""
+    if t.stride(-1) != 1 or t.stride(0) % 8 or t.stride(0) > _FAR or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 
@@ -255,7 +260,7 @@ class NF4Projection(torch.autograd.Function):
             rows = int(spec.weights[ad.seg][1].shape[0])
             dy_s = dy[:, offs[ad.seg]: offs[ad.seg] + rows]
             if dy_s.data_ptr() % 16:
-                dy_s = dy_s.contiguous()  # a copy only the job structs point to
+                dy_s = dy_s.clone(memory_format=torch.contiguous_format)  # only the job structs point to it
             da = torch.empty((x.shape[0], r), dtype=x.dtype, device=x.device)
             live += [dy_s, da]
             grad_b = torch.empty((rows, r), dtype=torch.float32, device=x.device)
@@ -308,8 +313,8 @@ def project(x, spec: ProjectionSpec, bias=None, lora_params=()):
 
 def _rows3(t):
     """A [tokens, heads, head_dim] tensor as the attention kernels take it (rows 16-byte aligned)."""
-    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.data_ptr() % 16:
-        return t.contiguous()
+    if t.stride(2) != 1 or t.stride(0) % 8 or t.stride(1) % 8 or t.stride(0) > _FAR or t.data_ptr() % 16:
+        return t.clone(memory_format=torch.contiguous_format)
     return t
 
 

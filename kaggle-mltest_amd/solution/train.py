@@ -18,12 +18,18 @@ from .layer import LoraAdapter, ProjectionSpec, project, rope_attention
 from .mlp import RecomputedMLP
 
 
+def _rows2(t):
+    """A [tokens, hidden] tensor as the norm's kernels take it: contiguous, 16-byte aligned."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+
+
 class AddNorm(torch.autograd.Function):
     """apply(x, d or None, weight, eps, dtype) -> (x + d, RMSNorm(x + d) in the GEMM dtype); the norm's
     weight is frozen."""
 
     @staticmethod
     def forward(ctx, x, d, weight, eps, dtype):
+        x, d = _rows2(x), None if d is None else _rows2(d)
         y, rstd = kernels.add_rmsnorm(x, weight, eps, d=d, dtype=dtype)
         ctx.save_for_backward(x, d, weight, rstd)
         ctx.dtype = dtype
@@ -33,8 +39,7 @@ class AddNorm(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dres, dy):
         x, d, weight, rstd = ctx.saved_tensors
-        dx = kernels.rmsnorm_bwd(x, weight, rstd, dy=dy.contiguous(), d=d, dres=dres.contiguous(),
-                                 dtype=ctx.dtype)
+        dx = kernels.rmsnorm_bwd(x, weight, rstd, dy=_rows2(dy), d=d, dres=_rows2(dres), dtype=ctx.dtype)
         return dx, None if d is None else dx.to(d.dtype), None, None, None
 
 

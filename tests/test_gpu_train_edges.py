@@ -6,11 +6,21 @@ import copy
 import pytest
 import torch
 
-from tests.gpu_util import banner, random_weight
+from tests import train_ref as ref
+from tests.gpu_util import banner, oracle_w16, random_weight
+from tests.test_gpu_attention import make, run
+from tests.test_gpu_train import tables
 
 pytestmark = pytest.mark.gpu
 
 F16, BF16 = torch.float16, torch.bfloat16
+
+
+def offset(t):
+    """t's values in a contiguous tensor whose start is not 16-byte aligned."""
+    flat = torch.empty(t.numel() + 1, dtype=t.dtype, device=t.device)
+    flat[1:] = t.detach().reshape(-1)
+    return flat[1:].view(t.shape)
 
 
 # ------------------------------------------------------------------ a spec that changes
@@ -62,6 +72,123 @@ def test_a_spec_changed_before_the_backward_pass(cuda, change):
 
 # -------------------------------------------------------------- views at any address
 
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("which", ["q", "k", "v", "dout"])
+def test_attention_of_an_offset_view(cuda, dtype, which):
+    from solution.layer import attention
+
+    q, k, v, dout, cu = make(cuda, dtype, 4, 2, 64, (70, 9), seed=80, layout="plain")
+    c = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    want = run(q, k, v, dout, cu)
+    args = {"q": q, "k": k, "v": v, "dout": dout}
+    args[which] = offset(args[which])
+    assert args[which].data_ptr() % 16 and args[which].is_contiguous()
+    leaves = [args[n].requires_grad_() for n in "qkv"]
+    out = attention(*leaves, c)
+    out.backward(args["dout"])
+    assert torch.equal(out, want["out"])
+    assert all(torch.equal(t.grad, want["d" + n]) for n, t in zip("qkv", leaves))
+
+
+def test_attention_of_rows_far_apart(cuda):
+    """More elements between two tokens than the kernels take."""
+    from solution.layer import attention, rope_attention
+
+    q, k, v, dout, cu = make(cuda, BF16, 4, 2, 64, (3,), seed=81, layout="plain")
+    want = run(q, k, v, dout, cu)
+    far = (1 << 23) + 8
+    big = torch.zeros(2 * far + 4 * 64, dtype=BF16, device=cuda)
+
+    def place(t):
+        x = torch.as_strided(big, t.shape, (far, 64, 1) if t.dim() == 3 else (far, 1))
+        x.copy_(t)
+        return x
+
+    for i in range(3):
+        leaves = [t.clone() for t in (q, k, v)]
+        leaves[i] = place(leaves[i])
+        for t in leaves:
+            t.requires_grad_()
+        out = attention(*leaves)
+        out.backward(dout)
+        assert torch.equal(out, want["out"])
+        assert all(torch.equal(t.grad, want["d" + n]) for n, t in zip("qkv", leaves))
+    assert torch.equal(attention(q, k, v.requires_grad_()), want["out"])
+    v.grad = None
+    attention(q, k, v).backward(place(dout))
+    assert torch.equal(v.grad, want["dv"])
+    cos, sin = tables([0, 1, 2], 64, cuda)
+    qkv = torch.cat([t.detach().flatten(1) for t in (q, k[:, :1], v[:, :1])], 1)  # 4 heads over 1
+    a, b = qkv.clone().requires_grad_(), torch.as_strided(torch.zeros(2 * far + 384, dtype=BF16, device=cuda), (3, 384), (far, 1))
+    b.copy_(qkv)
+    b.requires_grad_()
+    for t in (a, b):
+        rope_attention(t, cos, sin, 4, 1).backward(dout)
+    assert torch.equal(a.grad, b.grad)
+
+
+def test_rope_attention_of_an_offset_view(cuda):
+    from solution.layer import rope_attention
+
+    g = torch.Generator().manual_seed(82)
+    qkv = torch.randn(50, 8 * 64, generator=g).half().to(cuda)
+    dout = torch.randn(50, 4, 64, generator=g).half().to(cuda)
+    cos, sin = tables(range(50), 64, cuda)
+    a, b = qkv.clone().requires_grad_(), offset(qkv).requires_grad_()
+    ya, yb = (rope_attention(t, cos, sin, 4, 2) for t in (a, b))
+    ya.backward(dout)
+    yb.backward(offset(dout))
+    assert torch.equal(ya, yb) and torch.equal(a.grad, b.grad)
+
+
+@pytest.mark.parametrize("m", [1, 40, 200])
+def test_projection_of_offset_views(cuda, m):
+    """x, dY and adapters in the GEMM dtype that start anywhere; segments whose columns do."""
+    from solution.layer import LoraAdapter, ProjectionSpec, project
+
+    segs = [random_weight(n, 128, seed=83 + i, dev=cuda) for i, n in enumerate((64, 128))]
+    g = torch.Generator().manual_seed(84)
+    rnd = lambda *s: torch.randn(*s, generator=g).half().to(cuda)  # noqa: E731
+    x, dy = rnd(m, 128), rnd(m, 192)
+    params = [rnd(8, 128), rnd(64, 8), rnd(8, 128), rnd(128, 8)]
+    spec = ProjectionSpec(segs, [LoraAdapter(0, 2.0, dropout=0.3, site=1), LoraAdapter(1, 1.0)],
+                          torch.tensor([9, 4], device=cuda))
+    got = []
+    for place in (torch.clone, offset):
+        leaves = [place(t).requires_grad_() for t in (x, *params)]
+        y = project(leaves[0], spec, None, leaves[1:])
+        y.backward(place(dy))
+        got.append([y] + [t.grad for t in leaves])
+    assert all(torch.equal(a, b) for a, b in zip(got[0][1:], got[1][1:]))
+    # y: an adapter's B that is not 16-byte aligned may be summed in another order, each sum in fp32 and
+    # rounded once.  A sum of n terms is off by n half steps of fp32 of what its terms' sizes add up to, and
+    # the two results by half a step of fp16 each: |dy| <= 2 (2^-11 |y| + (128 + 8 + 2) 2^-24 size + 2^-25),
+    # with t of at most its terms' sizes (1.01: its own rounding), scaled by the share kept.
+    size = []
+    for (w, qs), ad, a, b in zip(segs, spec.loras, params[::2], params[1::2]):
+        t = 1.01 * ref.drop_scale(ad.dropout) * (x.double().abs() @ a.double().abs().t())
+        w16 = oracle_w16(w, qs).double().to(cuda)
+        size.append(x.double().abs() @ w16.abs().t() + ad.scale * t @ b.double().abs().t())
+    bound = 2 * (ref.HALF[F16] * got[0][0].double().abs() + 138 * ref.U32 * torch.cat(size, 1) + ref.TINY[F16])
+    assert ((got[0][0].double() - got[1][0].double()).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("m", [20, 100])
+def test_mlp_of_offset_views(cuda, m):
+    from solution.mlp import RecomputedMLP
+
+    w = [random_weight(*s, seed=85 + i, dev=cuda) for i, s in enumerate(((256, 128), (256, 128), (128, 256)))]
+    g = torch.Generator().manual_seed(86)
+    x, dy = (torch.randn(m, 128, generator=g).half().to(cuda) for _ in range(2))
+    got = []
+    for place in (torch.clone, offset):
+        leaf = place(x).requires_grad_()
+        y = RecomputedMLP.apply(leaf, *w[0], *w[1], *w[2])
+        y.backward(place(dy))
+        got.append((y, leaf.grad))
+    assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
 @pytest.mark.parametrize("m", [20, 100])
 def test_mlp_of_expanded_and_strided_tensors(cuda, m):
     """The gradient of a sum (one value, expanded), and every second column of a wider tensor."""
@@ -77,3 +204,34 @@ def test_mlp_of_expanded_and_strided_tensors(cuda, m):
         y.backward(one.contiguous() if dense else one)
         got.append((y, leaf.grad))
     assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def small_layer(dev, dropout=0.0):
+    from solution.train import TrainLayer
+
+    names = {"q": (128, 128), "k": (64, 128), "v": (64, 128), "o": (128, 128), "gate": (256, 128),
+             "up": (256, 128), "down": (128, 256)}
+    w = {n: random_weight(*s, seed=90 + i, dev=dev, std=0.06) for i, (n, s) in enumerate(names.items())}
+    g = torch.Generator().manual_seed(91)
+    lora = [(0.06 * torch.randn(*s, generator=g)).to(dev).requires_grad_()
+            for s in ((8, 128), (128, 8), (8, 128), (64, 8))]
+    one = torch.ones(128, device=dev)
+    return TrainLayer(w, one, one, 2, 1, lora, dropout=dropout, index=3), lora
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, torch.float32])
+def test_train_layer_of_offset_views(cuda, dtype):
+    layer, lora = small_layer(cuda, 0.2)
+    g = torch.Generator().manual_seed(92)
+    x, dy = (torch.randn(30, 128, generator=g).to(dtype).to(cuda) for _ in range(2))
+    cos, sin = tables(range(30), 64, cuda)
+    seed = torch.tensor([3, 1], device=cuda)
+    got = []
+    for place in (torch.clone, offset):
+        leaf = place(x).requires_grad_()
+        for t in lora:
+            t.grad = None
+        y = layer.forward(leaf, cos, sin, seed=seed)
+        y.backward(place(dy))
+        got.append([y, leaf.grad] + [t.grad for t in lora])
+    assert all(torch.equal(a, b) for a, b in zip(*got))
