@@ -374,7 +374,7 @@ class RopeAttention(torch.autograd.Function):
         dqkv = torch.empty((tokens, both + v.shape[1], dim), dtype=qk.dtype, device=qk.device)
         kernels.attention_bwd(_rows3(dout), qk[:, :n_heads], qk[:, n_heads:], v, out, stats, cu, *how,
                               grads=(dqkv[:, :n_heads], dqkv[:, n_heads:both], dqkv[:, both:]))
-        dqkv = dqkv.view(tokens, -1)
+        dqkv = dqkv.flatten(1)
         kernels.rope(dqkv, cos, sin, both, dim, inverse=True, out=dqkv)
         return dqkv, *[None] * 8
 

@@ -235,3 +235,21 @@ def test_train_layer_of_offset_views(cuda, dtype):
         y.backward(place(dy))
         got.append([y, leaf.grad] + [t.grad for t in lora])
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+# ----------------------------------------------------------------- nothing, and twice
+
+def test_no_tokens(cuda):
+    """An empty batch has empty results and gradients."""
+    from solution.layer import attention, rope_attention
+
+    for cu in (None, torch.zeros(1, dtype=torch.int32, device=cuda), torch.zeros(3, dtype=torch.int32, device=cuda)):
+        q, k, v = (torch.empty(0, h, 64, dtype=F16, device=cuda, requires_grad=True) for h in (4, 2, 2))
+        out = attention(q, k, v, cu)
+        out.backward(torch.empty_like(out))
+        assert out.shape == q.grad.shape == (0, 4, 64) and k.grad.shape == v.grad.shape == (0, 2, 64)
+        qkv = torch.empty(0, 8 * 64, dtype=F16, device=cuda, requires_grad=True)
+        table = torch.empty(0, 64, device=cuda)
+        out = rope_attention(qkv, table, table, 4, 2, cu)
+        out.backward(torch.empty_like(out))
+        assert out.shape == (0, 4, 64) and qkv.grad.shape == (0, 512)
