@@ -235,6 +235,7 @@ class NF4Projection(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         x, seed, *saved = ctx.saved_tensors
         spec = ctx.spec

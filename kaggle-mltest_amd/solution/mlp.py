@@ -22,6 +22,7 @@ GEMM dtype, as the reference's recomputing layers do (layer.py:986-990).
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib, kernels
 from .layer import _aligned_rows
@@ -67,6 +68,7 @@ class RecomputedMLP(torch.autograd.Function):
         return out.view(*shape[:-1], out.shape[-1])
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad):
         x2, gate_w, up_w, down_w = ctx.saved_tensors
         gate_qs, up_qs, down_qs = ctx.qs

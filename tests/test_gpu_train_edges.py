@@ -253,3 +253,23 @@ def test_no_tokens(cuda):
         out = rope_attention(qkv, table, table, 4, 2, cu)
         out.backward(torch.empty_like(out))
         assert out.shape == (0, 4, 64) and qkv.grad.shape == (0, 512)
+
+
+def test_second_derivatives_of_projection_and_mlp_raise(cuda):
+    """A penalty on their gradients has no derivative here: it raises rather than being left out."""
+    from solution.layer import LoraAdapter, ProjectionSpec, project
+    from solution.mlp import RecomputedMLP
+
+    w = [random_weight(*s, seed=95 + i, dev=cuda) for i, s in enumerate(((256, 128), (256, 128), (128, 256)))]
+    x = torch.randn(20, 128, device=cuda).half().requires_grad_()
+    a, b = torch.randn(8, 128, device=cuda).requires_grad_(), torch.randn(256, 8, device=cuda).requires_grad_()
+    seed = torch.tensor([1, 1], device=cuda)
+    for ad in (LoraAdapter(0, 1.0, dropout=0.5), LoraAdapter(0, 1.0)):
+        y = project(x, ProjectionSpec(w[:1], [ad], seed), None, (a, b))
+        for g in torch.autograd.grad(y.float().square().sum(), (x, a, b), create_graph=True):
+            with pytest.raises(RuntimeError, match="once_differentiable"):
+                g.float().square().sum().backward(retain_graph=True)
+    y = RecomputedMLP.apply(x, *w[0], *w[1], *w[2])
+    g, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.float().square().sum().backward()
