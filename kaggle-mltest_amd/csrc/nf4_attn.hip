@@ -646,7 +646,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     else if (nan) fill_of(acc, NAN);
     const bool f = fabsf(m) > kFar;
     float2 ml = make_float2(f ? m : m + kTop<DT>, f ? sum : __builtin_amdgcn_ldexpf(sum, -static_cast<int>(kTop<DT>)));
-    if (nan) ml.y = none ? 0.f : NAN;
+    if (nan) ml = none ? make_float2(m, 0.f) : make_float2(NAN, NAN);
     if (!some) ml = make_float2(0.f, 0.f);
     const bool mine_now = r < a.tokens && !(again >> n & 1);
     if (pieces > 1) {
@@ -704,7 +704,7 @@ __global__ __launch_bounds__(256) void attn_fwd_join_kernel(const Attn a, const 
         }
         if (l == 0.f && all_low) l = NAN;
         if (threadIdx.x < 32)
-            a.stats[static_cast<int64_t>(r) * a.n_heads + head] = l == 0.f ? make_float2(0.f, 0.f) : make_float2(m, l);
+            a.stats[static_cast<int64_t>(r) * a.n_heads + head] = l == 0.f ? make_float2(0.f, 0.f) : make_float2(l == l ? m : NAN, l);
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     float4_t o[D / 32];

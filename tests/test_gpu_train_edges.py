@@ -2,6 +2,8 @@
 address, empty batches, second derivatives, values that are not finite in a split launch."""
 
 import copy
+import ctypes
+import math
 
 import pytest
 import torch
@@ -273,3 +275,49 @@ def test_second_derivatives_of_projection_and_mlp_raise(cuda):
     g, = torch.autograd.grad(y.float().square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         g.float().square().sum().backward()
+
+
+# -------------------------------------------------------- launches of either kind
+
+def workspaces(q, k, v, max_len=0, window=0):
+    """(forward's, backward's) bytes: more of them where the work is in pieces or shares."""
+    from solution import _lib, kernels
+
+    c = torch.zeros(2, dtype=torch.int32, device=q.device)
+    d = ctypes.byref(kernels._attn_desc(q, k, v, c, None, window, max_len))
+    lib = _lib.load()
+    return lib.nf4_attn_fwd_workspace(d), lib.nf4_attn_bwd_workspace(d)
+
+
+def split(dev, dtype, seed):
+    """A forward pass whose tiles are in several pieces."""
+    q, k, v, dout, cu = make(dev, dtype, 4, 2, 64, (900,), seed=seed, layout="plain")
+    assert workspaces(q, k, v)[0] >= 8 * 4 * 3 * 128 * 264  # 8 tiles of 4 heads, 3 pieces at least
+    return q, k, v, dout, cu
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("pieces", [False, True])
+@pytest.mark.parametrize("value", [math.inf, math.nan, -math.inf])
+def test_statistics_of_scores_that_are_not_finite(cuda, dtype, pieces, value):
+    """A row that sees a score of NaN or +inf, or of -inf only, has NaN for its output and both statistics."""
+    banner("statistics", dtype, pieces, value)
+    if pieces:
+        q, k, v, dout, cu = split(cuda, dtype, 103)
+    else:
+        q, k, v, dout, cu = make(cuda, dtype, 4, 2, 64, (100,), seed=103, layout="plain")
+        assert workspaces(q, k, v)[0] == 0
+    n = q.shape[0]
+    q[:, :, 0], k[:, :, 0] = 1.0, 0.0
+    want = ref.attention(q, k, v, cu)
+    lo, hi = (0, 30) if value == -math.inf else (n - 30, n)  # the rows that are NaN
+    at = range(30) if value == -math.inf else [n - 30]
+    for i in at:
+        k[i, :, 0] = value
+    got = run(q, k, v, dout, cu)
+    assert torch.isnan(got["out"][lo:hi]).all() and torch.isnan(got["stats"][lo:hi]).all()
+    if value != -math.inf:
+        for name in ("out", "stats"):
+            ref.assert_within(got[name][:lo], tuple(t[:lo] for t in want[name]), name)
+    else:
+        assert not torch.isnan(got["out"][hi:]).any() and not torch.isnan(got["stats"][hi:]).any()
