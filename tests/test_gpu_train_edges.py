@@ -10,7 +10,7 @@ import torch
 
 from tests import train_ref as ref
 from tests.gpu_util import banner, oracle_w16, random_weight
-from tests.test_gpu_attention import make, run
+from tests.test_gpu_attention import check, make, run
 from tests.test_gpu_train import tables
 
 pytestmark = pytest.mark.gpu
@@ -289,11 +289,62 @@ def workspaces(q, k, v, max_len=0, window=0):
     return lib.nf4_attn_fwd_workspace(d), lib.nf4_attn_bwd_workspace(d)
 
 
+@pytest.mark.parametrize("dtype,dim", [(BF16, 64), (F16, 64), (BF16, 128)])
+def test_a_workgroup_a_tile_and_shares(cuda, dtype, dim):
+    """`max_len` below the longest sequence: a workgroup takes a tile of any length; as it is: shares."""
+    q, k, v, dout, cu = make(cuda, dtype, 16, 16, dim, (1100, 64, 964), seed=100)
+    tiles, shares = (workspaces(q, k, v, n)[1] for n in (64, 2000))
+    assert shares > tiles + (20 << 20)  # (2 * 16 slots a head of 64 KB and more, at the least)
+    want = ref.attention(q, k, v, cu, dout)
+    for n in (64, 2000):
+        got = run(q, k, v, dout, cu, max_len=n)
+        for name in got:
+            ref.assert_within(got[name], want[name], (name, n))
+
+
 def split(dev, dtype, seed):
     """A forward pass whose tiles are in several pieces."""
     q, k, v, dout, cu = make(dev, dtype, 4, 2, 64, (900,), seed=seed, layout="plain")
     assert workspaces(q, k, v)[0] >= 8 * 4 * 3 * 128 * 264  # 8 tiles of 4 heads, 3 pieces at least
     return q, k, v, dout, cu
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("at", [3, 500, 800])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_values_that_are_not_finite_in_pieces(cuda, dtype, at, value):
+    """A value of v that is not finite is in one channel of the rows that see it, and in nothing else."""
+    banner("pieces", dtype, at, value)
+    q, k, v, dout, cu = split(cuda, dtype, 101)
+    want = ref.attention(q, k, v, cu, dout)
+    v[at, 1, 5] = value  # of heads 2 and 3
+    got = run(q, k, v, dout, cu)
+    touched = torch.zeros(900, 4, 64, dtype=torch.bool)
+    touched[at:, 2:, 5] = True
+    there = got["out"].cpu()[touched].float()
+    assert torch.isnan(there).all() if math.isnan(value) else (there == value).all()
+    ref.assert_within(got["out"].cpu()[~touched], tuple(t[~touched] for t in want["out"]), "out")
+    ref.assert_within(got["stats"], want["stats"], "stats")
+    ref.assert_within(got["dq"][:at], tuple(t[:at] for t in want["dq"]), "dq")
+    for name in ("dk", "dv"):
+        ref.assert_within(got[name][:, 0], tuple(t[:, 0] for t in want[name]), name)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+def test_keys_of_no_weight_in_pieces(cuda, dtype):
+    """The first 300 keys have scores of -inf: rows before 300 are NaN, the others those of a sequence that
+    begins there, though their first pieces saw nothing else."""
+    q, k, v, dout, cu = split(cuda, dtype, 102)
+    q[:, :, 0], k[:, :, 0] = 1.0, 0.0
+    want = ref.attention(q[300:], k[300:], v[300:], [0, 600], dout[300:])
+    k[:300, :, 0] = -math.inf
+    got = run(q, k, v, dout, cu)
+    for name in ("out", "dk", "dv"):
+        ref.assert_within(got[name][300:], want[name], name)
+        assert torch.isnan(got[name][:300]).all()
+    ref.assert_within(got["stats"][300:], want["stats"], "stats")
+    ref.assert_within(got["dq"][300:, :, 1:], tuple(t[..., 1:] for t in want["dq"]), "dq")
+    assert torch.isnan(got["dq"][:300]).all()
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16])
@@ -321,3 +372,19 @@ def test_statistics_of_scores_that_are_not_finite(cuda, dtype, pieces, value):
             ref.assert_within(got[name][:lo], tuple(t[:lo] for t in want[name]), name)
     else:
         assert not torch.isnan(got["out"][hi:]).any() and not torch.isnan(got["stats"][hi:]).any()
+
+
+def test_the_generators_published_output(cuda):
+    """Philox4x32-10 of counter and key 0 is 6627e8d5 e169c58d bc57ac4c 9b00dbd8: an element is kept up to its
+    own number, and no further."""
+    from solution import kernels
+
+    numbers = [0xe8d5, 0x6627, 0xc58d, 0xe169, 0xac4c, 0xbc57, 0xdbd8, 0x9b00]
+    x = torch.ones(1, 8, dtype=F16, device=cuda)
+    seed = torch.zeros(2, dtype=torch.int64, device=cuda)
+    for n in numbers:
+        for cut in (n, n + 1):
+            (y,) = kernels.dropout(x, cut / 65536, seed, [0])
+            assert [bool(t) for t in y[0]] == [u >= cut for u in numbers]
+            dx = kernels.dropout_bwd([x], cut / 65536, seed, [0])
+            assert torch.equal(dx, y)

@@ -1,9 +1,12 @@
-"""How the training operators' calls find their tensors' device, and what they refuse (no GPU needed)."""
+"""How the training operators' calls find their tensors' device, what they refuse and what they hand on,
+and the generator's published outputs (no GPU needed)."""
 
 import contextlib
 
 import pytest
 import torch
+
+from tests import train_ref as ref
 
 
 class Tensor:
@@ -100,3 +103,15 @@ def test_the_mlp_hands_on_rows(monkeypatch):
         for grad in (torch.ones((), dtype=torch.half).expand(rows, 128), wide):
             with pytest.raises(Stop):
                 mlp.RecomputedMLP.backward(Ctx(), grad)
+
+
+@pytest.mark.parametrize("counter,key,words", [
+    ((0, 0, 0, 0), (0, 0), (0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8)),
+    ((0xffffffff,) * 4, (0xffffffff,) * 2, (0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd)),
+    ((0x243f6a88, 0x85a308d3, 0x13198a2e, 0x03707344), (0xa4093822, 0x299f31d0),
+     (0xd16cfe09, 0x94fdcceb, 0x5001e420, 0x24126ea1)),
+])
+def test_the_generators_published_outputs(counter, key, words):
+    """Philox4x32-10's known answers, against which the tests' own definition stands."""
+    got = ref.philox(key[0] | key[1] << 32, counter[2], counter[3], [counter[0] | counter[1] << 32])
+    assert got[0].tolist() == [w >> s & 0xffff for w in words for s in (0, 16)]
