@@ -136,17 +136,22 @@ __device__ __forceinline__ float lane_value(float v, int l) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
 }
 
-// acc += f * this lane's channels of a row
+// this lane's channels of a row (one in the low half, where it holds one)
+template <int D>
+__device__ __forceinline__ uint32_t channels_of(const uint16_t *row) {
+    const int l = thread_here() & 63;
+    if constexpr (D == 128) return *reinterpret_cast<const uint32_t *>(row + 2 * l);
+    else return row[l];
+}
+// acc += f * them
+template <int DT, int D>
+__device__ __forceinline__ void add_channels(float (&acc)[D / 64], float f, uint32_t w) {
+    acc[0] = fmaf(f, f32_of<DT>(w & 0xffffu), acc[0]);
+    if constexpr (D == 128) acc[1] = fmaf(f, f32_of<DT>(w >> 16), acc[1]);
+}
 template <int DT, int D>
 __device__ __forceinline__ void add_row(float (&acc)[D / 64], float f, const uint16_t *row) {
-    const int l = thread_here() & 63;
-    if constexpr (D == 128) {
-        const uint32_t w = *reinterpret_cast<const uint32_t *>(row + 2 * l);
-        acc[0] = fmaf(f, f32_of<DT>(w & 0xffffu), acc[0]);
-        acc[1] = fmaf(f, f32_of<DT>(w >> 16), acc[1]);
-    } else {
-        acc[0] = fmaf(f, f32_of<DT>(row[l]), acc[0]);
-    }
+    add_channels<DT, D>(acc, f, channels_of<D>(row));
 }
 
 template <int DT, int D>
@@ -163,28 +168,29 @@ __device__ __forceinline__ float wave_max(float v) {
     return v;
 }
 
-// (m, l) of row r over keys [k0, k1), and acc = sum 2^(t - m) v
+// acc = sum over keys [k0, k1) of 2^(t - m) v, of row r whose largest t is m; rows of v are asked for some
+// at a time
+constexpr int kAtOnce = 16;
 template <int DT, int D>
-__device__ __forceinline__ void row_forward(const Attn &a, int head, int r, int k0, int k1, float &m,
-                                            float &l, float (&acc)[D / 64]) {
+__device__ __forceinline__ void row_forward(const Attn &a, int head, int r, int k0, int k1, float m,
+                                            float (&acc)[D / 64]) {
     const int lane = thread_here() & 63, kvh = head / a.group;
     const uint16_t *q = a.q.at(r, head);
-    m = -INFINITY;
-    for (int k = k0; k < k1; k += 64)
-        if (k + lane < k1) m = fmaxf(m, dot_of<DT, D>(q, a.k.at(k + lane, kvh)) * a.c);
-    m = wave_max(m);
-    l = 0.f;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) acc[i] = 0.f;
     for (int k = k0; k < k1; k += 64) {
         float p = 0.f;
         if (k + lane < k1)
             p = __builtin_amdgcn_exp2f(exponent(dot_of<DT, D>(q, a.k.at(k + lane, kvh)), a.c, m));
-        l += p;
         const int n = k1 - k < 64 ? k1 - k : 64;
-        for (int i = 0; i < n; ++i) add_row<DT, D>(acc, lane_value(p, i), a.v.at(k + i, kvh));
+        for (int i = 0; i < n; i += kAtOnce) {
+            uint32_t w[kAtOnce];
+#pragma unroll
+            for (int u = 0; u < kAtOnce; ++u) w[u] = channels_of<D>(a.v.at(k + (i + u < n ? i + u : n - 1), kvh));
+#pragma unroll
+            for (int u = 0; u < kAtOnce && i + u < n; ++u) add_channels<DT, D>(acc, lane_value(p, i + u), w[u]);
+        }
     }
-    l = wave_sum(l);
 }
 
 // acc = sum over keys [k0, k1) of dS k
@@ -407,6 +413,45 @@ __device__ __forceinline__ void fill_of(float16_t (&v)[N], float f) {
     for (int x = 0; x < N; ++x)
 #pragma unroll
         for (int e = 0; e < 16; ++e) v[x][e] = f;
+}
+
+// Which of a wave's rows (bits) see a NaN of v, for each of a lane's channels D / 64 l ..: such a row's
+// sum in that channel is NaN.  `seen`: the keys of this lane's row; all rows' lie in [lo, hi).  One pass over v
+// for the 32 rows; formed again one by one, all rows behind an early NaN made the forward pass 110 times as long
+// at 2048 tokens, 280 times at 4096.
+template <int DT, int D>
+__device__ __forceinline__ void nan_values(const Attn &a, int kvh, int lo, int hi, int2 seen, uint32_t (&by)[D / 64]) {
+    constexpr uint32_t INF = DT == NF4_BF16 ? 0x7f80u : 0x7c00u;
+#pragma unroll
+    for (int i = 0; i < D / 64; ++i) by[i] = 0;
+    for (int k = lo; k < hi; k += kAtOnce) {
+        uint32_t w[kAtOnce];
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) w[u] = channels_of<D>(a.v.at(k + u < hi ? k + u : hi - 1, kvh));
+#pragma unroll
+        for (int u = 0; u < kAtOnce; ++u) {
+            const bool x = (w[u] & 0x7fffu) > INF, y = D == 128 && (w[u] >> 16 & 0x7fffu) > INF;
+            if (!__any(x || y)) continue;
+            const uint32_t rows = rows_where(seen.x <= k + u && k + u < seen.y);
+            if (x) by[0] |= rows;
+            if (y) by[D / 64 - 1] |= rows;
+        }
+    }
+}
+// A NaN of this lane's row in a channel for which `by` does not name the row.
+template <int D>
+__device__ __forceinline__ bool unexplained(const float16_t (&v)[D / 32], const uint32_t (&by)[D / 64]) {
+    const int l = thread_here() & 63;
+    bool z = false;
+#pragma unroll
+    for (int x = 0; x < D / 32; ++x)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const int c = x * 32 + 8 * (e >> 2) + 4 * (l >> 5) + (e & 3);  // (c and e are odd together)
+            const uint32_t rows = __shfl(by[e % (D / 64)], c / (D / 64));
+            z |= v[x][e] != v[x][e] && !(rows >> (l & 31) & 1);
+        }
+    return z;
 }
 
 // This lane's channels of its row, from a transposed result.
@@ -639,7 +684,12 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     const int64_t slot = ((static_cast<int64_t>(tile) * a.n_heads + head) * pc.most + piece) * kOwn + w * 32;
     const bool nan = some && !(sum > 0.f && fabsf(m) < INFINITY);  // a score is NaN or +inf, or all are -inf
     const bool none = nan && pieces > 1 && m == -INFINITY && sum == 0.f;  // (here: other pieces may have more)
-    const uint32_t again = rows_where(some && !nan && any_nan(acc));
+    uint32_t again = rows_where(some && !nan && any_nan(acc));
+    if (again) {  // but for what a NaN of v explains
+        uint32_t by[D / 64];
+        nan_values<DT, D>(a, kvh, sp.lo > first ? sp.lo : first, sp.hi < all.y ? sp.hi : all.y, part, by);
+        again &= rows_where(unexplained<D>(acc, by));
+    }
     // a row that sees nothing has zeros (its registers hold anything: no mask kept tiles from it that every
     // other row of its wave sees whole)
     if (!some || none) fill_of(acc, 0.f);
@@ -649,6 +699,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     if (nan) ml = none ? make_float2(m, 0.f) : make_float2(NAN, NAN);
     if (!some) ml = make_float2(0.f, 0.f);
     const bool mine_now = r < a.tokens && !(again >> n & 1);
+    if (pieces == 1 && r < a.tokens && g == 0) a.stats[static_cast<int64_t>(r) * a.n_heads + head] = ml;
     if (pieces > 1) {
         if (!f && some)
 #pragma unroll
@@ -659,24 +710,23 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
         const float inv = some ? 1.f / sum : 0.f;
         keep_finite<DT>(acc, inv);
         store_own<DT, D>(a.o.to(r, head), acc, DT == NF4_F16 ? 1.f : inv);
-        if (g == 0) a.stats[static_cast<int64_t>(r) * a.n_heads + head] = ml;
     }
     if (!again) return;
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (parts are there before their rows are written again)
 #pragma unroll 1
     for (uint32_t left = again; left; left &= left - 1) {
         const int i = __builtin_ctz(left), row = tile * kOwn + w * 32 + i;
-        float o[D / 64], rm, rl;
-        row_forward<DT, D>(a, head, row, __builtin_amdgcn_readlane(part.x, i), __builtin_amdgcn_readlane(part.y, i), rm, rl, o);
+        float o[D / 64];
+        row_forward<DT, D>(a, head, row, __builtin_amdgcn_readlane(part.x, i), __builtin_amdgcn_readlane(part.y, i),
+                           lane_value(ml.x, i), o);
         if (pieces > 1) {
             store_part_row<D>(pc.part + slot * D, i, o);
-            if (l == 0) pc.ml[slot + i] = make_float2(rm, rl);
             continue;
         }
+        const float rl = lane_value(ml.y, i);
 #pragma unroll
         for (int x = 0; x < D / 64; ++x) o[x] /= rl;
         store_row<DT, D>(a.o.to(row, head), o);
-        if (l == 0) a.stats[static_cast<int64_t>(row) * a.n_heads + head] = make_float2(rm, rl);
     }
 }
 

@@ -388,3 +388,60 @@ def test_the_generators_published_output(cuda):
             assert [bool(t) for t in y[0]] == [u >= cut for u in numbers]
             dx = kernels.dropout_bwd([x], cut / 65536, seed, [0])
             assert torch.equal(dx, y)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,lens,window,max_len", [
+    (64, (300,), 0, 300), (128, (300, 7, 130), 0, 300), (64, (400, 90), 70, 400), (128, (700,), 33, 700),
+    (128, (900, 60), 0, 900),
+])
+def test_values_that_are_not_finite_by_channel(cuda, dtype, dim, lens, window, max_len):
+    """NaN and infinities here and there in v: NaN in the channels and rows that see a NaN, an infinity in those
+    that see one and no NaN, and everything else as it is without them."""
+    banner("channels", dtype, dim, lens, window)
+    q, k, v, dout, cu = make(cuda, dtype, 4, 2, dim, lens, pad=5, seed=104, layout="plain")
+    want = ref.attention(q, k, v, cu, window=window)
+    n, g = sum(lens), torch.Generator().manual_seed(105)
+    nan, inf = (torch.zeros(n + 5, 2, dim, dtype=torch.bool) for _ in range(2))
+    for at in (2, 100, 129, 255, n - 3):
+        nan[at, at % 2, torch.randint(dim, (2,), generator=g)] = True
+    for at in (50, 140, n - 20):
+        inf[at, :, torch.randint(dim, (1,), generator=g)] = True
+    inf &= ~nan
+    v[nan.to(cuda)], v[inf.to(cuda)] = math.nan, math.inf
+    from solution import kernels
+
+    c = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    out, stats = (t.cpu() for t in kernels.attention_fwd(q, k, v, c, window=window, max_len=max_len))
+    sees = torch.zeros(n + 5, n + 5, dtype=torch.float64)
+    for a, b in zip(cu, cu[1:]):
+        sees[a:b, a:b] = (~ref.hidden(b - a, window)).double()
+    sees_nan, sees_inf = (((sees @ t.double().flatten(1)) > 0).view(-1, 2, dim).repeat_interleave(2, 1) for t in (nan, inf))
+    assert torch.equal(torch.isnan(out), sees_nan)
+    assert torch.equal(torch.isinf(out), sees_inf & ~sees_nan)
+    rest = ~(sees_nan | sees_inf)
+    ref.assert_within(out[rest], tuple(t[rest] for t in want["out"]), "out")
+    ref.assert_within(stats, want["stats"], "stats")
+
+
+def test_an_early_nan_of_v_costs_little(cuda):
+    """One pass over v says which rows see it: twice the time of finite values (formed again row by row, all
+    rows behind it took 110 times as long)."""
+    from solution import kernels
+
+    q, k, v, dout, cu = make(cuda, BF16, 12, 2, 128, (2048,), seed=106, layout="plain")
+
+    def us(v):
+        times = []
+        for _ in range(6):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            kernels.attention_fwd(q, k, v)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b) * 1e3)
+        return sorted(times)[2]
+
+    clean = us(v)
+    v[3, 0, 5] = math.nan
+    assert us(v) < 20 * clean + 100
