@@ -445,3 +445,83 @@ def test_an_early_nan_of_v_costs_little(cuda):
     clean = us(v)
     v[3, 0, 5] = math.nan
     assert us(v) < 20 * clean + 100
+
+
+# ------------------------------------------------------------- a layer's step, as it is used
+
+def test_a_captured_step_that_adds_to_its_seed(cuda):
+    """A layer's forward and backward pass and the step's increment in one graph: every replay has the next
+    step's masks, and what the eager calls give with that seed."""
+    layer, lora = small_layer(cuda, 0.3)
+    g = torch.Generator(device=cuda).manual_seed(110)
+    new = lambda *s: torch.randn(*s, generator=g, device=cuda)  # noqa: E731
+    x, dy = new(50, 128).half().requires_grad_(), new(50, 128).half()
+    cos, sin = tables([*range(30), *range(20)], 64, cuda)
+    cu = torch.tensor([0, 30, 50], dtype=torch.int32, device=cuda)
+    seed = torch.tensor([9, 4], device=cuda)
+
+    def step(seed):
+        y = layer.forward(x, cos, sin, cu, seed=seed)
+        return [y.detach(), *torch.autograd.grad(y, [x, *lora], dy)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(seed)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kept = step(seed)
+        seed[1] += 1
+    masks = set()
+    for i in range(4):
+        with torch.no_grad():
+            x.copy_(new(50, 128).half())
+        dy.copy_(new(50, 128).half())
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [t.clone() for t in kept]
+        assert seed.tolist() == [9, 5 + i]
+        want = step(torch.tensor([9, 4 + i], device=cuda))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+        masks.add(float(got[2].double().sum()))
+    assert len(masks) == 4
+
+
+def test_a_layer_whose_input_needs_no_gradient(cuda):
+    """The first layer behind frozen embeddings, and a second backward pass of the same graph: the adapters'
+    gradients are the same."""
+    layer, lora = small_layer(cuda, 0.2)
+    g = torch.Generator().manual_seed(111)
+    x, dy = (torch.randn(30, 128, generator=g).half().to(cuda) for _ in range(2))
+    cos, sin = tables(range(30), 64, cuda)
+    seed = torch.tensor([3, 1], device=cuda)
+    got = []
+    for leaf in (x.clone().requires_grad_(), x.clone()):
+        y = layer.forward(leaf, cos, sin, seed=seed)
+        for again in (True, False):
+            got.append(torch.autograd.grad(y, lora, dy, retain_graph=again))
+    for other in got[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(got[0], other))
+
+
+def test_two_adapters_of_one_site(cuda):
+    """Adapters that share a site have one mask."""
+    from solution.layer import LoraAdapter, ProjectionSpec, project
+
+    w = random_weight(64, 128, seed=112, dev=cuda)
+    g = torch.Generator().manual_seed(113)
+    x = torch.randn(20, 128, generator=g).half().to(cuda)
+    a, b = torch.randn(8, 128, generator=g).to(cuda), torch.randn(64, 8, generator=g).to(cuda)
+    seed = torch.tensor([2, 2], device=cuda)
+
+    def forward(*sites):
+        loras = [LoraAdapter(i, 1.0, dropout=0.4, site=s) for i, s in enumerate(sites)]
+        return project(x, ProjectionSpec([w] * len(sites), loras, seed), None, [a, b] * len(sites))
+
+    y = forward(7, 7)
+    assert torch.equal(y[:, :64], y[:, 64:])
+    y = forward(7, 8)
+    assert not torch.equal(y[:, :64], y[:, 64:])
