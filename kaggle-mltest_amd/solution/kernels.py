@@ -488,16 +488,17 @@ def qkv_rope_bwd(dq: torch.Tensor, dk: torch.Tensor, dv: torch.Tensor, cos: torc
 
 
 def _on_its_device(fn):
-    """Runs a call with the device of its first parameter (a tensor, or a list of them) as the current
-    one: launches go to the current device, and the handle of another's default stream is none of its
-    own.  Calls without such a tensor are refused by `fn` itself."""
-    first = next(iter(inspect.signature(fn).parameters))
+    """Runs a call (or method) with the device of its first parameter (a tensor, or a list of them) as the
+    current one: launches go to the current device, and the handle of another's default stream is none of
+    its own.  Calls without such a tensor are refused by `fn` itself."""
+    names = list(inspect.signature(fn).parameters)
+    at = int(names[0] == "self")
 
     @functools.wraps(fn)
     def call(*args, **kw):
         if _devices() < 2:
             return fn(*args, **kw)
-        t = args[0] if args else kw.get(first)
+        t = args[at] if len(args) > at else kw.get(names[at])
         if isinstance(t, (list, tuple)):
             t = t[0] if t else None
         if not getattr(t, "is_cuda", False) or t.get_device() == torch.cuda.current_device():

@@ -303,6 +303,7 @@ class NF4Projection(torch.autograd.Function):
         return (dx, dbias, None, *grads)
 
 
+@kernels._on_its_device
 def project(x, spec: ProjectionSpec, bias=None, lora_params=()):
     """Y = NF4Projection over a [..., K] input (the adapters' own inputs [..., K] too)."""
     shape = x.shape

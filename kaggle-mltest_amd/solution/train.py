@@ -62,6 +62,7 @@ class TrainLayer:
         self.loras = [LoraAdapter(seg, alpha / lora[2 * i].shape[0], dropout=dropout, site=2 * index + i)
                       for i, seg in enumerate((0, 2))]
 
+    @kernels._on_its_device
     def forward(self, x: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
                 cu_seqlens: torch.Tensor | None = None, max_len: int = 0,
                 seed: torch.Tensor | None = None, dtype=None) -> torch.Tensor:

@@ -27,8 +27,10 @@ def two_devices(monkeypatch):
     @contextlib.contextmanager
     def device(index):
         old, at[0] = at[0], index
-        yield
-        at[0] = old
+        try:
+            yield
+        finally:
+            at[0] = old
 
     monkeypatch.setattr(kernels, "_devices", lambda: 2)
     monkeypatch.setattr(torch.cuda, "current_device", lambda: at[0])
@@ -115,3 +117,39 @@ def test_the_generators_published_outputs(counter, key, words):
     """Philox4x32-10's known answers, against which the tests' own definition stands."""
     got = ref.philox(key[0] | key[1] << 32, counter[2], counter[3], [counter[0] | counter[1] << 32])
     assert got[0].tolist() == [w >> s & 0xffff for w in words for s in (0, 16)]
+
+
+def test_a_layers_calls_run_on_its_inputs_device(two_devices, monkeypatch):
+    """project and TrainLayer.forward launch on the device of x, also where another is the current one."""
+    from solution import layer, train
+
+    class X(Tensor):
+        shape = (3, 8)
+
+        def reshape(self, *shape):
+            return self
+
+    seen = []
+
+    class Stop(Exception):
+        pass
+
+    class Function:
+        @staticmethod
+        def apply(*args):
+            seen.append(two_devices[0])
+            raise Stop
+
+    monkeypatch.setattr(layer, "NF4Projection", Function)
+    monkeypatch.setattr(train, "AddNorm", Function)
+    spec = layer.ProjectionSpec([])
+    for call in (lambda: layer.project(X(1), spec), lambda: layer.project(spec=spec, x=X(1))):
+        with pytest.raises(Stop):
+            call()
+    a, b = torch.zeros(2, 8), torch.zeros(8, 2)
+    step = train.TrainLayer({n: None for n in ("q", "k", "v", "o", "gate", "up", "down")}, None, None, 1, 1, (a, b, a, b))
+    for call in (lambda: step.forward(X(1), None, None, dtype=torch.float16),
+                 lambda: step.forward(cos=None, sin=None, x=X(1), dtype=torch.float16)):
+        with pytest.raises(Stop):
+            call()
+    assert seen == [1] * 4 and two_devices == [0]
