@@ -275,13 +275,15 @@ struct Stager {
         pitch = static_cast<int>(x.tok) * 2;
         off = row * pitch + ((ch ^ swizzle<D>(row)) << 4);
     }
-    // the next tile to LDS address `at` (the wave's); rows from `rows` on are zeros, and not read
-    __device__ __forceinline__ void send(uint32_t at, int rows) {
-        const int n = rows < ROWS ? rows : ROWS;
-        const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint16_t *>(next), static_cast<short>(0),
+    // the next tile to LDS address `at` (the wave's); rows from `rows` on, and the first `skip`, are zeros, and not
+    // read (the buffer begins at row `skip`: offsets before it are negative, which is past its end)
+    __device__ __forceinline__ void send(uint32_t at, int rows, int skip = 0) {
+        const int n = (rows < ROWS ? rows : ROWS) - skip, before = skip * pitch;
+        const auto *first = reinterpret_cast<const char *>(next) + before;
+        const rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(first), static_cast<short>(0),
                                                            n > 0 ? (n - 1) * pitch + D * 2 : 0, 0x00020000);
 #pragma unroll
-        for (int x = 0; x < ROWS / RPP; ++x) lds_dma16(at + x * 4096, off + x * RPP * pitch, r, 0);
+        for (int x = 0; x < ROWS / RPP; ++x) lds_dma16(at + x * 4096, off + x * RPP * pitch - before, r, 0);
         next = reinterpret_cast<const uint16_t *>(reinterpret_cast<const char *>(next) + static_cast<int64_t>(ROWS) * pitch);
     }
 };
@@ -598,8 +600,11 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     for (int x = 0; x < DN; ++x) acc[x] = (float16_t){};
     int k = steps ? first : all.y, st = 0;
     if (k < all.y) {
-        sk.send(mine, all.y - k);
-        sv.send(mine + 2 * TB, all.y - k);
+        // (what lies before the rows' first key is not theirs: with a NaN in it every one of their sequence's
+        // rows was formed again)
+        const int skip = all.x > k ? all.x - k : 0;
+        sk.send(mine, all.y - k, skip);
+        sv.send(mine + 2 * TB, all.y - k, skip);
     }
     for (; k < all.y; k += kTile, st ^= 1) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -1070,8 +1075,9 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     const uint32_t mine = __builtin_amdgcn_readfirstlane(lds0 + w * 1024);
     int k = u.x < u.y ? first : last, st = 0;
     if (k < last) {
-        sk.send(mine, last - k);
-        sv.send(mine + 2 * TB, last - k);
+        const int skip = keys.x > k ? keys.x - k : 0;  // (as in the forward pass)
+        sk.send(mine, last - k, skip);
+        sv.send(mine + 2 * TB, last - k, skip);
     }
     // (what the rows see is found while all that is on its way)
     const int2 seen = keys_of(a, r);
@@ -1139,7 +1145,10 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
                 const uint64_t see = seen_bits(seen, k);
 #pragma unroll
                 for (int e = 0; e < 16; ++e)
-                    if (!bit_of(see, h, e)) sc[e] = a.c < 0.f && near ? INFINITY : -INFINITY;
+                    if (!bit_of(see, h, e)) {
+                        sc[e] = a.c < 0.f && near ? INFINITY : -INFINITY;
+                        dp[e] = 0.f;  // (a NaN of v that the row does not see)
+                    }
             }
 #pragma unroll
             for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], mul, -sub)) * dp[e];
@@ -1220,9 +1229,9 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
     };
     const float *rw_next = numbers(uh) + ut * 128;
     auto send = [&](int st) {
-        const int left = rows.y - (t0 + ut) * kRows;
-        sq.send(tiles0 + st * RB, left);
-        sg.send(tiles0 + (2 + st) * RB, left);
+        const int left = rows.y - (t0 + ut) * kRows, skip = ut ? 0 : rows.x - t0 * kRows;
+        sq.send(tiles0 + st * RB, left, skip);
+        sg.send(tiles0 + (2 + st) * RB, left, skip);
         if (w == 0)  // (512 bytes: the upper lanes' are past the end, zeros)
             lds_dma16(rows0 + st * 1024, l * 16, make_rsrc(reinterpret_cast<const float *>(uniform64(reinterpret_cast<int64_t>(rw_next))), 512), 0);
         rw_next += 128;
@@ -1318,7 +1327,10 @@ __device__ __forceinline__ void dkv_body(const Attn &a, const Back &b, int kvh, 
             const uint64_t see = seen_bits(seen, r);
 #pragma unroll
             for (int e = 0; e < 16; ++e)
-                if (!bit_of(see, 0, e)) sc[e] = -INFINITY;
+                if (!bit_of(see, 0, e)) {
+                    sc[e] = -INFINITY;
+                    dp[e] = 0.f;  // (a row's NaN that the key is not seen by)
+                }
         }
         read_t(0);
         __builtin_amdgcn_sched_barrier(0);

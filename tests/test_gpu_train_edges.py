@@ -525,3 +525,65 @@ def test_two_adapters_of_one_site(cuda):
     assert torch.equal(y[:, :64], y[:, 64:])
     y = forward(7, 8)
     assert not torch.equal(y[:, :64], y[:, 64:])
+
+
+# --------------------------------------------- what lies beside a sequence costs nothing
+
+def gpu_us(call):
+    times = []
+    for _ in range(6):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        call()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) * 1e3)
+    return sorted(times)[2]
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("value", [math.nan, math.inf])
+def test_rows_before_the_first_sequence(cuda, dtype, dim, value):
+    """Rows of no sequence in the first tile: results are the same bit for bit, and in about the same time
+    (each row formed again on its own: 55 times as long)."""
+    from solution import kernels
+
+    q, k, v, dout, _ = make(cuda, dtype, 4, 2, dim, (2148,), seed=107, layout="plain")
+    c = torch.tensor([101, 2148], dtype=torch.int32, device=cuda)
+
+    def both():
+        out, stats = kernels.attention_fwd(q, k, v, c)
+        return [out, stats, *kernels.attention_bwd(dout, q, k, v, out, stats, c)]
+
+    want, clean = both(), gpu_us(both)
+    for t in (q, k, v, dout):
+        t[:101] = value
+    assert all(torch.equal(a, b) for a, b in zip(both(), want))
+    assert gpu_us(both) < 5 * clean + 100
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_a_nan_of_v_beside_and_before(cuda, dtype, dim):
+    """A NaN of v at the end of a short sequence leaves the long one behind it as it is, and the keys and rows
+    before it have their gradients from the tiles: about the time of finite values (67 times as long before)."""
+    from solution import kernels
+
+    q, k, v, dout, cu = make(cuda, dtype, 4, 2, dim, (101, 2000), seed=108, layout="plain")
+    c = torch.tensor(cu, dtype=torch.int32, device=cuda)
+    out, stats = kernels.attention_fwd(q, k, v, c)
+    want = ref.attention(q, k, v, cu, dout)
+    clean = gpu_us(lambda: kernels.attention_bwd(dout, q, k, v, out, stats, c))
+    v[98, :, 5] = math.nan
+    out2, stats2 = kernels.attention_fwd(q, k, v, c)
+    assert torch.equal(out2[128:], out[128:]) and torch.equal(stats2, stats)
+    got = kernels.attention_bwd(dout, q, k, v, out2, stats2, c)
+    assert gpu_us(lambda: kernels.attention_bwd(dout, q, k, v, out2, stats2, c)) < 5 * clean + 100
+    # (not bit for bit: the outputs of rows 101 to 127, whose wave has rows that see it, are formed in fp32,
+    # so their D differs by a rounding)
+    for name, t in zip(("dq", "dk", "dv"), got):
+        ref.assert_within(t[101:], tuple(x[101:] for x in want[name]), name)  # another sequence's
+        assert torch.isnan(t[98:101]).all(), name
+    ref.assert_within(got[0][:98], tuple(x[:98] for x in want["dq"]), "dq")  # rows that do not see it
+    assert torch.isnan(got[1][:98]).all() and torch.isnan(got[2][:98]).all()  # keys that the NaN rows see
