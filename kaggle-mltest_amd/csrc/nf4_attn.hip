@@ -380,14 +380,19 @@ __device__ __forceinline__ bool bit_of(uint64_t m, int h, int e) {
     return static_cast<uint32_t>(m >> (32 * h)) >> (8 * (e >> 2) + (e & 3)) & 1;
 }
 
-// Probabilities are rounded to 16 bits for the second product; fp16's are 2^15 times as large, so that
-// those down to 2^-29 keep their bits (its least normal number is 2^-14).
+// Probabilities, and dS in the backward pass, are rounded to the inputs' 16 bits for the second product, half a
+// step each: they are operands of matrix instructions, which take fp32 at a sixteenth of the rate.  Against 64
+// bits, results are off by 1.1 (forward) to 1.4 times (backward) as much as with fp32 in their place, rounded once
+// at the end.  fp16's probabilities are 2^15 times as large, so that those down to 2^-29 keep their bits (its
+// least normal number is 2^-14).
 template <int DT>
 constexpr float kTop = DT == NF4_BF16 ? 0.f : 15.f;
 
 // Infinities and NaN.  A probability of 0 that stands for a key that is not seen makes NaN of an infinity
 // or NaN beside it in the tile.  So a row (or key) whose sums hold a NaN is formed again from what it
-// sees alone, by the functions above, unless what it sees says that it is NaN.
+// sees alone, by the functions above, unless what it sees says that it is NaN.  That takes 50 us for a row of 2000
+// keys, one behind the other: it is for the rows (or keys) that share a workgroup's 128 with some that see the
+// value, and what no row of a workgroup sees comes to LDS as zeros.
 template <int N>
 __device__ __forceinline__ bool any_nan(const float16_t (&v)[N]) {
     float odd = 0.f;
@@ -554,10 +559,12 @@ __device__ __forceinline__ void join_write(const Strided &out, int head, int r0,
 // ------------------------------------------------------------------------------ forward
 //
 // The running maximum and sum of a row stay in its lane; a wave whose rows' maxima all hold does not
-// rescale.  8192 tokens of 28 heads of 128 over 4, bf16: 495 us, 972 TFLOP/s.  A step of 64 keys for 128 rows
-// takes two workgroups on a CU 2.2 us: its matrix instructions alone, on values as these are, 1.27 at the
-// clock that the power cap leaves (0.93 on zeros), the exponentials, maxima and sums 0.24 more, reading k and v
-// out of LDS 0.26, barrier and DMA 0.2.  (The next step's scores formed between this one's exponentials, in the
+// rescale.  8192 tokens of 28 heads of 128 over 4, bf16: 490-505 us from card to card, 950-980 TFLOP/s.  A step
+// of 64 keys for 128 rows takes two workgroups on a CU 2.2 us.  In a loop of its own it takes 1.98: its matrix
+// instructions alone, on values as these are, 1.27 at the clock that the power cap leaves (0.93 on zeros), the
+// exponentials, maxima and sums 0.24 more, reading k and v out of LDS 0.27, barrier and DMA 0.2; where the other
+// 0.2 go was not found.  8192 tokens of 14 heads of 64 over 2, bf16: 181 us; a lane has as many exponentials for
+// half the products, and its vector instructions take about three quarters of the cycles.  (The next step's scores formed between this one's exponentials, in the
 // same wave: 20 % slower, and not faster without its spills, in steps of 32 keys.)
 template <int DT, int D>
 __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pieces pc, int tiles) {
@@ -803,16 +810,18 @@ constexpr float kNear = 256.f;
 // whatever the lengths of the sequences are (device data).  A step belongs to the share in which it
 // begins; a tile whose steps are in several leaves a part for each, and the join launch sums a tile's
 // parts in their order.  (Heads of 128, bf16, the whole pass: one sequence of 2048, 12 heads over 2: 81 us,
-// a fifth more with pieces of equal length; of 4096: 234, 28 % more; of 8192, 28 over 4: 1620, the same; 30
+// a fifth more with pieces of equal length; of 4096: 210, 28 % more; of 8192, 28 over 4: 1640, the same; 30
 // sequences of 200, 16 heads of 64: 50 with a workgroup a tile, 40 % more with shares.  Half as many shares,
 // one a CU: 2048 100 us, 8192 2270.)
 //
-// What bounds it, bf16, 8192 tokens of 28 heads of 128 over 4: the rows' launch 22 us, this one 1600, the join
-// 22.  It does 7 products where a formula's 5 would do (the scores and do.v are formed for the keys and for the
+// What bounds it, bf16, 8192 tokens of 28 heads of 128 over 4: the rows' launch 22 us, this one about 1600, the
+// join 22; 1590-1690 together, from card to card.  It does 7 products where a formula's 5 would do (the scores and do.v are formed for the keys and for the
 // rows again, since a sum of dq over the keys' workgroups would need atomics, whose order changes results):
 // 1.04 PFLOP/s of them, where a large matrix product by the library reaches 1.35.  The matrix pipe is busy 51 % of the
 // cycles, at 1.64 GHz: the power cap.  At 2048 tokens of 12 heads (65 us, the join 15) a workgroup has about 17
-// steps, and 55 MB of parts are written and read again.
+// steps, and 55 MB of parts are written and read again.  Both bodies, the rows and keys formed one by one and the
+// shares' bookkeeping are one kernel: with heads of 128 it has all 256 vector registers (bf16 one more, in scratch
+// memory) and about 230 scalar ones kept in lanes of them; with heads of 64 168 and 225.
 constexpr int kKeyCost = 20, kRowCost = 30, kItemCost = 80;  // a step of keys, of rows; a tile
 constexpr int kLeast = 160;                                  // a share
 
