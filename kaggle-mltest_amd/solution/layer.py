@@ -34,6 +34,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import kernels
+from .nf4 import _gemm_rows
 
 _CODE: dict = {}
 
@@ -124,11 +125,8 @@ _FAR = 1 << 23  # elements from a token's row to the next: the attention kernels
 
 
 def _aligned_rows(t: torch.Tensor) -> torch.Tensor:
-    """t [rows, cols] as the kernels take it: rows 16-byte aligned.  (A copy by clone: contiguous() gives
-    back a contiguous tensor that starts at another address as it is.)"""
-    if t.stride(-1) != 1 or t.stride(0) % 8 or t.stride(0) > _FAR or t.data_ptr() % 16:
-        return t.clone(memory_format=torch.contiguous_format)
-    return t
+    """t [rows, cols] as the kernels take it: rows 16-byte aligned (a copy where they are not)."""
+    return _gemm_rows(t.clone(memory_format=torch.contiguous_format) if t.stride(0) > _FAR else t)
 
 
 def _run_jobs(fn, jobs, like):

@@ -587,3 +587,35 @@ def test_a_nan_of_v_beside_and_before(cuda, dtype, dim):
         assert torch.isnan(t[98:101]).all(), name
     ref.assert_within(got[0][:98], tuple(x[:98] for x in want["dq"]), "dq")  # rows that do not see it
     assert torch.isnan(got[1][:98]).all() and torch.isnan(got[2][:98]).all()  # keys that the NaN rows see
+
+
+@pytest.mark.parametrize("widths", [(100,), (100, 64), (64, 100, 128)])
+@pytest.mark.parametrize("m", [1, 40])
+def test_projection_of_any_width(cuda, widths, m):
+    """Rows of Y and dY that are no multiple of 8 apart: the gradients of x and of the adapters, against the
+    products in 64 bits.  A sum of n terms is off by n half steps of fp32 of their sizes' sum, the operands that
+    are rounded on the way (t, da) and the result by half a step of fp16 each, and so is d(xd)."""
+    from solution import kernels
+    from solution.layer import LoraAdapter, ProjectionSpec, project
+
+    segs = [random_weight(n, 128, seed=120 + i, dev=cuda) for i, n in enumerate(widths)]
+    g = torch.Generator().manual_seed(121)
+    rnd = lambda *s: torch.randn(*s, generator=g).half().to(cuda)  # noqa: E731
+    n, p = sum(widths), 0.25
+    x, dy, a, b = rnd(m, 128).requires_grad_(), rnd(m, n), rnd(8, 128).requires_grad_(), rnd(widths[0], 8).requires_grad_()
+    seed = torch.tensor([4, 4], device=cuda)
+    project(x, ProjectionSpec(segs, [LoraAdapter(0, 2.0, dropout=p, site=3)], seed), None, (a, b)).backward(dy)
+    w = torch.cat([oracle_w16(*s) for s in segs]).double()
+    d0, d, a64, b64 = dy[:, :widths[0]].double().cpu(), dy.double().cpu(), a.detach().double().cpu(), b.detach().double().cpu()
+    xd = kernels.dropout(x.detach(), p, seed, [3])[0].double().cpu()
+    keep = ref.kept(4, 4, 3, m, 128, p).double() * ref.drop_scale(p)
+    half, terms = ref.HALF[F16], (n + 128 + 16) * ref.U32
+
+    def within(got, value, size, roundings):
+        ref.assert_within(got, (value, 1.01 * (roundings * half + terms) * size + ref.TINY[F16]), "gradient")
+
+    t, da = xd @ a64.t(), 2.0 * d0 @ b64
+    t_size, da_size = xd.abs() @ a64.abs().t(), 2.0 * d0.abs() @ b64.abs()
+    within(x.grad, d @ w + (da @ a64) * keep, d.abs() @ w.abs() + (da_size @ a64.abs()) * keep, 4)
+    within(a.grad, da.t() @ xd, da_size.t() @ xd.abs(), 2)
+    within(b.grad, 2.0 * d0.t() @ t, 2.0 * d0.abs().t() @ t_size, 2)
