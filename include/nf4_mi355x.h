@@ -495,7 +495,7 @@ int nf4_paged_attn(const nf4_paged_kv *kv, const void *q, int64_t ld_tok, int64_
  * max_len is the longest sequence as the host knows it (0: unknown): it chooses the launch shape
  * only, longer sequences are still right.
  * Supported: F16 and BF16, head_dim 64 or 128, pointers 16-byte aligned, strides multiples of 8 (a
- * dimension of one has no stride that counts) of at most 2^23, tokens at most 2^23 and
+ * dimension of one has no stride that counts), the tokens' at most 2^23, tokens at most 2^23 and
  * tokens * n_heads at most 2^30, n_heads at most 1024, batch at most 2^20; scale any number of
  * magnitude up to 2.3e38 (NaN and infinities: NF4_ERR_ARG). */
 typedef struct nf4_attn {

@@ -911,7 +911,7 @@ def attention_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
                   window: int = 0, max_len: int = 0, out: torch.Tensor | None = None):
     """Causal attention of a packed batch: (out [tokens, n_heads, head_dim], stats fp32
     [tokens, n_heads, 2]) of q [tokens, n_heads, head_dim], k and v [tokens, n_kv, head_dim] (any
-    strides, head_dim contiguous: columns of the projection's output as they are).  `cu_seqlens`:
+    strides of whole 16 bytes, head_dim contiguous: columns of the projection's output as they are).  `cu_seqlens`:
     int32 offsets of the sequences on the device (None: one sequence); row i of one sees its rows
     j <= i where window == 0 or j > i - window.  stats are (m, l): with t = scale log2(e) q.k, m =
     max t and l = sum 2^(t - m); a row behind the last sequence gives zeros and (0, 0).  `max_len`:
