@@ -422,22 +422,24 @@ __device__ __forceinline__ void fill_of(float16_t (&v)[N], float f) {
         for (int e = 0; e < 16; ++e) v[x][e] = f;
 }
 
-// Which of a wave's rows (bits) see a NaN of v, for each of a lane's channels D / 64 l ..: such a row's
-// sum in that channel is NaN.  `seen`: the keys of this lane's row; all rows' lie in [lo, hi).  One pass over v
-// for the 32 rows; formed again one by one, all rows behind an early NaN made the forward pass 110 times as long
-// at 2048 tokens, 280 times at 4096.
-template <int DT, int D>
-__device__ __forceinline__ void nan_values(const Attn &a, int kvh, int lo, int hi, int2 seen, uint32_t (&by)[D / 64]) {
-    constexpr uint32_t INF = DT == NF4_BF16 ? 0x7f80u : 0x7c00u;
+// Which of a wave's rows (bits) see a value x [keys, D] that makes its sum NaN, for each of a lane's channels
+// D / 64 l ..: a NaN of v in the forward pass, with INFS also an infinity, of k in the backward pass (a row that is
+// not NaN itself has a score of -inf with such a key, and 0 times an infinity in that channel).  `seen`: the
+// keys of this lane's row; all rows' lie in [lo, hi).  One pass over x for the 32 rows; formed again one by one, all
+// rows behind an early NaN of v made the forward pass 110 times as long at 2048 tokens, 280 times at 4096, and those
+// behind an infinite k the backward pass 40 and 60 times.
+template <int DT, int D, bool INFS>
+__device__ __forceinline__ void nan_by(const Strided &v, int head, int lo, int hi, int2 seen, uint32_t (&by)[D / 64]) {
+    constexpr uint32_t MOST = (DT == NF4_BF16 ? 0x7f80u : 0x7c00u) - INFS;
 #pragma unroll
     for (int i = 0; i < D / 64; ++i) by[i] = 0;
     for (int k = lo; k < hi; k += kAtOnce) {
         uint32_t w[kAtOnce];
 #pragma unroll
-        for (int u = 0; u < kAtOnce; ++u) w[u] = channels_of<D>(a.v.at(k + u < hi ? k + u : hi - 1, kvh));
+        for (int u = 0; u < kAtOnce; ++u) w[u] = channels_of<D>(v.at(k + u < hi ? k + u : hi - 1, head));
 #pragma unroll
         for (int u = 0; u < kAtOnce; ++u) {
-            const bool x = (w[u] & 0x7fffu) > INF, y = D == 128 && (w[u] >> 16 & 0x7fffu) > INF;
+            const bool x = (w[u] & 0x7fffu) > MOST, y = D == 128 && (w[u] >> 16 & 0x7fffu) > MOST;
             if (!__any(x || y)) continue;
             const uint32_t rows = rows_where(seen.x <= k + u && k + u < seen.y);
             if (x) by[0] |= rows;
@@ -699,7 +701,7 @@ __global__ __launch_bounds__(256, 2) void attn_fwd_kernel(const Attn a, const Pi
     uint32_t again = rows_where(some && !nan && any_nan(acc));
     if (again) {  // but for what a NaN of v explains
         uint32_t by[D / 64];
-        nan_values<DT, D>(a, kvh, sp.lo > first ? sp.lo : first, sp.hi < all.y ? sp.hi : all.y, part, by);
+        nan_by<DT, D, false>(a.v, kvh, sp.lo > first ? sp.lo : first, sp.hi < all.y ? sp.hi : all.y, part, by);
         again &= rows_where(unexplained<D>(acc, by));
     }
     // a row that sees nothing has zeros (its registers hold anything: no mask kept tiles from it that every
@@ -820,8 +822,8 @@ constexpr float kNear = 256.f;
 // 1.04 PFLOP/s of them, where a large matrix product by the library reaches 1.35.  The matrix pipe is busy 51 % of the
 // cycles, at 1.64 GHz: the power cap.  At 2048 tokens of 12 heads (65 us, the join 15) a workgroup has about 17
 // steps, and 55 MB of parts are written and read again.  Both bodies, the rows and keys formed one by one and the
-// shares' bookkeeping are one kernel: with heads of 128 it has all 256 vector registers (bf16 one more, in scratch
-// memory) and about 230 scalar ones kept in lanes of them; with heads of 64 168 and 225.
+// shares' bookkeeping are one kernel: with heads of 128 it has all 256 vector registers (bf16 two more, in scratch
+// memory) and about 220 scalar ones kept in lanes of them; with heads of 64 168 (fp16 one more) and 220 to 240.
 constexpr int kKeyCost = 20, kRowCost = 30, kItemCost = 80;  // a step of keys, of rows; a tile
 constexpr int kLeast = 160;                                  // a share
 
@@ -1174,7 +1176,12 @@ __device__ __forceinline__ void dq_body(const Attn &a, const Back &b, int head, 
     const bool some = own.x < own.y;
     if (part) part += w * 32 * D;
     const bool nan = some && base != base;
-    const uint32_t again = rows_where(some && !nan && any_nan(acc));
+    uint32_t again = rows_where(some && !nan && any_nan(acc));
+    if (again) {  // but for what an infinity of k explains
+        uint32_t by[D / 64];
+        nan_by<DT, D, true>(a.k, kvh, sp.lo > first ? sp.lo : first, sp.hi < last ? sp.hi : last, own, by);
+        again &= rows_where(unexplained<D>(acc, by));
+    }
     if (!some) fill_of(acc, 0.f);
     else if (nan) fill_of(acc, NAN);
     const float f = a.scale * (ldexpf(1.f, -static_cast<int>(kTop<DT>)) / fs);

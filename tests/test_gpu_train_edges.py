@@ -619,3 +619,33 @@ def test_projection_of_any_width(cuda, widths, m):
     within(x.grad, d @ w + (da @ a64) * keep, d.abs() @ w.abs() + (da_size @ a64.abs()) * keep, 4)
     within(a.grad, da.t() @ xd, da_size.t() @ xd.abs(), 2)
     within(b.grad, 2.0 * d0.t() @ t, 2.0 * d0.abs().t() @ t_size, 2)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("dim,value", [(64, math.inf), (128, -math.inf)])
+def test_an_infinite_key_of_no_weight(cuda, dtype, dim, value):
+    """The first key has a score of -inf with every later row, by an infinity in one channel: those rows are a
+    sequence that begins behind it, but for 0 times that infinity in their dq (formed again one by one, 40 times
+    as long for 2048 tokens)."""
+    from solution import kernels
+
+    q, k, v, dout, cu = make(cuda, dtype, 4, 2, dim, (1400,), seed=122, layout="plain")
+    q[:, :2, 5] = -1.0 if value > 0 else 1.0  # the heads of key head 0
+    k[:, 0, 5] = 0.25
+    clean = run(q, k, v, dout, cu)
+    want = ref.attention(q[1:], k[1:], v[1:], [0, 1399], dout[1:])
+    whole = ref.attention(q, k, v, cu, dout)
+    time = gpu_us(lambda: kernels.attention_bwd(dout, q, k, v, clean["out"], clean["stats"]))
+    k[0, 0, 5] = value
+    got = run(q, k, v, dout, cu)
+    assert gpu_us(lambda: kernels.attention_bwd(dout, q, k, v, got["out"], got["stats"])) < 10 * time + 100
+    other = [c for c in range(dim) if c != 5]
+    for name, n in (("out", 2), ("stats", 2), ("dq", 2), ("dk", 1), ("dv", 1)):
+        assert torch.isnan(got[name][0, :n]).all(), name
+        x, (val, bound) = got[name].cpu(), want[name]
+        if name == "dq":
+            assert torch.isnan(x[1:, :2, 5]).all()
+            ref.assert_within(x[1:, :2, other], (val[:, :2, other], bound[:, :2, other]), name)
+        else:
+            ref.assert_within(x[1:, :n], (val[:, :n], bound[:, :n]), name)
+        ref.assert_within(x[:, n:], tuple(t[:, n:] for t in whole[name]), name)
