@@ -561,7 +561,7 @@ __device__ __forceinline__ void join_write(const Strided &out, int head, int r0,
 // ------------------------------------------------------------------------------ forward
 //
 // The running maximum and sum of a row stay in its lane; a wave whose rows' maxima all hold does not rescale.  8192
-// tokens of 28 heads of 128 over 4, bf16: 490-505 us from card to card, 950-980 TFLOP/s.  A step of 64 keys for 128
+// tokens of 28 heads of 128 over 4, bf16: 490-512 us from card to card, 940-980 TFLOP/s.  A step of 64 keys for 128
 // rows takes two workgroups on a CU 2.2 us.  In a loop of its own it takes 1.98: its matrix instructions alone, on
 // values as these are, 1.27 at the clock that the power cap leaves (0.93 on zeros), the exponentials, maxima and
 // sums 0.24 more, reading k and v out of LDS 0.27, barrier and DMA 0.2; where the other 0.2 go was not found.  8192
@@ -817,7 +817,7 @@ constexpr float kNear = 256.f;
 // one a CU: 2048 100 us, 8192 2270.)
 //
 // What bounds it, bf16, 8192 tokens of 28 heads of 128 over 4: the rows' launch 22 us, this one about 1600, the
-// join 22; 1590-1690 together, from card to card.  It does 7 products where a formula's 5 would do (the scores and
+// join 22; 1590-1730 together, from card to card.  It does 7 products where a formula's 5 would do (the scores and
 // do.v are formed for the keys and for the rows again, since a sum of dq over the keys' workgroups would need
 // atomics, whose order changes results): 1.04 PFLOP/s of them, where a large matrix product by the library reaches
 // 1.35.  The matrix pipe is busy 51 % of the cycles, at 1.64 GHz: the power cap.  At 2048 tokens of 12 heads (65
